@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <new>
 #include <string>
@@ -317,6 +318,15 @@ int nomas_moe_forward_block(nomas_moe_t* h, const void* x, void* out, int64_t ro
     });
 }
 
+int nomas_moe_forward_routed(nomas_moe_t* h, const void* x, const int32_t* idx, const float* w, void* y,
+                             int64_t rows, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
+        return h->layer->forward_routed(x, {idx, w}, y, rows, static_cast<hipStream_t>(stream));
+    });
+}
+
 int nomas_moe_forward_host(nomas_moe_t* h, const void* x, void* y, int64_t rows) {
     return guarded(__func__, [&]() -> int {
         nomas::clear_error();
@@ -562,6 +572,229 @@ int nomas_gated_residual(int dtype, const void* x, const void* y, const float* g
                                                     (int)dim, seq, static_cast<hipStream_t>(stream));
         if (e != hipSuccess)
             return set_error(NOMAS_ERR_HIP, "gated residual launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
+namespace {
+
+bool misaligned(std::initializer_list<const void*> ps, uintptr_t to) {
+    for (const void* p : ps)
+        if (reinterpret_cast<uintptr_t>(p) % to) return true;
+    return false;
+}
+
+// What the seam and its gradients ask of their arguments alike.
+int check_block_seam(int dtype, int64_t rows, int64_t dim, int64_t seq, double residual_scale, double eps) {
+    if (dtype < 0 || dtype > 2) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (rows < 0 || rows > nomas::kMaxSeamRows)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
+    if (dim <= 0 || dim % 8 != 0 || dim > nomas::kMaxSeamDim)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dim must be a positive multiple of 8 up to %d (got %lld)",
+                         nomas::kMaxSeamDim, (long long)dim);
+    if (seq < 1 || rows % seq != 0)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT,
+                         "rows=%lld must be a whole number of sequences of seq=%lld",
+                         (long long)rows, (long long)seq);
+    if (!(eps >= 0.0)) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+    if (!std::isfinite(residual_scale))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "residual_scale must be finite");
+    return NOMAS_OK;
+}
+
+int check_route(int dtype, int64_t rows, int64_t experts, int64_t top_k, int scoring, double scale, double eps) {
+    if (dtype < 0 || dtype > 2) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (experts < 1 || top_k < 1 || top_k > experts)
+        return set_error(NOMAS_ERR_INVALID_CONFIG, "invalid MoE top_k/experts (top_k=%lld, experts=%lld)",
+                         (long long)top_k, (long long)experts);
+    if (experts > nomas::kMaxRouteExperts)
+        return set_error(NOMAS_ERR_INVALID_CONFIG, "experts=%lld exceeds the supported maximum %d",
+                         (long long)experts, nomas::kMaxRouteExperts);
+    if (rows < 0 || rows > 0x7fffffffLL)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
+    if (scoring != NOMAS_SOFTMAX && scoring != NOMAS_SIGMOID)
+        return set_error(NOMAS_ERR_INVALID_CONFIG, "unknown scoring %d", scoring);
+    if (!std::isfinite(scale)) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "scale must be finite");
+    if (!(eps >= 0.0) || !std::isfinite(eps))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be >= 0 and finite");
+    return NOMAS_OK;
+}
+
+}  // namespace
+
+int nomas_route(int dtype, const void* logits, int64_t rows, int64_t experts, int64_t top_k, int scoring,
+                const float* bias, int64_t groups, int64_t top_groups, int64_t group_top, int renormalize,
+                double scale, double eps, int32_t* idx, float* w, int32_t* counts, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        int rc = check_route(dtype, rows, experts, top_k, scoring, scale, eps);
+        if (rc != NOMAS_OK) return rc;
+        if (groups < 1 || groups > nomas::kMaxRouteGroups || experts % groups != 0)
+            return set_error(NOMAS_ERR_INVALID_CONFIG, "groups=%lld must divide experts=%lld and be at most %d",
+                             (long long)groups, (long long)experts, nomas::kMaxRouteGroups);
+        if (top_groups < 1 || top_groups > groups || experts / groups * top_groups < top_k)
+            return set_error(NOMAS_ERR_INVALID_CONFIG,
+                             "top_groups=%lld of %lld groups of %lld experts do not hold top_k=%lld",
+                             (long long)top_groups, (long long)groups, (long long)(experts / groups),
+                             (long long)top_k);
+        if (group_top != 1 && group_top != 2)
+            return set_error(NOMAS_ERR_INVALID_CONFIG, "group_top must be 1 or 2 (got %lld)", (long long)group_top);
+        if (rows > 0 && (!logits || !idx || !w))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "logits, idx and w must be non-null");
+        if (rows == 0 && !counts) return NOMAS_OK;
+        if (misaligned({logits}, dtype == NOMAS_F32 ? 4 : 2) || misaligned({bias, idx, w, counts}, 4))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "misaligned pointer");
+        nomas::RouteArgs a;
+        a.logits = logits;
+        a.bias = bias;
+        a.rows = rows;
+        a.E = (int)experts;
+        a.k = (int)top_k;
+        a.sigmoid = scoring == NOMAS_SIGMOID;
+        a.groups = (int)groups;
+        a.top_groups = (int)top_groups;
+        a.group_top = (int)group_top;
+        a.renormalize = renormalize != 0;
+        a.scale = scale;
+        a.eps = eps;
+        a.idx = idx;
+        a.w = w;
+        a.counts = counts;
+        const hipError_t e = nomas::launch_route(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return set_error(NOMAS_ERR_HIP, "route launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
+int nomas_route_backward(int dtype, const void* logits, const int32_t* idx, const float* dw, int64_t rows,
+                         int64_t experts, int64_t top_k, int scoring, int renormalize, double scale, double eps,
+                         void* dlogits, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        int rc = check_route(dtype, rows, experts, top_k, scoring, scale, eps);
+        if (rc != NOMAS_OK || rows == 0) return rc;
+        if (!logits || !idx || !dw || !dlogits)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "logits, idx, dw and dlogits must be non-null");
+        if (misaligned({logits, dlogits}, dtype == NOMAS_F32 ? 4 : 2) || misaligned({idx, dw}, 4))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "misaligned pointer");
+        nomas::RouteBackwardArgs a;
+        a.logits = logits;
+        a.idx = idx;
+        a.dw = dw;
+        a.rows = rows;
+        a.E = (int)experts;
+        a.k = (int)top_k;
+        a.sigmoid = scoring == NOMAS_SIGMOID;
+        a.renormalize = renormalize != 0;
+        a.scale = scale;
+        a.eps = eps;
+        a.dlogits = dlogits;
+        const hipError_t e =
+            nomas::launch_route_backward(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess)
+            return set_error(NOMAS_ERR_HIP, "route gradient launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
+int nomas_block_seam(int dtype, const void* x, const void* y, void* out, void* h, int64_t rows, int64_t dim,
+                     int64_t seq, const float* gate, int post_norm, const float* post_w, double residual_scale,
+                     const float* norm_w, const float* shift, const float* scale, double eps, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        int rc = check_block_seam(dtype, rows, dim, seq, residual_scale, eps);
+        if (rc != NOMAS_OK || rows == 0) return rc;
+        if (!x || !y || !out) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "x, y and out must be non-null");
+        if (h && (h == out))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "h and out must be different tensors");
+        if (misaligned({x, y, out, h, gate, post_w, norm_w, shift, scale}, 16))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+        nomas::BlockSeamArgs a;
+        a.x = x;
+        a.y = y;
+        a.out = out;
+        a.h = h;
+        a.rows = rows;
+        a.D = (int)dim;
+        a.seq = seq;
+        a.gate = gate;
+        a.post = post_norm != 0;
+        a.post_w = post_w;
+        a.alpha = (float)residual_scale;
+        a.norm_w = norm_w;
+        a.shift = shift;
+        a.scale = scale;
+        a.eps = (float)eps;
+        const hipError_t e =
+            nomas::launch_block_seam(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return set_error(NOMAS_ERR_HIP, "block seam launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
+int64_t nomas_block_seam_workspace(int64_t rows, int64_t dim, int64_t seq) {
+    if (rows < 1 || dim < 1 || seq < 1 || rows % seq != 0 || rows > nomas::kMaxSeamRows ||
+        dim > nomas::kMaxSeamDim)
+        return 0;
+    return nomas::block_seam_workspace(rows, dim, seq);
+}
+
+int nomas_block_seam_backward(int dtype, const void* dout, const void* dh, const void* out, const void* y,
+                              void* dx, void* dy, int64_t rows, int64_t dim, int64_t seq, const float* gate,
+                              int post_norm, const float* post_w, double residual_scale, const float* norm_w,
+                              const float* scale, double eps, float* dgate, float* dshift, float* dscale,
+                              float* dnorm_w, float* dpost_w, void* workspace, int64_t workspace_bytes,
+                              void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        int rc = check_block_seam(dtype, rows, dim, seq, residual_scale, eps);
+        if (rc != NOMAS_OK) return rc;
+        if (rows > 0 && !dout && !dh)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "one of dout and dh must be non-null");
+        if (rows > 0 && dh && !out) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dh needs out");
+        if (rows > 0 && !y && (dy || dgate || dpost_w))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dy, dgate and dpost_w need y");
+        if (rows > 0 && !dh && (dshift || dscale || dnorm_w))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dshift, dscale and dnorm_w need dh");
+        if (dpost_w && !post_norm)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dpost_w needs post_norm");
+        if (rows == 0 && !dnorm_w && !dpost_w) return NOMAS_OK;
+        if (dx && dx == dy) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dx and dy must be different tensors");
+        if (misaligned({dout, dh, out, y, dx, dy, gate, post_w, norm_w, scale, dgate, dshift, dscale, dnorm_w,
+                        dpost_w, workspace},
+                       16))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+        const int64_t need = nomas::block_seam_workspace(rows, dim, seq);
+        if (rows > 0 && (!workspace || workspace_bytes < need))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "the workspace holds %lld bytes, %lld are needed",
+                             (long long)(workspace ? workspace_bytes : 0), (long long)need);
+        nomas::BlockSeamBackwardArgs a;
+        a.dout = dout;
+        a.dh = dh;
+        a.out = dh ? out : nullptr;
+        a.y = y;
+        a.dx = dx;
+        a.dy = dy;
+        a.rows = rows;
+        a.D = (int)dim;
+        a.seq = seq;
+        a.gate = gate;
+        a.post = post_norm != 0;
+        a.post_w = post_w;
+        a.alpha = (float)residual_scale;
+        a.norm_w = norm_w;
+        a.scale = scale;
+        a.eps = (float)eps;
+        a.dgate = dgate;
+        a.dshift = dshift;
+        a.dscale = dscale;
+        a.dnorm_w = dnorm_w;
+        a.dpost_w = dpost_w;
+        a.workspace = workspace;
+        const hipError_t e =
+            nomas::launch_block_seam_backward(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess)
+            return set_error(NOMAS_ERR_HIP, "block seam gradient launch failed: %s", hipGetErrorString(e));
         return NOMAS_OK;
     });
 }

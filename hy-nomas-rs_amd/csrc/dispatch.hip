@@ -412,7 +412,8 @@ __global__ __launch_bounds__(kDispThreads) __attribute__((amdgpu_waves_per_eu(8)
 // (block.rs:101), its x and gate loaded with the first slots' loads.  kNt:
 // nontemporal output stores.  kBatch: 16-byte chunks per lane per pass (6: a
 // whole 3072-wide 16-bit row per pass, its slots' loads 4 at a time).
-template <typename T, bool kResid, bool kNt, int kBatch>
+// kHoles: rows may have empty slots, which add nothing, whatever y_perm holds.
+template <typename T, bool kResid, bool kNt, int kBatch, bool kHoles = false>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + wave;
@@ -457,7 +458,8 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
                     p[t] = a.tok_pos[row * k + j];
                     w[t] = a.topk_w[row * k + j];
                 }
-                // a slot without a position (none in a valid routing) adds 0 x row 0
+                // a slot without a position (only with kHoles) adds 0 x row 0, or
+                // zeros where row 0 may hold anything
                 const bool ok = p[t] >= 0 && p[t] < a.a_cap;
                 const int64_t pc = ok ? p[t] : 0;
                 w[t] = ok ? w[t] : 0.0f;
@@ -466,6 +468,7 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
                     // y_perm is read once: nontemporally, so that it does not
                     // push other data (the next forward's x) out of the caches
                     raw[t][u] = load16_nt(y + pc * a.D + (int64_t)min(c0 + u * kWave, nchunk - 1) * EPC);
+                    if constexpr (kHoles) raw[t][u] = ok ? raw[t][u] : make_uint4(0, 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -598,7 +601,11 @@ hipError_t launch_combine_t(const CombineArgs& a, hipStream_t s) {
     // pass measured the same as whole rows at top-2 with cached stores).
     // 16-bit types only, where it was measured.
     const bool whole = sizeof(T) == 2 && a.out_nt && (a.D / (16 / (int)sizeof(T))) % (kWave * 6) == 0;
-    auto kern = a.gate ? (a.out_nt ? combine_kernel<T, true, true, 2> : combine_kernel<T, true, false, 2>)
+    if (a.holes && a.gate) return hipErrorInvalidValue;
+    auto kern = a.holes ? (!a.out_nt ? combine_kernel<T, false, false, 2, true>
+                           : whole   ? combine_kernel<T, false, true, 6, true>
+                                     : combine_kernel<T, false, true, 2, true>)
+              : a.gate ? (a.out_nt ? combine_kernel<T, true, true, 2> : combine_kernel<T, true, false, 2>)
               : a.out_nt ? (whole ? combine_kernel<T, false, true, 6> : combine_kernel<T, false, true, 2>)
                          : combine_kernel<T, false, false, 2>;
     launch_kernel(kern, dim3(nblk), dim3(256), 0, s, a);

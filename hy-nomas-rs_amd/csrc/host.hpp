@@ -237,6 +237,13 @@ public:
         const float* gate;
     };
     int forward_block(const void* x, void* out, int64_t rows, const BlockArgs& b, hipStream_t s);
+    // forward() with the caller's routing (rows x top_k experts and weights on
+    // the device) in the place of the router's.
+    struct Given {
+        const int32_t* idx;
+        const float* w;
+    };
+    int forward_routed(const void* x, const Given& g, void* y, int64_t rows, hipStream_t s);
     int forward_host(const void* x, void* y, int64_t rows);
     int forward_host_pieces(const void* x, void* y, int64_t rows, int np, void* dx, void* dy);
     int routing(int32_t* idx, float* w, int32_t* counts, float* gap);
@@ -284,10 +291,11 @@ private:
     bool dense_only_ = false;
     int forward_dense(const void* x, void* y, int64_t rows, hipStream_t s);
     int check_forward(const void* x, const void* y, int64_t rows) const;
-    int forward_impl(const void* x, void* y, int64_t rows, hipStream_t s, const BlockArgs* blk);
+    int forward_impl(const void* x, void* y, int64_t rows, hipStream_t s, const BlockArgs* blk,
+                     const Given* given = nullptr);
     // the stages of a routed forward on the buffers of `w`
     int run_routed(const void* x, void* y, int64_t rows, hipStream_t s, const BlockArgs* blk,
-                   const Workspace& w);
+                   const Workspace& w, const Given* given = nullptr);
     int finish_forward(int64_t rows, hipStream_t s, const Workspace& w, int scratch_pieces = 1);
     void set_widths();
     bool want_block_ = false;  // the workspace holds h for forward_block

@@ -210,11 +210,96 @@ struct CombineArgs {
     const void* resid_x;  // rows x D, model dtype
     const float* gate;    // sequences x D
     int64_t seq;
+    // some slots are empty (tok_pos -1; the routing is the caller's)
+    bool holes = false;
     // write `out` with the nontemporal hint: when y_perm is larger than the
     // last-level cache, its reads stream through it and would evict the
     // output's dirty lines into the middle of them anyway
     int out_nt = 0;
 };
+
+// Routing to experts from logits (route.hip).
+constexpr int kMaxRouteExperts = 1024;
+constexpr int kMaxRouteGroups = 64;
+struct RouteArgs {
+    const void* logits;  // rows x E, model dtype
+    const float* bias;   // E, added to the scores for the choice (null: none)
+    int64_t rows;
+    int E, k;
+    int sigmoid;         // scores: 0 softmax, 1 sigmoid
+    int groups, top_groups, group_top;
+    int renormalize;
+    double scale, eps;
+    int32_t* idx;        // rows x k, ascending, -1 where no expert is left
+    float* w;            // rows x k
+    int32_t* counts;     // E: rows that chose each (null: not wanted)
+};
+struct RouteBackwardArgs {
+    const void* logits;  // rows x E
+    const int32_t* idx;  // rows x k (outside 0 .. E - 1: no expert)
+    const float* dw;     // rows x k
+    int64_t rows;
+    int E, k;
+    int sigmoid, renormalize;
+    double scale, eps;
+    void* dlogits;       // rows x E, model dtype
+};
+
+// The caller's routing, laid out as the router's: what dispatch and combine read.
+struct GivenRoutingArgs {
+    const int32_t* in_idx;  // rows x k
+    const float* in_w;
+    int64_t rows;
+    int E, E_cols, k, k_slots;
+    float dense_coef;
+    int32_t* idx;  // rows x k_slots
+    float* w;
+    int32_t* pos;  // rows x k_slots: -1 where the slot is empty (the dispatch writes the others)
+    float* gap;    // rows: +inf (no choice was made here)
+    int32_t* chunk_counts;  // ceil(rows / 64) x E_cols
+};
+
+// The seam between two branches of a block, and its gradients (block_seam.hip).
+constexpr int kMaxSeamDim = 16384;
+constexpr int64_t kMaxSeamRows = (int64_t)1 << 30;
+struct BlockSeamArgs {
+    const void *x, *y;  // rows x D, model dtype
+    void *out, *h;      // rows x D (h null: no norm before the next branch)
+    int64_t rows;
+    int D;
+    int64_t seq;        // rows per sequence
+    const float* gate;  // sequences x D (null: 1)
+    int post;           // whether y is normalised first
+    const float* post_w;  // D (null: 1)
+    float alpha;        // of x
+    const float* norm_w;  // D (null: 1)
+    const float *shift, *scale;  // sequences x D (null: 0)
+    float eps;
+};
+struct BlockSeamBackwardArgs {
+    const void *dout, *dh;  // rows x D (null: zero)
+    const void *out, *y;    // the forward's output and the branch's (null with dh, or without a branch)
+    void *dx, *dy;          // rows x D (null: not wanted)
+    int64_t rows;
+    int D;
+    int64_t seq;
+    const float* gate;
+    int post;
+    const float* post_w;
+    float alpha;
+    const float* norm_w;
+    const float* scale;
+    float eps;
+    float *dgate, *dshift, *dscale;  // sequences x D (null: not wanted)
+    float *dnorm_w, *dpost_w;        // D
+    void* workspace;                 // block_seam_workspace() bytes
+};
+int64_t block_seam_workspace(int64_t rows, int64_t D, int64_t seq);
+hipError_t launch_block_seam(DType dt, const BlockSeamArgs& a, hipStream_t s);
+hipError_t launch_block_seam_backward(DType dt, const BlockSeamBackwardArgs& a, hipStream_t s);
+hipError_t launch_route(DType dt, const RouteArgs& a, hipStream_t s);
+hipError_t launch_route_backward(DType dt, const RouteBackwardArgs& a, hipStream_t s);
+hipError_t launch_given_routing(const GivenRoutingArgs& a, hipStream_t s);
 
 size_t router_lds_bytes(int E);
 // Rows per router block (and per histogram it writes) for a launch of

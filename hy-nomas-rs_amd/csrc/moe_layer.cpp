@@ -486,8 +486,17 @@ int MoeLayer::forward_block(const void* x, void* out, int64_t rows, const BlockA
     return forward_impl(x, out, rows, s, &b);
 }
 
+int MoeLayer::forward_routed(const void* x, const Given& g, void* y, int64_t rows, hipStream_t s) {
+    if (dense_only_) return set_error(NOMAS_ERR_STATE, "a dense feed-forward has no routing");
+    if (rows > 0 && (!g.idx || !g.w))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "idx and w must be non-null");
+    if ((reinterpret_cast<uintptr_t>(g.idx) | reinterpret_cast<uintptr_t>(g.w)) & 3)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "idx and w must be 4-byte aligned");
+    return forward_impl(x, y, rows, s, nullptr, &g);
+}
+
 int MoeLayer::forward_impl(const void* x, void* y, int64_t rows, hipStream_t s,
-                           const BlockArgs* blk) {
+                           const BlockArgs* blk, const Given* given) {
     int rc = check_forward(x, y, rows);
     if (rc != NOMAS_OK) return rc;
     if (rows == 0) { last_rows_ = 0; last_in_scratch_ = false; return NOMAS_OK; }
@@ -500,7 +509,7 @@ int MoeLayer::forward_impl(const void* x, void* y, int64_t rows, hipStream_t s,
         if (blk) return set_error(NOMAS_ERR_STATE, "the fused block is implemented for the MoE layer");
         return forward_dense(x, y, rows, s);
     }
-    rc = run_routed(x, y, rows, s, blk, ws_);
+    rc = run_routed(x, y, rows, s, blk, ws_, given);
     if (rc != NOMAS_OK) {
         last_rows_ = -1;  // a failed forward may have overwritten the last one's routing
         return rc;
@@ -597,7 +606,7 @@ int MoeLayer::finish_forward(int64_t rows, hipStream_t s, const Workspace& w, in
 }
 
 int MoeLayer::run_routed(const void* x, void* y, int64_t rows, hipStream_t s,
-                         const BlockArgs* blk, const Workspace& w) {
+                         const BlockArgs* blk, const Workspace& w, const Given* given) {
     int rc;
     const int nch = (int)((rows + kRouterRows - 1) / kRouterRows);
     const GemmPlan plan = gemm_plan(rows);
@@ -639,21 +648,40 @@ int MoeLayer::run_routed(const void* x, void* y, int64_t rows, hipStream_t s,
         STAGE(launch_seam_h(dt_, sm, s), "norm/modulate");
         xr = w.block_h;
     }
-    RouterArgs ra;
-    ra.x = xr;
-    ra.wr = d_wr_;
-    ra.rows = rows;
-    ra.D = (int)D_;
-    ra.E = (int)E_;
-    ra.k = (int)k_;
-    ra.k_slots = (int)kslots_;
-    ra.dense_coef = (float)shared_dense_;
-    ra.topk_idx = w.idx;
-    ra.topk_w = w.w;
-    ra.gap = w.gap;
-    ra.chunk_counts = w.chunk_counts;
-    ra.block_rows = router_block_rows(dt_, rows, (int)D_, (int)E_);
-    STAGE(launch_router(dt_, ra, s), "router");
+    const int count_rows = given ? kRouterRows : router_block_rows(dt_, rows, (int)D_, (int)E_);
+    if (given) {
+        GivenRoutingArgs ga;
+        ga.in_idx = given->idx;
+        ga.in_w = given->w;
+        ga.rows = rows;
+        ga.E = (int)E_;
+        ga.E_cols = (int)Ecols_;
+        ga.k = (int)k_;
+        ga.k_slots = (int)kslots_;
+        ga.dense_coef = (float)shared_dense_;
+        ga.idx = w.idx;
+        ga.w = w.w;
+        ga.pos = w.pos;
+        ga.gap = w.gap;
+        ga.chunk_counts = w.chunk_counts;
+        STAGE(launch_given_routing(ga, s), "routing intake");
+    } else {
+        RouterArgs ra;
+        ra.x = xr;
+        ra.wr = d_wr_;
+        ra.rows = rows;
+        ra.D = (int)D_;
+        ra.E = (int)E_;
+        ra.k = (int)k_;
+        ra.k_slots = (int)kslots_;
+        ra.dense_coef = (float)shared_dense_;
+        ra.topk_idx = w.idx;
+        ra.topk_w = w.w;
+        ra.gap = w.gap;
+        ra.chunk_counts = w.chunk_counts;
+        ra.block_rows = count_rows;
+        STAGE(launch_router(dt_, ra, s), "router");
+    }
     if ((rc = mark(1))) return rc;
 
     // the scan of the chunk histograms is part of the dispatch kernel: the
@@ -669,7 +697,7 @@ int MoeLayer::run_routed(const void* x, void* y, int64_t rows, hipStream_t s,
     da.topk_idx = w.idx;
     da.chunk_counts = w.chunk_counts;
     da.nchunks = nch;
-    da.count_rows = ra.block_rows;
+    da.count_rows = count_rows;
     da.BM = plan.bm1;
     da.BM2 = plan.bm2;
     da.max_tiles = mt;
@@ -741,6 +769,7 @@ int MoeLayer::run_routed(const void* x, void* y, int64_t rows, hipStream_t s,
     ca.gate = blk ? blk->gate : nullptr;
     ca.seq = blk ? blk->seq : 1;
     ca.out_nt = g2.out_nt;
+    ca.holes = given != nullptr;
     STAGE(launch_combine(dt_, ca, s), "combine");
     if ((rc = mark(6))) return rc;
 #undef STAGE
@@ -1017,10 +1046,15 @@ int MoeLayer::routing(int32_t* idx, float* w, int32_t* counts, float* gap) {
         std::vector<float> hw((size_t)(rows * kslots_));
         HIP_TRY(hipMemcpy(hi.data(), s_idx, hi.size() * sizeof(int32_t), hipMemcpyDeviceToHost));
         HIP_TRY(hipMemcpy(hw.data(), s_w, hw.size() * sizeof(float), hipMemcpyDeviceToHost));
+        // (the shared dense branch's slot, expert E, is the last one taken: before
+        // the empty slots of a given routing)
         for (int64_t r = 0; r < rows; ++r)
-            for (int64_t j = 0; j < k_; ++j) {
-                if (idx) idx[r * k_ + j] = hi[(size_t)(r * kslots_ + j)];
-                if (w) w[r * k_ + j] = hw[(size_t)(r * kslots_ + j)];
+            for (int64_t j = 0, t = 0; t < kslots_ && j < k_; ++t) {
+                const size_t at = (size_t)(r * kslots_ + t);
+                if (hi[at] == E_) continue;
+                if (idx) idx[r * k_ + j] = hi[at];
+                if (w) w[r * k_ + j] = hw[at];
+                ++j;
             }
     }
     if (counts) {

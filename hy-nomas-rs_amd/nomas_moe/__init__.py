@@ -28,7 +28,7 @@ from ._lib import nomas_moe_config
 __all__ = [
     "DataType", "MoeConfig", "Weights", "MoeLayer", "FeedForward", "NomasError", "InvalidConfig",
     "WeightKey", "IoError", "path_seed", "randn_affine", "to_model_dtype", "norm_modulate",
-    "gated_residual",
+    "gated_residual", "block_seam", "block_seam_backward", "route", "route_backward",
 ]
 
 
@@ -230,6 +230,212 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor,
     return out
 
 
+# ---- the seam between two branches of a block, and routing to experts --------
+# Forward and gradient are calls of their own, as everything here: no autograd
+# graph is built or read.
+
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _same(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
+    """A second tensor of the activations' shape, dtype and device, contiguous."""
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise NomasError(2, f"{what}: expected {tuple(like.shape)} {like.dtype} on {like.device}, "
+                            f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
+def _param(t, like: torch.Tensor, shape: tuple, what: str):
+    """A parameter as contiguous f32 on the activations' device (None stays None)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise NomasError(2, f"{what}: expected {shape}, got {tuple(t.shape)}")
+    if t.dtype is torch.float32 and t.device == like.device and t.is_contiguous():
+        return t
+    return t.to(device=like.device, dtype=torch.float32).contiguous()
+
+
+def _call(fn, on: torch.Tensor, *args) -> None:
+    """fn(*args, stream): the current stream of `on`'s device, with that device current."""
+    index = on.device.index
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        _check(rc)
+
+
+def block_seam(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = None,
+               shift: torch.Tensor | None = None, scale: torch.Tensor | None = None, *,
+               post_norm: bool = False, post_w: torch.Tensor | None = None,
+               norm_w: torch.Tensor | None = None, residual_scale: float = 1.0,
+               eps: float = 1e-6, norm: bool = True, out: torch.Tensor | None = None,
+               h: torch.Tensor | None = None):
+    """What stands between two branches of a block, in one pass:
+
+        n   = y, or rmsnorm(y) * post_w with post_norm
+        out = residual_scale * x + n * gate
+        h   = rmsnorm(out) * norm_w * (1 + scale) + shift
+
+    x, y: (B, L, D) device tensors of one dtype; gate, shift, scale: (B, D);
+    post_w, norm_w: (D,); a parameter that is None is 1 (shift, scale: 0).
+    Returns (out, h); with norm=False h is None and not computed.  out may be x
+    or y, h the other of the two.  f32 between the tensors, one rounding each."""
+    xc = _seam_input(x)
+    yc = _same(y, xc, "y")
+    B, S, D = xc.shape
+    gate, shift, scale = (_param(t, xc, (B, D), n) for t, n in
+                          ((gate, "gate"), (shift, "shift"), (scale, "scale")))
+    norm_w, post_w = _param(norm_w, xc, (D,), "norm_w"), _param(post_w, xc, (D,), "post_w")
+    if not norm and any(t is not None for t in (h, shift, scale, norm_w)):
+        raise NomasError(2, "h, shift, scale and norm_w need norm=True")
+    if post_w is not None and not post_norm:
+        raise NomasError(2, "post_w needs post_norm=True")
+    out = torch.empty_like(xc) if out is None else _check_out(out, xc)
+    if norm:
+        h = torch.empty_like(xc) if h is None else _check_out(h, xc, "h")
+    _call(_lib.lib().nomas_block_seam, xc, _CODES[xc.dtype], xc.data_ptr(), yc.data_ptr(),
+          out.data_ptr(), _ptr(h), B * S, D, max(S, 1), _ptr(gate), int(post_norm), _ptr(post_w),
+          float(residual_scale), _ptr(norm_w), _ptr(shift), _ptr(scale), float(eps))
+    return out, h
+
+
+def block_seam_backward(dout: torch.Tensor | None, dh: torch.Tensor | None,
+                        out: torch.Tensor | None, y: torch.Tensor | None,
+                        gate: torch.Tensor | None = None, scale: torch.Tensor | None = None, *,
+                        post_norm: bool = False, post_w: torch.Tensor | None = None,
+                        norm_w: torch.Tensor | None = None, residual_scale: float = 1.0,
+                        eps: float = 1e-6) -> dict:
+    """The gradients of block_seam.
+
+    dout, dh: the gradients of its two results (None: zero; dh None: the seam
+    has no norm before the next branch).  out: its first result, as stored; y:
+    the branch's output (None: no branch, and out is norm_modulate's x).  The
+    rest as given to block_seam.  Returns a dict with ``dx``; ``dy`` and
+    ``dgate`` with a branch, ``dpost_w`` with post_norm; ``dshift``, ``dscale``
+    and ``dnorm_w`` with dh.  dx and dy are of the model dtype, the parameters'
+    gradients f32 (those of gate, shift and scale also where they were None)."""
+    first = dout if dout is not None else dh
+    if first is None:
+        raise NomasError(2, "one of dout and dh is needed")
+    first = _seam_input(first)
+    B, S, D = first.shape
+    if dh is not None and out is None:
+        raise NomasError(2, "dh needs out")
+    if y is None and post_norm:
+        raise NomasError(2, "post_norm needs y")
+    if post_w is not None and not post_norm:
+        raise NomasError(2, "post_w needs post_norm=True")
+    if y is None and gate is not None:
+        raise NomasError(2, "gate needs y")
+    if dh is None and (scale is not None or norm_w is not None):
+        raise NomasError(2, "scale and norm_w need dh")
+    dout, dh, y = (None if t is None else _same(t, first, n) for t, n in
+                   ((dout, "dout"), (dh, "dh"), (y, "y")))
+    out = None if dh is None else _same(out, first, "out")
+    gate, scale = _param(gate, first, (B, D), "gate"), _param(scale, first, (B, D), "scale")
+    norm_w, post_w = _param(norm_w, first, (D,), "norm_w"), _param(post_w, first, (D,), "post_w")
+    got = {"dx": torch.empty_like(first)}
+    if y is not None:
+        got["dy"] = torch.empty_like(first)
+    # the f32 gradients in one allocation, each at a multiple of 16 bytes
+    names = (["dgate"] if y is not None else []) + (["dshift", "dscale"] if dh is not None else [])
+    gains = (["dpost_w"] if post_norm else []) + (["dnorm_w"] if dh is not None else [])
+    make = torch.zeros if S == 0 else torch.empty
+    flat = make((len(names) * B + len(gains)) * D, dtype=torch.float32, device=first.device)
+    for i, n in enumerate(names):
+        got[n] = flat[i * B * D:(i + 1) * B * D].view(B, D)
+    for i, n in enumerate(gains):
+        got[n] = flat[(len(names) * B + i) * D:(len(names) * B + i + 1) * D]
+    if first.numel() == 0:
+        return {k: v.zero_() for k, v in got.items()}
+    L = _lib.lib()
+    need = L.nomas_block_seam_workspace(B * S, D, S)
+    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
+    _call(L.nomas_block_seam_backward, first, _CODES[first.dtype], _ptr(dout), _ptr(dh), _ptr(out),
+          _ptr(y), got["dx"].data_ptr(), _ptr(got.get("dy")), B * S, D, S, _ptr(gate),
+          int(post_norm), _ptr(post_w), float(residual_scale), _ptr(norm_w), _ptr(scale),
+          float(eps), _ptr(got.get("dgate")), _ptr(got.get("dshift")), _ptr(got.get("dscale")),
+          _ptr(got.get("dnorm_w")), _ptr(got.get("dpost_w")), ws.data_ptr(), need)
+    return got
+
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def _route_input(logits: torch.Tensor, scoring: str):
+    if logits.dim() < 1:
+        raise NomasError(2, "expected (..., E) logits")
+    if not logits.is_cuda:
+        raise NomasError(2, "routing takes device tensors")
+    if logits.dtype not in _CODES:
+        raise NomasError(2, f"logits must be f32, bf16 or f16, got {logits.dtype}")
+    if scoring not in _SCORING:
+        raise InvalidConfig(1, f"unknown scoring {scoring!r}")
+    return logits.contiguous()
+
+
+def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
+          bias: torch.Tensor | None = None, groups: int = 1, top_groups: int | None = None,
+          group_top: int = 2, renormalize: bool = True, scale: float = 1.0, eps: float = 1e-9,
+          counts: bool = True):
+    """Routing to experts: (idx, w, counts) from a router's logits (..., E).
+
+        s = softmax(logits) or sigmoid(logits)       (scoring)
+        the choice goes by s + bias (E,): of `groups` equal groups of experts the
+        top_groups with the largest sum of their group_top (1 or 2) best, and of
+        those groups' experts the top_k best, ties to the lowest index
+        w = scale * s / (sum of the chosen s + eps), or scale * s
+
+    idx (..., top_k) int32 in ascending order, w (..., top_k) f32, counts (E,)
+    int32: how many rows chose each expert (None with counts=False).  A logit
+    of -inf masks its expert: it is never chosen, and slots that stay empty
+    hold -1 with weight 0 (MoeLayer.forward_routed skips them).  A NaN logit is
+    chosen first and makes its row's weights NaN.  The choice is made as in 64 bits."""
+    lc = _route_input(logits, scoring)
+    E, k = lc.shape[-1], int(top_k)
+    rows = lc.numel() // E if E else 0
+    if k < 1 or k > E:
+        raise InvalidConfig(1, f"invalid MoE top_k/experts (top_k={k}, experts={E})")
+    bias = _param(bias, lc, (E,), "bias")
+    shape = lc.shape[:-1] + (k,)
+    idx = torch.empty(shape, dtype=torch.int32, device=lc.device)
+    w = torch.empty(shape, dtype=torch.float32, device=lc.device)
+    n = torch.empty(E, dtype=torch.int32, device=lc.device) if counts else None
+    _call(_lib.lib().nomas_route, lc, _CODES[lc.dtype], lc.data_ptr(), rows, E, k,
+          _SCORING[scoring], _ptr(bias), int(groups),
+          int(groups if top_groups is None else top_groups), int(group_top), int(renormalize),
+          float(scale), float(eps), idx.data_ptr(), w.data_ptr(), _ptr(n))
+    return idx, w, n
+
+
+def route_backward(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, *,
+                   scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                   eps: float = 1e-9) -> torch.Tensor:
+    """The gradient of route's weights with respect to the logits, of the logits'
+    shape and dtype.  idx: route's choice (an index outside 0..E-1: an empty
+    slot); dw: the weights' gradient.  The choice itself has none, and so
+    neither has the bias."""
+    lc = _route_input(logits, scoring)
+    E = lc.shape[-1]
+    want = lc.shape[:-1]
+    for t, n, dt in ((idx, "idx", torch.int32), (dw, "dw", torch.float32)):
+        if t.shape[:-1] != want or t.shape != idx.shape or t.dtype != dt or t.device != lc.device:
+            raise NomasError(2, f"{n}: expected {tuple(want)} + (top_k,) {dt} on {lc.device}, got "
+                                f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    idx, dw = idx.contiguous(), dw.contiguous()
+    dl = torch.empty_like(lc)
+    rows = lc.numel() // E if E else 0
+    _call(_lib.lib().nomas_route_backward, lc, _CODES[lc.dtype], lc.data_ptr(), idx.data_ptr(),
+          dw.data_ptr(), rows, E, idx.shape[-1], _SCORING[scoring], int(renormalize), float(scale),
+          float(eps), dl.data_ptr())
+    return dl
+
+
 class Weights:
     """Where a module's parameters come from (mod.rs:20-45).
 
@@ -374,6 +580,31 @@ class MoeLayer:
         return out
 
     __call__ = forward
+
+    def forward_routed(self, x: torch.Tensor, idx: torch.Tensor, w: torch.Tensor,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+        """forward with the caller's routing in the place of the layer's router:
+        the sum over a row's slots of w times the expert's output (plus the
+        shared dense branch, where there is one).  x: (..., D) on the layer's
+        GPU; idx: (..., top_k) int32 and w: (..., top_k) f32, as route gives
+        them, in any order.  An index outside 0..E-1 is an empty slot, which
+        adds nothing; an expert named twice in a row has the sum of its weights."""
+        if x.dim() < 1 or x.shape[-1] != self.dim:
+            raise NomasError(2, f"expected last dim {self.dim}, got shape {tuple(x.shape)}")
+        if x.dtype != self.dtype.torch:
+            raise NomasError(2, f"expected dtype {self.dtype.torch}, got {x.dtype}")
+        if not x.is_cuda or x.device.index != self.device:
+            raise NomasError(2, f"forward_routed takes tensors on the layer's GPU, got {x.device}")
+        want = x.shape[:-1] + (self.top_k,)
+        for t, n, dt in ((idx, "idx", torch.int32), (w, "w", torch.float32)):
+            if t.shape != want or t.dtype != dt or t.device != x.device:
+                raise NomasError(2, f"{n}: expected {tuple(want)} {dt} on {x.device}, got "
+                                    f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        xc, idx, w = x.contiguous(), idx.contiguous(), w.contiguous()
+        out = torch.empty_like(xc) if out is None else _check_out(out, xc)
+        _call(_lib.lib().nomas_moe_forward_routed, xc, self._h, xc.data_ptr(), idx.data_ptr(),
+              w.data_ptr(), out.data_ptr(), xc.numel() // self.dim)
+        return out
 
     # -- the FFN half of DiTBlock::forward (block.rs:96-101) ------------------
     def forward_block(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,

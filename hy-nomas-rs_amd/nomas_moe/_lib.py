@@ -96,6 +96,22 @@ def lib() -> C.CDLL:
     L.nomas_norm_modulate.restype = i32
     L.nomas_gated_residual.argtypes = [i32, vp, vp, vp, vp, i64, i64, i64, vp]
     L.nomas_gated_residual.restype = i32
+    f64 = C.c_double
+    L.nomas_moe_forward_routed.argtypes = [vp, vp, vp, vp, vp, i64, vp]
+    L.nomas_moe_forward_routed.restype = i32
+    L.nomas_route.argtypes = [i32, vp, i64, i64, i64, i32, vp, i64, i64, i64, i32, f64, f64, vp, vp,
+                              vp, vp]
+    L.nomas_route.restype = i32
+    L.nomas_route_backward.argtypes = [i32, vp, vp, vp, i64, i64, i64, i32, i32, f64, f64, vp, vp]
+    L.nomas_route_backward.restype = i32
+    L.nomas_block_seam.argtypes = [i32, vp, vp, vp, vp, i64, i64, i64, vp, i32, vp, f64, vp, vp, vp,
+                                   f64, vp]
+    L.nomas_block_seam.restype = i32
+    L.nomas_block_seam_workspace.argtypes = [i64, i64, i64]
+    L.nomas_block_seam_workspace.restype = i64
+    L.nomas_block_seam_backward.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, i32, vp,
+                                            f64, vp, vp, f64, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.nomas_block_seam_backward.restype = i32
     L.nomas_ffn_destroy.argtypes = [vp]
     L.nomas_ffn_destroy.restype = None
     L.nomas_moe_last_error.argtypes = []

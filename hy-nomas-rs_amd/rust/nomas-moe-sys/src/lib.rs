@@ -24,6 +24,10 @@ pub const NOMAS_F32: c_int = 0;
 pub const NOMAS_BF16: c_int = 1;
 pub const NOMAS_F16: c_int = 2;
 
+// enum nomas_scoring
+pub const NOMAS_SOFTMAX: c_int = 0;
+pub const NOMAS_SIGMOID: c_int = 1;
+
 /// MoeConfig (nomas-core config.rs:202-213), field for field.
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
@@ -67,6 +71,9 @@ extern "C" {
                              stream: *mut c_void) -> c_int;
     pub fn nomas_moe_forward_noalloc(h: *mut nomas_moe_t, x: *const c_void, y: *mut c_void,
                                      rows: i64, stream: *mut c_void) -> c_int;
+    pub fn nomas_moe_forward_routed(h: *mut nomas_moe_t, x: *const c_void, idx: *const i32,
+                                    w: *const f32, y: *mut c_void, rows: i64,
+                                    stream: *mut c_void) -> c_int;
     pub fn nomas_moe_forward_block(h: *mut nomas_moe_t, x: *const c_void, out: *mut c_void,
                                    rows: i64, seq: i64, norm_w: *const f32, eps: f64,
                                    shift: *const f32, scale: *const f32, gate: *const f32,
@@ -109,6 +116,31 @@ extern "C" {
     pub fn nomas_gated_residual(dtype: c_int, x: *const c_void, y: *const c_void,
                                 gate: *const f32, out: *mut c_void, rows: i64, dim: i64,
                                 seq: i64, stream: *mut c_void) -> c_int;
+
+    pub fn nomas_route(dtype: c_int, logits: *const c_void, rows: i64, experts: i64, top_k: i64,
+                       scoring: c_int, bias: *const f32, groups: i64, top_groups: i64,
+                       group_top: i64, renormalize: c_int, scale: f64, eps: f64, idx: *mut i32,
+                       w: *mut f32, counts: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn nomas_route_backward(dtype: c_int, logits: *const c_void, idx: *const i32,
+                                dw: *const f32, rows: i64, experts: i64, top_k: i64,
+                                scoring: c_int, renormalize: c_int, scale: f64, eps: f64,
+                                dlogits: *mut c_void, stream: *mut c_void) -> c_int;
+
+    pub fn nomas_block_seam(dtype: c_int, x: *const c_void, y: *const c_void, out: *mut c_void,
+                            h: *mut c_void, rows: i64, dim: i64, seq: i64, gate: *const f32,
+                            post_norm: c_int, post_w: *const f32, residual_scale: f64,
+                            norm_w: *const f32, shift: *const f32, scale: *const f32, eps: f64,
+                            stream: *mut c_void) -> c_int;
+    pub fn nomas_block_seam_workspace(rows: i64, dim: i64, seq: i64) -> i64;
+    pub fn nomas_block_seam_backward(dtype: c_int, dout: *const c_void, dh: *const c_void,
+                                     out: *const c_void, y: *const c_void, dx: *mut c_void,
+                                     dy: *mut c_void, rows: i64, dim: i64, seq: i64,
+                                     gate: *const f32, post_norm: c_int, post_w: *const f32,
+                                     residual_scale: f64, norm_w: *const f32, scale: *const f32,
+                                     eps: f64, dgate: *mut f32, dshift: *mut f32,
+                                     dscale: *mut f32, dnorm_w: *mut f32, dpost_w: *mut f32,
+                                     workspace: *mut c_void, workspace_bytes: i64,
+                                     stream: *mut c_void) -> c_int;
 
     pub fn nomas_moe_last_error() -> *const c_char;
     pub fn nomas_path_seed(seed: u64, path: *const c_char) -> u64;

@@ -118,6 +118,17 @@ int nomas_moe_forward(nomas_moe_t *h, const void *x, void *y, int64_t rows, void
  * handle is NOMAS_ERR_STATE. */
 int nomas_moe_forward_noalloc(nomas_moe_t *h, const void *x, void *y, int64_t rows, void *stream);
 
+/* No counterpart in the reference: nomas_moe_forward with the caller's routing in
+ * the place of the router's.  idx and w are (rows, top_k) on the device (4-byte
+ * aligned), as nomas_route writes them but in any order: y = sum over a row's
+ * slots of w * FFN_idx(x), plus the shared dense branch where the layer has
+ * one.  An index outside 0 .. E - 1 is an empty slot: it adds nothing and
+ * costs no product.  An expert named twice in a row has the sum of its
+ * weights.  nomas_moe_routing() reports the routing as it was run (ascending,
+ * -1 for empty slots, gap +inf). */
+int nomas_moe_forward_routed(nomas_moe_t *h, const void *x, const int32_t *idx, const float *w,
+                             void *y, int64_t rows, void *stream);
+
 /* The FFN half of DiTBlock::forward around the MoE (block.rs:96-101), fused
  * into the MoE's own kernels:
  *   h   = modulate(norm2(x), shift, scale)     (norm.rs:55-65, modulate.rs:69-79)
@@ -248,6 +259,75 @@ int nomas_norm_modulate(int dtype, const void *x, void *h, int64_t rows, int64_t
 /* out = x + y * gate  (block.rs:101), y the FFN output; out may alias x or y. */
 int nomas_gated_residual(int dtype, const void *x, const void *y, const float *gate, void *out,
                          int64_t rows, int64_t dim, int64_t seq, void *stream);
+
+/* ---- Routing to experts on its own --------------------------------------------
+ * No counterpart in the reference beyond the router inside MoeLayer::forward
+ * (moe.rs:67-95): scores, a bias for balance, groups and weights, from logits
+ * that the caller has, for nomas_moe_forward_routed or its own experts.  Device
+ * pointers, asynchronous on `stream` (of the current device); nothing is allocated. */
+
+enum nomas_scoring { NOMAS_SOFTMAX = 0, NOMAS_SIGMOID = 1 };
+
+/* logits: (rows, experts) in `dtype`.  s = softmax or sigmoid of a row; the choice
+ * goes by s + bias (bias: experts f32 or NULL).  The experts form `groups` equal
+ * groups (1: none); the top_groups groups with the largest sum of their group_top
+ * (1 or 2) largest unmasked choice values stay, and of their experts the top_k
+ * largest are chosen; ties go to the lowest index, in groups and experts, and
+ * differences count as in 64 bits.  (Without bias and groups the order is the
+ * logits' own.)  idx: (rows, top_k) in ascending order; w: scale * s / (sum of the
+ * chosen s + eps) with renormalize, else scale * s; counts: (experts) rows
+ * that chose each, or NULL.  A logit of -inf masks its expert, which is never
+ * chosen; slots that stay empty hold -1 and weight 0.  A NaN counts as the largest
+ * value.  Up to 1,024 experts and 64 groups. */
+int nomas_route(int dtype, const void *logits, int64_t rows, int64_t experts, int64_t top_k,
+                int scoring, const float *bias, int64_t groups, int64_t top_groups,
+                int64_t group_top, int renormalize, double scale, double eps, int32_t *idx,
+                float *w, int32_t *counts, void *stream);
+
+/* dlogits (rows, experts; every element is written) from dw, the gradient of
+ * nomas_route's w, for the choice idx (an index outside 0 .. experts - 1 is an
+ * empty slot).  The other arguments as in the forward call; dlogits may alias
+ * logits. */
+int nomas_route_backward(int dtype, const void *logits, const int32_t *idx, const float *dw,
+                         int64_t rows, int64_t experts, int64_t top_k, int scoring,
+                         int renormalize, double scale, double eps, void *dlogits, void *stream);
+
+/* ---- The seam between two branches of a block ------------------------------------
+ * No single counterpart in the reference: the end of one branch and the start of
+ * the next (block.rs:95-96, 101 with the next block's norm1) in one pass, with a
+ * norm after the branch and a scale on the residual as other DiTs have them:
+ *   n   = y, or y / rms(y) * post_w with post_norm
+ *   out = residual_scale * x + n * gate
+ *   h   = out / rms(out) * norm_w * (1 + scale) + shift       (h NULL: not computed)
+ * with rms(v) = sqrt(mean(v^2) + eps).  Tensors (rows, dim) in `dtype`, f32
+ * parameters: gate, shift, scale (rows / seq, dim), post_w, norm_w (dim); a NULL
+ * one is 1 (shift, scale: 0).  Everything 16-byte aligned, dim % 8 == 0 and at most
+ * 16,384.  f32 between the tensors: each output is rounded once, h is made from out before its
+ * rounding, and sums over a row are trees (nomas_norm_modulate and
+ * nomas_gated_residual round where the reference does instead).  out may alias x or y,
+ * and h the other one.  Asynchronous on `stream` (of the current device). */
+int nomas_block_seam(int dtype, const void *x, const void *y, void *out, void *h, int64_t rows,
+                     int64_t dim, int64_t seq, const float *gate, int post_norm,
+                     const float *post_w, double residual_scale, const float *norm_w,
+                     const float *shift, const float *scale, double eps, void *stream);
+
+/* Bytes of device workspace that nomas_block_seam_backward needs (0: invalid sizes). */
+int64_t nomas_block_seam_workspace(int64_t rows, int64_t dim, int64_t seq);
+
+/* The gradients of nomas_block_seam: dout and dh those of its results (either may
+ * be NULL: zero), out its first result as stored (read with dh only), y the branch's
+ * output (NULL: no branch, as before a first norm_modulate), the rest as in the forward
+ * call.  dx, dy (rows, dim) in `dtype`; dgate, dshift, dscale (rows / seq, dim) and
+ * dnorm_w, dpost_w (dim) f32; each may be NULL (not wanted).  The sums over rows
+ * have a fixed order: the same call gives the same bits.  workspace: 16-byte aligned, of
+ * nomas_block_seam_workspace() bytes, the call's own while it runs. */
+int nomas_block_seam_backward(int dtype, const void *dout, const void *dh, const void *out,
+                              const void *y, void *dx, void *dy, int64_t rows, int64_t dim,
+                              int64_t seq, const float *gate, int post_norm, const float *post_w,
+                              double residual_scale, const float *norm_w, const float *scale,
+                              double eps, float *dgate, float *dshift, float *dscale,
+                              float *dnorm_w, float *dpost_w, void *workspace,
+                              int64_t workspace_bytes, void *stream);
 
 /* Message of the last failure on this thread ("" if none). */
 const char *nomas_moe_last_error(void);
