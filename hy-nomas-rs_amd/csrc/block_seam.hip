@@ -20,15 +20,24 @@ namespace {
 
 // Blocks of a call that fills the chip: enough waves for the loads in flight, rows
 // enough per block for its parameters to be read from L2 seldom.
-constexpr int64_t kForwardBlocks = 2048;
+#ifndef V_FB
+#define V_FB 2048
+#endif
+#ifndef V_FT
+#define V_FT 256
+#endif
+constexpr int64_t kForwardBlocks = V_FB;
+constexpr int kForwardThreads = V_FT;
 
 template <typename T, bool kPost, bool kNorm, int L, int C>
-__global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel(BlockSeamArgs a, SeamPlan p) {
+__global__ __launch_bounds__(kSeamThreads) void block_seam_kernel(BlockSeamArgs a, SeamPlan p) {
     constexpr int R = sizeof(T) == 4 || C > 1 ? 1 : 2;  // rows of a step
-    __shared__ float s_part[L ? 1 : 2 * (kSeamWide / kWave) * R];
+    __shared__ __align__(16) float s_part[sums_floats<L, R>()];
     const int D = a.D;
-    const int t = L ? threadIdx.x % (L ? L : 1) : threadIdx.x, W = L ? L : blockDim.x;
-    const int g = L ? threadIdx.x / (L ? L : 1) : 0, G = L ? kSeamNarrow / (L ? L : 1) : 1;
+    const int W = L ? L : p.row_threads, G = p.groups;
+    // (the same for a wave where a row takes whole ones)
+    const int g = L && L < 64 ? threadIdx.x / W : __builtin_amdgcn_readfirstlane(threadIdx.x / W);
+    const int t = threadIdx.x - g * W;
     int col[C];
     bool live[C];
 #pragma unroll
@@ -75,8 +84,8 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel
             row[r] = min(at + r * stride, end - 1);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                ry[r][c] = fetch8(y + row[r] * D + col[c]);
-                rx[r][c] = fetch8(x + row[r] * D + col[c]);
+                ry[r][c] = fetch8(y + row[r] * D, col[c]);
+                rx[r][c] = fetch8(x + row[r] * D, col[c]);
             }
         }
         float v[R][C][8], s[R];
@@ -92,7 +101,7 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel
                 s[r] += live[c] ? q : 0.0f;
             }
         }
-        if constexpr (kPost) row_sums<L>(s, s_part, turn++);
+        if constexpr (kPost) row_sums<L>(s, s_part, turn++, W / kWave);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float n = kPost ? rsqrtf(s[r] * inv_d + a.eps) : 1.0f;
@@ -107,11 +116,11 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel
                     q += v[r][c][i] * v[r][c][i];
                 }
                 s[r] += live[c] ? q : 0.0f;
-                if (live[c] && busy && at + r * stride < end) put8(out + row[r] * D + col[c], v[r][c]);
+                if (live[c] && busy && at + r * stride < end) put8(out + row[r] * D, col[c], v[r][c]);
             }
         }
         if constexpr (kNorm) {
-            row_sums<L>(s, s_part, turn++);
+            row_sums<L>(s, s_part, turn++, W / kWave);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const float n = rsqrtf(s[r] * inv_d + a.eps);
@@ -119,7 +128,7 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel
                 for (int c = 0; c < C; ++c) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[r][c][i] = v[r][c][i] * n * f[c][i] + sh[c][i];
-                    if (live[c] && busy && at + r * stride < end) put8(h + row[r] * D + col[c], v[r][c]);
+                    if (live[c] && busy && at + r * stride < end) put8(h + row[r] * D, col[c], v[r][c]);
                 }
             }
         }
@@ -141,12 +150,12 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void block_seam_kernel
 
 template <typename T>
 hipError_t launch_seam_t(const BlockSeamArgs& a, hipStream_t s) {
-    const SeamPlan p = seam_plan(a.rows, a.D, a.seq, kForwardBlocks);
+    const SeamPlan p = seam_plan(a.rows, a.D, a.seq, kForwardBlocks, kForwardThreads);
     return with_seam_shape(p, [&](auto l, auto c) {
         constexpr int L = decltype(l)::value, C = decltype(c)::value;
         auto kern = a.post ? (a.h ? block_seam_kernel<T, true, true, L, C> : block_seam_kernel<T, true, false, L, C>)
                            : (a.h ? block_seam_kernel<T, false, true, L, C> : block_seam_kernel<T, false, false, L, C>);
-        launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.threads), 0, s, a, p);
+        launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.row_threads * p.groups), 0, s, a, p);
         return hipGetLastError();
     });
 }

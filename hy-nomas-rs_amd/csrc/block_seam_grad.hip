@@ -27,21 +27,41 @@ namespace {
 
 // Blocks of a call that fills the chip.  Each leaves 12 D bytes of sums, written and
 // read again.
-constexpr int64_t kGradBlocks = 768;
+#ifndef V_BLOCKS
+#define V_BLOCKS 768
+#endif
+#ifndef V_PRE
+#define V_PRE 1
+#endif
+#ifndef V_R
+#define V_R 2
+#endif
+#ifndef V_GT
+#define V_GT 512
+#endif
+constexpr int64_t kGradBlocks = V_BLOCKS;
+constexpr int kGradThreads = V_GT;
 
 // sums of a block's (or sequence's) columns: P, Q, R, each D floats
 constexpr int kSums = 3;
 
-template <typename T, bool kPost, bool kNorm, int L, int C>
-__global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
+template <typename T, bool kPost, bool kNorm, bool kWhole, int L, int C>
+__global__ __launch_bounds__(kSeamThreads)
+#ifdef V_WPE
+__attribute__((amdgpu_waves_per_eu(C == 1 ? V_WPE : 2)))
+#endif
+void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
                                                                                 float* sums) {
-    constexpr int R = sizeof(T) == 4 || C > 1 ? 1 : 2;     // rows of a step
+    constexpr int R = sizeof(T) == 4 || C > 1 ? 1 : V_R;     // rows of a step
     constexpr int N = (kNorm ? 2 : 0) + (kPost ? 2 : 0) + (kNorm && kPost ? 2 : 0);
     constexpr int NS = N ? N * R : 1;
-    __shared__ float s_part[L ? 1 : 2 * (kSeamWide / kWave) * NS];
+    __shared__ __align__(16) float s_part[sums_floats<L, NS>()];
+    __shared__ float s_v[kSeamThreads * 8];  // over_groups()
     const int D = a.D;
-    const int t = L ? threadIdx.x % (L ? L : 1) : threadIdx.x, W = L ? L : blockDim.x;
-    const int g = L ? threadIdx.x / (L ? L : 1) : 0, G = L ? kSeamNarrow / (L ? L : 1) : 1;
+    const int W = L ? L : p.row_threads, G = p.groups;
+    // (the same for a wave where a row takes whole ones)
+    const int g = L && L < 64 ? threadIdx.x / W : __builtin_amdgcn_readfirstlane(threadIdx.x / W);
+    const int t = threadIdx.x - g * W;
     int col[C];
     bool live[C];
 #pragma unroll
@@ -93,21 +113,21 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = min(at + r * stride, end - 1);
+            const int64_t o = row * D;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int64_t o = row * D + col[c];
                 if constexpr (kNorm) {
-                    q.dh[r][c] = fetch8(dh + o);
-                    q.out[r][c] = fetch8(out + o);
+                    q.dh[r][c] = fetch8(dh + o, col[c]);
+                    q.out[r][c] = fetch8(out + o, col[c]);
                 }
-                if (dout) q.dout[r][c] = fetch8(dout + o);
-                if (y) q.y[r][c] = fetch8(y + o);
+                if (dout) q.dout[r][c] = fetch8(dout + o, col[c]);
+                if (y) q.y[r][c] = fetch8(y + o, col[c]);
             }
         }
     };
     int turn = 0;
     // (rows as in block_seam_kernel)
-    auto step = [&](const Rows& q, int64_t at, int64_t stride, int64_t end, bool busy) {
+    auto step = [&](Rows& q, int64_t at, int64_t stride, int64_t end, bool busy) {
         float s[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) s[i] = 0.0f;
@@ -157,8 +177,21 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
                     for (int i = 0; i < N; ++i) s[r * N + i] += live[c] ? m[i] : 0.0f;
                 }
             }
-            row_sums<L>(s, s_part, turn++);
+            row_sums<L>(s, s_part, turn++, W / kWave);
         }
+#ifdef V_RENEW
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                renew(q.dout[r][c]);
+                if constexpr (kNorm) {
+                    renew(q.dh[r][c]);
+                    renew(q.out[r][c]);
+                }
+                renew(q.y[r][c]);
+            }
+#endif
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const float* m = s + r * N;
@@ -177,7 +210,7 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
             }
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int64_t o = min(at + r * stride, end - 1) * D + col[c];
+                const int64_t o = min(at + r * stride, end - 1) * D;
                 float d[8], v[8];
                 widen(q.dout[r][c], dout != nullptr, d);
                 if constexpr (kNorm) {
@@ -200,11 +233,11 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
                         w[i] = ry * (u[c][i] * d[i]);
                         if constexpr (kPost) w[i] -= k2 * vy[i];
                     }
-                    if (dy && on && live[c]) put8(dy + o, w);
+                    if (dy && on && live[c]) put8(dy + o, col[c], w);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = a.alpha * d[i];
-                if (dx && on && live[c]) put8(dx + o, v);
+                if (dx && on && live[c]) put8(dx + o, col[c], v);
             }
         }
     };
@@ -226,29 +259,23 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
             if (a.dgate) put8(a.dgate + o, v);
         }
     };
-    // The groups' values of a column, added up in the first group's lanes.
-    auto over_groups = [&](auto& v) {
-        if constexpr (L > 0) {
-            constexpr int kWaves = kSeamNarrow / kWave, n = sizeof(v) / sizeof(float);
-            __shared__ float s_v[kWaves - 1][n][L];
-            float* w = &v[0][0][0];
-            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // The groups' values of the columns added up, in the first group's lanes: by
+    // eights, every group's in LDS, in the groups' order.
+    auto over_groups = [&](float (&v)[C][8]) {
+        if (G == 1) return;
 #pragma unroll
-            for (int i = 0; i < n; ++i) {
-#pragma unroll
-                for (int o = L; o < kWave; o <<= 1) w[i] += __shfl_xor(w[i], o);
-                if (wave && lane < L) s_v[wave - 1][i][lane] = w[i];
-            }
+        for (int c = 0; c < C; ++c) {
             __syncthreads();
-            if (!wave && lane < L) {
 #pragma unroll
-                for (int i = 0; i < n; ++i)
+            for (int i = 0; i < 8; ++i) s_v[i * kSeamThreads + threadIdx.x] = v[c][i];
+            __syncthreads();
+            if (g == 0)
+                for (int o = 1; o < G; ++o)
 #pragma unroll
-                    for (int k = 0; k < kWaves - 1; ++k) w[i] += s_v[k][i][lane];
-            }
+                    for (int i = 0; i < 8; ++i) v[c][i] += s_v[i * kSeamThreads + o * W + t];
         }
     };
-    if (p.whole) {
+    if constexpr (kWhole) {
         const int64_t n = a.rows / a.seq;
         float gain[2][C][8];  // of norm_w and post_w
         clear(gain[0]);
@@ -278,7 +305,8 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
             clear(acc[1]);
             clear(acc[2]);
         }
-        over_groups(gain);
+        over_groups(gain[0]);
+        over_groups(gain[1]);
         if (g == 0) {
             float* o = sums + blockIdx.x * 2 * (int64_t)D;
 #pragma unroll
@@ -288,12 +316,11 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
                     put8(o + D + col[c], gain[1][c]);
                 }
         }
-        return;
-    }
+    } else {
     const int64_t b = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
     const int64_t first = b * a.seq + part * p.chunk, end = min(first + p.chunk, (b + 1) * a.seq);
     params(b);
-    if constexpr (C == 1) {
+    if constexpr (V_PRE && C == 1) {
         // the next step's rows are on their way during this one
         Rows q;
         load(q, first + g, G, end);
@@ -310,7 +337,9 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
             step(q, at + g, G, end, true);
         }
     }
-    over_groups(acc);
+    over_groups(acc[0]);
+    over_groups(acc[1]);
+    over_groups(acc[2]);
     if (g == 0) {
         float* o = sums + blockIdx.x * kSums * (int64_t)D;
 #pragma unroll
@@ -318,6 +347,7 @@ __global__ __launch_bounds__(L ? kSeamNarrow : kSeamWide) void seam_grad_kernel(
             if (live[c])
 #pragma unroll
                 for (int k = 0; k < kSums; ++k) put8(o + k * (int64_t)D + col[c], acc[k][c]);
+    }
     }
 }
 
@@ -391,7 +421,14 @@ __global__ __launch_bounds__(256) void zero_gains_kernel(float* p, float* q, int
     if (q) q[c] = 0.0f;
 }
 
-SeamPlan grad_plan(int64_t rows, int64_t D, int64_t seq) { return seam_plan(rows, D, seq, kGradBlocks); }
+SeamPlan grad_plan(int64_t rows, int64_t D, int64_t seq) {
+    return seam_plan(rows, D, seq, kGradBlocks, kGradThreads);
+}
+
+template <typename T, bool kPost, bool kNorm, int L, int C>
+auto grad_kernel(const SeamPlan& p) {
+    return p.whole ? seam_grad_kernel<T, kPost, kNorm, true, L, C> : seam_grad_kernel<T, kPost, kNorm, false, L, C>;
+}
 
 template <typename T>
 hipError_t launch_grad_t(const BlockSeamBackwardArgs& a, hipStream_t s) {
@@ -400,9 +437,9 @@ hipError_t launch_grad_t(const BlockSeamBackwardArgs& a, hipStream_t s) {
     const bool norm = a.dh != nullptr, post = a.post && a.y;
     const hipError_t e = with_seam_shape(p, [&](auto l, auto c) {
         constexpr int L = decltype(l)::value, C = decltype(c)::value;
-        auto kern = post ? (norm ? seam_grad_kernel<T, true, true, L, C> : seam_grad_kernel<T, true, false, L, C>)
-                         : (norm ? seam_grad_kernel<T, false, true, L, C> : seam_grad_kernel<T, false, false, L, C>);
-        launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.threads), 0, s, a, p, sums);
+        auto kern = post ? (norm ? grad_kernel<T, true, true, L, C>(p) : grad_kernel<T, true, false, L, C>(p))
+                         : (norm ? grad_kernel<T, false, true, L, C>(p) : grad_kernel<T, false, false, L, C>(p));
+        launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.row_threads * p.groups), 0, s, a, p, sums);
         return hipGetLastError();
     });
     if (e != hipSuccess || !(a.dgate || a.dshift || a.dscale || a.dnorm_w || a.dpost_w)) return e;
