@@ -655,8 +655,8 @@ int nomas_route(int dtype, const void* logits, int64_t rows, int64_t experts, in
         a.top_groups = (int)top_groups;
         a.group_top = (int)group_top;
         a.renormalize = renormalize != 0;
-        a.scale = scale;
-        a.eps = eps;
+        a.scale = (float)scale;
+        a.eps = (float)eps;
         a.idx = idx;
         a.w = w;
         a.counts = counts;

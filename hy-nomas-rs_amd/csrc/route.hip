@@ -18,14 +18,14 @@
 //    smallest of the lanes' maxima and the largest: each step counts the keys
 //    at or above the middle (two instructions a key) and most rows need five to
 //    eight steps.
-//  - Keys are f32, the definition's choice is made in 64 bits: where a key lies so
-//    near the border (of the experts, or of the groups) that its f32 error could
-//    carry it across, or a logit is NaN or +inf, the wave decides the row again in
-//    f64 (exact_row).  Without bias and groups the keys are the logits themselves:
-//    nothing is near, and ties are exact.
+//  - Keys are f32, the definition's choice is made in 64 bits: the keys that lie so
+//    near the border (of the experts, or of the groups) that their f32 error could
+//    carry them across are made again in f64, and decided among themselves.
+//    Without bias and groups the keys are the logits: nothing is near, ties are exact.
 //  - The chosen indices meet in LDS, and lane t of a row makes the weight of slot t.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kernels.hpp"
 
@@ -33,11 +33,20 @@ namespace nomas {
 
 namespace {
 
+#ifndef V_MAXV
+#define V_MAXV 16
+#endif
+#ifndef V_MINW
+#define V_MINW 4096
+#endif
+#ifndef V_RB
+#define V_RB 1024
+#endif
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWaves = kRouteThreads / kWave;
 // Blocks of a call that fills the chip (their rows are a loop, so that the bias is
 // loaded once and the histogram flushed once)
-constexpr int64_t kRouteBlocks = 1024;
+constexpr int64_t kRouteBlocks = V_RB;
 
 __device__ __forceinline__ double wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
@@ -46,121 +55,6 @@ __device__ __forceinline__ double wave_sum(double v) {
 __device__ __forceinline__ double wave_max(double v) {
     for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
     return v;
-}
-
-// ---- the choice in 64 bits, a wave a row ----------------------------------------
-
-// The wave's largest key and its lowest expert; -1 where every key is -inf.
-template <int V>
-__device__ int best_of(const double* key, double* best) {
-    const int lane = threadIdx.x & 63;
-    double b = -INFINITY;
-    int at = 1 << 30;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (key[j] > b) {
-            b = key[j];
-            at = lane + 64 * j;
-        }
-    for (int o = 32; o; o >>= 1) {
-        const double ob = __shfl_xor(b, o);
-        const int oa = __shfl_xor(at, o);
-        if (ob > b || (ob == b && oa < at)) {
-            b = ob;
-            at = oa;
-        }
-    }
-    *best = b;
-    return b == -INFINITY ? -1 : at;
-}
-
-// Writes a row's choice to `to` (ascending) and returns how many there are; lane
-// holds the experts lane, lane + 64, ...
-struct ExactRow {
-    const float* bias;
-    int E, k, sigmoid, groups, top_groups, group_top;
-};
-template <typename T, int V>
-__device__ __noinline__ int exact_row(ExactRow a, const T* l, int* to) {
-    const int lane = threadIdx.x & 63, E = a.E;
-    double raw[V], key[V];
-    double m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = lane + 64 * j;
-        raw[j] = e < E ? (double)Elt<T>::to_f32(l[e]) : -INFINITY;
-        m = fmax(m, raw[j]);
-    }
-    const bool scores = a.bias || a.groups > 1;
-    double z = 0.0;
-    if (scores && !a.sigmoid) m = wave_max(m);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        if (raw[j] == -INFINITY) key[j] = 0.0;
-        else if (!scores) key[j] = raw[j];
-        else if (a.sigmoid) key[j] = 1.0 / (1.0 + exp(-raw[j]));
-        else z += key[j] = exp(raw[j] - m);
-    }
-    if (scores && !a.sigmoid) z = wave_sum(z);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = lane + 64 * j;
-        if (scores && !a.sigmoid) key[j] /= z;
-        if (a.bias && e < E) key[j] += (double)a.bias[e];
-        if (key[j] != key[j]) key[j] = INFINITY;
-        if (raw[j] == -INFINITY) key[j] = -INFINITY;
-    }
-    if (a.groups > 1) {
-        const int per = E / a.groups;
-        double score = -INFINITY;  // of group `lane`
-        for (int g = 0; g < a.groups; ++g) {
-            double in[V], b1, b2 = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < V; ++j) in[j] = (lane + 64 * j) / per == g ? key[j] : -INFINITY;
-            const int at = best_of<V>(in, &b1);
-            if (a.group_top > 1 && at >= 0) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (lane + 64 * j == at) in[j] = -INFINITY;
-                if (best_of<V>(in, &b2) >= 0) b1 += b2;
-            }
-            if (lane == g) score = b1;
-        }
-        uint64_t kept = 0;
-        for (int t = 0; t < a.top_groups; ++t) {
-            double b;
-            const int g = best_of<1>(&score, &b);
-            if (g < 0) break;
-            kept |= 1ull << g;
-            if (lane == g) score = -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int g = (lane + 64 * j) / per;
-            if (g >= a.groups || !((kept >> g) & 1)) key[j] = -INFINITY;
-        }
-    }
-    unsigned chosen = 0;
-    for (int t = 0; t < a.k; ++t) {
-        double b;
-        const int at = best_of<V>(key, &b);
-        if (at < 0) break;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (lane + 64 * j == at) {
-                key[j] = -INFINITY;
-                chosen |= 1u << j;
-            }
-    }
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const bool in = (chosen >> j) & 1;
-        const uint64_t set = __ballot(in);
-        if (in) to[n + __popcll(set & ((1ull << lane) - 1))] = lane + 64 * j;
-        n += __popcll(set);
-    }
-    return n;
 }
 
 // ---- sums, extremes and scans over a row's L neighbouring lanes ------------------
@@ -211,6 +105,32 @@ __device__ __forceinline__ float lanes_maxf(float v) {
         return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
     }));
 }
+// The sum over the row's lanes up to and including this one (p: its place in the row).
+template <int L>
+__device__ __forceinline__ int lanes_scan(int v, int p) {
+#pragma unroll
+    for (int o = 1; o < (L < 16 ? L : 16); o <<= 1) {  // row_shr: o
+        const int t = o == 1 ? dpp_mov<0x111>(v, 0) : o == 2 ? dpp_mov<0x112>(v, 0) : o == 4 ? dpp_mov<0x114>(v, 0)
+                                                                                     : dpp_mov<0x118>(v, 0);
+        v += L < 16 && p < o ? 0 : t;
+    }
+    if constexpr (L >= 32) v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast: 15
+    if constexpr (L >= 64) v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast: 31
+    return v;
+}
+// The row's largest (d, lowest index), in all of its lanes.
+template <int L>
+__device__ __forceinline__ void lanes_best(double& d, int& e) {
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) {
+        const double od = __shfl_xor(d, o);
+        const int oe = __shfl_xor(e, o);
+        if (od > d || (od == d && oe < e)) {
+            d = od;
+            e = oe;
+        }
+    }
+}
 template <int L>
 __device__ __forceinline__ double lanes_addd(double v) {
 #pragma unroll
@@ -224,8 +144,6 @@ __device__ __forceinline__ int ordered(float v) {
     return b ^ ((b >> 31) & 0x7fffffff);
 }
 __device__ __forceinline__ float unordered(int b) { return __int_as_float(b ^ ((b >> 31) & 0x7fffffff)); }
-
-constexpr int kMasked = (int)0x807fffff;  // ordered(-inf)
 
 // How a row lies on its lanes: of `lanes` for each group (groups rounded up to a
 // power of two), lane p of group g holds the experts g per + p each .. + each - 1.
@@ -253,22 +171,82 @@ __device__ __forceinline__ void load_values(const T* p, float* v) {
     }
 }
 
-__global__ void zero_counts_kernel(int32_t* counts, int E) {
-    for (int e = threadIdx.x; e < E; e += blockDim.x) counts[e] = 0;
+// counts[e] += rows that chose e, of n indices: a histogram per block in LDS, added
+// with integer atomics (in any order the same).  Few blocks: their atomics meet at the
+// same E addresses (1,024 blocks that flush 256 counts each take 12 us).
+#ifndef V_CB
+#define V_CB 32
+#endif
+constexpr int kCountThreads = 1024, kCountBlocks = V_CB;
+__global__ __launch_bounds__(kCountThreads) void route_count_kernel(const int32_t* idx, int64_t n, int E,
+                                                                    int32_t* counts) {
+    __shared__ int s_n[kMaxRouteExperts];
+    for (int e = threadIdx.x; e < E; e += kCountThreads) s_n[e] = 0;
+    __syncthreads();
+    const int64_t stride = (int64_t)gridDim.x * kCountThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kCountThreads + threadIdx.x; i < n; i += 8 * stride) {
+        int e[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) e[u] = idx[min(i + u * stride, n - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i + u * stride < n && e[u] >= 0) atomicAdd(&s_n[e[u]], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kCountThreads)
+        if (s_n[e]) atomicAdd(&counts[e], s_n[e]);
 }
+
+// The keys that the choice goes by: f32 scores and bias, or f32 logits; or 16-bit
+// logits with the index behind them, in an integer, so that no two are equal.
+template <typename T, bool kKeys> struct RouteKey {
+    typedef float type;
+    static constexpr bool kUnique = false;
+};
+template <> struct RouteKey<__bf16, false> {
+    typedef int type;
+    static constexpr bool kUnique = true;
+    static constexpr int kDrop = 16;  // zero bits of the f32 value
+};
+template <> struct RouteKey<_Float16, false> {
+    typedef int type;
+    static constexpr bool kUnique = true;
+    static constexpr int kDrop = 13;
+};
+__device__ __forceinline__ float highest(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ int highest(int a, int b) { return max(a, b); }
+__device__ __forceinline__ float lowest(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ int lowest(int a, int b) { return min(a, b); }
+template <int L>
+__device__ __forceinline__ float lanes_highest(float v) { return lanes_maxf<L>(v); }
+template <int L>
+__device__ __forceinline__ int lanes_highest(int v) { return lanes_max<L>(v); }
+__device__ __forceinline__ int as_ordered(float v) { return ordered(v); }
+__device__ __forceinline__ int as_ordered(int v) { return v; }
+__device__ __forceinline__ float from_ordered(int v, float) { return unordered(v); }
+__device__ __forceinline__ int from_ordered(int v, int) { return v; }
+
+constexpr int kRounds = 16;  // the largest top_k whose keys are taken off one by one
+constexpr int kList = 4;     // keys that a lane keeps in order for that
 
 // kKeys: the keys are scores (bias or groups); else the logits.
 template <typename T, int L, int V, bool kKeys>
-__global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, RouteShape sh, int direct_counts) {
+__global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, RouteShape sh) {
     constexpr int kRows = kWave / L;  // rows of a wave at a time
+    constexpr bool kUnique = RouteKey<T, kKeys>::kUnique;
+    typedef typename RouteKey<T, kKeys>::type Key;
+    const Key kNone = kUnique ? (Key)INT_MIN : (Key)-INFINITY;  // masked, or no expert
     extern __shared__ int s_mem[];
     const int E = a.E, k = a.k;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % L, sub = lane / L;
     int* s_idx = s_mem + (wave * kRows + sub) * k;       // this row's choice
     int* s_hist = s_mem + kRouteWaves * kRows * k;       // [E]
-    if (a.counts) {
-        for (int e = threadIdx.x; e < E; e += kRouteThreads) s_hist[e] = 0;
-        __syncthreads();
+    // counts: a single block writes its histogram, others leave it to
+    // route_count_kernel, which adds to zeros
+    const bool hist = a.counts && gridDim.x == 1;
+    if (a.counts && blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < E; e += kRouteThreads) (hist ? s_hist : a.counts)[e] = 0;
+        if (hist) __syncthreads();
     }
     const int g = p / sh.lanes, at0 = (p - g * sh.lanes) * sh.each;
     const bool in_group = g < a.groups;
@@ -280,13 +258,6 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
 #pragma unroll
         for (int j = 0; j < V; ++j) bias[j] = a.bias && j < n ? a.bias[first + j] : 0.0f;
     }
-    // (a NaN or infinite bias: every row is decided in exact_row)
-    bool odd_bias = false;
-    if constexpr (kKeys) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) odd_bias |= !(fabsf(bias[j]) < INFINITY);
-    }
-    const ExactRow exact_args = {a.bias, E, k, a.sigmoid, a.groups, a.top_groups, a.group_top};
     const int64_t stride = (int64_t)gridDim.x * kRouteWaves * kRows;
     for (int64_t row0 = ((int64_t)blockIdx.x * kRouteWaves + wave) * kRows; row0 < a.rows; row0 += stride) {
         const int64_t row = min(row0 + sub, a.rows - 1);
@@ -302,199 +273,343 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
 #pragma unroll
             for (int j = 0; j < V; ++j) raw[j] = j < n ? Elt<T>::to_f32(l[first + j]) : -INFINITY;
         }
-        // +inf and NaN: decided in exact_row
-        float top = raw[0], all = raw[0];
-#pragma unroll
-        for (int j = 1; j < V; ++j) {
-            top = fmaxf(top, raw[j]);
-            all += raw[j];
-        }
-        bool odd = odd_bias || all != all || all == INFINITY;
-        float zsum = 1.0f;
+        // ---- keys ----
+        constexpr float kLog2e = 1.44269504f;
+        float top = 0.0f, zsum = 1.0f;  // of the softmax
         if (!a.sigmoid) {
-            top = lanes_maxf<L>(top);
-            float z = 0.0f;
-            const float c = top == -INFINITY ? 0.0f : top;
+            top = raw[0];
 #pragma unroll
-            for (int j = 0; j < V; ++j) z += __expf(raw[j] - c);
-            zsum = lanes_addf<L>(z);
-            top = c;
+            for (int j = 1; j < V; ++j) top = fmaxf(top, raw[j]);
+            top = lanes_maxf<L>(top);
+            if (top == -INFINITY) top = 0.0f;
+            zsum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < V; ++j) zsum += __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e);
+            zsum = lanes_addf<L>(zsum);
         }
-        int key[V];
+        Key key[V];
         float near = 0.0f;  // how far a key may be off
+        float all = 0.0f;   // a NaN if a key is one
         if constexpr (kKeys) {
+            // Errors of s, in half steps of f32: sigmoid, s (1 - s) (1.5 |l| + 2) + 3 s < 4;
+            // softmax, of 1 / Z at most: 2.5 |l - top| exp(l - top) + 2, and Z's own, below 30
             const float zi = 1.0f / zsum;
             near = a.sigmoid ? 0x1p-21f : 0x1p-19f * zi;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __expf(-raw[j])) : __expf(raw[j] - top) * zi;
-                key[j] = ordered(raw[j] == -INFINITY ? -INFINITY : s + bias[j]);
+                const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw[j] * -kLog2e))
+                                          : __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e) * zi;
+                const float q = s + bias[j];
+                all += q;
+                key[j] = raw[j] == -INFINITY ? -INFINITY : q;
+            }
+        } else if constexpr (kUnique) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                all += raw[j];
+                const int o = ordered(raw[j] != raw[j] ? INFINITY : raw[j]) >> RouteKey<T, kKeys>::kDrop;
+                key[j] = raw[j] == -INFINITY ? INT_MIN : o * kMaxRouteExperts + (kMaxRouteExperts - 1 - (first + j));
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) key[j] = ordered(raw[j]);
+            for (int j = 0; j < V; ++j) {
+                all += raw[j];
+                key[j] = raw[j];
+            }
         }
+        if constexpr (!kUnique) {
+            // a NaN counts as the largest (in a softmax all of the row's scores are NaN
+            // then, and after +inf too)
+            if (__ballot(all != all)) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (key[j] != key[j]) key[j] = INFINITY;
+            }
+        }
+        // The key of expert e in 64 bits.
+        double z64 = 0.0;
+        auto sum64 = [&]() {
+            if (a.sigmoid || z64 != 0.0) return;
+            for (int j = 0; j < n; ++j) {
+                const float v = Elt<T>::to_f32(l[first + j]);
+                if (v != -INFINITY) z64 += exp((double)v - (double)top);
+            }
+            z64 = lanes_addd<L>(z64);
+        };
+        auto key64 = [&](int e) {
+            const double v = Elt<T>::to_f32(l[e]);
+            double s = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / z64;
+            if (a.bias) s += (double)a.bias[e];
+            return s == s ? s : (double)INFINITY;
+        };
+        // the lane's largest keys in descending order
+        Key list[kList];
+#pragma unroll
+        for (int i = 0; i < kList; ++i) list[i] = kNone;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+#pragma unroll
+            for (int i = kList - 1; i > 0; --i) list[i] = highest(list[i], lowest(list[i - 1], key[j]));
+            list[0] = highest(list[0], key[j]);
+        }
+        bool kept = in_group;
         if constexpr (kKeys) {
             if (a.groups > 1) {
                 // the group's two largest, over its lanes
-                float m1 = -INFINITY, m2 = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float v = unordered(key[j]);
-                    m2 = fmaxf(m2, fminf(m1, v));
-                    m1 = fmaxf(m1, v);
-                }
+                float m1 = list[0], m2 = list[1];
                 for (int o = 1; o < sh.lanes; o <<= 1) {
                     const float o1 = __shfl_xor(m1, o), o2 = __shfl_xor(m2, o);
                     m2 = fmaxf(fmaxf(m2, o2), fminf(m1, o1));
                     m1 = fmaxf(m1, o1);
                 }
                 const float score = a.group_top > 1 && m2 != -INFINITY ? m1 + m2 : m1;
-                int before = 0;  // groups ahead of this one
-                float gap = INFINITY;  // to the nearest other group's score on the other side of the border
+                int ahead = 0;  // groups before this one
                 for (int q = 0; q < a.groups; ++q) {
                     const float o = __shfl(score, sub * L + q * sh.lanes);
-                    before += o > score || (o == score && q < g);
+                    ahead += o > score || (o == score && q < g);
                 }
-                const bool kept = before < a.top_groups && in_group;
+                kept &= ahead < a.top_groups;
                 const float low = -lanes_maxf<L>(kept ? -score : -INFINITY);
                 const float high = lanes_maxf<L>(kept || !in_group ? -INFINITY : score);
-                gap = low - high;
-                odd |= high != -INFINITY && !(gap > 4.0f * (near + 0x1p-22f * fabsf(high)));
+                const bool doubt = high != -INFINITY && low < INFINITY &&
+                                   !(low - high > 4.0f * (near + 0x1p-22f * fabsf(high)));
+                if (__ballot(doubt)) {
+                    sum64();
+                    // those that may be among the group's largest
+                    const float last = a.group_top > 1 ? m2 : m1;
+                    const float from = last - 2.0f * (near + 0x1p-22f * fabsf(last));
+                    double d1 = -INFINITY, d2 = -INFINITY;
+                    unsigned may = 0;
 #pragma unroll
-                for (int j = 0; j < V; ++j) key[j] = kept ? key[j] : kMasked;
-            }
-        }
-        // bisection: count(key >= lo) >= k > count(key >= hi)
-        int most = kMasked, least = INT_MAX, live = 0;
+                    for (int j = 0; j < V; ++j) may |= (unsigned)(key[j] != kNone && !(key[j] < from)) << j;
+                    if (!doubt) may = 0;
+                    for (; may; may &= may - 1) {
+                        const double d = key64(first + __ffs(may) - 1);
+                        d2 = fmax(d2, fmin(d1, d));
+                        d1 = fmax(d1, d);
+                    }
+                    for (int o = 1; o < sh.lanes; o <<= 1) {
+                        const double o1 = __shfl_xor(d1, o), o2 = __shfl_xor(d2, o);
+                        d2 = fmax(fmax(d2, o2), fmin(d1, o1));
+                        d1 = fmax(d1, o1);
+                    }
+                    const double exact = a.group_top > 1 && d2 != -INFINITY ? d1 + d2 : d1;
+                    ahead = 0;
+                    for (int q = 0; q < a.groups; ++q) {
+                        const double o = __shfl(exact, sub * L + q * sh.lanes);
+                        ahead += o > exact || (o == exact && q < g);
+                    }
+                    if (doubt) kept = ahead < a.top_groups && in_group;
+                }
+                if (!kept) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            most = max(most, key[j]);
-            live += key[j] != kMasked;
-        }
-        const int lanes_in = lanes_add<L>(most != kMasked);
-        const int total = lanes_add<L>(live);
-        if (lanes_in >= k) {
-            least = most == kMasked ? INT_MAX : most;
-        } else {
+                    for (int i = 0; i < kList; ++i) list[i] = kNone;
 #pragma unroll
-            for (int j = 0; j < V; ++j) least = min(least, key[j] == kMasked ? INT_MAX : key[j]);
-        }
-        int lo = lanes_min<L>(least), hi = lanes_max<L>(most);
-        bool done = total <= k;      // all of them
-        if (done) lo = kMasked + 1;
-        else hi = hi < INT_MAX ? hi + 1 : hi;
-        bool exact = done;           // count(key >= lo) is what is taken
-        // (32 steps halve any bracket to nothing; rows with a NaN may not end before)
-        for (int i = 0; i < 33 && __ballot(!done); ++i) {
-            // (lo + hi) / 2 without overflow, towards lo
-            const int mid = (lo & hi) + ((lo ^ hi) >> 1);
-            int c = 0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) c += key[j] >= mid;
-            c = lanes_add<L>(c);
-            if (!done) {
-                if (mid == lo) {     // lo is the k-th key, and there are more of it than places
-                    done = true;
-                } else if (c == k) {
-                    lo = mid;
-                    done = exact = true;
-                } else if (c > k) {
-                    lo = mid;
-                } else {
-                    hi = mid;
+                    for (int j = 0; j < V; ++j) key[j] = kNone;
                 }
             }
         }
-        unsigned chosen = 0;
+        // ---- the k-th key ----
+        Key border = kNone;  // chosen: the keys at or above it
+        bool found_it = false;
+        if (k <= kRounds) {
+            for (int i = 0; i < k; ++i) {
+                border = lanes_highest<L>(list[0]);
+                const bool off = list[0] == border;
 #pragma unroll
-        for (int j = 0; j < V; ++j) chosen |= (unsigned)(key[j] >= lo) << j;
+                for (int q = 0; q < kList; ++q) list[q] = off ? (q + 1 < kList ? list[min(q + 1, kList - 1)] : kNone) : list[q];
+            }
+        }
+        auto bits = [&](Key from) {  // of the lane's keys at or above `from` (kNone: above it)
+            unsigned m = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) m |= (unsigned)(from == kNone ? key[j] > from : key[j] >= from) << j;
+            return m;
+        };
+        unsigned chosen = bits(border);
+        int own = __popc(chosen);
+        int upto = lanes_scan<L>(own, p);
+        int found = lanes_max<L>(upto);
+        found_it = k <= kRounds && (border == kNone ? found <= k : found == k);
+        bool by_index = false;  // the places left go to the first of those with the key `border`
+        bool single = found_it; // no key is equal to the border on the other side of it
+        if (__ballot(!found_it)) {
+            // Bisection of the keys' bits: count(key >= lo) >= k > count(key >= hi).  For
+            // long choices, ties, and lanes that hold more of the best than their list.
+            int most = INT_MIN, least = INT_MAX, live = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (key[j] != kNone) {
+                    most = max(most, as_ordered(key[j]));
+                    least = min(least, as_ordered(key[j]));
+                    ++live;
+                }
+            live = lanes_add<L>(live);
+            int lo = lanes_min<L>(least), hi = lanes_max<L>(most);
+            bool done = found_it || live <= k, exact = done;
+            if (!found_it) border = kNone;
+            if (!done) hi = hi < INT_MAX ? hi + 1 : hi;
+            // (32 steps halve any bracket to nothing)
+            for (int i = 0; i < 33 && __ballot(!done); ++i) {
+                const int mid = (lo & hi) + ((lo ^ hi) >> 1);
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) c += key[j] != kNone && as_ordered(key[j]) >= mid;
+                c = lanes_add<L>(c);
+                if (!done) {
+                    if (mid == lo) {  // lo is the k-th key, and there are more of it than places
+                        done = true;
+                        border = from_ordered(lo, Key());
+                    } else if (c == k) {
+                        done = exact = true;
+                        border = from_ordered(mid, Key());
+                    } else if (c > k) {
+                        lo = mid;
+                    } else {
+                        hi = mid;
+                    }
+                }
+            }
+            if (!found_it) {
+                chosen = bits(border);
+                by_index = !exact;
+                single = exact;
+            }
+        }
         if constexpr (kKeys) {
-            if (total > k) {
-                const float border = unordered(lo);
-                float gap = INFINITY;
+            // the largest key that is left out: near the border?
+            float next = -INFINITY;
+            if (k <= kRounds) next = list[0];
+            if (__ballot(own >= kList || k > kRounds || !found_it)) {  // (its list may have ended before)
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    gap = fminf(gap, fabsf(unordered(key[j]) - border));
-                odd |= !exact || !(gap > near + 0x1p-22f * fabsf(border));
+                for (int j = 0; j < V; ++j) next = fmaxf(next, (chosen >> j) & 1 ? -INFINITY : key[j]);
             }
-        } else if (__ballot(!exact)) {
-            // of the experts at lo the first, in index order, for the places that are left
-            unsigned ties = 0;
+            next = lanes_maxf<L>(next);
+            const float off = 2.0f * (near + 0x1p-22f * fabsf(border));
+            const bool doubt = border > -INFINITY && border < INFINITY && next > -INFINITY &&
+                               (!single || !(border - next > off));
+            if (__ballot(doubt)) {
+                unsigned ties = 0, sure = 0;  // the doubtful ones, and those ahead of them
 #pragma unroll
-            for (int j = 0; j < V; ++j) ties |= (unsigned)(key[j] == lo) << j;
-            const int above = lanes_add<L>(__popc(chosen & ~ties));
-            int before = __popc(ties);
-            const int own = before;
-#pragma unroll
-            for (int o = 1; o < L; o <<= 1) {
-                const int t = __shfl_up(before, o, L);
-                if (p >= o) before += t;
+                for (int j = 0; j < V; ++j) {
+                    ties |= (unsigned)(fabsf(key[j] - border) <= off) << j;
+                    sure |= (unsigned)(key[j] > border + off) << j;
+                }
+                if (!doubt) ties = 0;
+                int places = doubt ? k - lanes_add<L>(__popc(sure)) : 0;
+                // the same logit and bias: a tie in 64 bits too
+                int l0 = INT_MAX, l1 = INT_MIN, b0 = INT_MAX, b1 = INT_MIN;
+                for (unsigned m = ties; m; m &= m - 1) {
+                    const int e = first + __ffs(m) - 1;
+                    const int v = ordered(Elt<T>::to_f32(l[e]) + 0.0f), w = a.bias ? ordered(a.bias[e] + 0.0f) : 0;
+                    l0 = min(l0, v);
+                    l1 = max(l1, v);
+                    b0 = min(b0, w);
+                    b1 = max(b1, w);
+                }
+                const bool same = lanes_min<L>(l0) == lanes_max<L>(l1) && lanes_min<L>(b0) == lanes_max<L>(b1);
+                if (doubt) chosen = sure;
+                if (__ballot(doubt && same)) {
+                    const int room = places - (lanes_scan<L>(__popc(ties), p) - __popc(ties));
+                    unsigned take = 0;
+                    int r = room;
+                    for (unsigned m = ties; m && r > 0; m &= m - 1, --r) take |= m & -m;
+                    if (doubt && same) {
+                        chosen = sure | take;
+                        places = 0;
+                    }
+                }
+                if (__ballot(places > 0)) {
+                    sum64();
+                    unsigned left = places > 0 ? ties : 0;
+                    double d = -INFINITY;  // the lane's best of those left
+                    int at = INT_MAX;
+                    bool again = true;
+                    while (__ballot(places > 0)) {
+                        if (again) {
+                            d = -INFINITY;
+                            at = INT_MAX;
+                            for (unsigned m = left; m; m &= m - 1) {
+                                const int e = first + __ffs(m) - 1;
+                                const double v = key64(e);
+                                if (v > d) {
+                                    d = v;
+                                    at = e;
+                                }
+                            }
+                        }
+                        double best = d;
+                        int e = at;
+                        lanes_best<L>(best, e);
+                        again = places > 0 && e == at && at != INT_MAX;
+                        if (again) {
+                            chosen |= 1u << (e - first);
+                            left &= ~(1u << (e - first));
+                        }
+                        --places;
+                    }
+                }
+                if (doubt) by_index = false;
             }
-            int room = k - above - (before - own);
+        }
+        if (__ballot(by_index)) {
+            unsigned ties = 0, sure = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ties |= (unsigned)(key[j] == border) << j;
+                sure |= (unsigned)(key[j] > border) << j;
+            }
+            int room = k - lanes_add<L>(__popc(sure)) - (lanes_scan<L>(__popc(ties), p) - __popc(ties));
             unsigned take = 0;
             for (unsigned m = ties; m && room > 0; m &= m - 1, --room) take |= m & -m;
-            if (!exact) chosen = (chosen & ~ties) | take;
+            if (by_index) chosen = sure | take;
         }
-        int before = __popc(chosen);
-        const int own = before;
-#pragma unroll
-        for (int o = 1; o < L; o <<= 1) {
-            const int t = __shfl_up(before, o, L);
-            if (p >= o) before += t;
-        }
-        int found = __shfl(before, sub * L + L - 1);
-        before -= own;
-        for (unsigned m = chosen; m; m &= m - 1, ++before)
-            if (before < k) s_idx[before] = first + __ffs(m) - 1;
-        uint64_t again = __ballot(odd && real);
-        while (again) {  // (the same for the whole wave)
-            const int r = __builtin_ctzll(again) / L;
-            again &= ~((L < 64 ? (1ull << (L & 63)) - 1 : ~0ull) << (r * L));
-            const int c = exact_row<T, (L * V + 63) / 64>(exact_args, logits + min(row0 + r, a.rows - 1) * E,
-                                                           s_mem + (wave * kRows + r) * k);
-            if (sub == r) found = c;
-        }
+        // ---- the choice, and its weights ----
+        own = __popc(chosen);
+        upto = lanes_scan<L>(own, p);
+        found = lanes_max<L>(upto);
+        int place = upto - own;
+        for (unsigned m = chosen; m; m &= m - 1, ++place)
+            if (place < k) s_idx[place] = first + __ffs(m) - 1;
         __builtin_amdgcn_wave_barrier();
-        found = min(found, k);
-        // slot t of the row: its weight, from f64 scores
-        double sum = 0.0;
-        for (int t0 = 0; t0 < k; t0 += L) {
-            const int t = t0 + p;
-            if (t < found) {
-                const double v = Elt<T>::to_f32(l[s_idx[t]]);
-                sum += a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / (double)zsum;
+        // lane t of the row: slot t
+        auto score = [&](int e) {
+            const float v = Elt<T>::to_f32(l[e]);
+            if (!a.sigmoid) return expf(v - top) / zsum;
+            const float q = expf(-fabsf(v));
+            return (v < 0.0f ? q : 1.0f) / (1.0f + q);  // (a NaN stays one)
+        };
+        int e0 = -1;
+        float s0 = 0.0f, sum = 0.0f;
+        for (int t = p; t < k; t += L) {
+            const int e = t < found ? s_idx[t] : -1;
+            const float s = e >= 0 ? score(e) : 0.0f;
+            if (t < L) {
+                e0 = e;
+                s0 = s;
             }
+            sum += s;
         }
-        if (a.renormalize) sum = lanes_addd<L>(sum) + a.eps;
-        for (int t0 = 0; t0 < k; t0 += L) {
-            const int t = t0 + p;
-            if (t >= k || !real) continue;
-            int e = -1;
-            float w = 0.0f;
-            if (t < found) {
-                e = s_idx[t];
-                const double v = Elt<T>::to_f32(l[e]);
-                const double s = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / (double)zsum;
-                w = (float)(a.scale * (a.renormalize ? s / sum : s));
-                if (a.counts) atomicAdd(&s_hist[e], 1);
-            }
+        float up = a.scale;
+        if (a.renormalize) up /= lanes_addf<L>(sum) + a.eps;
+        for (int t = p; t < k; t += L) {
+            if (!real) break;
+            const int e = t < L ? e0 : t < found ? s_idx[t] : -1;
+            const float s = t < L ? s0 : e >= 0 ? score(e) : 0.0f;
             a.idx[row * k + t] = e;
-            a.w[row * k + t] = w;
+            a.w[row * k + t] = e >= 0 ? up * s : 0.0f;
+            if (hist && e >= 0) atomicAdd(&s_hist[e], 1);
         }
         __builtin_amdgcn_wave_barrier();
     }
-    if (!a.counts) return;
+    if (!hist) return;
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
-        if (direct_counts) a.counts[e] = s_hist[e];
-        else if (s_hist[e]) atomicAdd(&a.counts[e], s_hist[e]);  // (integers: in any order)
-    }
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) a.counts[e] = s_hist[e];
 }
 
 // Lanes and values: the fewest lanes that hold a row with at most 16 values each,
 // each group on lanes of its own.
-RouteShape route_shape(int E, int groups) {
+RouteShape route_shape(int64_t rows, int E, int groups) {
     RouteShape s{};
     int gp = 1;
     while (gp < groups) gp <<= 1;
@@ -502,7 +617,7 @@ RouteShape route_shape(int E, int groups) {
     for (s.L = std::max(8, gp);; s.L <<= 1) {
         s.lanes = s.L / gp;
         s.each = (s.per + s.lanes - 1) / s.lanes;
-        if (s.each <= 16 || s.L == kWave) break;
+        if (s.L == kWave || (s.each <= V_MAXV && (s.each == 1 || rows * s.L / kWave >= V_MINW))) break;
     }
     for (s.V = 1; s.V < s.each; s.V <<= 1) {}
     return s;
@@ -668,17 +783,20 @@ hipError_t launch_route_shape(const RouteArgs& a, const RouteShape& sh, hipStrea
     constexpr int rows = kRouteWaves * (kWave / L);
     const int64_t need = (a.rows + rows - 1) / rows;
     const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min(need, kRouteBlocks));
-    const uint32_t lds = (uint32_t)(rows * a.k + (a.counts ? a.E : 0)) * 4;
-    const int direct = blocks == 1;
-    if (a.counts && !direct) launch_kernel(zero_counts_kernel, dim3(1), dim3(256), 0, s, a.counts, a.E);
+    const uint32_t lds = (uint32_t)(rows * a.k + (blocks == 1 ? a.E : 0)) * 4;
     auto kern = a.bias || a.groups > 1 ? route_kernel<T, L, V, true> : route_kernel<T, L, V, false>;
-    launch_kernel(kern, dim3(blocks), dim3(kRouteThreads), lds, s, a, sh, direct);
+    launch_kernel(kern, dim3(blocks), dim3(kRouteThreads), lds, s, a, sh);
+    if (a.counts && blocks > 1) {
+        const int64_t n = a.rows * a.k, most = (n + kCountThreads - 1) / kCountThreads;
+        launch_kernel(route_count_kernel, dim3((unsigned)std::min<int64_t>(kCountBlocks, most)), dim3(kCountThreads),
+                      0, s, (const int32_t*)a.idx, n, a.E, a.counts);
+    }
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch_route_t(const RouteArgs& a, hipStream_t s) {
-    RouteShape sh = route_shape(a.E, a.groups);
+    RouteShape sh = route_shape(a.rows, a.E, a.groups);
     const uintptr_t at = (uintptr_t)std::min<size_t>(16, sh.V * sizeof(T)) - 1;
     sh.vector = sh.each == sh.V && sh.per == sh.lanes * sh.V && !((uintptr_t)a.logits & at) &&
                 !((a.E * sizeof(T)) & at);
