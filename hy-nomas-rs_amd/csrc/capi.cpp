@@ -686,8 +686,8 @@ int nomas_route_backward(int dtype, const void* logits, const int32_t* idx, cons
         a.k = (int)top_k;
         a.sigmoid = scoring == NOMAS_SIGMOID;
         a.renormalize = renormalize != 0;
-        a.scale = scale;
-        a.eps = eps;
+        a.scale = (float)scale;
+        a.eps = (float)eps;
         a.dlogits = dlogits;
         const hipError_t e =
             nomas::launch_route_backward(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));

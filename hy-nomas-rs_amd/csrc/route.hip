@@ -33,29 +33,13 @@ namespace nomas {
 
 namespace {
 
-#ifndef V_MAXV
-#define V_MAXV 16
-#endif
-#ifndef V_MINW
-#define V_MINW 4096
-#endif
-#ifndef V_RB
-#define V_RB 1024
-#endif
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWaves = kRouteThreads / kWave;
 // Blocks of a call that fills the chip (their rows are a loop, so that the bias is
 // loaded once and the histogram flushed once)
-constexpr int64_t kRouteBlocks = V_RB;
-
-__device__ __forceinline__ double wave_sum(double v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-__device__ __forceinline__ double wave_max(double v) {
-    for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-    return v;
-}
+constexpr int64_t kRouteBlocks = 1024;
+constexpr int64_t kRouteGradBlocks = 8192;
+constexpr int64_t kRouteWavesMin = 1024;  // a wave for each SIMD
 
 // ---- sums, extremes and scans over a row's L neighbouring lanes ------------------
 
@@ -174,10 +158,7 @@ __device__ __forceinline__ void load_values(const T* p, float* v) {
 // counts[e] += rows that chose e, of n indices: a histogram per block in LDS, added
 // with integer atomics (in any order the same).  Few blocks: their atomics meet at the
 // same E addresses (1,024 blocks that flush 256 counts each take 12 us).
-#ifndef V_CB
-#define V_CB 32
-#endif
-constexpr int kCountThreads = 1024, kCountBlocks = V_CB;
+constexpr int kCountThreads = 1024, kCountBlocks = 32;
 __global__ __launch_bounds__(kCountThreads) void route_count_kernel(const int32_t* idx, int64_t n, int E,
                                                                     int32_t* counts) {
     __shared__ int s_n[kMaxRouteExperts];
@@ -197,34 +178,26 @@ __global__ __launch_bounds__(kCountThreads) void route_count_kernel(const int32_
         if (s_n[e]) atomicAdd(&counts[e], s_n[e]);
 }
 
-// The keys that the choice goes by: f32 scores and bias, or f32 logits; or 16-bit
-// logits with the index behind them, in an integer, so that no two are equal.
+// The keys that the choice goes by, as integers in their order: f32 scores and bias,
+// or f32 logits; of 16-bit logits the bits that they have, with the index behind
+// them, so that no two are equal.
 template <typename T, bool kKeys> struct RouteKey {
-    typedef float type;
+    static constexpr int kDrop = 0;  // zero bits of the f32 value
     static constexpr bool kUnique = false;
 };
 template <> struct RouteKey<__bf16, false> {
-    typedef int type;
+    static constexpr int kDrop = 16;
     static constexpr bool kUnique = true;
-    static constexpr int kDrop = 16;  // zero bits of the f32 value
 };
 template <> struct RouteKey<_Float16, false> {
-    typedef int type;
-    static constexpr bool kUnique = true;
     static constexpr int kDrop = 13;
+    static constexpr bool kUnique = true;
 };
-__device__ __forceinline__ float highest(float a, float b) { return fmaxf(a, b); }
-__device__ __forceinline__ int highest(int a, int b) { return max(a, b); }
-__device__ __forceinline__ float lowest(float a, float b) { return fminf(a, b); }
-__device__ __forceinline__ int lowest(int a, int b) { return min(a, b); }
-template <int L>
-__device__ __forceinline__ float lanes_highest(float v) { return lanes_maxf<L>(v); }
-template <int L>
-__device__ __forceinline__ int lanes_highest(int v) { return lanes_max<L>(v); }
-__device__ __forceinline__ int as_ordered(float v) { return ordered(v); }
-__device__ __forceinline__ int as_ordered(int v) { return v; }
-__device__ __forceinline__ float from_ordered(int v, float) { return unordered(v); }
-__device__ __forceinline__ int from_ordered(int v, int) { return v; }
+__device__ __forceinline__ int middle(int a, int b, int c) {
+    int r;
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 constexpr int kRounds = 16;  // the largest top_k whose keys are taken off one by one
 constexpr int kList = 4;     // keys that a lane keeps in order for that
@@ -234,8 +207,7 @@ template <typename T, int L, int V, bool kKeys>
 __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, RouteShape sh) {
     constexpr int kRows = kWave / L;  // rows of a wave at a time
     constexpr bool kUnique = RouteKey<T, kKeys>::kUnique;
-    typedef typename RouteKey<T, kKeys>::type Key;
-    const Key kNone = kUnique ? (Key)INT_MIN : (Key)-INFINITY;  // masked, or no expert
+    constexpr int kNone = kUnique ? INT_MIN : (int)0x807fffff;  // masked, or no expert: -inf
     extern __shared__ int s_mem[];
     const int E = a.E, k = a.k;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % L, sub = lane / L;
@@ -253,11 +225,6 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
     const int first = in_group ? g * sh.per + at0 : 0;      // the lane's experts: first .. first + n - 1
     const int n = in_group ? max(0, min(sh.each, sh.per - at0)) : 0;
     const T* logits = static_cast<const T*>(a.logits);
-    float bias[V];
-    if constexpr (kKeys) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) bias[j] = a.bias && j < n ? a.bias[first + j] : 0.0f;
-    }
     const int64_t stride = (int64_t)gridDim.x * kRouteWaves * kRows;
     for (int64_t row0 = ((int64_t)blockIdx.x * kRouteWaves + wave) * kRows; row0 < a.rows; row0 += stride) {
         const int64_t row = min(row0 + sub, a.rows - 1);
@@ -273,6 +240,15 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
 #pragma unroll
             for (int j = 0; j < V; ++j) raw[j] = j < n ? Elt<T>::to_f32(l[first + j]) : -INFINITY;
         }
+        float bias[V];  // (read again for each row: kept, its registers cost a wave per SIMD)
+        if constexpr (kKeys) {
+            if (a.bias && sh.vector) {
+                load_values<float, V>(a.bias + first, bias);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) bias[j] = a.bias && j < n ? a.bias[first + j] : 0.0f;
+            }
+        }
         // ---- keys ----
         constexpr float kLog2e = 1.44269504f;
         float top = 0.0f, zsum = 1.0f;  // of the softmax
@@ -287,43 +263,49 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             for (int j = 0; j < V; ++j) zsum += __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e);
             zsum = lanes_addf<L>(zsum);
         }
-        Key key[V];
+        int key[V];
         float near = 0.0f;  // how far a key may be off
         float all = 0.0f;   // a NaN if a key is one
         if constexpr (kKeys) {
             // Errors of s, in half steps of f32: sigmoid, s (1 - s) (1.5 |l| + 2) + 3 s < 4;
             // softmax, of 1 / Z at most: 2.5 |l - top| exp(l - top) + 2, and Z's own, below 30
-            const float zi = 1.0f / zsum;
-            near = a.sigmoid ? 0x1p-21f : 0x1p-19f * zi;
+            float s[V];
+            if (a.sigmoid) {
+                near = 0x1p-21f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw[j] * -kLog2e))
-                                          : __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e) * zi;
-                const float q = s + bias[j];
-                all += q;
-                key[j] = raw[j] == -INFINITY ? -INFINITY : q;
+                for (int j = 0; j < V; ++j)
+                    s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw[j] * -kLog2e));
+            } else {
+                const float zi = 1.0f / zsum;
+                near = 0x1p-19f * zi;
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] = __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e) * zi;
             }
-        } else if constexpr (kUnique) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                all += raw[j];
-                const int o = ordered(raw[j] != raw[j] ? INFINITY : raw[j]) >> RouteKey<T, kKeys>::kDrop;
-                key[j] = raw[j] == -INFINITY ? INT_MIN : o * kMaxRouteExperts + (kMaxRouteExperts - 1 - (first + j));
+                s[j] += bias[j];
+                all += s[j];
+                key[j] = ordered(raw[j] == -INFINITY ? -INFINITY : s[j]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 all += raw[j];
-                key[j] = raw[j];
+                key[j] = ordered(raw[j]);
+                if constexpr (kUnique)
+                    key[j] = raw[j] == -INFINITY ? kNone
+                                                 : (key[j] >> RouteKey<T, kKeys>::kDrop) * kMaxRouteExperts +
+                                                       (kMaxRouteExperts - 1 - first - j);
             }
         }
-        if constexpr (!kUnique) {
-            // a NaN counts as the largest (in a softmax all of the row's scores are NaN
-            // then, and after +inf too)
-            if (__ballot(all != all)) {
+        // a NaN counts as the largest (in a softmax all of the row's scores are NaN then,
+        // and after +inf too)
+        if (__ballot(all != all)) {
+            constexpr int kInf = 0x7f800000 >> RouteKey<T, kKeys>::kDrop;
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (key[j] != key[j]) key[j] = INFINITY;
+            for (int j = 0; j < V; ++j) {
+                const float v = kKeys ? unordered(key[j]) : raw[j];
+                if (v != v) key[j] = kUnique ? kInf * kMaxRouteExperts + (kMaxRouteExperts - 1 - first - j) : kInf;
             }
         }
         // The key of expert e in 64 bits.
@@ -343,25 +325,26 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             return s == s ? s : (double)INFINITY;
         };
         // the lane's largest keys in descending order
-        Key list[kList];
+        int list[kList];
 #pragma unroll
         for (int i = 0; i < kList; ++i) list[i] = kNone;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
 #pragma unroll
-            for (int i = kList - 1; i > 0; --i) list[i] = highest(list[i], lowest(list[i - 1], key[j]));
-            list[0] = highest(list[0], key[j]);
+            for (int i = kList - 1; i > 0; --i) list[i] = middle(list[i], list[i - 1], key[j]);
+            list[0] = max(list[0], key[j]);
         }
         bool kept = in_group;
         if constexpr (kKeys) {
             if (a.groups > 1) {
                 // the group's two largest, over its lanes
-                float m1 = list[0], m2 = list[1];
+                int i1 = list[0], i2 = list[1];
                 for (int o = 1; o < sh.lanes; o <<= 1) {
-                    const float o1 = __shfl_xor(m1, o), o2 = __shfl_xor(m2, o);
-                    m2 = fmaxf(fmaxf(m2, o2), fminf(m1, o1));
-                    m1 = fmaxf(m1, o1);
+                    const int o1 = __shfl_xor(i1, o), o2 = __shfl_xor(i2, o);
+                    i2 = max(max(i2, o2), min(i1, o1));
+                    i1 = max(i1, o1);
                 }
+                const float m1 = unordered(i1), m2 = unordered(i2);
                 const float score = a.group_top > 1 && m2 != -INFINITY ? m1 + m2 : m1;
                 int ahead = 0;  // groups before this one
                 for (int q = 0; q < a.groups; ++q) {
@@ -381,7 +364,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                     double d1 = -INFINITY, d2 = -INFINITY;
                     unsigned may = 0;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) may |= (unsigned)(key[j] != kNone && !(key[j] < from)) << j;
+                    for (int j = 0; j < V; ++j) may |= (unsigned)(key[j] != kNone && !(unordered(key[j]) < from)) << j;
                     if (!doubt) may = 0;
                     for (; may; may &= may - 1) {
                         const double d = key64(first + __ffs(may) - 1);
@@ -410,40 +393,38 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             }
         }
         // ---- the k-th key ----
-        Key border = kNone;  // chosen: the keys at or above it
-        bool found_it = false;
+        int border = kNone;  // chosen: the keys at or above it, but for kNone
         if (k <= kRounds) {
             for (int i = 0; i < k; ++i) {
-                border = lanes_highest<L>(list[0]);
+                border = lanes_max<L>(list[0]);
                 const bool off = list[0] == border;
 #pragma unroll
-                for (int q = 0; q < kList; ++q) list[q] = off ? (q + 1 < kList ? list[min(q + 1, kList - 1)] : kNone) : list[q];
+                for (int q = 0; q < kList; ++q)
+                    list[q] = off ? (q + 1 < kList ? list[min(q + 1, kList - 1)] : kNone) : list[q];
             }
         }
-        auto bits = [&](Key from) {  // of the lane's keys at or above `from` (kNone: above it)
+        auto bits = [&](int from) {  // of the lane's keys at or above `from`
             unsigned m = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) m |= (unsigned)(from == kNone ? key[j] > from : key[j] >= from) << j;
+            for (int j = V - 1; j >= 0; --j) m = m + m + (key[j] >= from);
             return m;
         };
-        unsigned chosen = bits(border);
+        unsigned chosen = bits(max(border, kNone + 1));
         int own = __popc(chosen);
         int upto = lanes_scan<L>(own, p);
         int found = lanes_max<L>(upto);
-        found_it = k <= kRounds && (border == kNone ? found <= k : found == k);
-        bool by_index = false;  // the places left go to the first of those with the key `border`
-        bool single = found_it; // no key is equal to the border on the other side of it
+        const bool found_it = k <= kRounds && (border == kNone ? found <= k : found == k);
+        bool by_index = false;   // the places left go to the first of those with the key `border`
         if (__ballot(!found_it)) {
             // Bisection of the keys' bits: count(key >= lo) >= k > count(key >= hi).  For
             // long choices, ties, and lanes that hold more of the best than their list.
-            int most = INT_MIN, least = INT_MAX, live = 0;
+            int most = kNone, least = INT_MAX, live = 0;
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (key[j] != kNone) {
-                    most = max(most, as_ordered(key[j]));
-                    least = min(least, as_ordered(key[j]));
-                    ++live;
-                }
+            for (int j = 0; j < V; ++j) {
+                most = max(most, key[j]);
+                least = min(least, key[j] == kNone ? INT_MAX : key[j]);
+                live += key[j] != kNone;
+            }
             live = lanes_add<L>(live);
             int lo = lanes_min<L>(least), hi = lanes_max<L>(most);
             bool done = found_it || live <= k, exact = done;
@@ -454,15 +435,15 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                 const int mid = (lo & hi) + ((lo ^ hi) >> 1);
                 int c = 0;
 #pragma unroll
-                for (int j = 0; j < V; ++j) c += key[j] != kNone && as_ordered(key[j]) >= mid;
+                for (int j = 0; j < V; ++j) c += key[j] >= mid;  // (lo, and so mid, is above kNone)
                 c = lanes_add<L>(c);
                 if (!done) {
                     if (mid == lo) {  // lo is the k-th key, and there are more of it than places
                         done = true;
-                        border = from_ordered(lo, Key());
+                        border = lo;
                     } else if (c == k) {
                         done = exact = true;
-                        border = from_ordered(mid, Key());
+                        border = mid;
                     } else if (c > k) {
                         lo = mid;
                     } else {
@@ -471,29 +452,28 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                 }
             }
             if (!found_it) {
-                chosen = bits(border);
+                chosen = bits(max(border, kNone + 1));
                 by_index = !exact;
-                single = exact;
             }
         }
         if constexpr (kKeys) {
             // the largest key that is left out: near the border?
-            float next = -INFINITY;
-            if (k <= kRounds) next = list[0];
-            if (__ballot(own >= kList || k > kRounds || !found_it)) {  // (its list may have ended before)
+            int next = k <= kRounds ? list[0] : kNone;
+            if (__ballot(own >= kList || !found_it)) {  // (the list may have ended before it)
 #pragma unroll
-                for (int j = 0; j < V; ++j) next = fmaxf(next, (chosen >> j) & 1 ? -INFINITY : key[j]);
+                for (int j = 0; j < V; ++j) next = max(next, (chosen >> j) & 1 ? kNone : key[j]);
             }
-            next = lanes_maxf<L>(next);
-            const float off = 2.0f * (near + 0x1p-22f * fabsf(border));
-            const bool doubt = border > -INFINITY && border < INFINITY && next > -INFINITY &&
-                               (!single || !(border - next > off));
+            next = lanes_max<L>(next);
+            const float edge = unordered(border);
+            const float off = 2.0f * (near + 0x1p-22f * fabsf(edge));
+            const bool doubt = border != kNone && edge < INFINITY && next != kNone &&
+                               (by_index || !(edge - unordered(next) > off));
             if (__ballot(doubt)) {
                 unsigned ties = 0, sure = 0;  // the doubtful ones, and those ahead of them
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    ties |= (unsigned)(fabsf(key[j] - border) <= off) << j;
-                    sure |= (unsigned)(key[j] > border + off) << j;
+                    ties |= (unsigned)(fabsf(unordered(key[j]) - edge) <= off) << j;
+                    sure |= (unsigned)(unordered(key[j]) > edge + off) << j;
                 }
                 if (!doubt) ties = 0;
                 int places = doubt ? k - lanes_add<L>(__popc(sure)) : 0;
@@ -607,8 +587,11 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
     for (int e = threadIdx.x; e < E; e += kRouteThreads) a.counts[e] = s_hist[e];
 }
 
-// Lanes and values: the fewest lanes that hold a row with at most 16 values each,
-// each group on lanes of its own.
+// Lanes and values: the fewest lanes that hold a row with at most 16 values each, each
+// group on lanes of its own; more lanes where the call has too few rows to give every
+// SIMD a wave (4,744 rows of 64 bf16: 8 lanes, 593 waves, 11.5 us; 16, 1,186 waves, 4.9;
+// 64, 4,744 waves, 7.2).  32,768 rows of 256: 16 lanes 21.8 us, 32 lanes 29, 64 lanes 48 (what
+// a row costs beyond its keys is then paid for fewer rows at once).
 RouteShape route_shape(int64_t rows, int E, int groups) {
     RouteShape s{};
     int gp = 1;
@@ -617,7 +600,7 @@ RouteShape route_shape(int64_t rows, int E, int groups) {
     for (s.L = std::max(8, gp);; s.L <<= 1) {
         s.lanes = s.L / gp;
         s.each = (s.per + s.lanes - 1) / s.lanes;
-        if (s.L == kWave || (s.each <= V_MAXV && (s.each == 1 || rows * s.L / kWave >= V_MINW))) break;
+        if (s.L == kWave || (s.each <= 16 && (s.each == 1 || rows * s.L / kWave >= kRouteWavesMin))) break;
     }
     for (s.V = 1; s.V < s.each; s.V <<= 1) {}
     return s;
@@ -625,78 +608,181 @@ RouteShape route_shape(int64_t rows, int E, int groups) {
 
 
 // ---- the gradient -----------------------------------------------------------------
-
-template <typename T, int V>
-__device__ void row_scores(const T* l, int E, int sigmoid, double* raw, double* s) {
-    const int lane = threadIdx.x & 63;
-    double m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = lane + 64 * j;
-        raw[j] = e < E ? (double)Elt<T>::to_f32(l[e]) : -INFINITY;
-        m = fmax(m, raw[j]);
-    }
-    double z = 0.0;
-    if (!sigmoid) m = wave_max(m);
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        if (raw[j] == -INFINITY) s[j] = 0.0;
-        else if (sigmoid) s[j] = 1.0 / (1.0 + exp(-raw[j]));
-        else z += s[j] = exp(raw[j] - m);
-    }
-    if (sigmoid) return;
-    z = wave_sum(z);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (raw[j] != -INFINITY) s[j] /= z;
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBackwardArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * kRouteWaves + (threadIdx.x >> 6);
-    if (row >= a.rows) return;
+//
+//   S = sum of the chosen s + eps, A = sum of dw s over the chosen
+//   ds_i = scale (dw_i - A / S) / S (renormalised) or scale dw_i, 0 where not chosen
+//   sigmoid: dl_i = ds_i s_i (1 - s_i)
+//   softmax: dl_e = s_e (ds_e - B), B = sum s ds: of renormalised weights scale A eps / S^2
+//
+// HBM bound: a softmax reads the row once, a sigmoid its chosen logits; every element of
+// dlogits is written once.  The lanes of a row hold 16-byte chunks of it; the chosen
+// elements are scattered into the row in LDS, and it is stored from there in whole chunks.
+template <typename T, int L, int C, bool kSigmoid>
+__global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBackwardArgs a, int vector) {
+    constexpr int W = 16 / (int)sizeof(T), kRows = kWave / L;
+    extern __shared__ __align__(16) float s_rows[];
     const int E = a.E, k = a.k;
-    double raw[V], s[V], ds[V];
-    row_scores<T, V>(static_cast<const T*>(a.logits) + row * E, E, a.sigmoid, raw, s);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % L, sub = lane / L;
+    float* s_row = s_rows + (wave * kRows + sub) * (L * C * W);
+    const int64_t stride = (int64_t)gridDim.x * kRouteWaves * kRows;
+    for (int64_t row0 = ((int64_t)blockIdx.x * kRouteWaves + wave) * kRows; row0 < a.rows; row0 += stride) {
+        const int64_t row = min(row0 + sub, a.rows - 1);
+        const bool real = row0 + sub < a.rows;
+        const T* l = static_cast<const T*>(a.logits) + row * E;
+        // the first slots, and where they lead
+        const int32_t* idx = a.idx + row * k;
+        const float* dw = a.dw + row * k;
+        const int e0 = p < k ? idx[p] : -1;
+        const float d0 = p < k ? dw[p] : 0.0f;
+        const float v0 = e0 >= 0 && e0 < E ? Elt<T>::to_f32(l[e0]) : 0.0f;
+        float s[C][W], top = 0.0f, zi = 1.0f;
+        if constexpr (!kSigmoid) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) ds[j] = 0.0;
-    // the chosen scores' sum, and their sum weighed by dw
-    double total = 0.0, dot = 0.0;
-    for (int t = 0; t < k; ++t) {
-        const int e = a.idx[row * k + t];
-        const double d = a.dw[row * k + t];
+            for (int c = 0; c < C; ++c) {
+                const int at = (c * L + p) * W;
+                if (vector && at < E) {
+                    load16(l + at, s[c]);
+                } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (lane + 64 * j == e && e < E) {
-                total += s[j];
-                dot += d * s[j];
-                ds[j] += d;
+                    for (int i = 0; i < W; ++i) s[c][i] = at + i < E ? Elt<T>::to_f32(l[at + i]) : -INFINITY;
+                }
             }
-    }
-    total = wave_sum(total) + a.eps;
-    dot = wave_sum(dot);
-    // ds_i = scale (dw_i - dot / total) / total for the chosen; the softmax's
-    // inner product sum_j s_j ds_j is then scale dot eps / total^2
-    const double mean = a.renormalize ? dot / total : 0.0;
-    const double up = a.renormalize ? a.scale / total : a.scale;
-    const double inner = a.sigmoid ? 0.0 : a.renormalize ? up * mean * a.eps : up * dot;
-    for (int t = 0; t < k; ++t) {
-        const int e = a.idx[row * k + t];
+            top = s[0][0];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (lane + 64 * j == e && e < E) ds[j] -= mean;
-    }
-    T* out = static_cast<T*>(a.dlogits) + row * E;
+            for (int c = 0; c < C; ++c)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int e = lane + 64 * j;
-        if (e >= E) continue;
-        const double d = up * ds[j] - inner;
-        const double r = raw[j] == -INFINITY ? 0.0 : a.sigmoid ? d * s[j] * (1.0 - s[j]) : d * s[j];
-        out[e] = Elt<T>::from_f32((float)r);
+                for (int i = 0; i < W; ++i) top = fmaxf(top, s[c][i]);
+            top = lanes_maxf<L>(top);
+            if (top == -INFINITY) top = 0.0f;
+            float z = 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < W; ++i) z += s[c][i] = __builtin_amdgcn_exp2f((s[c][i] - top) * 1.44269504f);
+            z = lanes_addf<L>(z);
+            zi = z == 0.0f ? 0.0f : 1.0f / z;
+        }
+        // a slot's score, and what dl is of ds
+        auto score = [&](float v, float* slope) {
+            if constexpr (!kSigmoid) return *slope = __builtin_amdgcn_exp2f((v - top) * 1.44269504f) * zi;
+            const float q = expf(-fabsf(v)), r = 1.0f / (1.0f + q);
+            *slope = q * r * r;
+            return (v < 0.0f ? q : 1.0f) * r;
+        };
+        auto slot = [&](int t, int* e, float* d, float* slope) {  // its score; e = -1: empty
+            *e = t < L ? e0 : idx[t];
+            *d = t < L ? d0 : dw[t];
+            *slope = 0.0f;
+            if (t >= k || *e < 0 || *e >= E) {
+                *e = -1;
+                return 0.0f;
+            }
+            return score(t < L ? v0 : Elt<T>::to_f32(l[*e]), slope);
+        };
+        float sum = 0.0f, dot = 0.0f;
+        bool some = false, twice = false;
+        for (int t = p; t < k; t += L) {
+            int e;
+            float d, slope;
+            const float w = slot(t, &e, &d, &slope);
+            sum += w;
+            dot += d * w;
+            some |= e >= 0;
+            if (e >= 0) reinterpret_cast<int*>(s_row)[e] = t;
+        }
+        __builtin_amdgcn_wave_barrier();
+        for (int t = p; t < k; t += L) {
+            const int e = t < L ? e0 : idx[t];
+            if (e >= 0 && e < E) twice |= reinterpret_cast<int*>(s_row)[e] != t;
+        }
+        __builtin_amdgcn_wave_barrier();
+        sum = lanes_addf<L>(sum);
+        dot = lanes_addf<L>(dot);
+        float mean = 0.0f, up = 0.0f, inner = 0.0f;
+        if (lanes_max<L>(some)) {
+            const float total = sum + a.eps;
+            mean = a.renormalize ? dot / total : 0.0f;
+            up = a.renormalize ? a.scale / total : a.scale;
+            inner = a.renormalize ? up * mean * a.eps : up * dot;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if constexpr (!kSigmoid) {
+                    const float f = -inner * zi;
+                    b = make_float4(f * s[c][i], f * s[c][i + 1], f * s[c][i + 2], f * s[c][i + 3]);
+                }
+                *reinterpret_cast<float4*>(s_row + (c * L + p) * W + i) = b;
+            }
+        __builtin_amdgcn_wave_barrier();
+        const bool again = __ballot(twice) != 0;
+        for (int t = p; t < k; t += L) {
+            int e;
+            float d, slope;
+            slot(t, &e, &d, &slope);
+            if (e < 0) continue;
+            float ds = up * (d - mean);
+            if (again) {  // an expert named twice: all its slots' shares, in their order
+                ds = 0.0f;
+                for (int u = 0; u < k; ++u)
+                    if (idx[u] == e) ds += up * (dw[u] - mean);
+            }
+            s_row[e] = slope * (kSigmoid ? ds : ds - inner);
+        }
+        __builtin_amdgcn_wave_barrier();
+        T* out = static_cast<T*>(a.dlogits) + row * E;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int at = (c * L + p) * W;
+            float v[W];
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(s_row + at + i);
+                v[i] = b.x;
+                v[i + 1] = b.y;
+                v[i + 2] = b.z;
+                v[i + 3] = b.w;
+            }
+            if (!real || at >= E) continue;
+            if (vector) {
+                store16(out + at, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (at + i < E) out[at + i] = Elt<T>::from_f32(v[i]);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
+
+template <typename T, int L, int C>
+hipError_t launch_route_backward_shape(const RouteBackwardArgs& a, hipStream_t s) {
+    constexpr int W = 16 / (int)sizeof(T), rows = kRouteWaves * (kWave / L);
+    const int vector = a.E % W == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.dlogits) & 15);
+    const int64_t blocks = std::min<int64_t>((a.rows + rows - 1) / rows, kRouteGradBlocks);
+    launch_kernel(a.sigmoid ? route_backward_kernel<T, L, C, true> : route_backward_kernel<T, L, C, false>,
+                  dim3((unsigned)blocks), dim3(kRouteThreads), rows * L * C * W * 4, s, a, vector);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_route_backward_t(const RouteBackwardArgs& a, hipStream_t s) {
+    constexpr int W = 16 / (int)sizeof(T);
+    const int chunks = (a.E + W - 1) / W;
+    // four chunks a lane where the row has them: more rows of a wave share its work on the
+    // slots (32,768 rows of 256 f32: one chunk 15.0 us, two 11.8, four 10.9)
+    if (chunks <= 8) return launch_route_backward_shape<T, 8, 1>(a, s);
+    if (chunks <= 16) return launch_route_backward_shape<T, 8, 2>(a, s);
+    if (chunks <= 32) return launch_route_backward_shape<T, 8, 4>(a, s);
+    if (chunks <= 64) return launch_route_backward_shape<T, 16, 4>(a, s);
+    if (chunks <= 128) return launch_route_backward_shape<T, 32, 4>(a, s);
+    return launch_route_backward_shape<T, 64, 4>(a, s);
+}
+
+// ---- the caller's routing -----------------------------------------------------------
 
 // The routing of the caller in the form that the router leaves for the
 // dispatch: per row distinct experts in ascending order, then -1; an expert
@@ -768,16 +854,6 @@ __global__ __launch_bounds__(kRouteThreads) void given_kernel(GivenRoutingArgs a
         a.chunk_counts[(int64_t)blockIdx.x * a.E_cols + e] = s_hist[e];
 }
 
-// Calls f with the number of values that a lane holds of E experts.
-template <typename F>
-hipError_t with_values(int E, F f) {
-    if (E <= 64) return f(std::integral_constant<int, 1>{});
-    if (E <= 128) return f(std::integral_constant<int, 2>{});
-    if (E <= 256) return f(std::integral_constant<int, 4>{});
-    if (E <= 512) return f(std::integral_constant<int, 8>{});
-    return f(std::integral_constant<int, 16>{});
-}
-
 template <typename T, int L, int V>
 hipError_t launch_route_shape(const RouteArgs& a, const RouteShape& sh, hipStream_t s) {
     constexpr int rows = kRouteWaves * (kWave / L);
@@ -799,7 +875,7 @@ hipError_t launch_route_t(const RouteArgs& a, hipStream_t s) {
     RouteShape sh = route_shape(a.rows, a.E, a.groups);
     const uintptr_t at = (uintptr_t)std::min<size_t>(16, sh.V * sizeof(T)) - 1;
     sh.vector = sh.each == sh.V && sh.per == sh.lanes * sh.V && !((uintptr_t)a.logits & at) &&
-                !((a.E * sizeof(T)) & at);
+                !((a.E * sizeof(T)) & at) && !((uintptr_t)a.bias & (std::min<size_t>(16, sh.V * 4) - 1));
     switch (sh.L * 64 + sh.V) {
 #define ROUTE_SHAPE(l, v) \
     case l * 64 + v: return launch_route_shape<T, l, v>(a, sh, s);
@@ -827,17 +903,6 @@ hipError_t launch_route_t(const RouteArgs& a, hipStream_t s) {
 #undef ROUTE_SHAPE
     }
     return hipErrorInvalidValue;
-}
-
-template <typename T>
-hipError_t launch_route_backward_t(const RouteBackwardArgs& a, hipStream_t s) {
-    const int64_t nblk = (a.rows + kRouteWaves - 1) / kRouteWaves;
-    if (nblk > 0x7fffffff) return hipErrorInvalidValue;
-    return with_values(a.E, [&](auto v) {
-        launch_kernel(route_backward_kernel<T, decltype(v)::value>, dim3((unsigned)nblk), dim3(kRouteThreads), 0,
-                      s, a);
-        return hipGetLastError();
-    });
 }
 
 }  // namespace
