@@ -29,8 +29,8 @@ struct SeamPlan {
 };
 
 // `target`: blocks that fill the chip; `most`: threads of a block (a row may need
-// more).  Sequences are shared by blocks unless they are shorter than two steps or
-// there are enough of them to fill the chip.
+// more).  Sequences are shared by blocks unless they are shorter than two rows of
+// each group or there are enough of them to fill the chip.
 inline SeamPlan seam_plan(int64_t rows, int64_t D, int64_t seq, int64_t target, int most) {
     SeamPlan p{};
     const int64_t chunks = D / kSeamCols;

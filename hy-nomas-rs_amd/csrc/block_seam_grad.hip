@@ -27,36 +27,30 @@ namespace {
 
 // Blocks of a call that fills the chip.  Each leaves 12 D bytes of sums, written and
 // read again.
-#ifndef V_BLOCKS
-#define V_BLOCKS 768
-#endif
-#ifndef V_PRE
-#define V_PRE 1
-#endif
-#ifndef V_R
-#define V_R 2
-#endif
-#ifndef V_GT
-#define V_GT 512
-#endif
-constexpr int64_t kGradBlocks = V_BLOCKS;
-constexpr int kGradThreads = V_GT;
+// Blocks and threads of a call that fills the chip: two blocks a CU, at 128 registers
+// all of them at once.  Each leaves 12 D bytes of sums, written and read again: 1,024
+// smaller blocks took as long, 768 blocks, of which a third run in a second round, 83 us
+// where 512 took 60 (14,232 rows of 1,536 bf16).
+constexpr int64_t kGradBlocks = 512;
+constexpr int kGradThreads = 384;
 
 // sums of a block's (or sequence's) columns: P, Q, R, each D floats
 constexpr int kSums = 3;
 
+// LDS: the parameters of a block's sequence, f and u [D] each, and later a group's
+// sums of eight columns a thread.
+__host__ __device__ inline uint32_t grad_lds(const SeamPlan& p, int D) {
+    const uint32_t params = p.whole ? 0 : 2 * (uint32_t)D * 4, sums = (uint32_t)(p.row_threads * p.groups) * 8 * 4;
+    return params > sums ? params : sums;
+}
+
 template <typename T, bool kPost, bool kNorm, bool kWhole, int L, int C>
-__global__ __launch_bounds__(kSeamThreads)
-#ifdef V_WPE
-__attribute__((amdgpu_waves_per_eu(C == 1 ? V_WPE : 2)))
-#endif
-void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
-                                                                                float* sums) {
-    constexpr int R = sizeof(T) == 4 || C > 1 ? 1 : V_R;     // rows of a step
+__global__ __launch_bounds__(kSeamThreads) __attribute__((amdgpu_waves_per_eu(C == 1 && !kWhole ? 4 : 2)))
+void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
     constexpr int N = (kNorm ? 2 : 0) + (kPost ? 2 : 0) + (kNorm && kPost ? 2 : 0);
-    constexpr int NS = N ? N * R : 1;
+    constexpr int NS = N ? N : 1;
     __shared__ __align__(16) float s_part[sums_floats<L, NS>()];
-    __shared__ float s_v[kSeamThreads * 8];  // over_groups()
+    extern __shared__ __align__(16) float s_dyn[];
     const int D = a.D;
     const int W = L ? L : p.row_threads, G = p.groups;
     // (the same for a wave where a row takes whole ones)
@@ -77,202 +71,180 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
     T* dy = static_cast<T*>(a.dy);
     const float inv_d = 1.0f / (float)D;
 
-    float f[C][8], u[C][8];
-    auto params = [&](int64_t b) {
+    // f = norm_w (1 + scale) and u = gate post_w for eight columns of sequence b
+    auto factors = [&](int64_t b, int at, float* f, float* u) {
+        float w[8];
+        params8(a.gate, b * D + at, 1.0f, u);
+        if constexpr (kPost) {
+            params8(a.post_w, at, 1.0f, w);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float w[8];
-            params8(a.gate, b * D + col[c], 1.0f, u[c]);
-            if constexpr (kPost) {
-                params8(a.post_w, col[c], 1.0f, w);
+            for (int i = 0; i < 8; ++i) u[i] *= w[i];
+        }
+        if constexpr (kNorm) {
+            params8(a.scale, b * D + at, 0.0f, f);
+            params8(a.norm_w, at, 1.0f, w);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[c][i] *= w[i];
-            }
-            if constexpr (kNorm) {
-                params8(a.scale, b * D + col[c], 0.0f, f[c]);
-                params8(a.norm_w, col[c], 1.0f, w);
+            for (int i = 0; i < 8; ++i) f[i] = w[i] * (1.0f + f[i]);
+        }
+    };
+    float own[2][kWhole ? C : 1][8];  // kWhole: this group's f and u (else they are in LDS)
+    auto get_f = [&](int c, float* f) {
+        if constexpr (kWhole) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[c][i] = w[i] * (1.0f + f[c][i]);
-            }
+            for (int i = 0; i < 8; ++i) f[i] = own[0][c][i];
+        } else {
+            load_f32s<8>(s_dyn + col[c], f);
+        }
+    };
+    auto get_u = [&](int c, float* u) {
+        if constexpr (kWhole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = own[1][c][i];
+        } else {
+            load_f32s<8>(s_dyn + D + col[c], u);
         }
     };
     float acc[kSums][C][8];
-    auto clear = [&](auto& v) {
+    auto clear = [&](float (&v)[C][8]) {
 #pragma unroll
-        for (auto& w : v)
+        for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = 0.0f;
+            for (int i = 0; i < 8; ++i) v[c][i] = 0.0f;
     };
     clear(acc[0]);
     clear(acc[1]);
     clear(acc[2]);
-    struct Rows {
-        Raw8<T> dout[R][C], dh[R][C], out[R][C], y[R][C];
-    };
-    auto load = [&](Rows& q, int64_t at, int64_t stride, int64_t end) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int64_t row = min(at + r * stride, end - 1);
-            const int64_t o = row * D;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                if constexpr (kNorm) {
-                    q.dh[r][c] = fetch8(dh + o, col[c]);
-                    q.out[r][c] = fetch8(out + o, col[c]);
-                }
-                if (dout) q.dout[r][c] = fetch8(dout + o, col[c]);
-                if (y) q.y[r][c] = fetch8(y + o, col[c]);
-            }
-        }
-    };
     int turn = 0;
-    // (rows as in block_seam_kernel)
-    auto step = [&](Rows& q, int64_t at, int64_t stride, int64_t end, bool busy) {
-        float s[NS];
+    // One row of each group; `on`: it is a row of this group (all lanes run the same
+    // steps, those without a row compute one that nothing is kept of).
+    auto step = [&](int64_t row, bool on) {
+        const int64_t o = row * D;
+        Raw8<T> rd[C], rh[C], ro[C], ry[C];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) s[i] = 0.0f;
-        auto widen = [&](const Raw8<T>& raw, bool there, float* o) {
-            if (there) {
-                widen8(raw, o);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = 0.0f;
+        for (int c = 0; c < C; ++c) {
+            if constexpr (kNorm) {
+                rh[c] = fetch8(dh + o, col[c]);
+                ro[c] = fetch8(out + o, col[c]);
             }
-        };
+            rd[c] = {};
+            if (dout) rd[c] = fetch8(dout + o, col[c]);
+            ry[c] = {};
+            if (kPost || y) ry[c] = fetch8(y + o, col[c]);
+        }
+        float m[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) m[i] = 0.0f;
         if constexpr (N > 0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+            for (int c = 0; c < C; ++c) {
+                float vo[8], vh[8], vy[8], vd[8], f[8], u[8], q[N];
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float vo[8], vh[8], vy[8], vd[8], m[N];
+                for (int i = 0; i < N; ++i) q[i] = 0.0f;
+                if constexpr (kNorm) {
+                    widen8(rh[c], vh);
+                    widen8(ro[c], vo);
+                    get_f(c, f);
+                }
+                if constexpr (kPost) {
+                    widen8(ry[c], vy);
+                    widen8(rd[c], vd);
+                    get_u(c, u);
+                }
 #pragma unroll
-                    for (int i = 0; i < N; ++i) m[i] = 0.0f;
+                for (int i = 0; i < 8; ++i) {
                     if constexpr (kNorm) {
-                        widen8(q.dh[r][c], vh);
-                        widen8(q.out[r][c], vo);
+                        vh[i] *= f[i];
+                        q[0] += vo[i] * vo[i];
+                        q[1] += vh[i] * vo[i];
                     }
                     if constexpr (kPost) {
-                        widen8(q.y[r][c], vy);
-                        widen(q.dout[r][c], dout != nullptr, vd);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                        constexpr int k = kNorm ? 2 : 0;
+                        q[k] += vy[i] * vy[i];
+                        const float uy = u[i] * vy[i];
+                        q[k + 1] += uy * vd[i];
                         if constexpr (kNorm) {
-                            vh[i] *= f[c][i];
-                            m[0] += vo[i] * vo[i];
-                            m[1] += vh[i] * vo[i];
-                        }
-                        if constexpr (kPost) {
-                            constexpr int k = kNorm ? 2 : 0;
-                            m[k] += vy[i] * vy[i];
-                            const float uy = u[c][i] * vy[i];
-                            m[k + 1] += uy * vd[i];
-                            if constexpr (kNorm) {
-                                m[k + 2] += uy * vh[i];
-                                m[k + 3] += uy * vo[i];
-                            }
+                            q[k + 2] += uy * vh[i];
+                            q[k + 3] += uy * vo[i];
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < N; ++i) s[r * N + i] += live[c] ? m[i] : 0.0f;
                 }
-            }
-            row_sums<L>(s, s_part, turn++, W / kWave);
-        }
-#ifdef V_RENEW
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+                for (int i = 0; i < N; ++i) m[i] += live[c] ? q[i] : 0.0f;
+            }
+            row_sums<L>(m, s_part, turn++, W / kWave);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                renew(q.dout[r][c]);
+                renew(rd[c]);
+                renew(ry[c]);
                 if constexpr (kNorm) {
-                    renew(q.dh[r][c]);
-                    renew(q.out[r][c]);
+                    renew(rh[c]);
+                    renew(ro[c]);
                 }
-                renew(q.y[r][c]);
-            }
-#endif
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float* m = s + r * N;
-            const bool on = busy && at + r * stride < end;
-            float rr = 0.0f, k1 = 0.0f, ry = 1.0f, k2 = 0.0f;
-            if constexpr (kNorm) {
-                rr = rsqrtf(m[0] * inv_d + a.eps);
-                k1 = rr * rr * rr * (m[1] * inv_d);  // of out in d
-            }
-            if constexpr (kPost) {
-                constexpr int k = kNorm ? 2 : 0;
-                ry = rsqrtf(m[k] * inv_d + a.eps);
-                float dot = m[k + 1];
-                if constexpr (kNorm) dot += rr * m[k + 2] - k1 * m[k + 3];
-                k2 = ry * ry * ry * (dot * inv_d);   // of y in dy
-            }
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int64_t o = min(at + r * stride, end - 1) * D;
-                float d[8], v[8];
-                widen(q.dout[r][c], dout != nullptr, d);
-                if constexpr (kNorm) {
-                    float vo[8], vh[8];
-                    widen8(q.dh[r][c], vh);
-                    widen8(q.out[r][c], vo);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (on) acc[0][c][i] += vh[i];
-                        if (on) acc[1][c][i] += (rr * vh[i]) * vo[i];
-                        d[i] += rr * (vh[i] * f[c][i]) - k1 * vo[i];
-                    }
-                }
-                if (y) {
-                    float vy[8], w[8];
-                    widen8(q.y[r][c], vy);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (on) acc[2][c][i] += d[i] * (ry * vy[i]);
-                        w[i] = ry * (u[c][i] * d[i]);
-                        if constexpr (kPost) w[i] -= k2 * vy[i];
-                    }
-                    if (dy && on && live[c]) put8(dy + o, col[c], w);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = a.alpha * d[i];
-                if (dx && on && live[c]) put8(dx + o, col[c], v);
             }
         }
-    };
-    // The parameters' gradients of sequence b from its sums.
-    auto finish = [&](int64_t b, const float (&s)[kSums][C][8]) {
+        if (!on) return;
+        float r = 0.0f, k1 = 0.0f, iy = 1.0f, k2 = 0.0f;
+        if constexpr (kNorm) {
+            r = rsqrtf(m[0] * inv_d + a.eps);
+            k1 = r * r * r * (m[1] * inv_d);  // of out in d
+        }
+        if constexpr (kPost) {
+            constexpr int k = kNorm ? 2 : 0;
+            iy = rsqrtf(m[k] * inv_d + a.eps);
+            float dot = m[k + 1];
+            if constexpr (kNorm) dot += r * m[k + 2] - k1 * m[k + 3];
+            k2 = iy * iy * iy * (dot * inv_d);  // of y in dy
+        }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (!live[c]) continue;
-            const int64_t o = b * D + col[c];
-            float w[8], v[8];
-            params8(a.norm_w, col[c], 1.0f, w);
-            if (a.dshift) put8(a.dshift + o, s[0][c]);
+            float d[8], v[8];
+            widen8(rd[c], d);
+            if constexpr (kNorm) {
+                float vo[8], vh[8], f[8];
+                widen8(rh[c], vh);
+                widen8(ro[c], vo);
+                get_f(c, f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = w[i] * s[1][c][i];
-            if (a.dscale) put8(a.dscale + o, v);
-            params8(kPost ? a.post_w : nullptr, col[c], 1.0f, w);
+                for (int i = 0; i < 8; ++i) {
+                    acc[0][c][i] += vh[i];
+                    vh[i] *= r;
+                    acc[1][c][i] += vh[i] * vo[i];
+                    d[i] += vh[i] * f[i] - k1 * vo[i];
+                }
+            }
+            if (kPost || y) {
+                float vy[8], w[8], u[8];
+                widen8(ry[c], vy);
+                get_u(c, u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = w[i] * s[2][c][i];
-            if (a.dgate) put8(a.dgate + o, v);
+                for (int i = 0; i < 8; ++i) {
+                    acc[2][c][i] += (iy * d[i]) * vy[i];
+                    w[i] = (iy * d[i]) * u[i];
+                    if constexpr (kPost) w[i] -= k2 * vy[i];
+                }
+                if (dy) put8(dy + o, col[c], w);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = a.alpha * d[i];
+            if (dx) put8(dx + o, col[c], v);
         }
     };
     // The groups' values of the columns added up, in the first group's lanes: by
     // eights, every group's in LDS, in the groups' order.
     auto over_groups = [&](float (&v)[C][8]) {
         if (G == 1) return;
+        const int n = W * G;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s_v[i * kSeamThreads + threadIdx.x] = v[c][i];
+            for (int i = 0; i < 8; ++i) s_dyn[i * n + threadIdx.x] = v[c][i];
             __syncthreads();
             if (g == 0)
-                for (int o = 1; o < G; ++o)
+                for (int q = 1; q < G; ++q)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[c][i] += s_v[i * kSeamThreads + o * W + t];
+                    for (int i = 0; i < 8; ++i) v[c][i] += s_dyn[i * n + q * W + t];
         }
     };
     if constexpr (kWhole) {
@@ -283,22 +255,29 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
         for (int64_t b0 = blockIdx.x * (int64_t)G; b0 < n; b0 += gridDim.x * (int64_t)G) {
             const bool busy = b0 + g < n;
             const int64_t b = min(b0 + g, n - 1);
-            params(b);
-            for (int64_t s = 0; s < a.seq; s += R) {
-                Rows q;
-                load(q, b * a.seq + s, 1, (b + 1) * a.seq);
-                step(q, b * a.seq + s, 1, (b + 1) * a.seq, busy);
-            }
-            if (busy) finish(b, acc);
+#pragma unroll
+            for (int c = 0; c < C; ++c) factors(b, col[c], own[0][c], own[1][c]);
+            for (int64_t s = 0; s < a.seq; ++s) step(b * a.seq + s, busy);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                float sc[8], gt[8];
-                params8(a.scale, b * D + col[c], 0.0f, sc);
-                params8(a.gate, b * D + col[c], 1.0f, gt);
+                if (!busy || !live[c]) continue;
+                const int64_t o = b * D + col[c];
+                float w[8], v[8];
+                params8(a.norm_w, col[c], 1.0f, w);
+                if (a.dshift) put8(a.dshift + o, acc[0][c]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = w[i] * acc[1][c][i];
+                if (a.dscale) put8(a.dscale + o, v);
+                params8(kPost ? a.post_w : nullptr, col[c], 1.0f, w);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = w[i] * acc[2][c][i];
+                if (a.dgate) put8(a.dgate + o, v);
+                params8(a.scale, o, 0.0f, w);
+                params8(a.gate, o, 1.0f, v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    gain[0][c][i] += (1.0f + sc[i]) * acc[1][c][i];  // (zero where not busy)
-                    gain[1][c][i] += gt[i] * acc[2][c][i];
+                    gain[0][c][i] += (1.0f + w[i]) * acc[1][c][i];
+                    gain[1][c][i] += v[i] * acc[2][c][i];
                 }
             }
             clear(acc[0]);
@@ -317,78 +296,77 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p,
                 }
         }
     } else {
-    const int64_t b = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
-    const int64_t first = b * a.seq + part * p.chunk, end = min(first + p.chunk, (b + 1) * a.seq);
-    params(b);
-    if constexpr (V_PRE && C == 1) {
-        // the next step's rows are on their way during this one
-        Rows q;
-        load(q, first + g, G, end);
-        for (int64_t at = first; at < end; at += (int64_t)G * R) {
-            Rows next;
-            load(next, at + (int64_t)G * R + g, G, end);
-            step(q, at + g, G, end, true);
-            q = next;
+        const int64_t b = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+        const int64_t first = b * a.seq + part * p.chunk, end = min(first + p.chunk, (b + 1) * a.seq);
+        for (int at = threadIdx.x * kSeamCols; at < D; at += blockDim.x * kSeamCols) {
+            float f[8], u[8];
+            factors(b, at, f, u);
+            if constexpr (kNorm) put8(s_dyn + at, f);
+            put8(s_dyn + D + at, u);
         }
-    } else {
-        for (int64_t at = first; at < end; at += (int64_t)G * R) {
-            Rows q;
-            load(q, at + g, G, end);
-            step(q, at + g, G, end, true);
+        __syncthreads();
+        for (int64_t at = first; at < end; at += G) step(min(at + g, end - 1), at + g < end);
+        over_groups(acc[0]);
+        over_groups(acc[1]);
+        over_groups(acc[2]);
+        if (g == 0) {
+            float* o = sums + blockIdx.x * kSums * (int64_t)D;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (live[c])
+#pragma unroll
+                    for (int k = 0; k < kSums; ++k) put8(o + k * (int64_t)D + col[c], acc[k][c]);
         }
-    }
-    over_groups(acc[0]);
-    over_groups(acc[1]);
-    over_groups(acc[2]);
-    if (g == 0) {
-        float* o = sums + blockIdx.x * kSums * (int64_t)D;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (live[c])
-#pragma unroll
-                for (int k = 0; k < kSums; ++k) put8(o + k * (int64_t)D + col[c], acc[k][c]);
-    }
     }
 }
 
-// Adds up the blocks' sums.  A block takes 64 columns (16 threads of four each) of one
-// sequence and one of its sums, blockIdx.z; 16 slices of the parts are added in LDS.
-//  parts > 0: sums [n][parts][3][D] of n sequences: dshift, dscale, dgate, and per
-//             sequence the gains' shares into `gains` [n][2][D] (n = 1: the gains' gradients)
+// Adds up the blocks' sums.  A block takes 32 columns (8 threads of four each) of one of
+// the sums, blockIdx.z; 32 slices of the parts are added in LDS.
+//  parts > 0: sums [n][parts][3][D] of n sequences: dshift, dscale, dgate.  The gains'
+//             gradients too where the block has all sequences (gridDim.y = 1), else
+//             their shares per sequence, blockIdx.y, into `gains` [n][2][D]
 //  parts = 0: gains [n][2][D] into dnorm_w and dpost_w
-constexpr int kSumSlices = 16;
-__global__ __launch_bounds__(256) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums, int64_t n,
-                                                        int64_t parts, float* gains) {
-    __shared__ float4 s_v[kSumSlices][16];
-    const int q = threadIdx.x & 15, slice = threadIdx.x >> 4;
-    const int col = blockIdx.x * 64 + q * 4;
+constexpr int kSumSlices = 32, kSumQuads = 8;
+// Sequences that a block takes together: their sums wait for one another only at the end
+// (three sequences in one kernel 5.5 us, in two kernels 4.4 each).
+constexpr int kSumSeqs = 4;
+__global__ __launch_bounds__(kSumSlices* kSumQuads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums,
+                                                                          int64_t n, int64_t parts, float* gains) {
+    __shared__ float4 s_v[kSumSeqs][kSumSlices][kSumQuads];
+    const int q = threadIdx.x % kSumQuads, slice = threadIdx.x / kSumQuads;
+    const int col = (blockIdx.x * kSumQuads + q) * 4;
     const bool live = col < a.D;
-    const int64_t D = a.D, b = blockIdx.y;
+    const int64_t D = a.D;
     const int k = blockIdx.z, per = parts ? kSums : 2;
     const int64_t m = parts ? parts : n;
-    const float* p = sums + (parts ? b * parts * per * D : 0) + k * D + (live ? col : 0);
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](const float4& o) {
+    const int seqs = parts && gridDim.y == 1 ? (int)n : 1;
+    auto add = [](float4& v, const float4& o) {
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
         v.w += o.w;
     };
-    constexpr int kFlight = 4;
-    int64_t i = slice;
-    for (; i + (kFlight - 1) * kSumSlices < m; i += kFlight * kSumSlices) {
-        float4 o[kFlight];
+    for (int i = 0; i < seqs; ++i) {
+        const float* p = sums + (parts ? (blockIdx.y + i) * parts * per * D : 0) + k * D + (live ? col : 0);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        constexpr int kFlight = 4;
+        int64_t r = slice;
+        for (; r + (kFlight - 1) * kSumSlices < m; r += kFlight * kSumSlices) {
+            float4 o[kFlight];
 #pragma unroll
-        for (int j = 0; j < kFlight; ++j)
-            o[j] = *reinterpret_cast<const float4*>(p + (i + j * kSumSlices) * per * D);
+            for (int j = 0; j < kFlight; ++j)
+                o[j] = *reinterpret_cast<const float4*>(p + (r + j * kSumSlices) * per * D);
 #pragma unroll
-        for (int j = 0; j < kFlight; ++j) add(o[j]);
+            for (int j = 0; j < kFlight; ++j) add(v, o[j]);
+        }
+        for (; r < m; r += kSumSlices) add(v, *reinterpret_cast<const float4*>(p + r * per * D));
+        s_v[i][slice][q] = v;
     }
-    for (; i < m; i += kSumSlices) add(*reinterpret_cast<const float4*>(p + i * per * D));
-    s_v[slice][q] = v;
     __syncthreads();
-    if (slice || !live) return;
-    for (int w = 1; w < kSumSlices; ++w) add(s_v[w][q]);
+    // one slice's threads for each sequence
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (slice < seqs)
+        for (int w = 0; w < kSumSlices; ++w) add(v, s_v[slice][w][q]);
     auto put = [&](float* to, const float* w, float off, const float4& x) {
         const float4 g = w ? *reinterpret_cast<const float4*>(w) : make_float4(1.0f - off, 1.0f - off, 1.0f - off, 1.0f - off);
         *reinterpret_cast<float4*>(to) =
@@ -396,22 +374,32 @@ __global__ __launch_bounds__(256) void seam_sums_kernel(BlockSeamBackwardArgs a,
     };
     if (!parts) {
         float* to = k ? a.dpost_w : a.dnorm_w;
-        if (to) put(to + col, nullptr, 0.0f, v);
+        if (to && slice == 0 && live) put(to + col, nullptr, 0.0f, v);
         return;
     }
-    const int64_t o = b * D + col;
+    const int64_t b = blockIdx.y + slice, o = b * D + col;
+    const bool mine = slice < seqs && live, scale = k == 1;
     if (k == 0) {
-        if (a.dshift) put(a.dshift + o, nullptr, 0.0f, v);
+        if (a.dshift && mine) put(a.dshift + o, nullptr, 0.0f, v);
         return;
     }
-    const bool scale = k == 1;
-    if (float* to = scale ? a.dscale : a.dgate)
+    if (float* to = scale ? a.dscale : a.dgate; to && mine)
         put(to + o, scale ? (a.norm_w ? a.norm_w + col : nullptr) : a.post && a.post_w ? a.post_w + col : nullptr, 0.0f,
             v);
-    float* to = n > 1 ? gains + (b * 2 + k - 1) * D : scale ? a.dnorm_w : a.dpost_w;
-    if (!to) return;
-    if (scale) put(to + col, a.scale ? a.scale + o : nullptr, 1.0f, v);
-    else put(to + col, a.gate ? a.gate + o : nullptr, 0.0f, v);
+    // the gains' share of the sequence
+    __syncthreads();
+    float* share = gridDim.y > 1 ? gains + (b * 2 + k - 1) * D + col : reinterpret_cast<float*>(&s_v[0][slice][q]);
+    if (mine) {
+        if (scale) put(share, a.scale ? a.scale + o : nullptr, 1.0f, v);
+        else put(share, a.gate ? a.gate + o : nullptr, 0.0f, v);
+    }
+    if (gridDim.y > 1) return;
+    __syncthreads();
+    float* to = scale ? a.dnorm_w : a.dpost_w;
+    if (slice || !live || !to) return;
+    v = s_v[0][0][q];
+    for (int i = 1; i < seqs; ++i) add(v, s_v[0][i][q]);
+    put(to + col, nullptr, 0.0f, v);
 }
 
 __global__ __launch_bounds__(256) void zero_gains_kernel(float* p, float* q, int D) {
@@ -425,36 +413,47 @@ SeamPlan grad_plan(int64_t rows, int64_t D, int64_t seq) {
     return seam_plan(rows, D, seq, kGradBlocks, kGradThreads);
 }
 
-template <typename T, bool kPost, bool kNorm, int L, int C>
-auto grad_kernel(const SeamPlan& p) {
-    return p.whole ? seam_grad_kernel<T, kPost, kNorm, true, L, C> : seam_grad_kernel<T, kPost, kNorm, false, L, C>;
+template <typename T, bool kWhole, int L, int C>
+hipError_t launch_grad_shape(const BlockSeamBackwardArgs& a, const SeamPlan& p, float* sums, hipStream_t s) {
+    const bool norm = a.dh != nullptr, post = a.post && a.y;
+    auto kern = post ? (norm ? seam_grad_kernel<T, true, true, kWhole, L, C> : seam_grad_kernel<T, true, false, kWhole, L, C>)
+                     : (norm ? seam_grad_kernel<T, false, true, kWhole, L, C> : seam_grad_kernel<T, false, false, kWhole, L, C>);
+    const uint32_t lds = grad_lds(p, a.D);
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.row_threads * p.groups), lds, s, a, p, sums);
+    return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch_grad_t(const BlockSeamBackwardArgs& a, hipStream_t s) {
     const SeamPlan p = grad_plan(a.rows, a.D, a.seq);
     float* sums = static_cast<float*>(a.workspace);
-    const bool norm = a.dh != nullptr, post = a.post && a.y;
-    const hipError_t e = with_seam_shape(p, [&](auto l, auto c) {
-        constexpr int L = decltype(l)::value, C = decltype(c)::value;
-        auto kern = post ? (norm ? grad_kernel<T, true, true, L, C>(p) : grad_kernel<T, true, false, L, C>(p))
-                         : (norm ? grad_kernel<T, false, true, L, C>(p) : grad_kernel<T, false, false, L, C>(p));
-        launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.row_threads * p.groups), 0, s, a, p, sums);
-        return hipGetLastError();
-    });
+    const hipError_t e =
+        p.whole ? with_seam_shape(p, [&](auto l, auto c) {
+            return launch_grad_shape<T, true, decltype(l)::value, decltype(c)::value>(a, p, sums, s);
+        })
+                : with_seam_shape(p, [&](auto l, auto c) {
+                      return launch_grad_shape<T, false, decltype(l)::value, decltype(c)::value>(a, p, sums, s);
+                  });
     if (e != hipSuccess || !(a.dgate || a.dshift || a.dscale || a.dnorm_w || a.dpost_w)) return e;
     const int64_t n = a.rows / a.seq;
-    const unsigned cols = (unsigned)((a.D + 63) / 64);
-    float* gains = sums;
-    int64_t ng = p.blocks;
-    if (!p.whole) {
-        gains = sums + p.blocks * kSums * a.D;
-        ng = n;
-        launch_kernel(seam_sums_kernel, dim3(cols, (unsigned)n, kSums), dim3(256), 0, s, a, (const float*)sums, n,
-                      p.parts, gains);
+    const unsigned cols = (unsigned)((a.D + 4 * kSumQuads - 1) / (4 * kSumQuads));
+    const dim3 block(kSumSlices * kSumQuads);
+    if (p.whole) {  // each block's shares of the gains
+        if (a.dnorm_w || a.dpost_w)
+            launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), block, 0, s, a, (const float*)sums, p.blocks, (int64_t)0,
+                          (float*)nullptr);
+        return hipGetLastError();
     }
-    if ((p.whole || n > 1) && (a.dnorm_w || a.dpost_w))
-        launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), dim3(256), 0, s, a, (const float*)gains, ng, (int64_t)0,
+    float* gains = sums + p.blocks * kSums * a.D;
+    const bool together = n <= kSumSeqs;
+    launch_kernel(seam_sums_kernel, dim3(cols, together ? 1 : (unsigned)n, kSums), block, 0, s, a, (const float*)sums, n,
+                  p.parts, gains);
+    if (!together && (a.dnorm_w || a.dpost_w))
+        launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), block, 0, s, a, (const float*)gains, n, (int64_t)0,
                       (float*)nullptr);
     return hipGetLastError();
 }

@@ -256,10 +256,15 @@ def _param(t, like: torch.Tensor, shape: tuple, what: str):
     return t.to(device=like.device, dtype=torch.float32).contiguous()
 
 
+# the handle of a device's current stream, without making a Stream object where torch can
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn, on: torch.Tensor, *args) -> None:
     """fn(*args, stream): the current stream of `on`'s device, with that device current."""
-    index = on.device.index
-    stream = torch.cuda.current_stream(index).cuda_stream
+    index = on.get_device()
+    stream = _raw_stream(index)
     if index == torch.cuda.current_device():
         rc = fn(*args, stream)
     else:
