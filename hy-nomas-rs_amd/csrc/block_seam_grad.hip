@@ -349,17 +349,17 @@ __global__ __launch_bounds__(kSumSlices* kSumQuads) void seam_sums_kernel(BlockS
     for (int i = 0; i < seqs; ++i) {
         const float* p = sums + (parts ? (blockIdx.y + i) * parts * per * D : 0) + k * D + (live ? col : 0);
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        constexpr int kFlight = 4;
-        int64_t r = slice;
-        for (; r + (kFlight - 1) * kSumSlices < m; r += kFlight * kSumSlices) {
+        // (unconditional loads, past the end of the last row: all of a flight at once)
+        constexpr int kFlight = 8;
+        for (int64_t r = slice; r < m; r += kFlight * kSumSlices) {
             float4 o[kFlight];
 #pragma unroll
             for (int j = 0; j < kFlight; ++j)
-                o[j] = *reinterpret_cast<const float4*>(p + (r + j * kSumSlices) * per * D);
+                o[j] = *reinterpret_cast<const float4*>(p + min(r + j * kSumSlices, m - 1) * per * D);
 #pragma unroll
-            for (int j = 0; j < kFlight; ++j) add(v, o[j]);
+            for (int j = 0; j < kFlight; ++j)
+                if (r + j * kSumSlices < m) add(v, o[j]);
         }
-        for (; r < m; r += kSumSlices) add(v, *reinterpret_cast<const float4*>(p + r * per * D));
         s_v[i][slice][q] = v;
     }
     __syncthreads();

@@ -122,7 +122,15 @@ __device__ __forceinline__ double lanes_addd(double v) {
     return v;
 }
 
-// Floats in the order of their values as integers (-inf first), and back.
+// What the wave's lanes have written to LDS is there for all of them: LDS takes a
+// wave's operations in order, so this only keeps the compiler from moving them.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Floats in the order of their values as integers (-inf first; not for -0), and back.
 __device__ __forceinline__ int ordered(float v) {
     const int b = __float_as_int(v);
     return b ^ ((b >> 31) & 0x7fffffff);
@@ -291,7 +299,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 all += raw[j];
-                key[j] = ordered(raw[j]);
+                key[j] = ordered(raw[j] + 0.0f);  // (-0 is 0)
                 if constexpr (kUnique)
                     key[j] = raw[j] == -INFINITY ? kNone
                                                  : (key[j] >> RouteKey<T, kKeys>::kDrop) * kMaxRouteExperts +
@@ -354,8 +362,11 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                 kept &= ahead < a.top_groups;
                 const float low = -lanes_maxf<L>(kept ? -score : -INFINITY);
                 const float high = lanes_maxf<L>(kept || !in_group ? -INFINITY : score);
-                const bool doubt = high != -INFINITY && low < INFINITY &&
-                                   !(low - high > 4.0f * (near + 0x1p-22f * fabsf(high)));
+                // two keys' errors on either side; a key's grows with it, not with the sum
+                const float size = fabsf(m1) + (m2 == -INFINITY ? 0.0f : fabsf(m2));
+                const float most = lanes_maxf<L>(in_group && size < INFINITY ? size : 0.0f);
+                const bool doubt =
+                    high != -INFINITY && low < INFINITY && !(low - high > 4.0f * near + 0x1p-21f * most);
                 if (__ballot(doubt)) {
                     sum64();
                     // those that may be among the group's largest
@@ -466,14 +477,15 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             next = lanes_max<L>(next);
             const float edge = unordered(border);
             const float off = 2.0f * (near + 0x1p-22f * fabsf(edge));
-            const bool doubt = border != kNone && edge < INFINITY && next != kNone &&
-                               (by_index || !(edge - unordered(next) > off));
+            const bool doubt = border != kNone && edge < INFINITY &&
+                               (by_index || (next != kNone && !(edge - unordered(next) > off)));
             if (__ballot(doubt)) {
                 unsigned ties = 0, sure = 0;  // the doubtful ones, and those ahead of them
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    ties |= (unsigned)(fabsf(unordered(key[j]) - edge) <= off) << j;
-                    sure |= (unsigned)(unordered(key[j]) > edge + off) << j;
+                    const bool tie = fabsf(unordered(key[j]) - edge) <= off;
+                    ties |= (unsigned)tie << j;
+                    sure |= (unsigned)(key[j] > border && !tie) << j;
                 }
                 if (!doubt) ties = 0;
                 int places = doubt ? k - lanes_add<L>(__popc(sure)) : 0;
@@ -551,7 +563,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
         int place = upto - own;
         for (unsigned m = chosen; m; m &= m - 1, ++place)
             if (place < k) s_idx[place] = first + __ffs(m) - 1;
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         // lane t of the row: slot t
         auto score = [&](int e) {
             const float v = Elt<T>::to_f32(l[e]);
@@ -580,7 +592,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             a.w[row * k + t] = e >= 0 ? up * s : 0.0f;
             if (hist && e >= 0) atomicAdd(&s_hist[e], 1);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
     if (!hist) return;
     __syncthreads();
@@ -688,14 +700,14 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
             sum += w;
             dot += d * w;
             some |= e >= 0;
-            if (e >= 0) reinterpret_cast<int*>(s_row)[e] = t;
+            if (e >= 0) s_row[e] = (float)t;  // (who is there: an expert named twice has another slot)
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         for (int t = p; t < k; t += L) {
             const int e = t < L ? e0 : idx[t];
-            if (e >= 0 && e < E) twice |= reinterpret_cast<int*>(s_row)[e] != t;
+            if (e >= 0 && e < E) twice |= s_row[e] != (float)t;
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         sum = lanes_addf<L>(sum);
         dot = lanes_addf<L>(dot);
         float mean = 0.0f, up = 0.0f, inner = 0.0f;
@@ -716,7 +728,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
                 }
                 *reinterpret_cast<float4*>(s_row + (c * L + p) * W + i) = b;
             }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         const bool again = __ballot(twice) != 0;
         for (int t = p; t < k; t += L) {
             int e;
@@ -731,7 +743,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
             }
             s_row[e] = slope * (kSigmoid ? ds : ds - inner);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
         T* out = static_cast<T*>(a.dlogits) + row * E;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -754,7 +766,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
                     if (at + i < E) out[at + i] = Elt<T>::from_f32(v[i]);
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
 }
 
@@ -791,9 +803,10 @@ hipError_t launch_route_backward_t(const RouteBackwardArgs& a, hipStream_t s) {
 __global__ __launch_bounds__(kRouteThreads) void given_kernel(GivenRoutingArgs a) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     const int k = a.k, ks = a.k_slots, n = kRouterRows * k;
-    int* s_e = reinterpret_cast<int*>(s_raw);           // [64 k] expert, -1 where none or named before
+    int* s_e = reinterpret_cast<int*>(s_raw);           // [64 k] expert, -1 where none
     float* s_w = reinterpret_cast<float*>(s_e + n);     // [64 k]
-    int* s_hist = reinterpret_cast<int*>(s_w + n);      // [E_cols]
+    int* s_first = reinterpret_cast<int*>(s_w + n);     // [64 k] expert, -1 where named before too
+    int* s_hist = s_first + n;                          // [E_cols]
     const int tid = threadIdx.x;
     const int64_t row0 = (int64_t)blockIdx.x * kRouterRows;
     const int nrows = (int)min<int64_t>(kRouterRows, a.rows - row0);
@@ -805,24 +818,22 @@ __global__ __launch_bounds__(kRouteThreads) void given_kernel(GivenRoutingArgs a
     }
     __syncthreads();
     for (int i = tid; i < nrows * k; i += kRouteThreads) {
-        const int r = i / k, e = s_e[i];
-        const int* re = s_e + r * k;
+        const int r = i / k * k, e = s_e[i];
+        bool first = e >= 0;
+        for (int t = r; t < i; ++t) first &= s_e[t] != e;
+        s_first[i] = first ? e : -1;
+    }
+    __syncthreads();
+    for (int i = tid; i < nrows * k; i += kRouteThreads) {
+        const int r = i / k, e = s_first[i];
         if (e < 0) continue;
-        // its place: distinct experts below it; a later mention adds its weight
+        // its place: the experts below it; later mentions add their weights
         int at = 0;
-        bool first = true;
         float w = 0.0f;
-        for (int t = 0; t < k; ++t) {
-            if (re[t] == e) {
-                if (r * k + t < i) first = false;
-                w += s_w[r * k + t];
-            } else if (re[t] >= 0 && re[t] < e) {
-                bool again = false;
-                for (int u = 0; u < t; ++u) again |= re[u] == re[t];
-                at += !again;
-            }
+        for (int t = r * k; t < r * k + k; ++t) {
+            at += s_first[t] >= 0 && s_first[t] < e;
+            if (s_e[t] == e) w += s_w[t];
         }
-        if (!first) continue;
         a.idx[(row0 + r) * ks + at] = e;
         a.w[(row0 + r) * ks + at] = w;
         atomicAdd(&s_hist[e], 1);
@@ -830,11 +841,7 @@ __global__ __launch_bounds__(kRouteThreads) void given_kernel(GivenRoutingArgs a
     // the empty slots (the dense slot, where there is one, comes last of those taken)
     for (int r = tid; r < nrows; r += kRouteThreads) {
         int live = 0;
-        for (int t = 0; t < k; ++t) {
-            bool again = s_e[r * k + t] < 0;
-            for (int u = 0; u < t; ++u) again |= s_e[r * k + u] == s_e[r * k + t];
-            live += !again;
-        }
+        for (int t = 0; t < k; ++t) live += s_first[r * k + t] >= 0;
         const int64_t o = (row0 + r) * ks;
         if (ks > k) {
             a.idx[o + live] = a.E;
@@ -930,7 +937,7 @@ hipError_t launch_route_backward(DType dt, const RouteBackwardArgs& a, hipStream
 }
 
 hipError_t launch_given_routing(const GivenRoutingArgs& a, hipStream_t s) {
-    const size_t lds = (size_t)kRouterRows * a.k * 8 + (size_t)a.E_cols * 4;
+    const size_t lds = (size_t)kRouterRows * a.k * 12 + (size_t)a.E_cols * 4;
     if (a.rows < 1 || a.k < 1 || a.k > a.E || lds > 160 * 1024) return hipErrorInvalidValue;
     const hipError_t e = hipFuncSetAttribute((const void*)given_kernel,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -239,7 +239,7 @@ _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 def _same(t: torch.Tensor, like: torch.Tensor, what: str) -> torch.Tensor:
     """A second tensor of the activations' shape, dtype and device, contiguous."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != like.shape or t.dtype is not like.dtype or t.device != like.device:
         raise NomasError(2, f"{what}: expected {tuple(like.shape)} {like.dtype} on {like.device}, "
                             f"got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.contiguous()
@@ -249,7 +249,7 @@ def _param(t, like: torch.Tensor, shape: tuple, what: str):
     """A parameter as contiguous f32 on the activations' device (None stays None)."""
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise NomasError(2, f"{what}: expected {shape}, got {tuple(t.shape)}")
     if t.dtype is torch.float32 and t.device == like.device and t.is_contiguous():
         return t
@@ -293,10 +293,10 @@ def block_seam(x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor | None = Non
     xc = _seam_input(x)
     yc = _same(y, xc, "y")
     B, S, D = xc.shape
-    gate, shift, scale = (_param(t, xc, (B, D), n) for t, n in
-                          ((gate, "gate"), (shift, "shift"), (scale, "scale")))
-    norm_w, post_w = _param(norm_w, xc, (D,), "norm_w"), _param(post_w, xc, (D,), "post_w")
-    if not norm and any(t is not None for t in (h, shift, scale, norm_w)):
+    gate, shift = _param(gate, xc, (B, D), "gate"), _param(shift, xc, (B, D), "shift")
+    scale, norm_w = _param(scale, xc, (B, D), "scale"), _param(norm_w, xc, (D,), "norm_w")
+    post_w = _param(post_w, xc, (D,), "post_w")
+    if not norm and not (h is shift is scale is norm_w is None):
         raise NomasError(2, "h, shift, scale and norm_w need norm=True")
     if post_w is not None and not post_norm:
         raise NomasError(2, "post_w needs post_norm=True")

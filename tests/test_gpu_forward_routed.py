@@ -117,8 +117,9 @@ def test_a_wide_output_past_the_last_level_cache():
     assert rel_err(got.float().cpu().numpy()[sel], want) <= TOL["bf16"]
 
 
-def test_many_experts_and_slots():
-    rows, D, E, k, H = 150, 64, 256, 20, 32
+@pytest.mark.parametrize("k", [20, 136])  # 136: the most that 256 experts allow
+def test_many_experts_and_slots(k):
+    rows, D, E, H = 150, 64, 256, 32
     layer, x, xm, p, _ = case(rows, D, E, k, H, "bf16", 59)
     g = np.random.default_rng(60)
     idx = g.permuted(np.tile(np.arange(E), (rows, 1)), axis=1)[:, :k].astype(np.int32)

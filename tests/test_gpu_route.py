@@ -95,6 +95,40 @@ def test_near_ties_are_decided_in_64_bits():
             check(l, k, scoring=scoring, bias=bias, groups=G, top_groups=4 if G > 1 else 1)
 
 
+def test_signed_zeros_tie():
+    for dtype in ("f32", "bf16", "f16"):
+        l = torch.zeros(30, 40, dtype=ref.TORCH[dtype])
+        l[torch.from_numpy(np.random.default_rng(12).random((30, 40)) < 0.5)] = -0.0
+        for bias in (None, torch.zeros(40), -torch.zeros(40)):
+            for k in (3, 20):
+                idx, _ = check(l, k, bias=bias)
+                assert (idx.cpu() == torch.arange(k)).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_large_biases_near_ties(scoring):
+    # f32 sums of score and bias have lost what decides: keys around +-1000, groups whose
+    # two best cancel, and differences in the scores alone
+    T, E, G = 64, 64, 8
+    g = np.random.default_rng(19)
+    l = torch.from_numpy((0.001 * g.standard_normal((T, E))).astype(np.float32))
+    bias = torch.full((E,), -1000.0)
+    bias[::8] = 1000.0
+    check(l, 6, scoring=scoring, bias=bias, groups=G, top_groups=3)
+    check(l, 12, scoring=scoring, bias=bias)
+    check(l, 30, scoring=scoring, bias=torch.full((E,), 4096.0))
+
+
+def test_scores_that_saturate():
+    # equal in f32 (0 or 1), not in 64 bits
+    l = torch.linspace(18, 30, 48).repeat(20, 1)
+    l = l.gather(1, torch.from_numpy(np.random.default_rng(20).permuted(np.tile(np.arange(48), (20, 1)), axis=1)))
+    for bias in (torch.zeros(48), torch.full((48,), 0.25)):
+        check(l, 7, scoring="sigmoid", bias=bias, groups=4, top_groups=2)
+        check(-l, 7, scoring="sigmoid", bias=torch.zeros(48))
+        check(l * 8 - 200, 7, scoring="softmax", bias=torch.zeros(48))
+
+
 @pytest.mark.parametrize("E,G", [(8, 1), (40, 4), (64, 8), (256, 8), (300, 1)])
 def test_masked_experts_and_rows(E, G):
     for dtype in ("f32", "f16"):
@@ -275,3 +309,75 @@ def test_in_place_gradient_graph_and_streams():
     assert rc == 0
     l2 = keep.flip(0)  # (the last replay's)
     assert torch.equal(l, nm.route_backward(l2, idx, dw, scoring="sigmoid"))
+
+
+def test_two_streams_at_once():
+    l = [logits_of(4000, 128, 30 + i, "f32").cuda() for i in range(2)]
+    b = torch.linspace(-0.1, 0.1, 128, device="cuda")
+    want = [nm.route(x, 6, scoring="sigmoid", bias=b) for x in l]
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for x, st in zip(l, s):
+            with torch.cuda.stream(st):
+                got.append(nm.route(x, 6, scoring="sigmoid", bias=b))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for u, v in zip(got, want) for p, q in zip(u, v))
+
+
+def test_gradient_of_repeated_experts_has_the_same_bits():
+    l = logits_of(64, 32, 33, "f32").cuda()
+    idx = torch.from_numpy(np.random.default_rng(34).integers(0, 4, (64, 16)).astype(np.int32)).cuda()
+    dw = torch.randn(64, 16, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    for scoring in ("softmax", "sigmoid"):
+        want = nm.route_backward(l, idx, dw, scoring=scoring)
+        check_grad(l.cpu(), idx.cpu(), dw.cpu(), "f32", scoring=scoring)
+        assert all(torch.equal(nm.route_backward(l, idx, dw, scoring=scoring), want) for _ in range(3))
+
+
+def plain_choice(l, k, scoring, bias, groups, top_groups, group_top):
+    """The choice in f64 torch operations, for many rows at once."""
+    T, E = l.shape
+    s = torch.sigmoid(l.double()) if scoring == "sigmoid" else torch.softmax(l.double(), -1)
+    key = l.double() if bias is None and groups == 1 else s if bias is None else s + bias.double()
+    out = l == -float("inf")
+    key = key.masked_fill(out, -float("inf"))
+    if groups > 1:
+        best = key.view(T, groups, -1).sort(-1, descending=True).values[..., :group_top]
+        score = best.masked_fill(best == -float("inf"), 0).sum(-1)
+        score = score.masked_fill(best[..., 0] == -float("inf"), -float("inf"))
+        kept = score.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        keep = torch.zeros(T, groups, dtype=torch.bool, device=l.device).scatter_(1, kept, True)
+        key = key.masked_fill(~keep.repeat_interleave(E // groups, 1), -float("inf"))
+    top = key.sort(dim=-1, descending=True, stable=True)
+    idx = top.indices[:, :k].masked_fill(top.values[:, :k] == -float("inf"), E).sort(-1).values
+    return idx.masked_fill(idx == E, -1).int()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_crowded_borders(seed):
+    # logits and biases of few levels, a few of them moved by an f32 step or so: ties and
+    # near ties at the borders of experts and groups in most rows
+    g = np.random.default_rng(1000 + seed)
+    G = int(g.choice([1, 1, 2, 4, 5, 8, 16]))
+    E = G * int(g.integers(2, max(3, min(600, 1024) // G)))
+    tg = int(g.integers(1, G + 1))
+    k = int(min(g.choice([1, 2, 4, 8, 8, 12, 16, 17, 40]), E // G * tg))
+    T = int(g.choice([7, 300, 3000]))
+    levels = int(g.choice([2, 5, 40, 400]))
+    l = torch.from_numpy((g.integers(-levels, levels + 1, (T, E)) * (3.0 / levels)).astype(np.float32))
+    moved = torch.from_numpy(g.random((T, E)) < 0.2)
+    l = torch.where(moved, l * (1 + 2.0 ** -22 * torch.from_numpy(g.integers(-2, 3, (T, E)).astype(np.float32))), l)
+    l[torch.from_numpy(g.random((T, E)) < 0.05)] = -float("inf")
+    l = l.to(ref.TORCH[str(g.choice(["f32", "f32", "bf16", "f16"]))]).cuda()
+    bias = [None, torch.zeros(E), torch.from_numpy((g.integers(-3, 4, E) * 0.05).astype(np.float32)),
+            torch.from_numpy((100 * g.standard_normal(E)).astype(np.float32))][int(g.integers(4))]
+    bias = None if bias is None else bias.cuda()
+    for scoring in ("sigmoid", "softmax"):
+        for top in (1, 2):
+            idx, w, counts = nm.route(l, k, scoring=scoring, bias=bias, groups=G, top_groups=tg, group_top=top)
+            want = plain_choice(l, k, scoring, bias, G, tg, top)
+            bad = (idx != want).any(1).nonzero().flatten()
+            assert not bad.numel(), (E, G, tg, k, levels, scoring, top, int(bad[0]), idx[bad[0]], want[bad[0]])
+            assert torch.equal(counts, torch.bincount(want[want >= 0], minlength=E).int())
