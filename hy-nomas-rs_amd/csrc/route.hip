@@ -43,18 +43,20 @@ constexpr int64_t kRouteWavesMin = 1024;  // a wave for each SIMD
 
 // ---- sums, extremes and scans over a row's L neighbouring lanes ------------------
 
+// Another lane's v (0 where there is none): in a form that the instruction that uses it
+// takes as its operand.
 template <int kCtrl>
-__device__ __forceinline__ int dpp_mov(int v, int old) {
-    return __builtin_amdgcn_update_dpp(old, v, kCtrl, 0xf, 0xf, false);
+__device__ __forceinline__ int dpp_mov(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, kCtrl, 0xf, 0xf, true);
 }
 // Combines each lane's v with those of the other lanes of its row, by `f`, in all of them.
 template <int L, typename F>
 __device__ __forceinline__ int over_lanes(int v, F f) {
     static_assert(L >= 8, "lanes of a row");
-    v = f(v, dpp_mov<0xb1>(v, v));     // lane ^ 1
-    v = f(v, dpp_mov<0x4e>(v, v));     // lane ^ 2
-    v = f(v, dpp_mov<0x141>(v, v));    // the other four of eight
-    if constexpr (L >= 16) v = f(v, dpp_mov<0x140>(v, v));  // the other eight of sixteen
+    v = f(v, dpp_mov<0xb1>(v));     // lane ^ 1
+    v = f(v, dpp_mov<0x4e>(v));     // lane ^ 2
+    v = f(v, dpp_mov<0x141>(v));    // the other four of eight
+    if constexpr (L >= 16) v = f(v, dpp_mov<0x140>(v));  // the other eight of sixteen
     if constexpr (L >= 32) {
         const auto s = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
         v = f((int)s[0], (int)s[1]);
@@ -94,8 +96,8 @@ template <int L>
 __device__ __forceinline__ int lanes_scan(int v, int p) {
 #pragma unroll
     for (int o = 1; o < (L < 16 ? L : 16); o <<= 1) {  // row_shr: o
-        const int t = o == 1 ? dpp_mov<0x111>(v, 0) : o == 2 ? dpp_mov<0x112>(v, 0) : o == 4 ? dpp_mov<0x114>(v, 0)
-                                                                                     : dpp_mov<0x118>(v, 0);
+        const int t = o == 1 ? dpp_mov<0x111>(v) : o == 2 ? dpp_mov<0x112>(v) : o == 4 ? dpp_mov<0x114>(v)
+                                                                                     : dpp_mov<0x118>(v);
         v += L < 16 && p < o ? 0 : t;
     }
     if constexpr (L >= 32) v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast: 15
@@ -332,21 +334,21 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
             if (a.bias) s += (double)a.bias[e];
             return s == s ? s : (double)INFINITY;
         };
-        // the lane's largest keys in descending order
-        int list[kList];
-#pragma unroll
-        for (int i = 0; i < kList; ++i) list[i] = kNone;
+        // the lane's largest keys in descending order (in four variables: of an array the
+        // compiler makes selections by index, twice the instructions of a round)
+        int t0 = kNone, t1 = kNone, t2 = kNone, t3 = kNone;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-#pragma unroll
-            for (int i = kList - 1; i > 0; --i) list[i] = middle(list[i], list[i - 1], key[j]);
-            list[0] = max(list[0], key[j]);
+            t3 = middle(t3, t2, key[j]);
+            t2 = middle(t2, t1, key[j]);
+            t1 = middle(t1, t0, key[j]);
+            t0 = max(t0, key[j]);
         }
         bool kept = in_group;
         if constexpr (kKeys) {
             if (a.groups > 1) {
                 // the group's two largest, over its lanes
-                int i1 = list[0], i2 = list[1];
+                int i1 = t0, i2 = t1;
                 for (int o = 1; o < sh.lanes; o <<= 1) {
                     const int o1 = __shfl_xor(i1, o), o2 = __shfl_xor(i2, o);
                     i2 = max(max(i2, o2), min(i1, o1));
@@ -396,8 +398,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                     if (doubt) kept = ahead < a.top_groups && in_group;
                 }
                 if (!kept) {
-#pragma unroll
-                    for (int i = 0; i < kList; ++i) list[i] = kNone;
+                    t0 = t1 = t2 = t3 = kNone;
 #pragma unroll
                     for (int j = 0; j < V; ++j) key[j] = kNone;
                 }
@@ -407,11 +408,12 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
         int border = kNone;  // chosen: the keys at or above it, but for kNone
         if (k <= kRounds) {
             for (int i = 0; i < k; ++i) {
-                border = lanes_max<L>(list[0]);
-                const bool off = list[0] == border;
-#pragma unroll
-                for (int q = 0; q < kList; ++q)
-                    list[q] = off ? (q + 1 < kList ? list[min(q + 1, kList - 1)] : kNone) : list[q];
+                border = lanes_max<L>(t0);
+                const bool off = t0 == border;
+                t0 = off ? t1 : t0;
+                t1 = off ? t2 : t1;
+                t2 = off ? t3 : t2;
+                t3 = off ? kNone : t3;
             }
         }
         auto bits = [&](int from) {  // of the lane's keys at or above `from`
@@ -469,7 +471,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
         }
         if constexpr (kKeys) {
             // the largest key that is left out: near the border?
-            int next = k <= kRounds ? list[0] : kNone;
+            int next = k <= kRounds ? t0 : kNone;
             if (__ballot(own >= kList || !found_it)) {  // (the list may have ended before it)
 #pragma unroll
                 for (int j = 0; j < V; ++j) next = max(next, (chosen >> j) & 1 ? kNone : key[j]);
