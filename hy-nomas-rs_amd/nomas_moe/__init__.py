@@ -339,33 +339,37 @@ def block_seam_backward(dout: torch.Tensor | None, dh: torch.Tensor | None,
         raise NomasError(2, "gate needs y")
     if dh is None and (scale is not None or norm_w is not None):
         raise NomasError(2, "scale and norm_w need dh")
-    dout, dh, y = (None if t is None else _same(t, first, n) for t, n in
-                   ((dout, "dout"), (dh, "dh"), (y, "y")))
+    dout = None if dout is None else _same(dout, first, "dout")
+    dh = None if dh is None else _same(dh, first, "dh")
+    y = None if y is None else _same(y, first, "y")
     out = None if dh is None else _same(out, first, "out")
     gate, scale = _param(gate, first, (B, D), "gate"), _param(scale, first, (B, D), "scale")
     norm_w, post_w = _param(norm_w, first, (D,), "norm_w"), _param(post_w, first, (D,), "post_w")
     got = {"dx": torch.empty_like(first)}
     if y is not None:
         got["dy"] = torch.empty_like(first)
-    # the f32 gradients in one allocation, each at a multiple of 16 bytes
-    names = (["dgate"] if y is not None else []) + (["dshift", "dscale"] if dh is not None else [])
-    gains = (["dpost_w"] if post_norm else []) + (["dnorm_w"] if dh is not None else [])
-    make = torch.zeros if S == 0 else torch.empty
-    flat = make((len(names) * B + len(gains)) * D, dtype=torch.float32, device=first.device)
-    for i, n in enumerate(names):
-        got[n] = flat[i * B * D:(i + 1) * B * D].view(B, D)
-    for i, n in enumerate(gains):
-        got[n] = flat[(len(names) * B + i) * D:(len(names) * B + i + 1) * D]
+    # the f32 gradients in one allocation
+    names = (("dgate",) if y is not None else ()) + (("dshift", "dscale") if dh is not None else ())
+    gains = (("dpost_w",) if post_norm else ()) + (("dnorm_w",) if dh is not None else ())
+    L = _lib.lib()
+    need = L.nomas_block_seam_workspace(B * S, D, max(S, 1))
+    ends = (len(names) * B + len(gains)) * D  # (a multiple of 8 floats)
+    flat = torch.empty(ends, dtype=torch.float32, device=first.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
+    at, ptr = 0, {}
+    base = flat.data_ptr()
+    for n in names:
+        got[n], ptr[n], at = flat[at:at + B * D].view(B, D), base + 4 * at, at + B * D
+    for n in gains:
+        got[n], ptr[n], at = flat[at:at + D], base + 4 * at, at + D
     if first.numel() == 0:
         return {k: v.zero_() for k, v in got.items()}
-    L = _lib.lib()
-    need = L.nomas_block_seam_workspace(B * S, D, S)
-    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
+    p = ptr.get
     _call(L.nomas_block_seam_backward, first, _CODES[first.dtype], _ptr(dout), _ptr(dh), _ptr(out),
           _ptr(y), got["dx"].data_ptr(), _ptr(got.get("dy")), B * S, D, S, _ptr(gate),
           int(post_norm), _ptr(post_w), float(residual_scale), _ptr(norm_w), _ptr(scale),
-          float(eps), _ptr(got.get("dgate")), _ptr(got.get("dshift")), _ptr(got.get("dscale")),
-          _ptr(got.get("dnorm_w")), _ptr(got.get("dpost_w")), ws.data_ptr(), need)
+          float(eps), p("dgate"), p("dshift"), p("dscale"), p("dnorm_w"), p("dpost_w"),
+          ws.data_ptr(), need)
     return got
 
 
