@@ -333,7 +333,7 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
 //  parts = 0: gains [n][2][D] into dnorm_w and dpost_w
 constexpr int kSumSlices = 32, kSumQuads = 8;
 // Sequences that a block takes together: their sums wait for one another only at the end
-// (three sequences in one kernel 5.5 us, in two kernels 4.4 each).
+// (three sequences in one kernel 6.3 us, in two kernels 4.5 each).
 constexpr int kSumSeqs = 4;
 __global__ __launch_bounds__(kSumSlices* kSumQuads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums,
                                                                           int64_t n, int64_t parts, float* gains) {

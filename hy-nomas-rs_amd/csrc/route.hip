@@ -282,7 +282,8 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
         float all = 0.0f;   // a NaN if a key is one
         if constexpr (kKeys) {
             // Errors of s, in half steps of f32: sigmoid, s (1 - s) (1.5 |l| + 2) + 3 s < 4;
-            // softmax, of 1 / Z at most: 2.5 |l - top| exp(l - top) + 2, and Z's own, below 30
+            // softmax, times 1 / Z: 2.5 |l - top| exp(l - top) + 2 < 3, and Z's own, at most
+            // 2.5 ln E + 2 of its terms and 37 of their sum
             float s[V];
             if (a.sigmoid) {
                 near = 0x1p-21f;
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                     s[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(raw[j] * -kLog2e));
             } else {
                 const float zi = 1.0f / zsum;
-                near = 0x1p-19f * zi;
+                near = 0x1p-18f * zi;
 #pragma unroll
                 for (int j = 0; j < V; ++j) s[j] = __builtin_amdgcn_exp2f((raw[j] - top) * kLog2e) * zi;
             }

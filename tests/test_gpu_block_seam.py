@@ -48,7 +48,7 @@ def check(t, dtype, post, alpha, drop=()):
 SHAPES = [
     (1, 1, 8), (1, 3, 16), (5, 1, 64), (2, 150, 256), (3, 7, 264), (1, 70, 1000), (4, 33, 512),
     (2, 19, 520), (1, 40, 2048), (7, 2, 1032), (1, 9, 4104), (2, 5, 8192), (1, 3, 8200), (1, 2, 16384), (300, 1, 128),
-    (2, 700, 64),
+    (2, 700, 64), (1, 13, 16384), (2, 9, 12296), (5, 60, 768), (6, 100, 1536),
 ]
 
 
@@ -239,6 +239,41 @@ def test_same_bits_again_in_place_and_captured():
                                      ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     assert torch.equal(t["dh"], want["dx"]) and torch.equal(t["y"], want["dy"]) and torch.equal(dg, want["dgate"])
+
+
+def test_two_streams_at_once():
+    t = [{k: dev(v) for k, v in inputs(2, 500, 640, "bf16", 40 + i, NAMES).items()} for i in range(2)]
+
+    def call(u):
+        o, h = nm.block_seam(u["dout"], u["y"], u["gate"], u["shift"], u["scale"], post_norm=True)
+        g = nm.block_seam_backward(u["dout"], u["dh"], u["out"], u["y"], u["gate"], u["scale"], post_norm=True)
+        return [o, h] + [g[k] for k in sorted(g)]
+
+    want = [call(u) for u in t]
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for u, st in zip(t, s):
+            with torch.cuda.stream(st):
+                got.append(call(u))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+def test_strided_inputs_and_parameters_of_other_types():
+    # the AdaLN chunks of one tensor, activations with a stride, 16-bit gains
+    B, S, D = 2, 30, 96
+    t = inputs(B, S, D, "bf16", 50)
+    six = torch.cat([t["gate"], t["shift"], t["scale"]], 1).cuda()
+    gate, shift, scale = six.chunk(3, 1)
+    wide = torch.empty(B, S, 2 * D, dtype=torch.bfloat16, device="cuda")
+    wide[..., :D], wide[..., D:] = t["x"].cuda(), t["y"].cuda()
+    w16 = t["norm_w"].bfloat16().cuda()
+    got = nm.block_seam(wide[..., :D], wide[..., D:], gate, shift, scale, norm_w=w16)
+    want = nm.block_seam(t["x"].cuda(), t["y"].cuda(), t["gate"].cuda(), t["shift"].cuda(), t["scale"].cuda(),
+                         norm_w=w16.float())
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
 def test_empty_batches():
