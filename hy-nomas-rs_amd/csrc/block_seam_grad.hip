@@ -326,18 +326,19 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
 }
 
 // Adds up the blocks' sums.  A block takes 32 columns (8 threads of four each) of one of
-// the sums, blockIdx.z; 32 slices of the parts are added in LDS.
+// the sums, blockIdx.z, in 64 slices of the parts: eight of a wave are added in
+// registers, the waves' in LDS.
 //  parts > 0: sums [n][parts][3][D] of n sequences: dshift, dscale, dgate.  The gains'
 //             gradients too where the block has all sequences (gridDim.y = 1), else
 //             their shares per sequence, blockIdx.y, into `gains` [n][2][D]
 //  parts = 0: gains [n][2][D] into dnorm_w and dpost_w
-constexpr int kSumSlices = 32, kSumQuads = 8;
-// Sequences that a block takes together: their sums wait for one another only at the end
-// (three sequences in one kernel 6.3 us, in two kernels 4.5 each).
+constexpr int kSumSlices = 64, kSumQuads = 8, kSumThreads = kSumSlices * kSumQuads;
+// Sequences that a block takes together: their sums wait for one another only at the end.
 constexpr int kSumSeqs = 4;
-__global__ __launch_bounds__(kSumSlices* kSumQuads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums,
-                                                                          int64_t n, int64_t parts, float* gains) {
-    __shared__ float4 s_v[kSumSeqs][kSumSlices][kSumQuads];
+__global__ __launch_bounds__(kSumThreads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums, int64_t n,
+                                                                int64_t parts, float* gains) {
+    constexpr int kWaves = kSumThreads / kWave;
+    __shared__ float4 s_v[kSumSeqs][kWaves][kSumQuads];
     const int q = threadIdx.x % kSumQuads, slice = threadIdx.x / kSumQuads;
     const int col = (blockIdx.x * kSumQuads + q) * 4;
     const bool live = col < a.D;
@@ -351,60 +352,78 @@ __global__ __launch_bounds__(kSumSlices* kSumQuads) void seam_sums_kernel(BlockS
         v.z += o.z;
         v.w += o.w;
     };
-    for (int i = 0; i < seqs; ++i) {
-        const float* p = sums + (parts ? (blockIdx.y + i) * parts * per * D : 0) + k * D + (live ? col : 0);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        // (unconditional loads, past the end of the last row: all of a flight at once)
-        constexpr int kFlight = 8;
-        for (int64_t r = slice; r < m; r += kFlight * kSumSlices) {
-            float4 o[kFlight];
+    // the sum over the wave's lanes with this lane's columns: 8, 16 and 32 lanes away
+    auto over_slices = [](float v) {
+        v = dpp_add<0x128>(v);  // row_ror: 8
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    };
+    const float* p = sums + (parts ? blockIdx.y * parts * per * D : 0) + k * D + (live ? col : 0);
+    float4 v[kSumSeqs];
+#pragma unroll
+    for (int i = 0; i < kSumSeqs; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // (unconditional loads, past the end of the last row: all sequences' of a flight at once)
+    constexpr int kFlight = 4;
+    for (int64_t r = slice; r < m; r += kFlight * kSumSlices) {
+        float4 o[kSumSeqs][kFlight];
+#pragma unroll
+        for (int i = 0; i < kSumSeqs; ++i)
+            if (i < seqs)
+#pragma unroll
+                for (int j = 0; j < kFlight; ++j)
+                    o[i][j] = *reinterpret_cast<const float4*>(p + (i * m + min(r + j * kSumSlices, m - 1)) * per * D);
+#pragma unroll
+        for (int i = 0; i < kSumSeqs; ++i)
 #pragma unroll
             for (int j = 0; j < kFlight; ++j)
-                o[j] = *reinterpret_cast<const float4*>(p + min(r + j * kSumSlices, m - 1) * per * D);
+                if (i < seqs && r + j * kSumSlices < m) add(v[i], o[i][j]);
+    }
 #pragma unroll
-            for (int j = 0; j < kFlight; ++j)
-                if (r + j * kSumSlices < m) add(v, o[j]);
-        }
-        s_v[i][slice][q] = v;
+    for (int i = 0; i < kSumSeqs; ++i) {
+        if (i >= seqs) break;
+        const float4 s = make_float4(over_slices(v[i].x), over_slices(v[i].y), over_slices(v[i].z), over_slices(v[i].w));
+        if ((threadIdx.x & 63) < kSumQuads) s_v[i][threadIdx.x / kWave][q] = s;
     }
     __syncthreads();
     // one slice's threads for each sequence
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (slice < seqs)
-        for (int w = 0; w < kSumSlices; ++w) add(v, s_v[slice][w][q]);
-    auto put = [&](float* to, const float* w, float off, const float4& x) {
+        for (int w = 0; w < kWaves; ++w) add(x, s_v[slice][w][q]);
+    auto put = [&](float* to, const float* w, float off, const float4& e) {
         const float4 g = w ? *reinterpret_cast<const float4*>(w) : make_float4(1.0f - off, 1.0f - off, 1.0f - off, 1.0f - off);
         *reinterpret_cast<float4*>(to) =
-            make_float4((off + g.x) * x.x, (off + g.y) * x.y, (off + g.z) * x.z, (off + g.w) * x.w);
+            make_float4((off + g.x) * e.x, (off + g.y) * e.y, (off + g.z) * e.z, (off + g.w) * e.w);
     };
     if (!parts) {
         float* to = k ? a.dpost_w : a.dnorm_w;
-        if (to && slice == 0 && live) put(to + col, nullptr, 0.0f, v);
+        if (to && slice == 0 && live) put(to + col, nullptr, 0.0f, x);
         return;
     }
     const int64_t b = blockIdx.y + slice, o = b * D + col;
     const bool mine = slice < seqs && live, scale = k == 1;
     if (k == 0) {
-        if (a.dshift && mine) put(a.dshift + o, nullptr, 0.0f, v);
+        if (a.dshift && mine) put(a.dshift + o, nullptr, 0.0f, x);
         return;
     }
     if (float* to = scale ? a.dscale : a.dgate; to && mine)
         put(to + o, scale ? (a.norm_w ? a.norm_w + col : nullptr) : a.post && a.post_w ? a.post_w + col : nullptr, 0.0f,
-            v);
+            x);
     // the gains' share of the sequence
     __syncthreads();
-    float* share = gridDim.y > 1 ? gains + (b * 2 + k - 1) * D + col : reinterpret_cast<float*>(&s_v[0][slice][q]);
+    float* share = gridDim.y > 1 ? gains + (b * 2 + k - 1) * D + col : reinterpret_cast<float*>(&s_v[0][slice % kSumSeqs][q]);
     if (mine) {
-        if (scale) put(share, a.scale ? a.scale + o : nullptr, 1.0f, v);
-        else put(share, a.gate ? a.gate + o : nullptr, 0.0f, v);
+        if (scale) put(share, a.scale ? a.scale + o : nullptr, 1.0f, x);
+        else put(share, a.gate ? a.gate + o : nullptr, 0.0f, x);
     }
     if (gridDim.y > 1) return;
     __syncthreads();
     float* to = scale ? a.dnorm_w : a.dpost_w;
     if (slice || !live || !to) return;
-    v = s_v[0][0][q];
-    for (int i = 1; i < seqs; ++i) add(v, s_v[0][i][q]);
-    put(to + col, nullptr, 0.0f, v);
+    x = s_v[0][0][q];
+    for (int i = 1; i < seqs; ++i) add(x, s_v[0][i][q]);
+    put(to + col, nullptr, 0.0f, x);
 }
 
 __global__ __launch_bounds__(256) void zero_gains_kernel(float* p, float* q, int D) {
@@ -446,7 +465,7 @@ hipError_t launch_grad_t(const BlockSeamBackwardArgs& a, hipStream_t s) {
     if (e != hipSuccess || !(a.dgate || a.dshift || a.dscale || a.dnorm_w || a.dpost_w)) return e;
     const int64_t n = a.rows / a.seq;
     const unsigned cols = (unsigned)((a.D + 4 * kSumQuads - 1) / (4 * kSumQuads));
-    const dim3 block(kSumSlices * kSumQuads);
+    const dim3 block(kSumThreads);
     if (p.whole) {  // each block's shares of the gains
         if (a.dnorm_w || a.dpost_w)
             launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), block, 0, s, a, (const float*)sums, p.blocks, (int64_t)0,
