@@ -194,3 +194,37 @@ def test_chain_of_a_block_eager_and_captured():
         eager = chain()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager)), r
+
+
+def test_refusals_with_a_layer():
+    layer, x, *_ = case(40, 64, 4, 2, 96, "bf16", 71)
+    i = torch.zeros(40, 2, dtype=torch.int32, device="cuda")
+    w = torch.ones(40, 2, device="cuda")
+    L, p = nm._lib.lib(), x.data_ptr()
+    y = torch.empty_like(x)
+    for args in ((p, None, w.data_ptr()), (p, i.data_ptr(), None), (None, i.data_ptr(), w.data_ptr()),
+                 (p + 2, i.data_ptr(), w.data_ptr()), (p, i.data_ptr() + 2, w.data_ptr())):
+        assert L.nomas_moe_forward_routed(layer._h, *args, y.data_ptr(), 40, None) == 2
+    assert L.nomas_moe_forward_routed(layer._h, p, i.data_ptr(), w.data_ptr(), y.data_ptr(), -1, None) == 2
+    for bad in ((x, i.long(), w), (x, i, w.half()), (x, i[:, :1], w), (x, i, w[:20]), (x, i.cpu(), w), (x.float(), i, w)):
+        with pytest.raises(nm.NomasError):
+            layer.forward_routed(*bad)
+
+
+def test_streams_are_ordered():
+    # forwards of one handle on different streams share its workspace and wait for each other
+    layer, x, *_ = case(900, 128, 8, 2, 192, "bf16", 73)
+    want = layer.forward(x)
+    idx, w, _, _ = layer.routing(900)
+    idx, w = torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda()
+    flip = layer.forward_routed(x, idx.flip(0), w)
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(6):
+        with torch.cuda.stream(s[0]):
+            a = layer.forward_routed(x, idx, w)
+        with torch.cuda.stream(s[1]):
+            b = layer.forward_routed(x, idx.flip(0), w)
+        c = layer.forward(x)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want) and torch.equal(b, flip) and torch.equal(c, want)
