@@ -20,8 +20,8 @@
 // leaves its sums in the workspace, and seam_sums_kernel adds them up in a
 // fixed order: no atomics, the same bits every time.
 //
-// 14,232 rows of 1,536 bf16 (262 MB and 9 MB of sums): 60 us, 4.5 TB/s, and 6 for the sums; 5,998 rows of
-// 1,000 f32: 32 us and 6.  Loading the next row ahead takes registers that are worth more
+// 14,232 rows of 1,536 bf16 (262 MB and 9 MB of sums): 60 us, 4.5 TB/s, and 5.6 for the sums; 5,998 rows of
+// 1,000 f32: 32 us and 4.6.  Loading the next row ahead takes registers that are worth more
 // as waves (114 us), a wave a row of three chunks a lane measured 58.5 and 37 us.  Rows past 8,192
 // columns hold four chunks a thread and spill: 1.9 TB/s at 16,384.
 #include "block_seam.hpp"
@@ -325,105 +325,147 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
     }
 }
 
-// Adds up the blocks' sums.  A block takes 32 columns (8 threads of four each) of one of
-// the sums, blockIdx.z, in 64 slices of the parts: eight of a wave are added in
-// registers, the waves' in LDS.
-//  parts > 0: sums [n][parts][3][D] of n sequences: dshift, dscale, dgate.  The gains'
-//             gradients too where the block has all sequences (gridDim.y = 1), else
-//             their shares per sequence, blockIdx.y, into `gains` [n][2][D]
-//  parts = 0: gains [n][2][D] into dnorm_w and dpost_w
+// ---- the blocks' sums added up ----
+//
+// A block takes 32 columns (8 threads of four each) of one of the sums, blockIdx.z; the
+// rows of sums are dealt out to 64 slices, eight a wave.
+
 constexpr int kSumSlices = 64, kSumQuads = 8, kSumThreads = kSumSlices * kSumQuads;
-// Sequences that a block takes together: their sums wait for one another only at the end.
+constexpr int kSumWaves = kSumThreads / kWave, kSumWaveSlices = kSumSlices / kSumWaves;
+// Sequences whose sums one block adds, so that it can finish the gains too.
 constexpr int kSumSeqs = 4;
-__global__ __launch_bounds__(kSumThreads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums, int64_t n,
-                                                                int64_t parts, float* gains) {
-    constexpr int kWaves = kSumThreads / kWave;
-    __shared__ float4 s_v[kSumSeqs][kWaves][kSumQuads];
-    const int q = threadIdx.x % kSumQuads, slice = threadIdx.x / kSumQuads;
-    const int col = (blockIdx.x * kSumQuads + q) * 4;
-    const bool live = col < a.D;
-    const int64_t D = a.D;
-    const int k = blockIdx.z, per = parts ? kSums : 2;
-    const int64_t m = parts ? parts : n;
-    const int seqs = parts && gridDim.y == 1 ? (int)n : 1;
-    auto add = [](float4& v, const float4& o) {
-        v.x += o.x;
-        v.y += o.y;
-        v.z += o.z;
-        v.w += o.w;
-    };
-    // the sum over the wave's lanes with this lane's columns: 8, 16 and 32 lanes away
-    auto over_slices = [](float v) {
-        v = dpp_add<0x128>(v);  // row_ror: 8
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-    };
-    const float* p = sums + (parts ? blockIdx.y * parts * per * D : 0) + k * D + (live ? col : 0);
-    float4 v[kSumSeqs];
-#pragma unroll
-    for (int i = 0; i < kSumSeqs; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    // (unconditional loads, past the end of the last row: all sequences' of a flight at once)
+
+__device__ __forceinline__ void add4(float4& v, const float4& o) {
+    v.x += o.x;
+    v.y += o.y;
+    v.z += o.z;
+    v.w += o.w;
+}
+
+// v[i], i < seqs: the sum of rows slice, slice + slices, ... of the m rows of sequence i
+// (`pitch` floats apart), added over the slices that the wave holds.  The loads of a
+// flight, of all sequences, are unconditional, clamped to the last row: they wait once.
+template <int N>
+__device__ __forceinline__ void sum_rows(const float* p, int64_t m, int64_t pitch, int seqs, int slice, int slices,
+                                         float4 (&v)[N]) {
     constexpr int kFlight = 4;
-    for (int64_t r = slice; r < m; r += kFlight * kSumSlices) {
-        float4 o[kSumSeqs][kFlight];
 #pragma unroll
-        for (int i = 0; i < kSumSeqs; ++i)
+    for (int i = 0; i < N; ++i) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int64_t r = slice; r < m; r += kFlight * slices) {
+        float4 o[N][kFlight];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
             if (i < seqs)
 #pragma unroll
                 for (int j = 0; j < kFlight; ++j)
-                    o[i][j] = *reinterpret_cast<const float4*>(p + (i * m + min(r + j * kSumSlices, m - 1)) * per * D);
+                    o[i][j] = *reinterpret_cast<const float4*>(p + (i * m + min(r + j * slices, m - 1)) * pitch);
 #pragma unroll
-        for (int i = 0; i < kSumSeqs; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < kFlight; ++j)
-                if (i < seqs && r + j * kSumSlices < m) add(v[i], o[i][j]);
+                if (i < seqs && r + j * slices < m) add4(v[i], o[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < kSumSeqs; ++i) {
-        if (i >= seqs) break;
-        const float4 s = make_float4(over_slices(v[i].x), over_slices(v[i].y), over_slices(v[i].z), over_slices(v[i].w));
-        if ((threadIdx.x & 63) < kSumQuads) s_v[i][threadIdx.x / kWave][q] = s;
-    }
-    __syncthreads();
-    // one slice's threads for each sequence
-    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (slice < seqs)
-        for (int w = 0; w < kWaves; ++w) add(x, s_v[slice][w][q]);
-    auto put = [&](float* to, const float* w, float off, const float4& e) {
-        const float4 g = w ? *reinterpret_cast<const float4*>(w) : make_float4(1.0f - off, 1.0f - off, 1.0f - off, 1.0f - off);
-        *reinterpret_cast<float4*>(to) =
-            make_float4((off + g.x) * e.x, (off + g.y) * e.y, (off + g.z) * e.z, (off + g.w) * e.w);
+    // lanes with the same columns are 8, 16 and 32 apart
+    auto over_slices = [](float x) {
+        x = dpp_add<0x128>(x);  // row_ror: 8
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
     };
-    if (!parts) {
-        float* to = k ? a.dpost_w : a.dnorm_w;
-        if (to && slice == 0 && live) put(to + col, nullptr, 0.0f, x);
-        return;
-    }
-    const int64_t b = blockIdx.y + slice, o = b * D + col;
-    const bool mine = slice < seqs && live, scale = k == 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < seqs) v[i] = make_float4(over_slices(v[i].x), over_slices(v[i].y), over_slices(v[i].z), over_slices(v[i].w));
+}
+
+// x times four of w (1 where there is none), or of 1 + w (w 0 where there is none)
+__device__ __forceinline__ float4 times(const float4& x, const float* w, bool plus_one) {
+    if (!w) return x;
+    float4 g = *reinterpret_cast<const float4*>(w);
+    const float c = plus_one ? 1.0f : 0.0f;
+    return make_float4((c + g.x) * x.x, (c + g.y) * x.y, (c + g.z) * x.z, (c + g.w) * x.w);
+}
+__device__ __forceinline__ void put4(float* to, const float4& x) { *reinterpret_cast<float4*>(to) = x; }
+
+// From x, sum k (P, Q, R) of four columns of sequence b: that parameter's gradient; what
+// it adds to the gradient of norm_w (Q) or post_w (R) is returned.
+__device__ __forceinline__ float4 finish_sequence(const BlockSeamBackwardArgs& a, int k, int64_t b, int col, const float4& x) {
+    const int64_t o = b * a.D + col;
     if (k == 0) {
-        if (a.dshift && mine) put(a.dshift + o, nullptr, 0.0f, x);
-        return;
+        if (a.dshift) put4(a.dshift + o, x);
+        return x;
     }
-    if (float* to = scale ? a.dscale : a.dgate; to && mine)
-        put(to + o, scale ? (a.norm_w ? a.norm_w + col : nullptr) : a.post && a.post_w ? a.post_w + col : nullptr, 0.0f,
-            x);
-    // the gains' share of the sequence
+    if (k == 1) {
+        if (a.dscale) put4(a.dscale + o, times(x, a.norm_w ? a.norm_w + col : nullptr, false));
+        return times(x, a.scale ? a.scale + o : nullptr, true);
+    }
+    if (a.dgate) put4(a.dgate + o, times(x, a.post && a.post_w ? a.post_w + col : nullptr, false));
+    return times(x, a.gate ? a.gate + o : nullptr, false);
+}
+
+// n <= kSumSeqs sequences of `parts` rows [3][D]: all gradients of parameters.
+__global__ __launch_bounds__(kSumThreads) void seam_sums_kernel(BlockSeamBackwardArgs a, const float* sums, int n,
+                                                                int64_t parts) {
+    __shared__ float4 s_v[kSumSeqs][kSumWaves][kSumQuads];
+    const int q = threadIdx.x % kSumQuads, slice = threadIdx.x / kSumQuads, wave = threadIdx.x / kWave;
+    const int col = (blockIdx.x * kSumQuads + q) * 4, k = blockIdx.z;
+    const bool live = col < a.D;
+    float4 v[kSumSeqs];
+    sum_rows(sums + (int64_t)k * a.D + (live ? col : 0), parts, kSums * (int64_t)a.D, n, slice, kSumSlices, v);
+#pragma unroll
+    for (int i = 0; i < kSumSeqs; ++i)
+        if ((threadIdx.x & 63) < kSumQuads) s_v[i][wave][q] = v[i];
     __syncthreads();
-    float* share = gridDim.y > 1 ? gains + (b * 2 + k - 1) * D + col : reinterpret_cast<float*>(&s_v[0][slice % kSumSeqs][q]);
+    // slice i's threads finish sequence i
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const bool mine = slice < n && live;
     if (mine) {
-        if (scale) put(share, a.scale ? a.scale + o : nullptr, 1.0f, x);
-        else put(share, a.gate ? a.gate + o : nullptr, 0.0f, x);
+        for (int w = 0; w < kSumWaves; ++w) add4(x, s_v[slice][w][q]);
+        x = finish_sequence(a, k, slice, col, x);
     }
-    if (gridDim.y > 1) return;
+    float* to = k == 0 ? nullptr : k == 1 ? a.dnorm_w : a.dpost_w;
+    if (!to) return;
     __syncthreads();
-    float* to = scale ? a.dnorm_w : a.dpost_w;
-    if (slice || !live || !to) return;
-    x = s_v[0][0][q];
-    for (int i = 1; i < seqs; ++i) add(x, s_v[0][i][q]);
-    put(to + col, nullptr, 0.0f, x);
+    if (mine) s_v[slice][0][q] = x;
+    __syncthreads();
+    if (slice || !live) return;
+    for (int i = 1; i < n; ++i) add4(x, s_v[i][0][q]);
+    put4(to + col, x);
+}
+
+// More sequences, a wave each: their gradients, and the shares of the gains [n][2][D].
+// (A block of 64 slices for each would stand idle where a sequence has few rows of sums:
+// the backward pass of 64 x 16 rows of 1,536 takes 26 us, and took 45 so.)
+__global__ __launch_bounds__(kSumThreads) void seam_sequence_sums_kernel(BlockSeamBackwardArgs a, const float* sums,
+                                                                         int64_t n, int64_t parts, float* gains) {
+    const int q = threadIdx.x % kSumQuads, slice = threadIdx.x % kWave / kSumQuads;
+    const int col = (blockIdx.x * kSumQuads + q) * 4, k = blockIdx.z;
+    const int64_t b = blockIdx.y * (int64_t)kSumWaves + threadIdx.x / kWave;
+    if (b >= n) return;
+    const bool live = col < a.D;
+    float4 v[1];
+    sum_rows(sums + (b * parts * kSums + k) * a.D + (live ? col : 0), parts, kSums * (int64_t)a.D, 1, slice,
+             kSumWaveSlices, v);
+    if (slice || !live) return;
+    const float4 x = finish_sequence(a, k, b, col, v[0]);
+    if (k) put4(gains + (b * 2 + k - 1) * a.D + col, x);
+}
+
+// Shares [n][2][D] of the gains, of sequences or of blocks: dnorm_w and dpost_w.
+__global__ __launch_bounds__(kSumThreads) void seam_gain_sums_kernel(BlockSeamBackwardArgs a, const float* gains, int64_t n) {
+    __shared__ float4 s_v[kSumWaves][kSumQuads];
+    float* to = blockIdx.z ? a.dpost_w : a.dnorm_w;
+    if (!to) return;
+    const int q = threadIdx.x % kSumQuads, slice = threadIdx.x / kSumQuads;
+    const int col = (blockIdx.x * kSumQuads + q) * 4;
+    const bool live = col < a.D;
+    float4 v[1];
+    sum_rows(gains + (int64_t)blockIdx.z * a.D + (live ? col : 0), n, 2 * (int64_t)a.D, 1, slice, kSumSlices, v);
+    if ((threadIdx.x & 63) < kSumQuads) s_v[threadIdx.x / kWave][q] = v[0];
+    __syncthreads();
+    if (slice || !live) return;
+    for (int w = 1; w < kSumWaves; ++w) add4(v[0], s_v[w][q]);
+    put4(to + col, v[0]);
 }
 
 __global__ __launch_bounds__(256) void zero_gains_kernel(float* p, float* q, int D) {
@@ -465,20 +507,22 @@ hipError_t launch_grad_t(const BlockSeamBackwardArgs& a, hipStream_t s) {
     if (e != hipSuccess || !(a.dgate || a.dshift || a.dscale || a.dnorm_w || a.dpost_w)) return e;
     const int64_t n = a.rows / a.seq;
     const unsigned cols = (unsigned)((a.D + 4 * kSumQuads - 1) / (4 * kSumQuads));
-    const dim3 block(kSumThreads);
+    const bool want_gains = a.dnorm_w || a.dpost_w;
+    auto gain_sums = [&](const float* gains, int64_t rows) {
+        if (want_gains)
+            launch_kernel(seam_gain_sums_kernel, dim3(cols, 1, 2), dim3(kSumThreads), 0, s, a, gains, rows);
+    };
     if (p.whole) {  // each block's shares of the gains
-        if (a.dnorm_w || a.dpost_w)
-            launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), block, 0, s, a, (const float*)sums, p.blocks, (int64_t)0,
-                          (float*)nullptr);
-        return hipGetLastError();
+        gain_sums(sums, p.blocks);
+    } else if (n <= kSumSeqs) {
+        launch_kernel(seam_sums_kernel, dim3(cols, 1, kSums), dim3(kSumThreads), 0, s, a, (const float*)sums, (int)n,
+                      p.parts);
+    } else {
+        float* gains = sums + p.blocks * kSums * a.D;
+        launch_kernel(seam_sequence_sums_kernel, dim3(cols, (unsigned)((n + kSumWaves - 1) / kSumWaves), kSums),
+                      dim3(kSumThreads), 0, s, a, (const float*)sums, n, p.parts, gains);
+        gain_sums(gains, n);
     }
-    float* gains = sums + p.blocks * kSums * a.D;
-    const bool together = n <= kSumSeqs;
-    launch_kernel(seam_sums_kernel, dim3(cols, together ? 1 : (unsigned)n, kSums), block, 0, s, a, (const float*)sums, n,
-                  p.parts, gains);
-    if (!together && (a.dnorm_w || a.dpost_w))
-        launch_kernel(seam_sums_kernel, dim3(cols, 1, 2), block, 0, s, a, (const float*)gains, n, (int64_t)0,
-                      (float*)nullptr);
     return hipGetLastError();
 }
 

@@ -144,6 +144,12 @@ def test_gradients(dtype, B, S, D):
     check_grad(t, dtype, False, 0.5)
 
 
+@pytest.mark.parametrize("drop", [(), ("scale", "norm_w"), ("gate", "post_w")])
+@pytest.mark.parametrize("B,S,D", [(4, 40, 1032), (13, 40, 1032), (64, 16, 1536), (9, 300, 72), (17, 120, 264)])
+def test_gradients_of_many_sequences(drop, B, S, D):
+    check_grad(inputs(B, S, D, "f32", 17, NAMES), "f32", True, 1.0, drop)
+
+
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("B,S,D", [(2, 37, 136), (3, 300, 512), (40, 3, 1032)])
 @pytest.mark.parametrize("drop", [("gate",), ("scale",), ("norm_w",), ("post_w",), ("dout",),
