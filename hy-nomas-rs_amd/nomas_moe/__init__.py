@@ -359,9 +359,9 @@ def block_seam_backward(dout: torch.Tensor | None, dh: torch.Tensor | None,
     at, ptr = 0, {}
     base = flat.data_ptr()
     for n in names:
-        got[n], ptr[n], at = flat[at:at + B * D].view(B, D), base + 4 * at, at + B * D
+        got[n], ptr[n], at = flat.as_strided((B, D), (D, 1), at), base + 4 * at, at + B * D
     for n in gains:
-        got[n], ptr[n], at = flat[at:at + D], base + 4 * at, at + D
+        got[n], ptr[n], at = flat.as_strided((D,), (1,), at), base + 4 * at, at + D
     if first.numel() == 0:
         return {k: v.zero_() for k, v in got.items()}
     p = ptr.get
@@ -413,7 +413,7 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
     bias = _param(bias, lc, (E,), "bias")
     shape = lc.shape[:-1] + (k,)
     idx = torch.empty(shape, dtype=torch.int32, device=lc.device)
-    w = torch.empty(shape, dtype=torch.float32, device=lc.device)
+    w = torch.empty_like(idx, dtype=torch.float32)
     n = torch.empty(E, dtype=torch.int32, device=lc.device) if counts else None
     _call(_lib.lib().nomas_route, lc, _CODES[lc.dtype], lc.data_ptr(), rows, E, k,
           _SCORING[scoring], _ptr(bias), int(groups),
