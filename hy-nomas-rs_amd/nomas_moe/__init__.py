@@ -47,8 +47,11 @@ class DataType(enum.IntEnum):
         if isinstance(dt, DataType):
             return dt
         if isinstance(dt, torch.dtype):
-            return {torch.float32: cls.F32, torch.bfloat16: cls.Bf16, torch.float16: cls.F16}[dt]
+            return _OF_TORCH[dt]
         return {"f32": cls.F32, "bf16": cls.Bf16, "f16": cls.F16}[str(dt).lower()]
+
+
+_OF_TORCH = {t.torch: t for t in DataType}
 
 
 def _check_out(out: torch.Tensor, like: torch.Tensor, what: str = "out") -> torch.Tensor:
@@ -348,28 +351,26 @@ def block_seam_backward(dout: torch.Tensor | None, dh: torch.Tensor | None,
     got = {"dx": torch.empty_like(first)}
     if y is not None:
         got["dy"] = torch.empty_like(first)
-    # the f32 gradients in one allocation
-    names = (("dgate",) if y is not None else ()) + (("dshift", "dscale") if dh is not None else ())
-    gains = (("dpost_w",) if post_norm else ()) + (("dnorm_w",) if dh is not None else ())
-    L = _lib.lib()
-    need = L.nomas_block_seam_workspace(B * S, D, max(S, 1))
-    ends = (len(names) * B + len(gains)) * D  # (a multiple of 8 floats)
-    flat = torch.empty(ends, dtype=torch.float32, device=first.device)
-    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
-    at, ptr = 0, {}
-    base = flat.data_ptr()
-    for n in names:
-        got[n], ptr[n], at = flat.as_strided((B, D), (D, 1), at), base + 4 * at, at + B * D
-    for n in gains:
-        got[n], ptr[n], at = flat.as_strided((D,), (1,), at), base + 4 * at, at + D
+    # (a parameter of the same shape makes its gradient fastest)
+    like = gate if gate is not None else scale
+    for n in (("dgate",) if y is not None else ()) + (("dshift", "dscale") if dh is not None else ()):
+        like = got[n] = torch.empty((B, D), dtype=torch.float32, device=first.device) \
+            if like is None else torch.empty_like(like)
+    like = norm_w if norm_w is not None else post_w
+    for n in (("dpost_w",) if post_norm else ()) + (("dnorm_w",) if dh is not None else ()):
+        like = got[n] = torch.empty(D, dtype=torch.float32, device=first.device) \
+            if like is None else torch.empty_like(like)
     if first.numel() == 0:
         return {k: v.zero_() for k, v in got.items()}
-    p = ptr.get
+    L = _lib.lib()
+    need = L.nomas_block_seam_workspace(B * S, D, S)
+    ws = torch.empty(need, dtype=torch.uint8, device=first.device)
+    p = got.get
     _call(L.nomas_block_seam_backward, first, _CODES[first.dtype], _ptr(dout), _ptr(dh), _ptr(out),
-          _ptr(y), got["dx"].data_ptr(), _ptr(got.get("dy")), B * S, D, S, _ptr(gate),
-          int(post_norm), _ptr(post_w), float(residual_scale), _ptr(norm_w), _ptr(scale),
-          float(eps), p("dgate"), p("dshift"), p("dscale"), p("dnorm_w"), p("dpost_w"),
-          ws.data_ptr(), need)
+          _ptr(y), got["dx"].data_ptr(), _ptr(p("dy")), B * S, D, S, _ptr(gate), int(post_norm),
+          _ptr(post_w), float(residual_scale), _ptr(norm_w), _ptr(scale), float(eps),
+          _ptr(p("dgate")), _ptr(p("dshift")), _ptr(p("dscale")), _ptr(p("dnorm_w")),
+          _ptr(p("dpost_w")), ws.data_ptr(), need)
     return got
 
 
