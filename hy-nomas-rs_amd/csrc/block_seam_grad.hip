@@ -486,7 +486,9 @@ hipError_t launch_grad_shape(const BlockSeamBackwardArgs& a, const SeamPlan& p, 
                      : (norm ? seam_grad_kernel<T, false, true, kWhole, L, C> : seam_grad_kernel<T, false, false, kWhole, L, C>);
     const uint32_t lds = grad_lds(p, a.D);
     if (lds > 48 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        // (the widest row's: calls of several threads set the same value)
+        const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 2 * kMaxSeamDim * 4);
         if (e != hipSuccess) return e;
     }
     launch_kernel(kern, dim3((unsigned)p.blocks), dim3(p.row_threads * p.groups), lds, s, a, p, sums);

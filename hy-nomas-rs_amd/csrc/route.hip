@@ -946,10 +946,14 @@ hipError_t launch_route_backward(DType dt, const RouteBackwardArgs& a, hipStream
 
 hipError_t launch_given_routing(const GivenRoutingArgs& a, hipStream_t s) {
     const size_t lds = (size_t)kRouterRows * a.k * 12 + (size_t)a.E_cols * 4;
-    if (a.rows < 1 || a.k < 1 || a.k > a.E || lds > 160 * 1024) return hipErrorInvalidValue;
-    const hipError_t e = hipFuncSetAttribute((const void*)given_kernel,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
+    constexpr size_t kMost = 160 * 1024;
+    if (a.rows < 1 || a.k < 1 || a.k > a.E || lds > kMost) return hipErrorInvalidValue;
+    if (lds > 48 * 1024) {
+        // (all that there is: calls of several threads set the same value)
+        const hipError_t e =
+            hipFuncSetAttribute((const void*)given_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
+        if (e != hipSuccess) return e;
+    }
     launch_kernel(given_kernel, dim3((unsigned)((a.rows + kRouterRows - 1) / kRouterRows)), dim3(kRouteThreads),
                   (uint32_t)lds, s, a);
     return hipGetLastError();

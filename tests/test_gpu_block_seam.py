@@ -1,6 +1,8 @@
 """The seam between two branches of a block (nm.block_seam) and its gradients on
 the GPU, against their formulas in 64 bits, with bounds on the errors that the
 f32 evaluation and the outputs' types allow (tests/_block_ops.py)."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -265,6 +267,23 @@ def test_two_streams_at_once():
                 got.append(call(u))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+def test_two_host_threads():
+    # wide rows of two widths: each call asks for its own share of LDS
+    t = [{k: dev(v) for k, v in inputs(1, 9, D, "bf16", D, NAMES).items()} for D in (8192, 16384)]
+
+    def call(u):
+        g = nm.block_seam_backward(u["dout"], u["dh"], u["out"], u["y"], u["gate"], u["scale"], post_norm=True)
+        return [g[k] for k in sorted(g)]
+
+    want = [call(u) for u in t]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(2) as pool:
+        for _ in range(20):
+            got = list(pool.map(call, t))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
 
 
 def test_strided_inputs_and_parameters_of_other_types():
