@@ -328,7 +328,8 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
 // ---- the blocks' sums added up ----
 //
 // A block takes 32 columns (8 threads of four each) of one of the sums, blockIdx.z; the
-// rows of sums are dealt out to 64 slices, eight a wave.
+// rows of sums are dealt out to 64 slices, eight a wave.  32 columns are a line of 128 bytes:
+// with 16, and 128 slices in twice the blocks, the 512 rows of 1,536 take 7.5 us instead of 5.5.
 
 constexpr int kSumSlices = 64, kSumQuads = 8, kSumThreads = kSumSlices * kSumQuads;
 constexpr int kSumWaves = kSumThreads / kWave, kSumWaveSlices = kSumSlices / kSumWaves;
