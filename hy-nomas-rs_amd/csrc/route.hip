@@ -628,7 +628,8 @@ RouteShape route_shape(int64_t rows, int E, int groups) {
 
 // ---- the gradient -----------------------------------------------------------------
 //
-//   S = sum of the chosen s + eps, A = sum of dw s over the chosen
+//   S = sum of the chosen s + eps, A = sum of dw s over the chosen (an empty slot, or a masked
+//   expert's, has no part in them: its dw is not used)
 //   ds_i = scale (dw_i - A / S) / S (renormalised) or scale dw_i, 0 where not chosen
 //   sigmoid: dl_i = ds_i s_i (1 - s_i)
 //   softmax: dl_e = s_e (ds_e - B), B = sum s ds: of renormalised weights scale A eps / S^2
@@ -688,15 +689,17 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
             *slope = q * r * r;
             return (v < 0.0f ? q : 1.0f) * r;
         };
-        auto slot = [&](int t, int* e, float* d, float* slope) {  // its score; e = -1: empty
+        // its score; e = -1: empty (no expert, or a masked one), whatever its value is
+        auto slot = [&](int t, int* e, float* d, float* slope) {
             *e = t < L ? e0 : idx[t];
-            *d = t < L ? d0 : dw[t];
-            *slope = 0.0f;
-            if (t >= k || *e < 0 || *e >= E) {
+            const float v = t < k && *e >= 0 && *e < E ? t < L ? v0 : Elt<T>::to_f32(l[*e]) : -INFINITY;
+            if (v == -INFINITY) {
                 *e = -1;
+                *d = *slope = 0.0f;
                 return 0.0f;
             }
-            return score(t < L ? v0 : Elt<T>::to_f32(l[*e]), slope);
+            *d = t < L ? d0 : dw[t];
+            return score(v, slope);
         };
         float sum = 0.0f, dot = 0.0f;
         bool some = false, twice = false;
@@ -711,8 +714,10 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
         }
         wave_sync();
         for (int t = p; t < k; t += L) {
-            const int e = t < L ? e0 : idx[t];
-            if (e >= 0 && e < E) twice |= s_row[e] != (float)t;
+            int e;
+            float d, slope;
+            slot(t, &e, &d, &slope);
+            if (e >= 0) twice |= s_row[e] != (float)t;
         }
         wave_sync();
         sum = lanes_addf<L>(sum);

@@ -427,8 +427,8 @@ def route_backward(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, *,
                    scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
                    eps: float = 1e-9) -> torch.Tensor:
     """The gradient of route's weights with respect to the logits, of the logits'
-    shape and dtype.  idx: route's choice (an index outside 0..E-1: an empty
-    slot); dw: the weights' gradient.  The choice itself has none, and so
+    shape and dtype.  idx: route's choice (an index outside 0..E-1, or of a masked
+    expert: an empty slot, whose dw is not used); dw: the weights' gradient.  The choice itself has none, and so
     neither has the bias."""
     lc = _route_input(logits, scoring)
     E = lc.shape[-1]

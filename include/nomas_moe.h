@@ -285,8 +285,8 @@ int nomas_route(int dtype, const void *logits, int64_t rows, int64_t experts, in
                 float *w, int32_t *counts, void *stream);
 
 /* dlogits (rows, experts; every element is written) from dw, the gradient of
- * nomas_route's w, for the choice idx (an index outside 0 .. experts - 1 is an
- * empty slot).  The other arguments as in the forward call; dlogits may alias
+ * nomas_route's w, for the choice idx (an index outside 0 .. experts - 1, or of a
+ * masked expert, is an empty slot, whose dw is not used).  The other arguments as in the forward call; dlogits may alias
  * logits. */
 int nomas_route_backward(int dtype, const void *logits, const int32_t *idx, const float *dw,
                          int64_t rows, int64_t experts, int64_t top_k, int scoring,
