@@ -656,7 +656,7 @@ int nomas_route(int dtype, const void* logits, int64_t rows, int64_t experts, in
         a.group_top = (int)group_top;
         a.renormalize = renormalize != 0;
         a.scale = (float)scale;
-        a.eps = (float)eps;
+        a.log_eps = (float)std::log(eps);
         a.idx = idx;
         a.w = w;
         a.counts = counts;

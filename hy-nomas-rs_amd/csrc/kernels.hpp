@@ -229,7 +229,7 @@ struct RouteArgs {
     int sigmoid;         // scores: 0 softmax, 1 sigmoid
     int groups, top_groups, group_top;
     int renormalize;
-    float scale, eps;
+    float scale, log_eps;  // (log of the eps in the weights' sum: -inf without one)
     int32_t* idx;        // rows x k, ascending, -1 where no expert is left
     float* w;            // rows x k
     int32_t* counts;     // E: rows that chose each (null: not wanted)

@@ -571,30 +571,46 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
         for (unsigned m = chosen; m; m &= m - 1, ++place)
             if (place < k) s_idx[place] = first + __ffs(m) - 1;
         wave_sync();
-        // lane t of the row: slot t
-        auto score = [&](int e) {
-            const float v = Elt<T>::to_f32(l[e]);
-            if (!a.sigmoid) return expf(v - top) / zsum;
+        // lane t of the row: slot t.  Renormalised weights come from scores (and eps) relative to the
+        // largest chosen one or eps, whichever is larger: at their own scale all of the chosen may
+        // underflow (a softmax whose bias chooses far below the row's largest logit, a sigmoid of
+        // low logits), at the scores' eps may overflow.
+        float m = 0.0f;  // a softmax's scores are exp(v - top - m), a sigmoid's s exp(-m), m <= 0
+        auto score = [&](float v) {
+            if (!a.sigmoid) return expf(v - top - m);
             const float q = expf(-fabsf(v));
-            return (v < 0.0f ? q : 1.0f) / (1.0f + q);  // (a NaN stays one)
+            return (v < 0.0f ? expf(v - m) : 1.0f) / (1.0f + q);  // (a NaN stays one)
         };
         int e0 = -1;
-        float s0 = 0.0f, sum = 0.0f;
+        float v0 = -INFINITY, most = -INFINITY;
         for (int t = p; t < k; t += L) {
             const int e = t < found ? s_idx[t] : -1;
-            const float s = e >= 0 ? score(e) : 0.0f;
+            const float v = e >= 0 ? Elt<T>::to_f32(l[e]) : -INFINITY;
             if (t < L) {
                 e0 = e;
-                s0 = s;
+                v0 = v;
             }
+            most = fmaxf(most, v);
+        }
+        float log_eps = 0.0f;
+        if (a.renormalize) {
+            most = lanes_maxf<L>(most);
+            log_eps = a.log_eps + (a.sigmoid ? 0.0f : logf(zsum));
+            m = a.sigmoid ? fminf(fmaxf(most, log_eps), 0.0f) : fmaxf(most - top, log_eps);
+        }
+        float s0 = 0.0f, sum = 0.0f;
+        for (int t = p; t < k; t += L) {
+            const int e = t < L ? e0 : t < found ? s_idx[t] : -1;
+            const float s = e >= 0 ? score(t < L ? v0 : Elt<T>::to_f32(l[e])) : 0.0f;
+            if (t < L) s0 = s;
             sum += s;
         }
-        float up = a.scale;
-        if (a.renormalize) up /= lanes_addf<L>(sum) + a.eps;
+        float up = a.sigmoid ? a.scale : a.scale / zsum;
+        if (a.renormalize) up = a.scale / (lanes_addf<L>(sum) + expf(log_eps - m));
         for (int t = p; t < k; t += L) {
             if (!real) break;
             const int e = t < L ? e0 : t < found ? s_idx[t] : -1;
-            const float s = t < L ? s0 : e >= 0 ? score(e) : 0.0f;
+            const float s = t < L ? s0 : e >= 0 ? score(Elt<T>::to_f32(l[e])) : 0.0f;
             a.idx[row * k + t] = e;
             a.w[row * k + t] = e >= 0 ? up * s : 0.0f;
             if (hist && e >= 0) atomicAdd(&s_hist[e], 1);
