@@ -650,28 +650,52 @@ RouteShape route_shape(int64_t rows, int E, int groups) {
 //   sigmoid: dl_i = ds_i s_i (1 - s_i)
 //   softmax: dl_e = s_e (ds_e - B), B = sum s ds: of renormalised weights scale A eps / S^2
 //
+// dw_i - A / S and ds_i - B cancel: a row's only survivor keeps eps' share of dw_i, equal dw no
+// more.  So the kernel sums differences.  With eps (a softmax's: eps R / (1 + eps), R the
+// scores of the experts not chosen, summed as such) as one more slot of dw 0, A / M is the
+// slots' mean, M = sum s + that; from c, the dw of the largest of them,
+//   dw_i - A / M = (dw_i - c) + (c eps' - sum s (dw - c)) / M
+// and with N = S (softmax: in units in which the row's scores sum to Z, S Z)
+//   sigmoid: dl_i = scale s_i (1 - s_i) (dw_i - A / M) / N, M = N
+//   softmax: dl_i = scale s_i (dw_i - A / M) / N (chosen: N = M (1 + eps)),
+//            dl_e = -scale s_e eps A / N^2 (not chosen)
+// A softmax that is not renormalised is the same with R in the place of eps', M = N = Z and
+// dl_e = -scale s_e A / N^2.  Where an expert is named twice its slots count each, but its score
+// only once in Z: then eps' = eps Z, M = N, and B (as above) is taken off the sum of its slots.
+//
 // HBM bound: a softmax reads the row once, a sigmoid its chosen logits; every element of
 // dlogits is written once.  The lanes of a row hold 16-byte chunks of it; the chosen
 // elements are scattered into the row in LDS, and it is stored from there in whole chunks.
 template <typename T, int L, int C, bool kSigmoid>
 __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBackwardArgs a, int vector) {
     constexpr int W = 16 / (int)sizeof(T), kRows = kWave / L;
+    static_assert(C * W <= 32, "a bit for each of a lane's elements");
     extern __shared__ __align__(16) float s_rows[];
     const int E = a.E, k = a.k;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, p = lane % L, sub = lane / L;
     float* s_row = s_rows + (wave * kRows + sub) * (L * C * W);
+    unsigned* s_bits = reinterpret_cast<unsigned*>(s_row);  // [L] the chosen of each lane's elements, at first
     const int64_t stride = (int64_t)gridDim.x * kRouteWaves * kRows;
     for (int64_t row0 = ((int64_t)blockIdx.x * kRouteWaves + wave) * kRows; row0 < a.rows; row0 += stride) {
         const int64_t row = min(row0 + sub, a.rows - 1);
         const bool real = row0 + sub < a.rows;
         const T* l = static_cast<const T*>(a.logits) + row * E;
-        // the first slots, and where they lead
+        // a slot's expert (-1: empty, whatever its value is), value and logit
         const int32_t* idx = a.idx + row * k;
         const float* dw = a.dw + row * k;
-        const int e0 = p < k ? idx[p] : -1;
-        const float d0 = p < k ? dw[p] : 0.0f;
-        const float v0 = e0 >= 0 && e0 < E ? Elt<T>::to_f32(l[e0]) : 0.0f;
-        float s[C][W], top = 0.0f, zi = 1.0f;
+        auto read = [&](int t, float* d, float* v) {
+            const int e = idx[t];
+            *d = dw[t];
+            *v = e >= 0 && e < E ? Elt<T>::to_f32(l[e]) : -INFINITY;
+            if (*v != -INFINITY) return e;
+            *d = 0.0f;
+            return -1;
+        };
+        // lane t's first slot is slot t
+        int e0 = -1;
+        float d0 = 0.0f, v0 = -INFINITY;
+        if (p < k) e0 = read(p, &d0, &v0);
+        float s[C][W], top = 0.0f, z = 1.0f;
         if constexpr (!kSigmoid) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -690,86 +714,127 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
                 for (int i = 0; i < W; ++i) top = fmaxf(top, s[c][i]);
             top = lanes_maxf<L>(top);
             if (top == -INFINITY) top = 0.0f;
-            float z = 0.0f;
+            z = 0.0f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int i = 0; i < W; ++i) z += s[c][i] = __builtin_amdgcn_exp2f((s[c][i] - top) * 1.44269504f);
             z = lanes_addf<L>(z);
-            zi = z == 0.0f ? 0.0f : 1.0f / z;
         }
-        // a slot's score, and what dl is of ds
+        // what is chosen, and whether anything is twice
+        s_bits[p] = 0;
+        wave_sync();
+        bool some = false, twice = false;
+        float most = -INFINITY;
+        for (int t = p; t < k; t += L) {
+            int e = e0;
+            float d = d0, v = v0;
+            if (t >= L) e = read(t, &d, &v);
+            if (e < 0) continue;
+            const int chunk = e / W;
+            const unsigned bit = 1u << (chunk / L * W + e % W);
+            twice |= (atomicOr(&s_bits[chunk % L], bit) & bit) != 0;
+            some = true;
+            most = fmaxf(most, v);
+        }
+        wave_sync();
+        const unsigned chosen = s_bits[p];
+        wave_sync();
+        some = lanes_max<L>(some);
+        twice = lanes_max<L>(twice);
+        // a slot's score (a softmax's: times z), and how that moves with the logit
         auto score = [&](float v, float* slope) {
-            if constexpr (!kSigmoid) return *slope = __builtin_amdgcn_exp2f((v - top) * 1.44269504f) * zi;
+            if constexpr (!kSigmoid) return *slope = __builtin_amdgcn_exp2f((v - top) * 1.44269504f);
             const float q = expf(-fabsf(v)), r = 1.0f / (1.0f + q);
             *slope = q * r * r;
             return (v < 0.0f ? q : 1.0f) * r;
         };
-        // its score; e = -1: empty (no expert, or a masked one), whatever its value is
-        auto slot = [&](int t, int* e, float* d, float* slope) {
-            *e = t < L ? e0 : idx[t];
-            const float v = t < k && *e >= 0 && *e < E ? t < L ? v0 : Elt<T>::to_f32(l[*e]) : -INFINITY;
-            if (v == -INFINITY) {
-                *e = -1;
-                *d = *slope = 0.0f;
-                return 0.0f;
+        float u0 = 0.0f, slope0 = 0.0f;
+        if (e0 >= 0) u0 = score(v0, &slope0);
+        // of slot t, with its score and slope
+        auto slot = [&](int t, float* d, float* u, float* slope) {
+            if (t < L) {
+                *d = d0;
+                *u = u0;
+                *slope = slope0;
+                return e0;
             }
-            *d = t < L ? d0 : dw[t];
-            return score(v, slope);
+            float v;
+            const int e = read(t, d, &v);
+            *u = *slope = 0.0f;
+            if (e >= 0) *u = score(v, slope);
+            return e;
         };
-        float sum = 0.0f, dot = 0.0f;
-        bool some = false, twice = false;
-        for (int t = p; t < k; t += L) {
-            int e;
-            float d, slope;
-            const float w = slot(t, &e, &d, &slope);
-            sum += w;
-            dot += d * w;
-            some |= e >= 0;
-            if (e >= 0) s_row[e] = (float)t;  // (who is there: an expert named twice has another slot)
-        }
-        wave_sync();
-        for (int t = p; t < k; t += L) {
-            int e;
-            float d, slope;
-            slot(t, &e, &d, &slope);
-            if (e >= 0) twice |= s_row[e] != (float)t;
-        }
-        wave_sync();
-        sum = lanes_addf<L>(sum);
-        dot = lanes_addf<L>(dot);
-        float mean = 0.0f, up = 0.0f, inner = 0.0f;
-        if (lanes_max<L>(some)) {
-            const float total = sum + a.eps;
-            mean = a.renormalize ? dot / total : 0.0f;
-            up = a.renormalize ? a.scale / total : a.scale;
-            inner = a.renormalize ? up * mean * a.eps : up * dot;
+        float up = 0.0f, base = 0.0f, center = 0.0f, shift = 0.0f, inner = 0.0f;
+        if (kSigmoid && !a.renormalize) {
+            up = a.scale;
+        } else {
+            most = lanes_maxf<L>(most);
+            float sum = 0.0f, dot = 0.0f, rest = 0.0f;
+            center = -INFINITY;
+            for (int t = p; t < k; t += L) {
+                float d, u, slope;
+                const int e = slot(t, &d, &u, &slope);
+                sum += u;
+                dot += d * u;
+                if (e >= 0 && (t < L ? v0 : Elt<T>::to_f32(l[e])) == most) center = fmaxf(center, d);
+            }
+            if constexpr (!kSigmoid) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) rest += (chosen >> (c * W + i)) & 1 ? 0.0f : s[c][i];
+                rest = lanes_addf<L>(rest);
+            }
+            sum = lanes_addf<L>(sum);
+            dot = lanes_addf<L>(dot);
+            center = lanes_maxf<L>(center);
+            // eps (or the rest) as a slot, and the sum of all
+            float other = a.eps, total = sum + a.eps;
+            if constexpr (!kSigmoid) {
+                other = !a.renormalize ? rest : twice ? a.eps * z : a.eps * rest / (1.0f + a.eps);
+                total = a.renormalize ? sum + a.eps * z : z;
+            }
+            float slope;
+            const bool plain = !a.renormalize && twice;  // (its slots' values as they are)
+            if (plain || other > score(most, &slope) || !(fabsf(center) < INFINITY)) center = 0.0f;
+            float off = 0.0f;
+            for (int t = p; t < k; t += L) {
+                float d, u;
+                if (slot(t, &d, &u, &slope) >= 0) off += u * (d - center);
+            }
+            off = lanes_addf<L>(off);
+            if (some) {
+                up = a.scale / total;
+                if (!plain) shift = (center * other - off) / (sum + other);
+                if constexpr (!kSigmoid) {
+                    const float mean = dot / total * (a.renormalize ? a.eps : 1.0f);
+                    base = -up * mean;
+                    if (twice) inner = mean;
+                }
+            }
         }
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < W; i += 4) {
                 float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if constexpr (!kSigmoid) {
-                    const float f = -inner * zi;
-                    b = make_float4(f * s[c][i], f * s[c][i + 1], f * s[c][i + 2], f * s[c][i + 3]);
-                }
+                if constexpr (!kSigmoid)
+                    b = make_float4(base * s[c][i], base * s[c][i + 1], base * s[c][i + 2], base * s[c][i + 3]);
                 *reinterpret_cast<float4*>(s_row + (c * L + p) * W + i) = b;
             }
         wave_sync();
-        const bool again = __ballot(twice) != 0;
         for (int t = p; t < k; t += L) {
-            int e;
-            float d, slope;
-            slot(t, &e, &d, &slope);
+            float d, u, slope;
+            const int e = slot(t, &d, &u, &slope);
             if (e < 0) continue;
-            float ds = up * (d - mean);
-            if (again) {  // an expert named twice: all its slots' shares, in their order
-                ds = 0.0f;
-                for (int u = 0; u < k; ++u)
-                    if (idx[u] == e) ds += up * (dw[u] - mean);
+            float ds = (d - center) + shift;
+            if (twice) {  // an expert named twice: all its slots' shares, in their order
+                ds = -inner;
+                for (int o = 0; o < k; ++o)
+                    if (idx[o] == e) ds += (dw[o] - center) + shift;
             }
-            s_row[e] = slope * (kSigmoid ? ds : ds - inner);
+            s_row[e] = slope * (up * ds);
         }
         wave_sync();
         T* out = static_cast<T*>(a.dlogits) + row * E;

@@ -105,3 +105,120 @@ def test_weights_of_masked_rows_without_eps():
     l[3, :2] = -200.0
     for scoring in ("softmax", "sigmoid"):
         check_weights(l, 4, scoring, 0.0)
+
+
+# ---- gradients in which all but eps' share cancels -----------------------------------
+
+def grad(logits, idx, dw, scoring, renormalize, scale, eps):
+    """(dlogits, magnitudes): the definition, and the size of the terms that it has when it is
+    written without cancellation.  A chosen expert i has scale s_i / S^2 times
+    sum_j s_j (d_i - d_j) + eps d_i (1 - s_i for a softmax): its terms' magnitudes."""
+    T, E = logits.shape
+    dl, mag = np.zeros((T, E), X), np.zeros((T, E), X)
+    for r in range(T):
+        s = scores(logits[r], scoring)
+        sel = [(e, X(dw[r, t])) for t, e in enumerate(idx[r]) if 0 <= e < E and logits[r, e] != -np.inf]
+        if not sel:
+            continue
+        S = sum(s[e] for e, _ in sel) + X(eps) if renormalize else X(1)
+        A = sum(s[e] * d for e, d in sel)
+        B = sum(s[e] * abs(d) for e, d in sel)
+        ds = np.zeros(E, X)
+        for e, d in sel:
+            ds[e] += scale * ((d - A / S) / S if renormalize else d)
+        chosen = {e for e, _ in sel}
+        rest = sum(s[e] for e in range(E) if e not in chosen)
+        if scoring == "sigmoid":
+            dl[r] = ds * s * (1 - s)
+        else:
+            dl[r] = s * (ds - (s * ds).sum())
+            mag[r] = s * scale * B * (X(eps) / S / S if renormalize else 1)
+        for e, d in sel:
+            others = sum(s[f] * abs(d - g) for f, g in sel)
+            if renormalize:
+                own = X(eps) * abs(d) * (rest if scoring == "softmax" else 1)
+                m = (others * (1 + X(eps)) + own) / S / S
+            else:
+                m = others + rest * abs(d) if scoring == "softmax" else abs(d)
+            mag[r, e] = scale * s[e] * m * ((1 - s[e]) if scoring == "sigmoid" else 1)
+    return dl, mag
+
+
+def check_grad(l, idx, dw, dtype="f32", scoring="softmax", renormalize=True, scale=1.5, eps=1e-9):
+    """The kernel sums differences from the dominant slot's value; against the terms above,
+    differences from each slot's own, their magnitudes are 3 k + 5 times as large at most
+    (|d_i - c| <= (k + 1) of them, since the dominant score is a (k + 1)-th of the sum; the sum
+    of the others' and eps' share as much again).  Their roundings: exponentials, whose arguments'
+    errors are `spread` half steps, sums (trees) and quotients, 48 besides."""
+    got = nm.route_backward(l.cuda(), idx.cuda(), dw.cuda(), scoring=scoring, renormalize=renormalize, scale=scale,
+                            eps=eps).double().cpu().numpy()
+    k = idx.shape[1]
+    l64 = l.double().numpy()
+    want, mag = grad(l64, idx.numpy(), dw.double().numpy(), scoring, renormalize, scale, np.float32(eps))
+    e = (4 * ref.spread(l64, scoring) + 48) * ref.F32 * (3 * k + 5) * mag
+    tol = e + ref.HALF[dtype] * (np.abs(want) + e) + max(ref.TINY[dtype], 2.0 ** -148)
+    over = ~(np.abs(got - want) <= tol)
+    assert not over.any(), (over.sum(), np.argwhere(over)[0], got[over][0], float(want[over][0]), float(tol[over][0]))
+    return got
+
+
+def route_of(l, k, scoring):
+    return nm.route(l.cuda(), k, scoring=scoring, counts=False)[0].cpu()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("eps", [1e-9, 1e-2, 1.0])
+@pytest.mark.parametrize("dtype,E", [("f32", 2), ("f32", 16), ("bf16", 64), ("f16", 100), ("f32", 256), ("f32", 1000)])
+def test_gradient_of_a_single_survivor(scoring, eps, dtype, E):
+    l = logits_of(33, E, E, dtype)
+    got = check_grad(l, route_of(l, 1, scoring), values(33, 1, E), dtype, scoring, eps=eps)
+    if dtype == "f32":
+        assert (got != 0).any(1).all()
+    # the same with slots to spare, all but one expert masked
+    k = min(E, 6)
+    for r in range(33):
+        keep = l[r, r % E].clone()
+        l[r] = -float("inf")
+        l[r, r % E] = keep
+    idx = route_of(l, k, scoring)
+    assert ((idx >= 0).sum(1) == 1).all()
+    check_grad(l, idx, values(33, k, E + 1), dtype, scoring, eps=eps)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("eps", [1e-9, 1e-2])
+@pytest.mark.parametrize("E,k", [(8, 2), (64, 8), (100, 20), (256, 8), (1024, 70)])
+def test_gradient_of_equal_values_and_dominant_experts(scoring, eps, E, k):
+    T = 21
+    l = logits_of(T, E, E + k, "f32")
+    l[::3, E // 3] = 9.0                       # nearly all of the row's weight
+    l[1::3] -= 12.0                            # (sigmoid: eps beside small scores)
+    idx = route_of(l, k, scoring)
+    d = values(T, k, E)
+    check_grad(l, idx, d, "f32", scoring, eps=eps)
+    d[:, :] = d[:, :1]                         # no weight can gain from another
+    check_grad(l, idx, d, "f32", scoring, eps=eps)
+    d[:, k // 2] += 1e-3
+    check_grad(l, idx, 1000 + d, "f32", scoring, eps=eps)
+    check_grad(l, idx, d, "f32", scoring, renormalize=False)
+
+
+@pytest.mark.parametrize("dtype,E,k", [("f32", 16, 4), ("bf16", 64, 8), ("f32", 256, 40)])
+def test_gradient_of_scores_that_are_not_renormalised(dtype, E, k):
+    # all of the softmax's weight on the chosen: what is left is the rest's share
+    l = logits_of(18, E, 7, dtype)
+    l[:, :k] += 10.0
+    idx = route_of(l, k, "softmax")
+    d = values(18, k, 8)
+    check_grad(l, idx, d, dtype, "softmax", renormalize=False)
+    check_grad(l, idx, d[:, :1].repeat(1, k), dtype, "softmax", renormalize=False)
+
+
+def test_gradient_of_a_training_step_keeps_its_digits():
+    # top-1 of a batch: the 2-norm's error, not only each element's bound
+    l = logits_of(4000, 64, 9, "f32")
+    for scoring in ("softmax", "sigmoid"):
+        idx, d = route_of(l, 1, scoring), values(4000, 1, 10)
+        got = nm.route_backward(l.cuda(), idx.cuda(), d.cuda(), scoring=scoring).double().cpu().numpy()
+        want, _ = grad(l.double().numpy(), idx.numpy(), d.double().numpy(), scoring, True, 1.0, np.float32(1e-9))
+        assert np.linalg.norm((got - want).astype(float)) <= 1e-5 * np.linalg.norm(want.astype(float))
