@@ -688,6 +688,7 @@ int nomas_route_backward(int dtype, const void* logits, const int32_t* idx, cons
         a.renormalize = renormalize != 0;
         a.scale = (float)scale;
         a.eps = (float)eps;
+        a.log_eps = (float)std::log(eps);
         a.dlogits = dlogits;
         const hipError_t e =
             nomas::launch_route_backward(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));

@@ -241,7 +241,7 @@ struct RouteBackwardArgs {
     int64_t rows;
     int E, k;
     int sigmoid, renormalize;
-    float scale, eps;
+    float scale, eps, log_eps;
     void* dlogits;       // rows x E, model dtype
 };
 

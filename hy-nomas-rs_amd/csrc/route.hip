@@ -742,12 +742,22 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
         wave_sync();
         some = lanes_max<L>(some);
         twice = lanes_max<L>(twice);
-        // a slot's score (a softmax's: times z), and how that moves with the logit
+        // Renormalised: scores and eps relative to the larger of the largest chosen one and eps, as
+        // the forward's weights (a softmax's scores are exp(v - top - m), a sigmoid's s exp(-m)).
+        float m = 0.0f, eps = 0.0f;  // eps: times z for a softmax
+        if (a.renormalize) {
+            most = lanes_maxf<L>(most);
+            const float log_eps = a.log_eps + (kSigmoid ? 0.0f : logf(z));
+            m = kSigmoid ? fminf(fmaxf(most, log_eps), 0.0f) : fmaxf(most - top, log_eps);
+            eps = expf(log_eps - m);
+        }
+        // a slot's score, and how that moves with the logit
         auto score = [&](float v, float* slope) {
-            if constexpr (!kSigmoid) return *slope = __builtin_amdgcn_exp2f((v - top) * 1.44269504f);
+            if constexpr (!kSigmoid) return *slope = expf(v - top - m);
             const float q = expf(-fabsf(v)), r = 1.0f / (1.0f + q);
-            *slope = q * r * r;
-            return (v < 0.0f ? q : 1.0f) * r;
+            const float u = v < 0.0f ? expf(v - m) * r : r;
+            *slope = u * (v < 0.0f ? r : q * r);
+            return u;
         };
         float u0 = 0.0f, slope0 = 0.0f;
         if (e0 >= 0) u0 = score(v0, &slope0);
@@ -769,7 +779,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
         if (kSigmoid && !a.renormalize) {
             up = a.scale;
         } else {
-            most = lanes_maxf<L>(most);
+            if (!a.renormalize) most = lanes_maxf<L>(most);
             float sum = 0.0f, dot = 0.0f, rest = 0.0f;
             center = -INFINITY;
             for (int t = p; t < k; t += L) {
@@ -790,10 +800,14 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
             dot = lanes_addf<L>(dot);
             center = lanes_maxf<L>(center);
             // eps (or the rest) as a slot, and the sum of all
-            float other = a.eps, total = sum + a.eps;
+            float other = eps, total = sum + eps;
             if constexpr (!kSigmoid) {
-                other = !a.renormalize ? rest : twice ? a.eps * z : a.eps * rest / (1.0f + a.eps);
-                total = a.renormalize ? sum + a.eps * z : z;
+                if (!a.renormalize) {
+                    other = rest;
+                    total = z;
+                } else if (!twice) {
+                    other = eps * (rest / z) / (1.0f + a.eps);
+                }
             }
             float slope;
             const bool plain = !a.renormalize && twice;  // (its slots' values as they are)
@@ -808,9 +822,9 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteBack
                 up = a.scale / total;
                 if (!plain) shift = (center * other - off) / (sum + other);
                 if constexpr (!kSigmoid) {
-                    const float mean = dot / total * (a.renormalize ? a.eps : 1.0f);
-                    base = -up * mean;
-                    if (twice) inner = mean;
+                    const float mean = dot / total;
+                    base = -up * mean * (a.renormalize ? eps / z : 1.0f);
+                    if (twice) inner = a.renormalize ? a.eps * mean : mean;
                 }
             }
         }

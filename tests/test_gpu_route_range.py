@@ -110,11 +110,14 @@ def test_weights_of_masked_rows_without_eps():
 # ---- gradients in which all but eps' share cancels -----------------------------------
 
 def grad(logits, idx, dw, scoring, renormalize, scale, eps):
-    """(dlogits, magnitudes): the definition, and the size of the terms that it has when it is
+    """(dlogits, magnitudes, own): the definition, and the size of the terms that it has when it is
     written without cancellation.  A chosen expert i has scale s_i / S^2 times
-    sum_j s_j (d_i - d_j) + eps d_i (1 - s_i for a softmax): its terms' magnitudes."""
+    sum_j s_j (d_i - d_j) + eps d_i (a softmax: times the scores not chosen): its terms' magnitudes.
+    own: the roundings of this very evaluation, 2^-64 of the terms that cancel in it, for each of the E + k
+    terms of its sums and 8 operations besides (all there is where eps is 0: without a second slot the
+    gradient is 0 then)."""
     T, E = logits.shape
-    dl, mag = np.zeros((T, E), X), np.zeros((T, E), X)
+    dl, mag, own = np.zeros((T, E), X), np.zeros((T, E), X), np.zeros((T, E), X)
     for r in range(T):
         s = scores(logits[r], scoring)
         sel = [(e, X(dw[r, t])) for t, e in enumerate(idx[r]) if 0 <= e < E and logits[r, e] != -np.inf]
@@ -136,12 +139,17 @@ def grad(logits, idx, dw, scoring, renormalize, scale, eps):
         for e, d in sel:
             others = sum(s[f] * abs(d - g) for f, g in sel)
             if renormalize:
-                own = X(eps) * abs(d) * (rest if scoring == "softmax" else 1)
-                m = (others * (1 + X(eps)) + own) / S / S
+                left = X(eps) * abs(d) * (rest if scoring == "softmax" else 1)
+                m = (others * (1 + X(eps)) + left) / S / S
             else:
                 m = others + rest * abs(d) if scoring == "softmax" else abs(d)
-            mag[r, e] = scale * s[e] * m * ((1 - s[e]) if scoring == "sigmoid" else 1)
-    return dl, mag
+            slope = scale * s[e] * ((1 - s[e]) if scoring == "sigmoid" else 1)
+            mag[r, e] = slope * m
+            noise = X(2) ** -64 * (E + len(sel) + 8) * scale * 2 * (abs(d) + B / S) / S  # of ds[e]
+            own[r, e] += s[e] * noise
+            if scoring == "softmax":
+                own[r] += s * s[e] * noise     # by way of the inner product
+    return dl, mag, own
 
 
 def check_grad(l, idx, dw, dtype="f32", scoring="softmax", renormalize=True, scale=1.5, eps=1e-9):
@@ -154,9 +162,9 @@ def check_grad(l, idx, dw, dtype="f32", scoring="softmax", renormalize=True, sca
                             eps=eps).double().cpu().numpy()
     k = idx.shape[1]
     l64 = l.double().numpy()
-    want, mag = grad(l64, idx.numpy(), dw.double().numpy(), scoring, renormalize, scale, np.float32(eps))
+    want, mag, own = grad(l64, idx.numpy(), dw.double().numpy(), scoring, renormalize, scale, np.float32(eps))
     e = (4 * ref.spread(l64, scoring) + 48) * ref.F32 * (3 * k + 5) * mag
-    tol = e + ref.HALF[dtype] * (np.abs(want) + e) + max(ref.TINY[dtype], 2.0 ** -148)
+    tol = e + ref.HALF[dtype] * (np.abs(want) + e) + max(ref.TINY[dtype], 2.0 ** -148) + own
     over = ~(np.abs(got - want) <= tol)
     assert not over.any(), (over.sum(), np.argwhere(over)[0], got[over][0], float(want[over][0]), float(tol[over][0]))
     return got
@@ -220,5 +228,33 @@ def test_gradient_of_a_training_step_keeps_its_digits():
     for scoring in ("softmax", "sigmoid"):
         idx, d = route_of(l, 1, scoring), values(4000, 1, 10)
         got = nm.route_backward(l.cuda(), idx.cuda(), d.cuda(), scoring=scoring).double().cpu().numpy()
-        want, _ = grad(l.double().numpy(), idx.numpy(), d.double().numpy(), scoring, True, 1.0, np.float32(1e-9))
+        want, _, _ = grad(l.double().numpy(), idx.numpy(), d.double().numpy(), scoring, True, 1.0, np.float32(1e-9))
         assert np.linalg.norm((got - want).astype(float)) <= 1e-5 * np.linalg.norm(want.astype(float))
+
+
+# ---- gradients of scores that underflow ------------------------------------------------
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-9])
+@pytest.mark.parametrize("E,k", [(16, 1), (16, 4), (64, 8), (256, 30)])
+def test_gradient_of_scores_that_underflow(scoring, eps, E, k):
+    l = logits_of(20, E, E + k, "f32", std=2.0)
+    idx = torch.from_numpy(np.random.default_rng(k).permuted(np.tile(np.arange(E // 2, dtype=np.int32), (20, 1)), axis=1)
+                           [:, :k] + E // 2)
+    for low in (20.0, 95.0, 130.0, 300.0):
+        far = l.clone()
+        if scoring == "sigmoid":
+            far -= low
+        else:
+            far[:, E // 2:] -= low             # chosen far below the row's best
+        check_grad(far, idx, values(20, k, 11), "f32", scoring, eps=eps)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_gradient_of_masked_choices_without_eps(scoring):
+    l = logits_of(5, 24, 12, "f32")
+    l[1] = -float("inf")
+    l[2, 3] = l[2, 5] = -float("inf")
+    idx = torch.tensor([[1, 2], [3, 5], [3, 5], [-1, -1], [3, 4]], dtype=torch.int32)
+    got = check_grad(l, idx, values(5, 2, 13), "f32", scoring, eps=0.0)
+    assert (got[1:4] == 0).all()
