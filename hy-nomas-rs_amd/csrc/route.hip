@@ -359,8 +359,9 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                     i2 = max(max(i2, o2), min(i1, o1));
                     i1 = max(i1, o1);
                 }
+                // (half of the sum, or of the one that there is: two biases' may pass f32's range)
                 const float m1 = unordered(i1), m2 = unordered(i2);
-                const float score = a.group_top > 1 && m2 != -INFINITY ? m1 + m2 : m1;
+                const float score = a.group_top > 1 && m2 != -INFINITY ? 0.5f * m1 + 0.5f * m2 : 0.5f * m1;
                 int ahead = 0;  // groups before this one
                 for (int q = 0; q < a.groups; ++q) {
                     const float o = __shfl(score, sub * L + q * sh.lanes);
@@ -370,10 +371,10 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a, Route
                 const float low = -lanes_maxf<L>(kept ? -score : -INFINITY);
                 const float high = lanes_maxf<L>(kept || !in_group ? -INFINITY : score);
                 // two keys' errors on either side; a key's grows with it, not with the sum
-                const float size = fabsf(m1) + (m2 == -INFINITY ? 0.0f : fabsf(m2));
+                const float size = 0.5f * fabsf(m1) + (m2 == -INFINITY ? 0.0f : 0.5f * fabsf(m2));
                 const float most = lanes_maxf<L>(in_group && size < INFINITY ? size : 0.0f);
                 const bool doubt =
-                    high != -INFINITY && low < INFINITY && !(low - high > 4.0f * near + 0x1p-21f * most);
+                    high != -INFINITY && low < INFINITY && !(low - high > 2.0f * near + 0x1p-21f * most);
                 if (__ballot(doubt)) {
                     sum64();
                     // those that may be among the group's largest

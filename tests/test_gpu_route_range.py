@@ -258,3 +258,18 @@ def test_gradient_of_masked_choices_without_eps(scoring):
     idx = torch.tensor([[1, 2], [3, 5], [3, 5], [-1, -1], [3, 4]], dtype=torch.int32)
     got = check_grad(l, idx, values(5, 2, 13), "f32", scoring, eps=0.0)
     assert (got[1:4] == 0).all()
+
+
+# ---- groups ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_group_scores_past_f32(scoring, sign):
+    # sums of two biases near the largest f32: infinite in 32 bits, told apart in 64
+    l = logits_of(9, 32, 14, "f32")
+    bias = torch.zeros(32)
+    for g, top in enumerate((3.0e38, 3.2e38, 2.9e38, 3.1e38)):
+        bias[8 * g:8 * g + 8] = sign * top
+    idx, _, _ = nm.route(l.cuda(), 4, scoring=scoring, bias=bias.cuda(), groups=4, top_groups=1)
+    best = 1 if sign > 0 else 2
+    assert (idx // 8 == best).all()
