@@ -191,14 +191,14 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
         float r = 0.0f, k1 = 0.0f, iy = 1.0f, k2 = 0.0f;
         if constexpr (kNorm) {
             r = rsqrtf(m[0] * inv_d + a.eps);
-            k1 = r * r * r * (m[1] * inv_d);  // of out in d
+            k1 = r * (r * (r * (m[1] * inv_d)));  // of out in d (r^3 by itself leaves f32's range at rms 1e13)
         }
         if constexpr (kPost) {
             constexpr int k = kNorm ? 2 : 0;
             iy = rsqrtf(m[k] * inv_d + a.eps);
             float dot = m[k + 1];
             if constexpr (kNorm) dot += r * m[k + 2] - k1 * m[k + 3];
-            k2 = iy * iy * iy * (dot * inv_d);  // of y in dy
+            k2 = iy * (iy * (dot * inv_d));  // of y in dy / iy
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -225,8 +225,7 @@ void seam_grad_kernel(BlockSeamBackwardArgs a, SeamPlan p, float* sums) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     acc[2][c][i] += (iy * d[i]) * vy[i];
-                    w[i] = (iy * d[i]) * u[i];
-                    if constexpr (kPost) w[i] -= k2 * vy[i];
+                    w[i] = kPost ? iy * (d[i] * u[i] - k2 * vy[i]) : d[i] * u[i];
                 }
                 if (dy) put8(dy + o, col[c], w);
             }
