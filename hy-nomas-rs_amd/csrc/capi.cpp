@@ -7,6 +7,7 @@
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
+#include <limits>
 #include <memory>
 #include <new>
 #include <string>
@@ -596,9 +597,12 @@ int check_block_seam(int dtype, int64_t rows, int64_t dim, int64_t seq, double r
         return set_error(NOMAS_ERR_INVALID_ARGUMENT,
                          "rows=%lld must be a whole number of sequences of seq=%lld",
                          (long long)rows, (long long)seq);
-    if (!(eps >= 0.0)) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be >= 0");
-    if (!std::isfinite(residual_scale))
-        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "residual_scale must be finite");
+    // (the kernels take both as f32: a smaller eps would be none, and a row of zeros NaN)
+    using F32 = std::numeric_limits<float>;
+    if (eps != 0.0 && !(eps >= F32::min() && eps <= F32::max()))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be 0 or a positive normal f32");
+    if (!(std::abs(residual_scale) <= F32::max()))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "residual_scale must be finite as an f32");
     return NOMAS_OK;
 }
 
@@ -614,9 +618,12 @@ int check_route(int dtype, int64_t rows, int64_t experts, int64_t top_k, int sco
         return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
     if (scoring != NOMAS_SOFTMAX && scoring != NOMAS_SIGMOID)
         return set_error(NOMAS_ERR_INVALID_CONFIG, "unknown scoring %d", scoring);
-    if (!std::isfinite(scale)) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "scale must be finite");
-    if (!(eps >= 0.0) || !std::isfinite(eps))
-        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be >= 0 and finite");
+    // (the kernels take both as f32)
+    using F32 = std::numeric_limits<float>;
+    if (!(std::abs(scale) <= F32::max()))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "scale must be finite as an f32");
+    if (!(eps >= 0.0 && eps <= F32::max()))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "eps must be >= 0 and finite as an f32");
     return NOMAS_OK;
 }
 

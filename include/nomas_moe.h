@@ -278,7 +278,7 @@ enum nomas_scoring { NOMAS_SOFTMAX = 0, NOMAS_SIGMOID = 1 };
  * chosen s + eps) with renormalize, else scale * s; counts: (experts) rows
  * that chose each, or NULL.  A logit of -inf masks its expert, which is never
  * chosen; slots that stay empty hold -1 and weight 0.  A NaN counts as the largest
- * value.  Up to 1,024 experts and 64 groups. */
+ * value.  Up to 1,024 experts and 64 groups; scale and eps finite as f32, eps >= 0. */
 int nomas_route(int dtype, const void *logits, int64_t rows, int64_t experts, int64_t top_k,
                 int scoring, const float *bias, int64_t groups, int64_t top_groups,
                 int64_t group_top, int renormalize, double scale, double eps, int32_t *idx,
@@ -302,7 +302,7 @@ int nomas_route_backward(int dtype, const void *logits, const int32_t *idx, cons
  * with rms(v) = sqrt(mean(v^2) + eps).  Tensors (rows, dim) in `dtype`, f32
  * parameters: gate, shift, scale (rows / seq, dim), post_w, norm_w (dim); a NULL
  * one is 1 (shift, scale: 0).  Everything 16-byte aligned, dim % 8 == 0 and at most
- * 16,384.  f32 between the tensors: each output is rounded once, h is made from out before its
+ * 16,384; residual_scale finite as f32, eps 0 or a positive normal f32.  f32 between the tensors: each output is rounded once, h is made from out before its
  * rounding, and sums over a row are trees (nomas_norm_modulate and
  * nomas_gated_residual round where the reference does instead).  out may alias x or y,
  * and h the other one.  Asynchronous on `stream` (of the current device). */

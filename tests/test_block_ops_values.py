@@ -1,0 +1,38 @@
+"""Scalars of the routing and the block seams that f32 does not hold, and tensors that the
+Python mirror has to refuse by its own error -- CPU only."""
+import pytest
+import torch
+
+import nomas_moe as nm
+from nomas_moe import _lib
+from test_block_ops_refusals import BACK, P, SEAM, fake, lib, no_lib, refused, route  # noqa: F401
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(scale=1e39), "scale"), (dict(scale=-1e300), "scale"), (dict(eps=1e39), "eps"), (dict(eps=1e300), "eps"),
+])
+def test_route_scalars_past_f32(kw, text):
+    assert route(**kw) == 2
+    assert text in _lib.last_error() and "f32" in _lib.last_error()
+    a = dict(dtype=0, logits=P, idx=P, dw=P, rows=4, experts=8, k=2, scoring=0, renorm=1, scale=1.0, eps=1e-9, dl=P)
+    assert lib().nomas_route_backward(*{**a, **kw}.values(), None) == 2
+    assert text in _lib.last_error() and "f32" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(alpha=1e39), "residual_scale"), (dict(alpha=-1e300), "residual_scale"), (dict(eps=1e-39), "eps"),
+    (dict(eps=1e-50), "eps"),
+])
+def test_seam_scalars_that_f32_does_not_hold(kw, text):
+    assert lib().nomas_block_seam(*{**SEAM, **kw}.values(), None) == 2
+    assert text in _lib.last_error()
+    assert lib().nomas_block_seam_backward(*{**BACK, **kw}.values(), None) == 2
+    assert text in _lib.last_error()
+
+
+def test_scalars_at_the_ends_of_f32_are_taken():
+    none = dict(rows=0, logits=None, idx=None, w=None)
+    assert route(**none, scale=3e38, eps=3e38) == 0 and route(**none, scale=-3e38, eps=0.0) == 0
+    none = dict(rows=0, x=None, y=None, out=None, h=None)
+    for eps in (0.0, 2.0 ** -126, 3e38):
+        assert lib().nomas_block_seam(*{**SEAM, **none, "eps": eps, "alpha": 3e38}.values(), None) == 0
