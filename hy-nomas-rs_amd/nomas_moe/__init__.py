@@ -182,7 +182,8 @@ def _seam_input(x: torch.Tensor) -> torch.Tensor:
         raise NomasError(2, f"expected (B, L, D) activations, got shape {tuple(x.shape)}")
     if not x.is_cuda:
         raise NomasError(2, "the block seams take device tensors")
-    DataType.of(x.dtype)
+    if x.dtype not in _OF_TORCH:
+        raise NomasError(2, f"activations must be f32, bf16 or f16, got {x.dtype}")
     return x.contiguous()
 
 
@@ -428,13 +429,14 @@ def route_backward(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, *,
                    eps: float = 1e-9) -> torch.Tensor:
     """The gradient of route's weights with respect to the logits, of the logits'
     shape and dtype.  idx: route's choice (an index outside 0..E-1, or of a masked
-    expert: an empty slot, whose dw is not used); dw: the weights' gradient.  The choice itself has none, and so
-    neither has the bias."""
+    expert: an empty slot, whose dw is not used); dw: the weights' gradient.  The
+    choice itself has none, and so neither has the bias."""
     lc = _route_input(logits, scoring)
     E = lc.shape[-1]
     want = lc.shape[:-1]
     for t, n, dt in ((idx, "idx", torch.int32), (dw, "dw", torch.float32)):
-        if t.shape[:-1] != want or t.shape != idx.shape or t.dtype != dt or t.device != lc.device:
+        if t.dim() != lc.dim() or t.shape[:-1] != want or t.shape != idx.shape or \
+                t.dtype != dt or t.device != lc.device:
             raise NomasError(2, f"{n}: expected {tuple(want)} + (top_k,) {dt} on {lc.device}, got "
                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
     idx, dw = idx.contiguous(), dw.contiguous()

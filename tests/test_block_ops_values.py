@@ -36,3 +36,14 @@ def test_scalars_at_the_ends_of_f32_are_taken():
     none = dict(rows=0, x=None, y=None, out=None, h=None)
     for eps in (0.0, 2.0 ** -126, 3e38):
         assert lib().nomas_block_seam(*{**SEAM, **none, "eps": eps, "alpha": 3e38}.values(), None) == 0
+
+
+def test_the_mirrors_own_error_for_types_and_shapes(no_lib):  # noqa: F811
+    x64 = fake(2, 3, 16, dtype=torch.float64)
+    refused("f32, bf16 or f16", nm.block_seam, x64, x64)
+    refused("f32, bf16 or f16", nm.block_seam_backward, x64, x64, x64, x64)
+    refused("f32, bf16 or f16", nm.norm_modulate, x64, fake(2, 16), fake(2, 16))
+    refused("f32, bf16 or f16", nm.gated_residual, x64, x64, fake(2, 16))
+    # a row of logits with a choice that has no slots' dimension
+    refused("idx", nm.route_backward, fake(8), fake(1, dtype=torch.int32)[0], fake(1)[0])
+    refused("dw", nm.route_backward, fake(8), fake(2, dtype=torch.int32), fake(1)[0])
