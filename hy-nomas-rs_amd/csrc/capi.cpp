@@ -585,6 +585,24 @@ bool misaligned(std::initializer_list<const void*> ps, uintptr_t to) {
     return false;
 }
 
+// Whether tensors of n bytes at p and q share some of their memory, but are not the same.
+bool partly_shared(const void* p, const void* q, int64_t n) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return p && q && a != b && (a < b ? b - a : a - b) < (uint64_t)n;
+}
+
+// Rows are read and written in any order: an output may be an input, not a part of one.
+bool outputs_partly_shared(std::initializer_list<const void*> outputs, std::initializer_list<const void*> inputs,
+                           int64_t n) {
+    for (const void* o : outputs) {
+        for (const void* i : inputs)
+            if (partly_shared(o, i, n)) return true;
+        for (const void* p : outputs)
+            if (partly_shared(o, p, n)) return true;
+    }
+    return false;
+}
+
 // What the seam and its gradients ask of their arguments alike.
 int check_block_seam(int dtype, int64_t rows, int64_t dim, int64_t seq, double residual_scale, double eps) {
     if (dtype < 0 || dtype > 2) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
@@ -684,6 +702,8 @@ int nomas_route_backward(int dtype, const void* logits, const int32_t* idx, cons
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "logits, idx, dw and dlogits must be non-null");
         if (misaligned({logits, dlogits}, dtype == NOMAS_F32 ? 4 : 2) || misaligned({idx, dw}, 4))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "misaligned pointer");
+        if (partly_shared(logits, dlogits, rows * experts * (int64_t)nomas::dtype_size(static_cast<DType>(dtype))))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dlogits overlaps a part of logits");
         nomas::RouteBackwardArgs a;
         a.logits = logits;
         a.idx = idx;
@@ -717,6 +737,9 @@ int nomas_block_seam(int dtype, const void* x, const void* y, void* out, void* h
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "h and out must be different tensors");
         if (misaligned({x, y, out, h, gate, post_w, norm_w, shift, scale}, 16))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+        if (outputs_partly_shared({out, h}, {x, y},
+                                  rows * dim * (int64_t)nomas::dtype_size(static_cast<DType>(dtype))))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "out or h overlaps a part of another tensor");
         nomas::BlockSeamArgs a;
         a.x = x;
         a.y = y;
@@ -772,6 +795,9 @@ int nomas_block_seam_backward(int dtype, const void* dout, const void* dh, const
                         dpost_w, workspace},
                        16))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+        if (outputs_partly_shared({dx, dy}, {dout, dh, dh ? out : nullptr, y},
+                                  rows * dim * (int64_t)nomas::dtype_size(static_cast<DType>(dtype))))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "dx or dy overlaps a part of another tensor");
         const int64_t need = nomas::block_seam_workspace(rows, dim, seq);
         if (rows > 0 && (!workspace || workspace_bytes < need))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "the workspace holds %lld bytes, %lld are needed",

@@ -286,8 +286,8 @@ int nomas_route(int dtype, const void *logits, int64_t rows, int64_t experts, in
 
 /* dlogits (rows, experts; every element is written) from dw, the gradient of
  * nomas_route's w, for the choice idx (an index outside 0 .. experts - 1, or of a
- * masked expert, is an empty slot, whose dw is not used).  The other arguments as in the forward call; dlogits may alias
- * logits. */
+ * masked expert, is an empty slot, whose dw is not used).  The other arguments as in the forward call; dlogits may be
+ * logits, but not overlap a part of it. */
 int nomas_route_backward(int dtype, const void *logits, const int32_t *idx, const float *dw,
                          int64_t rows, int64_t experts, int64_t top_k, int scoring,
                          int renormalize, double scale, double eps, void *dlogits, void *stream);
@@ -304,8 +304,9 @@ int nomas_route_backward(int dtype, const void *logits, const int32_t *idx, cons
  * one is 1 (shift, scale: 0).  Everything 16-byte aligned, dim % 8 == 0 and at most
  * 16,384; residual_scale finite as f32, eps 0 or a positive normal f32.  f32 between the tensors: each output is rounded once, h is made from out before its
  * rounding, and sums over a row are trees (nomas_norm_modulate and
- * nomas_gated_residual round where the reference does instead).  out may alias x or y,
- * and h the other one.  Asynchronous on `stream` (of the current device). */
+ * nomas_gated_residual round where the reference does instead).  out may be x or y,
+ * and h the other one; overlapping a part of a tensor is refused.  Asynchronous on `stream`
+ * (of the current device). */
 int nomas_block_seam(int dtype, const void *x, const void *y, void *out, void *h, int64_t rows,
                      int64_t dim, int64_t seq, const float *gate, int post_norm,
                      const float *post_w, double residual_scale, const float *norm_w,
@@ -320,7 +321,8 @@ int64_t nomas_block_seam_workspace(int64_t rows, int64_t dim, int64_t seq);
  * call.  dx, dy (rows, dim) in `dtype`; dgate, dshift, dscale (rows / seq, dim) and
  * dnorm_w, dpost_w (dim) f32; each may be NULL (not wanted).  The sums over rows
  * have a fixed order: the same call gives the same bits.  workspace: 16-byte aligned, of
- * nomas_block_seam_workspace() bytes, the call's own while it runs. */
+ * nomas_block_seam_workspace() bytes, the call's own while it runs.  dx and dy may be
+ * dout, dh, out or y (not both the same one); overlapping a part of one is refused. */
 int nomas_block_seam_backward(int dtype, const void *dout, const void *dh, const void *out,
                               const void *y, void *dx, void *dy, int64_t rows, int64_t dim,
                               int64_t seq, const float *gate, int post_norm, const float *post_w,

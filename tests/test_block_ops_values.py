@@ -47,3 +47,31 @@ def test_the_mirrors_own_error_for_types_and_shapes(no_lib):  # noqa: F811
     # a row of logits with a choice that has no slots' dimension
     refused("idx", nm.route_backward, fake(8), fake(1, dtype=torch.int32)[0], fake(1)[0])
     refused("dw", nm.route_backward, fake(8), fake(2, dtype=torch.int32), fake(1)[0])
+
+
+# 6 rows of 64 bf16 are 768 bytes, 4 rows of 8 f32 128: tensors that lie nearer share memory
+APART = {**SEAM, "y": 2 * P, "out": 3 * P, "h": 4 * P}
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=P + 128), dict(out=P - 640), dict(out=2 * P + 16), dict(out=2 * P - 752), dict(h=P + 640),
+    dict(h=2 * P - 128), dict(h=3 * P + 16), dict(out=4 * P + 752), dict(out=P, y=P + 256),
+])
+def test_seam_outputs_that_share_part_of_a_tensor(kw):
+    assert lib().nomas_block_seam(*{**APART, **kw}.values(), None) == 2
+    assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dx=P + 128), dict(dx=2 * P + 256), dict(dy=P + 752), dict(dh=2 * P + 16), dict(y=3 * P, dy=3 * P - 512),
+])
+def test_seam_gradients_that_share_part_of_a_tensor(kw):
+    assert lib().nomas_block_seam_backward(*{**BACK, **kw}.values(), None) == 2
+    assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("dl", [P + 4, P + 124, P - 32])
+def test_route_gradient_that_shares_part_of_the_logits(dl):
+    a = dict(dtype=0, logits=P, idx=P, dw=P, rows=4, experts=8, k=2, scoring=0, renorm=1, scale=1.0, eps=1e-9, dl=dl)
+    assert lib().nomas_route_backward(*a.values(), None) == 2
+    assert "overlap" in _lib.last_error()
