@@ -30,7 +30,9 @@ struct SeamPlan {
 
 // `target`: blocks that fill the chip; `most`: threads of a block (a row may need
 // more).  Sequences are shared by blocks unless they are shorter than two rows of
-// each group or there are enough of them to fill the chip.
+// each group or there are enough of them to fill the chip.  A few short sequences of narrow rows are then
+// walked row by row by a group each, with most of the chip idle: 191 rows of 64 take 160 us in the gradients,
+// 47 of 256 45, 8 x 11 of 1,024 19; in the forward pass 127 rows of 64 take 54 us.
 inline SeamPlan seam_plan(int64_t rows, int64_t D, int64_t seq, int64_t target, int most) {
     SeamPlan p{};
     const int64_t chunks = D / kSeamCols;

@@ -22,20 +22,24 @@
 //
 // 14,232 rows of 1,536 bf16 (262 MB and 9 MB of sums): 60 us, 4.5 TB/s, and 5.6 for the sums; 5,998 rows of
 // 1,000 f32: 32 us and 4.6.  Loading the next row ahead takes registers that are worth more
-// as waves (114 us), a wave a row of three chunks a lane measured 58.5 and 37 us.  Rows past 8,192
-// columns hold four chunks a thread and spill: 1.9 TB/s at 16,384.
+// as waves (114 us), a wave a row of three chunks a lane measured 58.5 and 37 us.  At 128 registers
+// the bf16 form with both norms spills 6 of them (28 bytes of scratch a lane), narrow f32 rows 2.
+// Rows past 8,192 columns hold four chunks a thread and spill 86 to 387 with both norms: 2,000 rows of 16,384
+// take 195 us in bf16 and 306 in f32 (1.8 and 2.4 TB/s with the sums).
 #include "block_seam.hpp"
 
 namespace nomas {
 
 namespace {
 
-// Blocks of a call that fills the chip.  Each leaves 12 D bytes of sums, written and
-// read again.
 // Blocks and threads of a call that fills the chip: two blocks a CU, at 128 registers
-// all of them at once.  Each leaves 12 D bytes of sums, written and read again: 1,024
-// smaller blocks took as long, 768 blocks, of which a third run in a second round, 83 us
-// where 512 took 60 (14,232 rows of 1,536 bf16).
+// all of them at once where a block has six waves (768 or 1,536 columns, or narrow rows).  Each leaves 12 D
+// bytes of sums, written and read again: 1,024 smaller blocks took as long, 768 blocks, of which a third run
+// in a second round, 83 us where 512 took 60 (14,232 rows of 1,536 bf16).
+// What the fixed number costs: rows of 2,048 columns have four waves a block, of 2,560 five, so that a CU is not
+// full (14,232 rows: 89 us, 3.9 TB/s, and 109, 4.0); and a number of sequences that does not divide 512 passes it,
+// since parts are rounded up (3 x 8,192 rows of 1,536 in 513 blocks 129 us, 3.5 TB/s; 24 x 592 in 528, 84 us, 3.1;
+// 3 x 4,744 in 510, 60 us, 4.4).
 constexpr int64_t kGradBlocks = 512;
 constexpr int kGradThreads = 384;
 

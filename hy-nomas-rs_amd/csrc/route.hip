@@ -24,9 +24,13 @@
 //    Without bias and groups the keys are the logits: nothing is near, ties are exact.
 //  - The chosen indices meet in LDS, and lane t of a row makes the weight of slot t.
 //
-// 32,768 rows of 256 f32, sigmoid and bias, 8 groups, top-8: 20.9 us (an f64 wave a row: 196),
-// of which the read 7.2, keys 2.5, lists and groups 2, rounds 4, choice and weights 4,
-// doubtful rows 2.3; 4,744 rows of 64 bf16 4.5 us; one row 4.4.  With the counts 3 us more.
+// 32,768 rows of 256 f32, sigmoid and bias, 8 groups, top-8: 21.5 us (an f64 wave a row: 196).
+// Leaving one part out at a time makes it shorter by: the read 7.2, keys 2.5, lists and groups 2,
+// rounds 4, choice and weights 4, doubtful rows 2.3 (they overlap somewhat).  The masks of the loads
+// that are no vector loads, kept for all rows, push 107 scalar registers into vector ones.  4,744 rows of
+// 64 bf16 4.6 us; one row 4.6.  The counts take 3 (4,744 rows) to 4 us more.  Top-24 of the same rows
+// (bisection) 37 us; 8,192 rows of 1,000 f32, softmax top-8, 37 us; of 1,020 in 60 groups, 32 values a
+// lane at 179 registers, top-32, 91 us.
 #include <algorithm>
 #include <climits>
 #include <type_traits>

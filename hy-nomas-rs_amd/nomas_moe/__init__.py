@@ -600,7 +600,9 @@ class MoeLayer:
         shared dense branch, where there is one).  x: (..., D) on the layer's
         GPU; idx: (..., top_k) int32 and w: (..., top_k) f32, as route gives
         them, in any order.  An index outside 0..E-1 is an empty slot, which
-        adds nothing; an expert named twice in a row has the sum of its weights."""
+        adds nothing; an expert named twice in a row has the sum of its weights.
+        Hidden activations and each expert's output are rounded to the model
+        dtype, as in forward, whose bits it gives for the router's own routing."""
         if x.dim() < 1 or x.shape[-1] != self.dim:
             raise NomasError(2, f"expected last dim {self.dim}, got shape {tuple(x.shape)}")
         if x.dtype != self.dtype.torch:

@@ -124,8 +124,11 @@ int nomas_moe_forward_noalloc(nomas_moe_t *h, const void *x, void *y, int64_t ro
  * slots of w * FFN_idx(x), plus the shared dense branch where the layer has
  * one.  An index outside 0 .. E - 1 is an empty slot: it adds nothing and
  * costs no product.  An expert named twice in a row has the sum of its
- * weights.  nomas_moe_routing() reports the routing as it was run (ascending,
- * -1 for empty slots, gap +inf). */
+ * weights.  The arithmetic is nomas_moe_forward's: the hidden activations and each
+ * expert's output are rounded to the handle's dtype before the weighted sum
+ * (a bf16 result is 2.9e-3 off, where one rounding of an f32 result is 1.7e-3); with the
+ * router's own routing the bits are the same.  nomas_moe_routing() reports the
+ * routing as it was run (ascending, -1 for empty slots, gap +inf). */
 int nomas_moe_forward_routed(nomas_moe_t *h, const void *x, const int32_t *idx, const float *w,
                              void *y, int64_t rows, void *stream);
 
