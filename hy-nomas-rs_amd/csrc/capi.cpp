@@ -833,6 +833,110 @@ int nomas_block_seam_backward(int dtype, const void* dout, const void* dh, const
     });
 }
 
+namespace {
+
+struct Span {
+    const void* p;
+    int64_t bytes;
+};
+// Whether the output shares memory with any of the inputs.
+bool shares(const Span& out, std::initializer_list<Span> inputs) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out.p);
+    for (const Span& in : inputs) {
+        const uintptr_t i = reinterpret_cast<uintptr_t>(in.p);
+        if (out.p && in.p && o < i + (uint64_t)in.bytes && i < o + (uint64_t)out.bytes) return true;
+    }
+    return false;
+}
+
+int64_t fp8_blocks(int64_t n) { return (n + nomas::kFp8Block - 1) / nomas::kFp8Block; }
+
+}  // namespace
+
+int nomas_quantize_fp8(int dtype, const void* x, int64_t rows, int64_t cols, int square, void* q, float* scale,
+                       void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (dtype < 0 || dtype > 2) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+        if (cols < 16 || cols % 16 != 0 || cols > 0x7fffff00)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "cols must be a positive multiple of 16 (got %lld)",
+                             (long long)cols);
+        if (rows < 0 || rows > 0x7fffffffLL || rows * fp8_blocks(cols) > 0x7fffffffLL ||
+            (square && fp8_blocks(rows) > 65535))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
+        if (rows == 0) return NOMAS_OK;
+        if (!x || !q || !scale) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "x, q and scale must be non-null");
+        if (misaligned({x, q}, 16) || misaligned({scale}, 4))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "misaligned pointer");
+        const Span sx{x, rows * cols * (int64_t)nomas::dtype_size(static_cast<DType>(dtype))}, sq{q, rows * cols},
+            ss{scale, (square ? fp8_blocks(rows) : rows) * fp8_blocks(cols) * 4};
+        if (shares(sq, {sx, ss}) || shares(ss, {sx}))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "q or scale shares memory with another tensor");
+        hipError_t e;
+        if (square) {
+            nomas::QuantSquareArgs a = {};
+            a.x = x;
+            a.q = static_cast<uint8_t*>(q);
+            a.scale = scale;
+            a.rows = (int)rows;
+            a.cols = (int)cols;
+            a.batch = 1;
+            a.x_step = 32;
+            a.x_row = cols;
+            a.row_group = 32;
+            a.ld_q = (int)cols;
+            e = nomas::launch_quant_squares(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        } else {
+            nomas::QuantArgs a;
+            a.x = x;
+            a.q = static_cast<uint8_t*>(q);
+            a.scale = scale;
+            a.rows = rows;
+            a.cols = a.ld_q = (int)cols;
+            e = nomas::launch_quant_rows(static_cast<DType>(dtype), a, static_cast<hipStream_t>(stream));
+        }
+        if (e != hipSuccess) return set_error(NOMAS_ERR_HIP, "quantize launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
+int nomas_matmul_fp8(int dtype, const void* a, const float* a_scale, const void* b, const float* b_scale,
+                     const float* bias, void* y, int64_t rows, int64_t n, int64_t k, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (dtype < 0 || dtype > 2) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+        if (k < 16 || k % 16 != 0 || k > nomas::kFp8MaxK)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "k must be a multiple of 16 up to %d (got %lld)",
+                             nomas::kFp8MaxK, (long long)k);
+        if (n < 0 || n > nomas::kFp8MaxN)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "n=%lld out of range", (long long)n);
+        if (rows < 0 || rows > nomas::kFp8MaxRows)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
+        if (rows == 0 || n == 0) return NOMAS_OK;
+        if (!a || !a_scale || !b || !b_scale || !y)
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "a, b, their scales and y must be non-null");
+        if (misaligned({a, b, y}, 16) || misaligned({a_scale, b_scale, bias}, 4))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "misaligned pointer");
+        if (shares({y, rows * n * (int64_t)nomas::dtype_size(static_cast<DType>(dtype))},
+                   {{a, rows * k}, {a_scale, rows * fp8_blocks(k) * 4}, {b, n * k},
+                    {b_scale, fp8_blocks(n) * fp8_blocks(k) * 4}, {bias, n * 4}}))
+            return set_error(NOMAS_ERR_INVALID_ARGUMENT, "y shares memory with an input");
+        nomas::Fp8GemmArgs g;
+        g.a = static_cast<const uint8_t*>(a);
+        g.as = a_scale;
+        g.b = static_cast<const uint8_t*>(b);
+        g.bs = b_scale;
+        g.bias = bias;
+        g.y = y;
+        g.M = rows;
+        g.N = (int)n;
+        g.K = (int)k;
+        const hipError_t e = nomas::launch_fp8_gemm(static_cast<DType>(dtype), g, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return set_error(NOMAS_ERR_HIP, "8-bit product launch failed: %s", hipGetErrorString(e));
+        return NOMAS_OK;
+    });
+}
+
 const char* nomas_moe_last_error(void) { return nomas::last_error(); }
 
 uint64_t nomas_path_seed(uint64_t seed, const char* path) {

@@ -294,6 +294,49 @@ struct BlockSeamBackwardArgs {
     float *dnorm_w, *dpost_w;        // D
     void* workspace;                 // block_seam_workspace() bytes
 };
+// 8-bit values with a scale for each block of 128 (fp8_quant.hip, fp8.hpp).
+struct QuantArgs {
+    const void* x;  // rows x cols, model dtype
+    uint8_t* q;     // rows x ld_q (columns past `cols` are written as zeros)
+    float* scale;   // rows x ceil(ld_q / 128)
+    int64_t rows;
+    int cols, ld_q;
+};
+// Squares of 128 x 128 of `batch` matrices.  Element (r, c) of x is at
+// c / 32 x_step + (r / 32 row_group + r % 32) x_row + c % 32, so that it may lie K-blocked and
+// with groups of 32 rows apart; its value at row r / 32 row_group + r % 32 of q.
+struct QuantSquareArgs {
+    const void* x;
+    uint8_t* q;
+    float* scale;  // ceil(rows / 128) x ceil(cols / 128) each
+    int rows, cols, batch;
+    int64_t x_batch, x_step, x_row, row_group;
+    int64_t q_batch, scale_batch;
+    int ld_q;        // of row-major q
+    int fragments;   // q in fragments of 16 rows x 64 columns (few.hip) of a matrix of q_rows rows
+    int64_t q_rows;
+};
+hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s);
+hipError_t launch_quant_squares(DType dt, const QuantSquareArgs& a, hipStream_t s);
+
+constexpr int kFp8Block = 128;
+// columns of a product (a tile of 256 rows: 2^30 bytes), its weight rows and rows
+constexpr int kFp8MaxK = 1 << 22;
+constexpr int kFp8MaxN = 1 << 24;
+constexpr int64_t kFp8MaxRows = (int64_t)1 << 30;
+// Products of 8-bit matrices with block scales (fp8_gemm.hip).
+struct Fp8GemmArgs {
+    const uint8_t* a;  // M x K
+    const float* as;   // M x ceil(K / 128)
+    const uint8_t* b;  // N x K
+    const float* bs;   // ceil(N / 128) x ceil(K / 128)
+    const float* bias; // N (null: none)
+    void* y;           // M x N
+    int64_t M;
+    int N, K;          // K % 16 == 0
+};
+// y = a b^T + bias in `dt`.
+hipError_t launch_fp8_gemm(DType dt, const Fp8GemmArgs& a, hipStream_t s);
 int64_t block_seam_workspace(int64_t rows, int64_t D, int64_t seq);
 hipError_t launch_block_seam(DType dt, const BlockSeamArgs& a, hipStream_t s);
 hipError_t launch_block_seam_backward(DType dt, const BlockSeamBackwardArgs& a, hipStream_t s);

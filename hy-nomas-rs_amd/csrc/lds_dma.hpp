@@ -36,6 +36,22 @@ __device__ __forceinline__ void lds_dma16_buf(__amdgpu_buffer_rsrc_t rsrc, uint3
                  : "v"(voff), "s"(rsrc), "s"(lds_base)
                  : "memory", "m0");
 }
+// The same with a uniform byte offset added to the address (not to what is checked
+// against num_records).
+__device__ __forceinline__ void lds_dma16_buf_s(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff,
+                                                uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds_base)
+                 : "memory", "m0");
+}
+// 4 bytes per lane: lane l's land at lds_base + 4 * l.
+__device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(voff), "s"(sbase), "s"(lds_base)
+                 : "memory", "m0");
+}
 // Groups of loads into consecutive 1 KB LDS blocks: M0 is written once per
 // group (set_lds_m0) and load q of the group carries q * 1024 in its
 // immediate offset, which the hardware adds to both the global (or buffer)

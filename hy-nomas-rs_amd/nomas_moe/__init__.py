@@ -29,6 +29,7 @@ __all__ = [
     "DataType", "MoeConfig", "Weights", "MoeLayer", "FeedForward", "NomasError", "InvalidConfig",
     "WeightKey", "IoError", "path_seed", "randn_affine", "to_model_dtype", "norm_modulate",
     "gated_residual", "block_seam", "block_seam_backward", "route", "route_backward",
+    "quantize_fp8", "matmul_fp8",
 ]
 
 
@@ -446,6 +447,85 @@ def route_backward(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, *,
           dw.data_ptr(), rows, E, idx.shape[-1], _SCORING[scoring], int(renormalize), float(scale),
           float(eps), dl.data_ptr())
     return dl
+
+
+# ---- 8-bit values with a scale for each block of 128 ---------------------------
+
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+def quantize_fp8(x: torch.Tensor, *, square: bool = False):
+    """(q, scale): x as e4m3 with an f32 scale for each block of 128.
+
+        scale = max(largest magnitude of the block / 448, 2^-126)
+        q     = x / scale, rounded to the nearest e4m3 (once)
+
+    x: (..., K) device tensor in f32 / bf16 / f16, K a multiple of 16.  Blocks are 128
+    columns of a row (activations; scale (..., ceil(K / 128))), or with square=True
+    squares of 128 x 128 of a matrix (weights; x (N, K), scale (ceil(N / 128), ceil(K / 128))).
+    A block with an infinity or a NaN becomes NaN, scale and values."""
+    if x.dim() < 1 or (square and x.dim() != 2):
+        raise NomasError(2, f"expected {'(N, K)' if square else '(..., K)'} values, got shape "
+                            f"{tuple(x.shape)}")
+    if not x.is_cuda:
+        raise NomasError(2, "quantize_fp8 takes device tensors")
+    if x.dtype not in _CODES:
+        raise NomasError(2, f"values must be f32, bf16 or f16, got {x.dtype}")
+    K = x.shape[-1]
+    if K < 16 or K % 16:
+        raise NomasError(2, f"the last dimension must be a positive multiple of 16, got {K}")
+    xc = x.contiguous()
+    rows = xc.numel() // K
+    q = torch.empty(xc.shape, dtype=FP8, device=xc.device)
+    lead = (_blocks(rows),) if square else xc.shape[:-1]
+    scale = torch.empty(lead + (_blocks(K),), dtype=torch.float32, device=xc.device)
+    _call(_lib.lib().nomas_quantize_fp8, xc, _CODES[xc.dtype], xc.data_ptr(), rows, K, int(square),
+          q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
+def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, *, dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """a b^T + bias (..., N) in `dtype` of 8-bit values with block scales.
+
+    a: (..., K) e4m3 with a_scale (..., ceil(K / 128)), as quantize_fp8 gives them; b: (N, K)
+    e4m3 with b_scale (ceil(N / 128), ceil(K / 128)), as quantize_fp8(square=True) does; any f32
+    scales.  K a multiple of 16; bias: (N,).  Sums in f32, rounded once; for 16-bit results the
+    matrix instructions keep 13 bits below the largest of each 8 products (1.4e-5 of a result on
+    random values), f32 results have exact products."""
+    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+        raise NomasError(2, f"expected (..., K) and (N, K) values, got {tuple(a.shape)} and "
+                            f"{tuple(b.shape)}")
+    if a.dtype is not FP8 or b.dtype is not FP8:
+        raise NomasError(2, f"a and b must be {FP8}, got {a.dtype} and {b.dtype}")
+    if not a.is_cuda or b.device != a.device:
+        raise NomasError(2, f"matmul_fp8 takes tensors on one GPU, got {a.device} and {b.device}")
+    if dtype not in _CODES:
+        raise NomasError(2, f"the result must be f32, bf16 or f16, got {dtype}")
+    N, K = b.shape
+    if K < 16 or K % 16:
+        raise NomasError(2, f"K must be a positive multiple of 16, got {K}")
+    for t, n, want in ((a_scale, "a_scale", a.shape[:-1] + (_blocks(K),)),
+                       (b_scale, "b_scale", (_blocks(N), _blocks(K)))):
+        if t.shape != want or t.dtype is not torch.float32 or t.device != a.device:
+            raise NomasError(2, f"{n}: expected {tuple(want)} f32 on {a.device}, got "
+                                f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    ac, bc, sa, sb = a.contiguous(), b.contiguous(), a_scale.contiguous(), b_scale.contiguous()
+    bias = _param(bias, ac, (N,), "bias")
+    shape = a.shape[:-1] + (N,)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=ac.device)
+    else:
+        _check_out(out, torch.empty((), dtype=dtype, device=ac.device).expand(shape))
+    _call(_lib.lib().nomas_matmul_fp8, ac, _CODES[dtype], ac.data_ptr(), sa.data_ptr(),
+          bc.data_ptr(), sb.data_ptr(), _ptr(bias), out.data_ptr(), ac.numel() // K, N, K)
+    return out
 
 
 class Weights:

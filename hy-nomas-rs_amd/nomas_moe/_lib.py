@@ -112,6 +112,10 @@ def lib() -> C.CDLL:
     L.nomas_block_seam_backward.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, i32, vp,
                                             f64, vp, vp, f64, vp, vp, vp, vp, vp, vp, i64, vp]
     L.nomas_block_seam_backward.restype = i32
+    L.nomas_quantize_fp8.argtypes = [i32, vp, i64, i64, i32, vp, vp, vp]
+    L.nomas_quantize_fp8.restype = i32
+    L.nomas_matmul_fp8.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp]
+    L.nomas_matmul_fp8.restype = i32
     L.nomas_ffn_destroy.argtypes = [vp]
     L.nomas_ffn_destroy.restype = None
     L.nomas_moe_last_error.argtypes = []

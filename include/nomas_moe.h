@@ -334,6 +334,31 @@ int nomas_block_seam_backward(int dtype, const void *dout, const void *dh, const
                               float *dnorm_w, float *dpost_w, void *workspace,
                               int64_t workspace_bytes, void *stream);
 
+/* ---- 8-bit values with a scale for each block of 128 ------------------------------
+ * No counterpart in the reference.  Values are e4m3 (1 sign, 4 exponent, 3 mantissa bits,
+ * largest 448, no infinities), a block's scale an f32:
+ *   scale = max(largest magnitude / 448, 2^-126), rounded to the nearest
+ *   q     = x / scale, rounded to the nearest e4m3 (once)
+ * A block with an infinity or a NaN has scale NaN and values NaN.  Device pointers,
+ * asynchronous on `stream` (of the current device); nothing is allocated. */
+
+/* x (rows, cols) in `dtype` -> q (rows, cols) and scale: (rows, ceil(cols / 128)) for blocks
+ * along the rows (activations), or (ceil(rows / 128), ceil(cols / 128)) with `square` for
+ * blocks of 128 x 128 (weights).  cols % 16 == 0; x and q 16-byte, scale 4-byte aligned; outputs
+ * share no memory with x or each other.  rows * ceil(cols / 128) < 2^31. */
+int nomas_quantize_fp8(int dtype, const void* x, int64_t rows, int64_t cols, int square, void* q, float* scale,
+                       void* stream);
+
+/* y (rows, n) in `dtype` = a b^T + bias, a (rows, k) with scales (rows, ceil(k / 128)), b (n, k)
+ * with scales (ceil(n / 128), ceil(k / 128)), any f32 values; bias n f32 or NULL.  A block's
+ * sums are scaled and added in f32, and rounded once.  For 16-bit results the 8-bit matrix
+ * instructions make them, which keep 13 bits below the largest of each 8 products (1.4e-5 of a
+ * result on random values); f32 results have exact products and f32 sums.  The order of the
+ * sums depends on the sizes.  1 <= k <= 2^22 with k % 16 == 0; a, b and y 16-byte, the
+ * others 4-byte aligned; y shares no memory with the inputs. */
+int nomas_matmul_fp8(int dtype, const void* a, const float* a_scale, const void* b, const float* b_scale,
+                     const float* bias, void* y, int64_t rows, int64_t n, int64_t k, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 const char *nomas_moe_last_error(void);
 
