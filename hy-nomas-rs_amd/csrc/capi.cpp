@@ -328,6 +328,24 @@ int nomas_moe_forward_routed(nomas_moe_t* h, const void* x, const int32_t* idx, 
     });
 }
 
+int nomas_moe_forward_few(nomas_moe_t* h, const void* x, const int32_t* idx, const float* w, int fp8, void* y,
+                          int64_t rows, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
+        const MoeLayer::Given given{idx, w};
+        return h->layer->forward_few(x, idx || w ? &given : nullptr, fp8 != 0, y, rows, static_cast<hipStream_t>(stream));
+    });
+}
+
+int nomas_moe_quantize(nomas_moe_t* h) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
+        return h->layer->quantize();
+    });
+}
+
 int nomas_moe_forward_host(nomas_moe_t* h, const void* x, void* y, int64_t rows) {
     return guarded(__func__, [&]() -> int {
         nomas::clear_error();
@@ -476,6 +494,22 @@ int nomas_ffn_forward(nomas_ffn_t* h, const void* x, void* y, int64_t rows, void
         nomas::clear_error();
         if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
         return h->layer->forward(x, y, rows, static_cast<hipStream_t>(stream));
+    });
+}
+
+int nomas_ffn_quantize(nomas_ffn_t* h) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
+        return h->layer->quantize();
+    });
+}
+
+int nomas_ffn_forward_fp8(nomas_ffn_t* h, const void* x, void* y, int64_t rows, void* stream) {
+    return guarded(__func__, [&]() -> int {
+        nomas::clear_error();
+        if (!h) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "null handle");
+        return h->layer->forward_fp8(x, y, rows, static_cast<hipStream_t>(stream));
     });
 }
 
@@ -921,7 +955,7 @@ int nomas_matmul_fp8(int dtype, const void* a, const float* a_scale, const void*
                    {{a, rows * k}, {a_scale, rows * fp8_blocks(k) * 4}, {b, n * k},
                     {b_scale, fp8_blocks(n) * fp8_blocks(k) * 4}, {bias, n * 4}}))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "y shares memory with an input");
-        nomas::Fp8GemmArgs g;
+        nomas::Fp8GemmArgs g = {};
         g.a = static_cast<const uint8_t*>(a);
         g.as = a_scale;
         g.b = static_cast<const uint8_t*>(b);

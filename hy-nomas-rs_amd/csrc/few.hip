@@ -1,0 +1,523 @@
+// The MoE layer on up to 64 rows: gate/up with SwiGLU, then down with the weighted sum, each one
+// kernel over all chosen experts.
+//
+//   h[e, r] = silu(x_r Wg_e^T + bg_e) (x_r Wu_e^T + bu_e)         for the rows r that chose e
+//   y_r     = sum over the chosen e, ascending, of w[r, e] (h[e, r] Wd_e^T + bd_e)
+//
+// What bounds such a call is the chosen experts' weights on their way from HBM, and for the
+// smallest ones the launches.  So there is no dispatch: as a block starts, it makes the lists of
+// the rows that chose each expert from the routing (a 64-bit mask per expert), and reads
+// rows where they are; and no combine: a block of the second kernel has a tile of 16
+// columns for all rows and experts, or shares it with a few others.  Weights are read in the layouts that
+// the layer keeps (K-blocked, kernels.hpp), a 16 x 16-byte fragment of an MFMA per instruction, straight
+// into registers, or as 8-bit values in fragment order, widened there.
+#include "fp8.hpp"
+#include "mfma.hpp"
+
+#include <algorithm>
+
+namespace nomas {
+
+namespace {
+
+constexpr int kFewThreads = 512;
+constexpr int kFewWaves = kFewThreads / kWave;
+
+// Fragments of a step of KS columns: two of 16 weight rows x 64 bytes, XL of 16 token rows x 16 bytes
+// a lane.  xk: the lane's column of the q-th token fragment in a step.
+template <typename T, bool W8> struct Step {
+    static constexpr int KS = W8 ? 128 : 128 / (int)sizeof(T), XL = W8 ? 4 : 2, CH = 16 / (int)sizeof(T);
+    static __device__ __forceinline__ int xk(int q, int lq) {
+        return W8 ? q / 2 * 64 + lq * 16 + q % 2 * 8 : q * (KS / 2) + lq * CH;
+    }
+};
+
+template <typename T> struct Widen8;
+template <> struct Widen8<__bf16> {
+    typedef __bf16 V2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ V2 run(uint32_t w, bool hi) {
+        return hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false);
+    }
+};
+template <> struct Widen8<_Float16> {
+    typedef _Float16 V2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ V2 run(uint32_t w, bool hi) {
+        return hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false);
+    }
+};
+
+// acc += the step's products.  `s`: the scale of 8-bit weights, else what f32 weights are taken down by.
+template <typename T, bool W8>
+__device__ __forceinline__ void multiply(f32x4_t& acc, const u32x4_t (&w)[2], const u32x4_t (&x)[Step<T, W8>::XL],
+                                         float s) {
+    if constexpr (W8) {
+        typedef typename Mfma<T>::V V;
+        f32x4_t t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            V a;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const auto v = Widen8<T>::run(w[q / 2][q % 2 * 2 + i], h);
+                    a[i * 4 + h * 2] = v[0];
+                    a[i * 4 + h * 2 + 1] = v[1];
+                }
+            t = Mfma<T>::run(a, __builtin_bit_cast(V, x[q]), t);
+        }
+        // The result is there 8 wait states after the last MFMA.  The compiler moved its use behind a
+        // branch that skips the next rows' products and counted the waits along the longer
+        // way only: every fourth column was wrong.  So the wait stands here.
+        asm volatile("s_nop 8" : "+v"(t));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(t[r], s, acc[r]);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                acc = mfma_f32(__uint_as_float(w[q][k]) * s, __uint_as_float(x[q][k]), acc);
+    } else {
+        typedef typename Mfma<T>::V V;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            acc = Mfma<T>::run(__builtin_bit_cast(V, w[q]), __builtin_bit_cast(V, x[q]), acc);
+    }
+}
+
+__device__ __forceinline__ u32x4_t load16u(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+
+// What a block knows of the routing.
+struct Lists {
+    uint64_t* mask;  // [Ecols] rows that chose the expert
+    int* live;       // [Ecols] the chosen experts, ascending
+    int* off;        // [Ecols] by place in `live`: the expert's first place in `row`
+    int* info;       // [16] scratch; [0]: chosen experts
+    uint8_t* row;    // [rows * slots] the experts' rows, one after another
+    float* gate;     // ... and their weights (second kernel)
+    static __host__ __device__ size_t bytes(int ecols, int places, bool gates) {
+        return (size_t)ecols * 16 + 64 + (size_t)(places + 15) / 16 * 16 + (gates ? (size_t)places * 4 : 0);
+    }
+    __device__ Lists(uint8_t* p, int ecols, int places) {
+        mask = reinterpret_cast<uint64_t*>(p);
+        live = reinterpret_cast<int*>(p + (size_t)ecols * 8);
+        off = live + ecols;
+        info = off + ecols;
+        row = reinterpret_cast<uint8_t*>(info + 16);
+        gate = reinterpret_cast<float*>(row + (places + 15) / 16 * 16);
+    }
+};
+
+// Experts named twice by a row have the sum of their weights, at the first mention.
+template <bool kGates>
+__device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
+    const int tid = threadIdx.x, n = a.rows * a.k, lane = tid & 63, wave = tid >> 6;
+    for (int e = tid; e < a.Ecols; e += kFewThreads)
+        l.mask[e] = e < a.E ? 0 : ~0ull >> (64 - a.rows);  // (the shared branch: all rows)
+    __syncthreads();
+    for (int i = tid; i < n; i += kFewThreads) {
+        const int e = a.idx[i];
+        if (e >= 0 && e < a.E) atomicOr(reinterpret_cast<unsigned long long*>(&l.mask[e]), 1ull << (i / a.k));
+    }
+    __syncthreads();
+    // places: the chosen experts before, and their rows (512 threads hold all experts)
+    static_assert(kMaxExperts + 1 <= kFewThreads, "an expert a thread");
+    const int c = tid < a.Ecols ? __popcll(l.mask[tid]) : 0;
+    const uint64_t some = __ballot(c > 0);
+    int sum = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 63) l.info[wave] = __popcll(some) << 16 | sum;
+    __syncthreads();
+    int before = 0, first = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) {
+        const int v = l.info[w];
+        all += v >> 16;
+        if (w < wave) {
+            before += v >> 16;
+            first += v & 0xffff;
+        }
+    }
+    __syncthreads();
+    if (c > 0) {
+        const int at = before + __popcll(some & ((1ull << lane) - 1));
+        l.live[at] = tid;
+        l.off[at] = first + sum - c;
+        int p = first + sum - c;
+        for (uint64_t m = l.mask[tid]; m; m &= m - 1) {
+            const int r = __builtin_ctzll(m);
+            l.row[p] = (uint8_t)r;
+            if constexpr (kGates) {
+                float w = tid < a.E ? 0.0f : a.dense_coef;
+                if (tid < a.E)
+                    for (int t = 0; t < a.k; ++t) w += a.idx[r * a.k + t] == tid ? a.w[r * a.k + t] : 0.0f;
+                l.gate[p] = w;
+            }
+            ++p;
+        }
+    }
+    if (tid == 0) l.info[0] = all;
+    __syncthreads();
+}
+
+// Waits for this wave's LDS traffic and for the other waves, not for loads in flight.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <typename T, bool W8>
+__device__ __forceinline__ uint32_t weight_lane(int l16, int lq) {
+    return W8 ? (uint32_t)(lq * 256 + l16 * 16) : (uint32_t)(l16 * 64 + lq * 16);
+}
+
+// S waves share a unit (16 hidden units of one expert: 16 gate and 16 up rows), each its own
+// share of the steps.
+template <typename T, bool W8, int NT, int S, int P>
+__global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
+    typedef Step<T, W8> St;
+    constexpr int GP = kFewWaves / S;  // units a block has at a time
+    extern __shared__ __align__(16) uint8_t s_dyn[];
+    __shared__ f32x4_t s_part[S > 1 ? kFewWaves : 1][2][NT][kWave];
+    const Lists l(s_dyn, a.Ecols, a.rows * (a.k + a.Ecols - a.E));
+    make_lists<false>(a, l);
+
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = wave / S, part = wave % S;
+    const int tiles = (a.H + 15) / 16, units = __builtin_amdgcn_readfirstlane(l.info[0]) * tiles;
+    const int steps = (a.D + St::KS - 1) / St::KS, s0 = steps * part / S, s1 = steps * (part + 1) / S;
+    const uint32_t wl = weight_lane<T, W8>(l16, lq);
+    const int64_t kstep = (int64_t)a.N1 * kKBlockBytes;
+
+    struct Unit {
+        int e, off, n, n0;         // expert, its first place and rows, the gate rows' place
+        const uint8_t* w;          // ... and address
+        const uint8_t* x[NT];      // the lane's token rows
+        const float *sg, *su;      // 8-bit weights: scales of its gate and up rows
+    };
+    auto unit = [&](int u, Unit& t) {
+        const int li = u / tiles, ht = u - li * tiles;
+        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
+        t.off = __builtin_amdgcn_readfirstlane(l.off[li]);
+        t.n = __popcll(l.mask[t.e]);
+        t.n = __builtin_amdgcn_readfirstlane(t.n);
+        t.n0 = ht / 2 * 64 + ht % 2 * 16;
+        t.w = static_cast<const uint8_t*>(a.w1) + (int64_t)t.e * a.w1_expert + (int64_t)t.n0 * kKBlockBytes;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            t.x[j] = static_cast<const uint8_t*>(a.x) + (int64_t)l.row[t.off + min(j * 16 + l16, t.n - 1)] * a.D * sizeof(T);
+        if constexpr (W8) {
+            t.sg = a.s1 + ((int64_t)t.e * 2 * a.hb + ht / 8) * a.kb1;
+            t.su = t.sg + (int64_t)a.hb * a.kb1;
+        }
+    };
+    struct Data {
+        u32x4_t w[2][2], x[NT][St::XL];
+        float s[2];
+    };
+    auto fetch = [&](const Unit& t, int st, Data& d) {
+        const uint8_t* p = t.w + 2 * st * kstep + wl;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) d.w[i][q] = load16u(p + q * kstep + i * 32 * kKBlockBytes);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            if (j * 16 >= t.n) break;
+#pragma unroll
+            for (int q = 0; q < St::XL; ++q) {
+                const int k = st * St::KS + St::xk(q, lq);
+                d.x[j][q] = u32x4_t{0, 0, 0, 0};
+                if (k < a.D) d.x[j][q] = load16u(t.x[j] + k * sizeof(T));
+            }
+        }
+        if constexpr (W8) {
+            d.s[0] = t.sg[st];
+            d.s[1] = t.su[st];
+        } else {
+            d.s[0] = d.s[1] = a.w1_down;
+        }
+    };
+    for (int u0 = blockIdx.x * GP; u0 < units; u0 += gridDim.x * GP) {
+        const bool mine = u0 + g < units;
+        Unit t;
+        f32x4_t acc[2][NT];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        unit(min(u0 + g, units - 1), t);
+        if (mine) {
+            Data d[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (s0 + p < s1) fetch(t, s0 + p, d[p]);
+            for (int st = s0; st < s1; st += P) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    if (st + p >= s1) break;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if (j * 16 >= t.n) break;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) multiply<T, W8>(acc[i][j], d[p].w[i], d[p].x[j], d[p].s[i]);
+                    }
+                    if (st + p + P < s1) fetch(t, st + p + P, d[p]);
+                }
+            }
+        }
+        // lane (l16, lq): token row j * 16 + l16, hidden units 4 lq + (0..3) of the tile
+        const int ht = t.n0 / 64 * 2 + t.n0 % 64 / 16, hc = ht * 16 + 4 * lq;
+        auto finish = [&](int j, const f32x4_t& gv, const f32x4_t& uv) {
+            const int m = j * 16 + l16;
+            if (m >= t.n) return;
+            const float* b = a.b1 + (int64_t)t.e * a.N1 + t.n0 + 4 * lq;
+            T o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                o[r] = Elt<T>::from_f32(hc + r < a.H ? swiglu<T>(gv[r] + b[r], uv[r] + b[32 + r]) : 0.0f);
+            typedef typename std::conditional<sizeof(T) == 2, uint2, uint4>::type Raw4;
+            Raw4 raw;
+            __builtin_memcpy(&raw, o, sizeof(raw));
+            *reinterpret_cast<Raw4*>(static_cast<T*>(a.h) + (int64_t)(t.off + m) * a.ldh + hc) = raw;
+        };
+        if constexpr (S == 1) {
+            if (mine)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) finish(j, acc[0][j], acc[1][j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) s_part[wave][i][j][lane] = acc[i][j];
+            lds_barrier();
+            if (mine)
+                for (int j = part; j < NT; j += S) {
+                    f32x4_t gv = s_part[g * S][0][j][lane], uv = s_part[g * S][1][j][lane];
+#pragma unroll
+                    for (int w = 1; w < S; ++w) {
+                        gv += s_part[g * S + w][0][j][lane];
+                        uv += s_part[g * S + w][1][j][lane];
+                    }
+                    finish(j, gv, uv);
+                }
+            lds_barrier();
+        }
+    }
+}
+
+// A block has 16 columns of y, or with parts > 1 a share of their sums' steps.
+template <typename T, bool W8, int NT, int P>
+__global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
+    typedef Step<T, W8> St;
+    extern __shared__ __align__(16) uint8_t s_dyn[];
+    __shared__ f32x4_t s_y[kFewWaves][16 * NT][4];  // [wave][row][4 columns each]
+    __shared__ int s_last;
+    const int slots = a.k + a.Ecols - a.E;
+    const Lists l(s_dyn, a.Ecols, a.rows * slots);
+    make_lists<true>(a, l);
+
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tile = blockIdx.x / a.parts, part = blockIdx.x % a.parts, n0 = tile * 16;
+    const int steps = (a.H + St::KS - 1) / St::KS;  // of an expert
+    const int total = __builtin_amdgcn_readfirstlane(l.info[0]) * steps, shares = a.parts * kFewWaves;
+    const int share = part * kFewWaves + wave;
+    const int s0 = (int)((int64_t)total * share / shares), s1 = (int)((int64_t)total * (share + 1) / shares);
+    const uint32_t wl = weight_lane<T, W8>(l16, lq);
+    const int64_t kstep = (int64_t)a.N2 * kKBlockBytes;
+    const int live_h = (a.H + 15) / 16 * 16;  // columns of h that are written
+
+    for (int r = lane; r < 16 * NT * 4; r += kWave) s_y[wave][r / 4][r % 4] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    struct Data {
+        u32x4_t w[2], x[NT][St::XL];
+        float s;
+    };
+    struct At {
+        int e, off, n;
+    };
+    auto place = [&](int li) {
+        At t;
+        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
+        t.off = __builtin_amdgcn_readfirstlane(l.off[li]);
+        t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
+        return t;
+    };
+    auto fetch = [&](int s, Data& d) {
+        const int li = s / steps, st = s - li * steps;
+        const At t = place(li);
+        const uint8_t* p = static_cast<const uint8_t*>(a.w2) + (int64_t)t.e * a.w2_expert + (int64_t)n0 * kKBlockBytes +
+                           2 * st * kstep + wl;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) d.w[q] = load16u(p + q * kstep);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            if (j * 16 >= t.n) break;
+            const T* h = static_cast<const T*>(a.h) + (int64_t)(t.off + min(j * 16 + l16, t.n - 1)) * a.ldh;
+#pragma unroll
+            for (int q = 0; q < St::XL; ++q) {
+                const int k = st * St::KS + St::xk(q, lq);
+                d.x[j][q] = u32x4_t{0, 0, 0, 0};
+                if (k < live_h) d.x[j][q] = load16u(h + k);
+            }
+        }
+        if constexpr (W8) d.s = a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + st];
+        else d.s = a.w2_down;
+    };
+    f32x4_t acc[NT];
+    auto clear = [&] {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    // the sums of expert `li` so far, weighed, to the rows' (each row of it is one lane's)
+    auto flush = [&](int li, bool bias) {
+        const At t = place(li);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int m = j * 16 + l16;
+            if (m < t.n) {
+                const float w = l.gate[t.off + m];
+                f32x4_t v = acc[j];
+                if (bias) {
+                    const float* b = a.b2 + (int64_t)t.e * a.N2 + n0 + 4 * lq;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] += b[r];
+                }
+                f32x4_t& to = s_y[wave][l.row[t.off + m]][lq];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[r] = __builtin_fmaf(v[r], w, to[r]);
+            }
+        }
+        clear();
+    };
+    clear();
+    Data d[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        if (s0 + p < s1) fetch(s0 + p, d[p]);
+    int li = s0 / steps, end = (li + 1) * steps, from = s0;
+    int n = s0 < s1 ? place(li).n : 0;
+    for (int s = s0; s < s1; s += P) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            if (s + p >= s1) break;
+            if (s + p == end) {
+                flush(li, from <= end - steps);
+                ++li;
+                from = end;
+                end += steps;
+                n = place(li).n;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (j * 16 >= n) break;
+                multiply<T, W8>(acc[j], d[p].w, d[p].x[j], d[p].s);
+            }
+            if (s + p + P < s1) fetch(s + p + P, d[p]);
+        }
+    }
+    if (s0 < s1) flush(li, from <= end - steps);
+    __syncthreads();
+    // the waves' sums in wave order; thread (row, column quarter)
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int row = tid / 4, c = tid % 4;
+    static_assert(kFewThreads >= 64 * 4, "a thread for 4 columns of each row");
+    if (row < a.rows) {
+        v = s_y[0][row][c];
+#pragma unroll
+        for (int w = 1; w < kFewWaves; ++w) v += s_y[w][row][c];
+    }
+    if (a.parts > 1) {
+        // the last block to arrive adds the shares, in their order
+        f32x4_t* ws = reinterpret_cast<f32x4_t*>(a.partial) + (int64_t)tile * a.parts * a.rows * 4;
+        if (row < a.rows) ws[((int64_t)part * a.rows + row) * 4 + c] = v;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0)
+            s_last = __hip_atomic_fetch_add(&a.arrived[tile], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+        __syncthreads();
+        if (!s_last) return;
+        __threadfence();
+        if (row < a.rows) {
+            v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int p = 0; p < a.parts; ++p) v += ws[((int64_t)p * a.rows + row) * 4 + c];
+        }
+        if (tid == 0) __hip_atomic_store(&a.arrived[tile], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const int col = n0 + 4 * c;
+    if (row < a.rows && col < a.D) {  // (D % 8 == 0: four columns are real or padding)
+        T o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = Elt<T>::from_f32(v[r]);
+        typedef typename std::conditional<sizeof(T) == 2, uint2, uint4>::type Raw4;
+        Raw4 raw;
+        __builtin_memcpy(&raw, o, sizeof(raw));
+        *reinterpret_cast<Raw4*>(static_cast<T*>(a.y) + (int64_t)row * a.D + col) = raw;
+    }
+}
+
+// The lists are dynamic LDS; more than 64 KB in a block has to be asked for.
+template <typename F>
+hipError_t launch(F kernel, int64_t grid, size_t fixed, size_t lds, const FewArgs& a, hipStream_t s) {
+    if (fixed + lds > 160 * 1024) return hipErrorInvalidValue;
+    if (fixed + lds > 64 * 1024) {
+        const hipError_t e =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    launch_kernel(kernel, dim3((unsigned)grid), dim3(kFewThreads), (uint32_t)lds, s, a);
+    return hipGetLastError();
+}
+
+constexpr int kTargetWaves = 256 * 8;  // that fill the chip
+
+template <typename T, bool W8, int NT>
+hipError_t launch_nt(FewArgs a, hipStream_t s) {
+    constexpr int P = W8 ? (NT == 1 ? 3 : NT == 2 ? 2 : 1) : NT == 1 ? 4 : 2;  // steps in flight
+    const int slots = a.k + a.Ecols - a.E, places = a.rows * slots;
+    const int tiles = (a.H + 15) / 16, live = std::min(a.E, a.rows * a.k) + a.Ecols - a.E;
+    const int64_t units = (int64_t)tiles * live;
+    const size_t lds1 = Lists::bytes(a.Ecols, places, false), lds2 = Lists::bytes(a.Ecols, places, true);
+    const int S = units * 2 > kTargetWaves ? 2 : units * 4 > kTargetWaves ? 4 : 8;
+    const int grid = (int)std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 512);
+    constexpr size_t fixed1 = kFewWaves * 2 * NT * kWave * 16, fixed2 = kFewWaves * NT * kWave * 16 + 16;
+    hipError_t e = S == 2   ? launch(few_up_kernel<T, W8, NT, 2, P>, grid, fixed1, lds1, a, s)
+                   : S == 4 ? launch(few_up_kernel<T, W8, NT, 4, P>, grid, fixed1, lds1, a, s)
+                            : launch(few_up_kernel<T, W8, NT, 8, P>, grid, fixed1, lds1, a, s);
+    if (e != hipSuccess) return e;
+    const int ntiles = (a.D + 15) / 16;
+    a.parts = std::max(1, std::min(kFewParts, 256 / ntiles));
+    return launch(few_down_kernel<T, W8, NT, P>, ntiles * a.parts, fixed2, lds2, a, s);
+}
+
+template <typename T, bool W8>
+hipError_t launch_few_t(const FewArgs& a, hipStream_t s) {
+    if (a.rows <= 16) return launch_nt<T, W8, 1>(a, s);
+    if (a.rows <= 32) return launch_nt<T, W8, 2>(a, s);
+    return launch_nt<T, W8, 4>(a, s);
+}
+
+}  // namespace
+
+hipError_t launch_few(DType dt, const FewArgs& a, hipStream_t s) {
+    if (a.rows < 1 || a.rows > kFewRows || a.D < 8 || a.D % 8 != 0 || a.E < 1 || a.E > kMaxExperts || a.k < 1 ||
+        a.k > a.Ecols || (a.D + 15) / 16 > a.tile_cap)
+        return hipErrorInvalidValue;
+    const bool w8 = a.s1 != nullptr;
+    switch (dt) {
+        case DType::F32: return w8 ? hipErrorInvalidValue : launch_few_t<float, false>(a, s);
+        case DType::BF16: return w8 ? launch_few_t<__bf16, true>(a, s) : launch_few_t<__bf16, false>(a, s);
+        case DType::F16: return w8 ? launch_few_t<_Float16, true>(a, s) : launch_few_t<_Float16, false>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace nomas

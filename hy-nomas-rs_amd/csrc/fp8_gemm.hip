@@ -13,20 +13,19 @@
 // from the same bytes (every e4m3 is a bf16): exact products, f32 sums, half the rate.
 #include "fp8.hpp"
 #include "lds_dma.hpp"
+#include "mfma.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nomas {
 
 namespace {
 
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ f32x4_t mfma_fp8(const i32x8_t& a, const i32x8_t& b) {
     const f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, z, 0, 0, 0, 0, 0, 0);
 }
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 // The lane's 32 values of a fragment, for 16-bit results as they are, for f32 ones widened.
@@ -79,12 +78,20 @@ __device__ __forceinline__ void put4(T* row, int n, int N, const f32x4_t& v, boo
     }
 }
 
+// What is made of the products:
+//  kStore  y (M x N) in T, with a bias
+//  kGlu    the hidden activations of a SwiGLU feed-forward: b's rows are its packed gate and up rows
+//          (32 of the one, 32 of the other), scales for squares of 128 gate rows, then of the up
+//          rows; silu(gate + bias) (up + bias) in f32 as 8-bit values with a scale for each
+//          128 of them (tile kernel: a tile has whole blocks) or as they are (few rows)
+enum { kStore = 0, kGlu = 1 };
+
 // ---- tiles through LDS ---------------------------------------------------------
 // A block's WN x WM waves share a tile of 16 NI WN weight rows and 16 NJ WM rows;
 // K-blocks of 128 bytes a row go through a ring of two LDS stages, filled by direct loads of
 // whole 128-byte rows.  16-byte chunk c of row r is kept at chunk c ^ (r % 8), so that the
 // fragment reads (one chunk of 8 rows at a time) touch every bank once.
-template <typename T, int NI, int NJ, int WN, int WM>
+template <typename T, int MODE, int NI, int NJ, int WN, int WM>
 __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a, int tiles_m, int tiles_n) {
     constexpr int NW = WN * WM, BN = 16 * NI * WN, BM = 16 * NJ * WM;
     constexpr int kStage = (BN + BM) * kFp8Block;
@@ -145,7 +152,10 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 
     // (a wave's weight rows lie in one block of 128)
     static_assert(kFp8Block % (16 * NI) == 0, "one weight scale a wave");
-    const float* __restrict__ bs = a.bs + (int64_t)min((n0 + wn * 16 * NI) / kFp8Block, (a.N - 1) / kFp8Block) * kb;
+    // (of the gate rows with kGlu, whose up rows' scales are `up` further on)
+    const float* __restrict__ bs =
+        a.bs + (int64_t)(MODE == kGlu ? tn : min((n0 + wn * 16 * NI) / kFp8Block, (a.N - 1) / kFp8Block)) * kb;
+    const int64_t up = MODE == kGlu ? (int64_t)tiles_n * kb : 0;
     const int sw = l16 & 7;
     const int c0 = (2 * lq) ^ sw, c1 = (2 * lq + 1) ^ sw;
 
@@ -162,13 +172,15 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             return join(*reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c0 * 16),
                         *reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c1 * 16));
         };
-        const float sb = bs[kt];
+        const float sb = bs[kt], sb2 = bs[up + kt];
         FragOf<T> x[NJ];
-        float s[NJ];
+        float s[NJ], s2[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             x[j].set(frag(xt, j));
-            s[j] = s_sa[kt & 1][wm * NJ * 16 + j * 16 + l16] * sb;
+            const float sa = s_sa[kt & 1][wm * NJ * 16 + j * 16 + l16];
+            s[j] = sa * sb;
+            s2[j] = MODE == kGlu ? sa * sb2 : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
@@ -178,11 +190,65 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             for (int j = 0; j < NJ; ++j) {
                 const f32x4_t t = dot(w, x[j]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(t[r], s[j], acc[i][j][r]);
+                for (int r = 0; r < 4; ++r)
+                    acc[i][j][r] = __builtin_fmaf(t[r], MODE == kGlu && i % 4 >= 2 ? s2[j] : s[j], acc[i][j][r]);
             }
         }
     }
 
+    if constexpr (MODE == kGlu) {
+        // a lane's gate values of weight blocks i and up values of i + 2 are of the same hidden
+        // units; the tile is 128 of them, a block of the output
+        static_assert(MODE != kGlu || (NI == 8 && WN == 2), "a tile is 128 hidden units");
+        const int H = a.N / 2, hb = H / kFp8Block;
+        uint32_t top[NJ];
+        int hc[4];  // the lane's four neighbouring units, four times
+#pragma unroll
+        for (int p = 0; p < 4; ++p) hc[p] = n0 / 2 + wn * 64 + p / 2 * 32 + p % 2 * 16 + 4 * lq;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) top[j] = 0;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int i = p / 2 * 4 + p % 2, at = n0 + wn * 128 + i * 16 + 4 * lq;
+            const float4 bg = *reinterpret_cast<const float4*>(a.bias + at);
+            const float4 bu = *reinterpret_cast<const float4*>(a.bias + at + 32);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                acc[i][j] += f32x4_t{bg.x, bg.y, bg.z, bg.w};
+                acc[i + 2][j] += f32x4_t{bu.x, bu.y, bu.z, bu.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float h = hc[p] + r < a.hidden ? swiglu<__bf16>(acc[i][j][r], acc[i + 2][j][r]) : 0.0f;
+                    acc[i][j][r] = h;
+                    top[j] = max(top[j], __float_as_uint(h) & 0x7fffffffu);
+                }
+            }
+        }
+        __syncthreads();  // (all have read the last stage)
+        uint32_t* s_top = reinterpret_cast<uint32_t*>(&s_ring[0][0]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 16));
+            top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 32));
+            if (lq == 0) s_top[((wm * NJ + j) * 16 + l16) * 2 + wn] = top[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int m = (wm * NJ + j) * 16 + l16;
+            if (m >= rows_m) continue;
+            const float s = fp8_scale(max(s_top[m * 2], s_top[m * 2 + 1]));
+            const Fp8Quot d(s);
+            uint8_t* q = static_cast<uint8_t*>(a.y) + (m0 + m) * H;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const f32x4_t& h = acc[p / 2 * 4 + p % 2][j];
+                *reinterpret_cast<uint32_t*>(q + hc[p]) = fp8_pack4(d(h[0]), d(h[1]), d(h[2]), d(h[3]));
+            }
+            if (wn == 0 && lq == 0) a.y_scale[(m0 + m) * hb + tn] = s;
+        }
+        return;
+    }
     T* y = static_cast<T*>(a.y);
     const bool whole = a.N % 4 == 0;
 #pragma unroll
@@ -203,7 +269,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 // ---- few rows --------------------------------------------------------------------
 // 16 NT rows x 16 NI weight rows a block; its NW waves take the K-blocks in turn, operands
 // straight from global memory, and add their sums in LDS in wave order.
-template <typename T, int NI, int NT, int NW, int P>
+template <typename T, int MODE, int NI, int NT, int NW, int P>
 __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
     constexpr int BN = 16 * NI, BM = 16 * NT;
     __shared__ f32x4_t s_part[NW][NI][NT][kWave];
@@ -225,8 +291,10 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
 
     struct Step {
         i32x4_t w[NI][2], x[NT][2];
-        float sa[NT], sb;
+        float sa[NT], sb, sb2;
     };
+    const int hb = a.N / 2 / kFp8Block;  // (kGlu)
+    const float* bs = a.bs + (int64_t)(MODE == kGlu ? n0 / 2 / kFp8Block : n0 / kFp8Block) * kb;
     auto load = [&](int kt, Step& s) {
         const int k = kt * kFp8Block + lq * 32;
         const bool ok0 = k < K, ok1 = k + 16 < K;  // (false in the last block only)
@@ -245,7 +313,8 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
             s.x[j][1] = ok1 ? *reinterpret_cast<const i32x4_t*>(p + 16) : z;
             s.sa[j] = as[(int64_t)min(j * 16 + l16, rows_m - 1) * kb + kt];
         }
-        s.sb = a.bs[(int64_t)(n0 / kFp8Block) * kb + kt];
+        s.sb = bs[kt];
+        s.sb2 = MODE == kGlu ? bs[(int64_t)hb * kb + kt] : 0.0f;
     };
     static_assert(kFp8Block % BN == 0, "one weight scale a block");
     f32x4_t acc[NI][NT];
@@ -267,14 +336,15 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
             for (int i = 0; i < NI; ++i) w[i].set(join(s.w[i][0], s.w[i][1]));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const float f = s.sa[j] * s.sb;
+                const float f = s.sa[j] * s.sb, f2 = s.sa[j] * s.sb2;
                 FragOf<T> x;
                 x.set(join(s.x[j][0], s.x[j][1]));
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
                     const f32x4_t t = dot(w[i], x);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(t[r], f, acc[i][j][r]);
+                    for (int r = 0; r < 4; ++r)
+                        acc[i][j][r] = __builtin_fmaf(t[r], MODE == kGlu && i >= 2 ? f2 : f, acc[i][j][r]);
                 }
             }
             if (k0 + (p + P) * NW < kb) load(k0 + (p + P) * NW, s);
@@ -285,6 +355,26 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) s_part[wave][i][j][lane] = acc[i][j];
     __syncthreads();
+    if constexpr (MODE == kGlu) {
+        static_assert(MODE != kGlu || NI == 4, "32 gate rows and their 32 up rows");
+        float* h = static_cast<float*>(a.y);
+        for (int it = wave; it < 2 * NT; it += NW) {
+            const int i = it % 2, j = it / 2, at = n0 + i * 16 + 4 * lq, hc = n0 / 2 + i * 16 + 4 * lq;
+            f32x4_t g = s_part[0][i][j][lane], u = s_part[0][(i + 2) % NI][j][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                g += s_part[w][i][j][lane];
+                u += s_part[w][(i + 2) % NI][j][lane];
+            }
+            f32x4_t o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                o[r] = hc + r < a.hidden ? swiglu<__bf16>(g[r] + a.bias[at + r], u[r] + a.bias[at + 32 + r]) : 0.0f;
+            const int m = j * 16 + l16;
+            if (m < rows_m) *reinterpret_cast<f32x4_t*>(h + (m0 + m) * (a.N / 2) + hc) = o;
+        }
+        return;
+    }
     T* y = static_cast<T*>(a.y);
     const bool whole = a.N % 4 == 0;
     for (int it = wave; it < NI * NT; it += NW) {
@@ -300,29 +390,29 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
     }
 }
 
-template <typename T, int NI, int NJ, int WN, int WM>
+template <typename T, int MODE, int NI, int NJ, int WN, int WM>
 hipError_t tile(const Fp8GemmArgs& a, hipStream_t s) {
     const int64_t tm = (a.M + 16 * NJ * WM - 1) / (16 * NJ * WM), tn = (a.N + 16 * NI * WN - 1) / (16 * NI * WN);
     if (tm * tn > 0x7fffff00) return hipErrorInvalidValue;
-    launch_kernel(fp8_tile_kernel<T, NI, NJ, WN, WM>, dim3((unsigned)round_up(tm * tn, kNumXcd)), dim3(WN * WM * kWave),
-                  0, s, a, (int)tm, (int)tn);
+    launch_kernel(fp8_tile_kernel<T, MODE, NI, NJ, WN, WM>, dim3((unsigned)round_up(tm * tn, kNumXcd)),
+                  dim3(WN * WM * kWave), 0, s, a, (int)tm, (int)tn);
     return hipGetLastError();
 }
-template <typename T, int NI, int NT, int NW, int P>
+template <typename T, int MODE, int NI, int NT, int NW, int P>
 hipError_t rows(const Fp8GemmArgs& a, hipStream_t s) {
     const int64_t tm = (a.M + 16 * NT - 1) / (16 * NT), tn = (a.N + 16 * NI - 1) / (16 * NI);
     if (tm > 65535) return hipErrorInvalidValue;
-    launch_kernel(fp8_rows_kernel<T, NI, NT, NW, P>, dim3((unsigned)tn, (unsigned)tm), dim3(NW * kWave), 0, s, a);
+    launch_kernel(fp8_rows_kernel<T, MODE, NI, NT, NW, P>, dim3((unsigned)tn, (unsigned)tm), dim3(NW * kWave), 0, s, a);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
-    if (a.M <= 16) return rows<T, 2, 1, 8, 2>(a, s);
-    if (a.M <= 32) return rows<T, 2, 2, 8, 2>(a, s);
-    if (a.M <= 512) return rows<T, 4, 4, 4, 2>(a, s);
-    if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<T, 4, 4, 2, 2>(a, s);
-    return tile<T, 8, 4, 2, 4>(a, s);
+    if (a.M <= 16) return rows<T, kStore, 2, 1, 8, 2>(a, s);
+    if (a.M <= 32) return rows<T, kStore, 2, 2, 8, 2>(a, s);
+    if (a.M <= 512) return rows<T, kStore, 4, 4, 4, 2>(a, s);
+    if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<T, kStore, 4, 4, 2, 2>(a, s);
+    return tile<T, kStore, 8, 4, 2, 4>(a, s);
 }
 
 }  // namespace
@@ -338,6 +428,21 @@ hipError_t launch_fp8_gemm(DType dt, const Fp8GemmArgs& a, hipStream_t s) {
         case DType::F16: return gemm<_Float16>(a, s);
     }
     return hipErrorInvalidValue;
+}
+
+bool fp8_glu_fused(int64_t M, int) { return M > kFp8GluRows; }
+
+hipError_t launch_fp8_glu(const Fp8GemmArgs& a, hipStream_t s) {
+    if (a.M < 1 || a.N < 256 || a.N % 256 != 0 || a.K < 128 || a.K % 128 != 0 || a.K > kFp8MaxK || a.N > kFp8MaxN ||
+        a.M > kFp8MaxRows || a.hidden < 1 || a.hidden > a.N / 2 || !a.bias)
+        return hipErrorInvalidValue;
+    if (!fp8_glu_fused(a.M, a.N)) {
+        if (a.M <= 16) return rows<__bf16, kGlu, 4, 1, 8, 2>(a, s);
+        if (a.M <= 32) return rows<__bf16, kGlu, 4, 2, 8, 2>(a, s);
+        return rows<__bf16, kGlu, 4, 4, 4, 2>(a, s);
+    }
+    if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<__bf16, kGlu, 8, 2, 2, 4>(a, s);
+    return tile<__bf16, kGlu, 8, 4, 2, 4>(a, s);
 }
 
 }  // namespace nomas

@@ -244,6 +244,14 @@ public:
         const float* w;
     };
     int forward_routed(const void* x, const Given& g, void* y, int64_t rows, hipStream_t s);
+    // Makes the 8-bit copy of the weights (16-bit models): of the experts for forward_few, of
+    // a dense feed-forward for forward_fp8.  Synchronises; a second call does nothing.
+    int quantize();
+    // forward() on up to kFewRows rows in few kernels, or with `g` forward_routed();
+    // with `fp8` on the 8-bit copy of the experts' weights.
+    int forward_few(const void* x, const Given* g, bool fp8, void* y, int64_t rows, hipStream_t s);
+    // The dense feed-forward on 8-bit weights and activations.
+    int forward_fp8(const void* x, void* y, int64_t rows, hipStream_t s);
     int forward_host(const void* x, void* y, int64_t rows);
     int forward_host_pieces(const void* x, void* y, int64_t rows, int np, void* dx, void* dy);
     int routing(int32_t* idx, float* w, int32_t* counts, float* gap);
@@ -310,6 +318,21 @@ private:
     // makes all its sums with f32 MFMAs (GemmArgs)
     float w1_scale_ = 1.0f, w2_scale_ = 1.0f;
     bool w1_all_f32_ = false, w2_all_f32_ = false;
+
+    // 8-bit weights: experts' in fragment order (few.hip), a dense feed-forward's row-major in
+    // the packed row order; scales of their squares of 128 x 128 (gate, then up)
+    uint8_t *d_q1_ = nullptr, *d_q2_ = nullptr;
+    float *d_s1_ = nullptr, *d_s2_ = nullptr;
+    // forward_few's workspace: one size for all calls, so that a captured call's stays where it is
+    void* d_few_ = nullptr;
+    Workspace few_ws_;
+    float* few_partial_ = nullptr;
+    int32_t* few_arrived_ = nullptr;
+    int ensure_few();
+    bool last_few_given_ = false;  // the last forward was forward_few under the caller's routing
+    // forward_fp8's: x and the hidden activations in 8 bits, and the latter in f32 where few
+    void* d_f8_ = nullptr;
+    int64_t f8_rows_ = 0;
 
     // the handle's workspace (sized for ws_.cap_rows rows)
     void* d_ws_ = nullptr;

@@ -316,6 +316,32 @@ struct QuantSquareArgs {
     int fragments;   // q in fragments of 16 rows x 64 columns (few.hip) of a matrix of q_rows rows
     int64_t q_rows;
 };
+// The MoE layer on few rows (few.hip).
+constexpr int kFewRows = 64;
+constexpr int kFewParts = 4;  // blocks that share 16 columns of y, at most
+struct FewArgs {
+    const void* x;       // rows x D, model dtype
+    void* y;
+    int rows, D, H, E, Ecols, k;  // Ecols: E, or E + 1 with the shared dense branch
+    const int32_t* idx;  // rows x k (outside 0 .. E - 1: an empty slot)
+    const float* w;
+    float dense_coef;
+    const void *w1, *w2;           // weights as the layer keeps them: K-blocked, N1 (2 padded H) and N2 rows
+    int64_t w1_expert, w2_expert;  // bytes from expert to expert
+    const float *b1, *b2;          // Ecols x N1, Ecols x N2
+    int N1, N2;
+    float w1_down, w2_down;        // f32: what takes the weights back to their values
+    // 8-bit weights (s1 non-null), in fragment order; scales Ecols x 2 x hb x kb1 and Ecols x nb2 x kb2
+    const float *s1, *s2;
+    int hb, kb1, nb2, kb2;
+    void* h;             // hidden activations, ldh columns a place
+    int64_t ldh;
+    float* partial;      // tile_cap x kFewParts x rows x 16 sums
+    int32_t* arrived;    // tile_cap counters, zero between calls
+    int tile_cap;
+    int parts;           // (set by the launch)
+};
+hipError_t launch_few(DType dt, const FewArgs& a, hipStream_t s);
 hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s);
 hipError_t launch_quant_squares(DType dt, const QuantSquareArgs& a, hipStream_t s);
 
@@ -334,9 +360,16 @@ struct Fp8GemmArgs {
     void* y;           // M x N
     int64_t M;
     int N, K;          // K % 16 == 0
+    int hidden;        // launch_fp8_glu: hidden units (those up to N / 2 come out as zeros)
+    float* y_scale;    // ... and M x N / 256 scales, where y is 8-bit
 };
 // y = a b^T + bias in `dt`.
 hipError_t launch_fp8_gemm(DType dt, const Fp8GemmArgs& a, hipStream_t s);
+// The hidden activations of a SwiGLU feed-forward from its packed gate and up weights (N % 256 == 0, K %
+// 128 == 0; scales 2 x N / 256 x K / 128): 8-bit (M x N / 2) with y_scale where fp8_glu_fused, else f32.
+constexpr int kFp8GluRows = 128;  // (more rows: always fused)
+bool fp8_glu_fused(int64_t M, int N);
+hipError_t launch_fp8_glu(const Fp8GemmArgs& a, hipStream_t s);
 int64_t block_seam_workspace(int64_t rows, int64_t D, int64_t seq);
 hipError_t launch_block_seam(DType dt, const BlockSeamArgs& a, hipStream_t s);
 hipError_t launch_block_seam_backward(DType dt, const BlockSeamBackwardArgs& a, hipStream_t s);

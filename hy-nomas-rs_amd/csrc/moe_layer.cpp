@@ -200,7 +200,8 @@ MoeLayer::~MoeLayer() {
     if (hs_copy_) (void)hipStreamSynchronize(hs_copy_);
     if (hs_comp_) (void)hipStreamSynchronize(hs_comp_);
     if (hs_out_) (void)hipStreamSynchronize(hs_out_);
-    for (void* p : {d_wr_, d_w1_, (void*)d_b1_, d_w2_, (void*)d_b2_, d_hio_, d_route_})
+    for (void* p : {d_wr_, d_w1_, (void*)d_b1_, d_w2_, (void*)d_b2_, d_hio_, d_route_, (void*)d_q1_, (void*)d_q2_,
+                    (void*)d_s1_, (void*)d_s2_, d_few_, d_f8_})
         if (p) (void)hipFree(p);
     for (hipEvent_t e : events_) (void)hipEventDestroy(e);
     for (int i = 0; i < kHostMaxPieces; ++i) {
@@ -598,6 +599,7 @@ int MoeLayer::finish_forward(int64_t rows, hipStream_t s, const Workspace& w, in
     HIP_TRY(hipEventRecord(done_, s));
     done_recorded_ = true;
     host_pieces_ = 0;  // routing() reads this forward's workspace
+    last_few_given_ = false;
     scratch_pieces_ = scratch_pieces;
     last_rows_ = rows;
     last_stream_ = s;
@@ -861,6 +863,265 @@ int MoeLayer::forward_dense(const void* x, void* y, int64_t rows, hipStream_t s)
     return finish_forward(rows, s, w);
 }
 
+// ---- 8-bit weights, few rows ----------------------------------------------------
+
+int MoeLayer::quantize() {
+    if (dt_ == DType::F32)
+        return set_error(NOMAS_ERR_INVALID_CONFIG, "8-bit weights are made of bf16 or f16 ones: this layer's are f32");
+    if (!d_w1_) return set_error(NOMAS_ERR_STATE, "weights have not been uploaded");
+    if (d_s2_) return NOMAS_OK;
+    DeviceGuard g(device_);
+    if (!g.ok) return set_error(NOMAS_ERR_HIP, "hipSetDevice(%d) failed", device_);
+    const int64_t N1 = 2 * Hp_, kb1 = Dk_ / kFp8Block, kb2 = Hp_ / kFp8Block, hb = Hp_ / kFp8Block, nb2 = Dn_ / kFp8Block;
+    if (Dk_ > kFp8MaxK || Hp_ > kFp8MaxK || Dn_ > kFp8MaxN || N1 > kFp8MaxN)
+        return set_error(NOMAS_ERR_INVALID_CONFIG, "dim=%lld, hidden=%lld are too wide for 8-bit weights", (long long)D_,
+                         (long long)H_);
+    struct Buffers {  // until all of it is made
+        void* p[4] = {};
+        ~Buffers() {
+            for (void* q : p)
+                if (q) (void)hipFree(q);
+        }
+    } b;
+    HIP_TRY(hipMalloc(&b.p[0], (size_t)(Ecols_ * N1 * Dk_)));
+    HIP_TRY(hipMalloc(&b.p[1], (size_t)(Ecols_ * Dn_ * Hp_)));
+    HIP_TRY(hipMalloc(&b.p[2], (size_t)(Ecols_ * 2 * hb * kb1) * sizeof(float)));
+    HIP_TRY(hipMalloc(&b.p[3], (size_t)(Ecols_ * nb2 * kb2) * sizeof(float)));
+    constexpr int64_t KB = kKBlockBytes / 2;
+    for (int64_t e = 0; e < Ecols_; ++e) {
+        // gate and up: squares of 128 hidden units, whose rows lie in groups of 32 gate, 32 up
+        QuantSquareArgs a = {};
+        a.x = static_cast<const uint16_t*>(d_w1_) + e * N1 * Dk_;
+        a.q = static_cast<uint8_t*>(b.p[0]) + e * N1 * Dk_;
+        a.scale = static_cast<float*>(b.p[2]) + e * 2 * hb * kb1;
+        a.rows = (int)Hp_;
+        a.cols = (int)Dk_;
+        a.batch = 2;
+        a.x_batch = 32 * KB;
+        a.x_step = N1 * KB;
+        a.x_row = KB;
+        a.row_group = 64;
+        a.fragments = !dense_only_;
+        // (32 rows on: two fragments, or 32 rows of Dk)
+        a.q_batch = dense_only_ ? 32 * Dk_ : 2 * 1024;
+        a.scale_batch = hb * kb1;
+        a.ld_q = (int)Dk_;
+        a.q_rows = N1;
+        HIP_TRY(launch_quant_squares(dt_, a, nullptr));
+        a.x = static_cast<const uint16_t*>(d_w2_) + e * Dn_ * Hp_;
+        a.q = static_cast<uint8_t*>(b.p[1]) + e * Dn_ * Hp_;
+        a.scale = static_cast<float*>(b.p[3]) + e * nb2 * kb2;
+        a.rows = (int)Dn_;
+        a.cols = (int)Hp_;
+        a.batch = 1;
+        a.x_step = Dn_ * KB;
+        a.row_group = 32;
+        a.ld_q = (int)Hp_;
+        a.q_rows = Dn_;
+        HIP_TRY(launch_quant_squares(dt_, a, nullptr));
+    }
+    HIP_TRY(hipDeviceSynchronize());
+    d_q1_ = static_cast<uint8_t*>(b.p[0]);
+    d_q2_ = static_cast<uint8_t*>(b.p[1]);
+    d_s1_ = static_cast<float*>(b.p[2]);
+    d_s2_ = static_cast<float*>(b.p[3]);
+    for (void*& p : b.p) p = nullptr;
+    return NOMAS_OK;
+}
+
+int MoeLayer::ensure_few() {
+    if (d_few_) return NOMAS_OK;
+    const int64_t tiles = (D_ + 15) / 16;
+    Workspace w;
+    size_t off = 0;
+    uint8_t* base = nullptr;
+    auto take = [&](size_t bytes) {
+        const size_t o = off;
+        off += align256(bytes);
+        return base ? base + o : nullptr;
+    };
+    auto lay = [&] {
+        off = 0;
+        few_arrived_ = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * tiles));
+        w.idx = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * kFewRows * kslots_));
+        w.w = reinterpret_cast<float*>(take(sizeof(float) * kFewRows * kslots_));
+        w.gap = reinterpret_cast<float*>(take(sizeof(float) * kFewRows));
+        w.expert_count = w.chunk_counts = reinterpret_cast<int32_t*>(
+            take(sizeof(int32_t) * (kFewRows / kMinRouterBlockRows) * Ecols_));
+        w.h = take(dtype_size(dt_) * kFewRows * kslots_ * round_up(H_, 16));
+        few_partial_ = reinterpret_cast<float*>(take(sizeof(float) * tiles * kFewParts * kFewRows * 16));
+    };
+    lay();
+    void* p = nullptr;
+    HIP_TRY(hipMalloc(&p, off));
+    base = static_cast<uint8_t*>(p);
+    lay();
+    const hipError_t e = hipMemset(few_arrived_, 0, sizeof(int32_t) * tiles);
+    if (e != hipSuccess || hipDeviceSynchronize() != hipSuccess) {
+        (void)hipFree(p);
+        return set_error(NOMAS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
+    }
+    few_ws_ = w;
+    d_few_ = p;
+    return NOMAS_OK;
+}
+
+int MoeLayer::forward_few(const void* x, const Given* g, bool fp8, void* y, int64_t rows, hipStream_t s) {
+    if (dense_only_) return set_error(NOMAS_ERR_STATE, "the forward of few rows is implemented for the MoE layer");
+    if (rows > kFewRows)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld: the forward of few rows takes up to %d", (long long)rows,
+                         kFewRows);
+    if (rows > 0 && g && (!g->idx || !g->w))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "idx and w must both be given");
+    if (g && (reinterpret_cast<uintptr_t>(g->idx) | reinterpret_cast<uintptr_t>(g->w)) & 3)
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "idx and w must be 4-byte aligned");
+    if (fp8 && !d_s2_) return set_error(NOMAS_ERR_STATE, "the layer has no 8-bit weights: quantize it first");
+    int rc = check_forward(x, y, rows);
+    if (rc != NOMAS_OK) return rc;
+    if (rows == 0) { last_rows_ = 0; last_in_scratch_ = false; return NOMAS_OK; }
+    DeviceGuard guard(device_);
+    if (!guard.ok) return set_error(NOMAS_ERR_HIP, "hipSetDevice(%d) failed", device_);
+    rc = ensure_few();
+    if (rc != NOMAS_OK) return rc;
+    if (done_recorded_ && s != last_stream_) HIP_TRY(hipStreamWaitEvent(s, done_, 0));
+    const Workspace& w = few_ws_;
+    int count_rows = kRouterRows;
+    last_rows_ = -1;  // (until all is launched)
+    if (!g) {
+        count_rows = router_block_rows(dt_, rows, (int)D_, (int)E_);
+        RouterArgs ra;
+        ra.x = x;
+        ra.wr = d_wr_;
+        ra.rows = rows;
+        ra.D = (int)D_;
+        ra.E = (int)E_;
+        ra.k = (int)k_;
+        ra.k_slots = (int)kslots_;
+        ra.dense_coef = (float)shared_dense_;
+        ra.topk_idx = w.idx;
+        ra.topk_w = w.w;
+        ra.gap = w.gap;
+        ra.chunk_counts = w.chunk_counts;
+        ra.block_rows = count_rows;
+        HIP_TRY(launch_router(dt_, ra, s));
+    }
+    FewArgs a = {};
+    a.x = x;
+    a.y = y;
+    a.rows = (int)rows;
+    a.D = (int)D_;
+    a.H = (int)H_;
+    a.E = (int)E_;
+    a.Ecols = (int)Ecols_;
+    // (the router's slots with the shared branch's last one, which is not below E)
+    a.k = (int)(g ? k_ : kslots_);
+    a.idx = g ? g->idx : w.idx;
+    a.w = g ? g->w : w.w;
+    a.dense_coef = (float)shared_dense_;
+    const int64_t N1 = 2 * Hp_, es = fp8 ? 1 : (int64_t)dtype_size(dt_);
+    a.w1 = fp8 ? static_cast<const void*>(d_q1_) : d_w1_;
+    a.w2 = fp8 ? static_cast<const void*>(d_q2_) : d_w2_;
+    a.w1_expert = N1 * Dk_ * es;
+    a.w2_expert = Dn_ * Hp_ * es;
+    a.b1 = d_b1_;
+    a.b2 = d_b2_;
+    a.N1 = (int)N1;
+    a.N2 = (int)Dn_;
+    a.w1_down = 1.0f / w1_scale_;
+    a.w2_down = 1.0f / w2_scale_;
+    if (fp8) {
+        a.s1 = d_s1_;
+        a.s2 = d_s2_;
+        a.hb = a.kb2 = (int)(Hp_ / kFp8Block);
+        a.kb1 = (int)(Dk_ / kFp8Block);
+        a.nb2 = (int)(Dn_ / kFp8Block);
+    }
+    a.h = w.h;
+    a.ldh = round_up(H_, 16);
+    a.partial = few_partial_;
+    a.arrived = few_arrived_;
+    a.tile_cap = (int)((D_ + 15) / 16);
+    HIP_TRY(launch_few(dt_, a, s));
+    last_in_scratch_ = false;
+    rc = finish_forward(rows, s, w, (int)((rows + count_rows - 1) / count_rows));
+    last_few_given_ = g != nullptr;
+    return rc;
+}
+
+int MoeLayer::forward_fp8(const void* x, void* y, int64_t rows, hipStream_t s) {
+    if (!dense_only_) return set_error(NOMAS_ERR_STATE, "the 8-bit forward is implemented for the dense feed-forward");
+    if (!d_s2_) return set_error(NOMAS_ERR_STATE, "the feed-forward has no 8-bit weights: quantize it first");
+    int rc = check_forward(x, y, rows);
+    if (rc != NOMAS_OK) return rc;
+    if (rows > kFp8MaxRows / std::max<int64_t>(1, std::max(Dk_, Hp_) / kFp8Block))
+        return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld exceed the supported range", (long long)rows);
+    if (rows == 0) return NOMAS_OK;
+    DeviceGuard g(device_);
+    if (!g.ok) return set_error(NOMAS_ERR_HIP, "hipSetDevice(%d) failed", device_);
+    const int64_t kb1 = Dk_ / kFp8Block, kb2 = Hp_ / kFp8Block;
+    auto lay = [&](int64_t cap, uint8_t* base, QuantArgs* x8, QuantArgs* h8) {
+        size_t off = 0;
+        auto take = [&](size_t bytes) {
+            const size_t o = off;
+            off += align256(bytes);
+            return base + o;
+        };
+        x8->q = take((size_t)(cap * Dk_));
+        x8->scale = reinterpret_cast<float*>(take(sizeof(float) * cap * kb1));
+        h8->q = take((size_t)(cap * Hp_));
+        h8->scale = reinterpret_cast<float*>(take(sizeof(float) * cap * kb2));
+        h8->x = take(sizeof(float) * std::min<int64_t>(cap, kFp8GluRows) * Hp_);
+        return off;
+    };
+    QuantArgs x8 = {}, h8 = {};
+    if (rows > f8_rows_) {
+        const int64_t cap = round_up(std::max(rows, f8_rows_ + f8_rows_ / 2), kRouterRows);
+        const size_t bytes = lay(cap, nullptr, &x8, &h8);
+        if (d_f8_) HIP_TRY(hipFree(d_f8_));
+        d_f8_ = nullptr;
+        f8_rows_ = 0;
+        HIP_TRY(hipMalloc(&d_f8_, bytes));
+        f8_rows_ = cap;
+    }
+    lay(f8_rows_, static_cast<uint8_t*>(d_f8_), &x8, &h8);
+    if (done_recorded_ && s != last_stream_) HIP_TRY(hipStreamWaitEvent(s, done_, 0));
+    x8.x = x;
+    x8.rows = rows;
+    x8.cols = (int)D_;
+    x8.ld_q = (int)Dk_;
+    HIP_TRY(launch_quant_rows(dt_, x8, s));
+    Fp8GemmArgs a = {};
+    a.a = x8.q;
+    a.as = x8.scale;
+    a.b = d_q1_;
+    a.bs = d_s1_;
+    a.bias = d_b1_;
+    a.M = rows;
+    a.N = (int)(2 * Hp_);
+    a.K = (int)Dk_;
+    a.hidden = (int)H_;
+    const bool fused = fp8_glu_fused(rows, a.N);
+    a.y = fused ? static_cast<void*>(h8.q) : const_cast<void*>(h8.x);
+    a.y_scale = h8.scale;
+    HIP_TRY(launch_fp8_glu(a, s));
+    if (!fused) {
+        h8.rows = rows;
+        h8.cols = h8.ld_q = (int)Hp_;
+        HIP_TRY(launch_quant_rows(DType::F32, h8, s));
+    }
+    a.a = h8.q;
+    a.as = h8.scale;
+    a.b = d_q2_;
+    a.bs = d_s2_;
+    a.bias = d_b2_;
+    a.y = y;
+    a.N = (int)D_;
+    a.K = (int)Hp_;
+    HIP_TRY(launch_fp8_gemm(dt_, a, s));
+    last_in_scratch_ = false;
+    return finish_forward(rows, s, ws_);
+}
+
 int MoeLayer::forward_host(const void* x, void* y, int64_t rows) {
     if (rows < 0) return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows must be >= 0");
     if (rows == 0) { last_rows_ = 0; return NOMAS_OK; }
@@ -1021,6 +1282,8 @@ int MoeLayer::forward_host_pieces(const void* x, void* y, int64_t rows, int np, 
 int MoeLayer::routing(int32_t* idx, float* w, int32_t* counts, float* gap) {
     if (dense_only_) return set_error(NOMAS_ERR_STATE, "a dense feed-forward has no routing");
     if (last_rows_ < 0) return set_error(NOMAS_ERR_STATE, "no forward has run on this handle");
+    if (last_few_given_)
+        return set_error(NOMAS_ERR_STATE, "the last forward of few rows ran under the caller's routing");
     if (last_in_scratch_ && last_rows_ > 0 && scratch_generation(device_) != last_scratch_gen_)
         return set_error(NOMAS_ERR_STATE,
                          "the routing of this handle's last (no-allocation) forward was overwritten "

@@ -700,6 +700,45 @@ class MoeLayer:
               w.data_ptr(), out.data_ptr(), xc.numel() // self.dim)
         return out
 
+    # -- few rows ------------------------------------------------------------
+    FEW_ROWS = 64
+
+    def quantize(self) -> None:
+        """Adds an 8-bit copy of the experts' weights (and the shared branch's) to a bf16 or f16
+        layer, for forward_few(fp8=True): as quantize_fp8(square=True) makes them of each
+        (out, in) weight.  The other forwards stay as they are.  Synchronises."""
+        _check(_lib.lib().nomas_moe_quantize(self._h))
+
+    def forward_few(self, x: torch.Tensor, idx: torch.Tensor | None = None,
+                    w: torch.Tensor | None = None, *, fp8: bool = False,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+        """The layer for calls of few rows (up to 64: single tokens, small decoding batches),
+        without a dispatch and a combine.  x: (..., D) on the layer's GPU; idx and w: the
+        caller's routing as in forward_routed, or None for the router's; fp8: on the
+        experts' 8-bit weights (quantize), with activations in the model dtype.  out may be x.
+        The result is forward's (or forward_routed's) but for the order of sums, and each
+        expert's output stays in f32 up to the weighted sum."""
+        if x.dim() < 1 or x.shape[-1] != self.dim:
+            raise NomasError(2, f"expected last dim {self.dim}, got shape {tuple(x.shape)}")
+        if x.dtype != self.dtype.torch:
+            raise NomasError(2, f"expected dtype {self.dtype.torch}, got {x.dtype}")
+        if not x.is_cuda or x.device.index != self.device:
+            raise NomasError(2, f"forward_few takes tensors on the layer's GPU, got {x.device}")
+        if (idx is None) != (w is None):
+            raise NomasError(2, "idx and w must both be given")
+        xc = x.contiguous()
+        if idx is not None:
+            want = x.shape[:-1] + (self.top_k,)
+            for t, n, dt in ((idx, "idx", torch.int32), (w, "w", torch.float32)):
+                if t.shape != want or t.dtype != dt or t.device != x.device:
+                    raise NomasError(2, f"{n}: expected {tuple(want)} {dt} on {x.device}, got "
+                                        f"{tuple(t.shape)} {t.dtype} on {t.device}")
+            idx, w = idx.contiguous(), w.contiguous()
+        out = torch.empty_like(xc) if out is None else _check_out(out, xc)
+        _call(_lib.lib().nomas_moe_forward_few, xc, self._h, xc.data_ptr(), _ptr(idx), _ptr(w),
+              int(fp8), out.data_ptr(), xc.numel() // self.dim)
+        return out
+
     # -- the FFN half of DiTBlock::forward (block.rs:96-101) ------------------
     def forward_block(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
                       gate: torch.Tensor, norm_w: torch.Tensor | None = None, eps: float = 1e-6,
@@ -843,6 +882,27 @@ class FeedForward:
         return out
 
     __call__ = forward
+
+    def quantize(self) -> None:
+        """Adds an 8-bit copy of the weights to a bf16 or f16 feed-forward, for forward_fp8: as
+        quantize_fp8(square=True) makes them of each (out, in) weight.  Synchronises."""
+        _check(_lib.lib().nomas_ffn_quantize(self._h))
+
+    def forward_fp8(self, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+        """forward on 8-bit weights (quantize) and activations: x and the hidden activations in
+        blocks of 128 of a row, as quantize_fp8 makes them.  x: (..., D) in the model dtype on
+        the layer's GPU; out may be x."""
+        if x.dim() < 1 or x.shape[-1] != self.dim:
+            raise NomasError(2, f"expected last dim {self.dim}, got shape {tuple(x.shape)}")
+        if x.dtype != self.dtype.torch:
+            raise NomasError(2, f"expected dtype {self.dtype.torch}, got {x.dtype}")
+        if not x.is_cuda or x.device.index != self.device:
+            raise NomasError(2, f"forward_fp8 takes tensors on the layer's GPU, got {x.device}")
+        xc = x.contiguous()
+        out = torch.empty_like(xc) if out is None else _check_out(out, xc)
+        _call(_lib.lib().nomas_ffn_forward_fp8, xc, self._h, xc.data_ptr(), out.data_ptr(),
+              xc.numel() // self.dim)
+        return out
 
     def n_params(self) -> int:
         """mlp.rs:50-58."""

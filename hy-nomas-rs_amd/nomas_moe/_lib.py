@@ -112,6 +112,14 @@ def lib() -> C.CDLL:
     L.nomas_block_seam_backward.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp, i32, vp,
                                             f64, vp, vp, f64, vp, vp, vp, vp, vp, vp, i64, vp]
     L.nomas_block_seam_backward.restype = i32
+    L.nomas_moe_forward_few.argtypes = [vp, vp, vp, vp, i32, vp, i64, vp]
+    L.nomas_moe_forward_few.restype = i32
+    L.nomas_moe_quantize.argtypes = [vp]
+    L.nomas_moe_quantize.restype = i32
+    L.nomas_ffn_quantize.argtypes = [vp]
+    L.nomas_ffn_quantize.restype = i32
+    L.nomas_ffn_forward_fp8.argtypes = [vp, vp, vp, i64, vp]
+    L.nomas_ffn_forward_fp8.restype = i32
     L.nomas_quantize_fp8.argtypes = [i32, vp, i64, i64, i32, vp, vp, vp]
     L.nomas_quantize_fp8.restype = i32
     L.nomas_matmul_fp8.argtypes = [i32, vp, vp, vp, vp, vp, vp, i64, i64, i64, vp]

@@ -156,6 +156,25 @@ int nomas_moe_forward_block(nomas_moe_t *h, const void *x, void *out, int64_t ro
                             const float *norm_w, double eps, const float *shift,
                             const float *scale, const float *gate, void *stream);
 
+/* No counterpart in the reference: the layer for calls of few rows (up to 64: single tokens,
+ * small decoding batches), whose time is the weights' way from memory and the launches.
+ * Two kernels behind the router: no dispatch and no combine.  x, y and `stream` as in
+ * nomas_moe_forward (y may be x).  idx and w: the caller's routing as in
+ * nomas_moe_forward_routed, or both NULL for the router's.  fp8 != 0: the experts' (and the shared
+ * branch's) weights in 8 bits, which nomas_moe_quantize has made; activations stay in the
+ * handle's dtype.  The hidden activations are rounded to the handle's dtype, the rest is
+ * f32 up to y: results are those of nomas_moe_forward but for the order of sums and its rounding of
+ * each expert's output.  The first call on a handle allocates a workspace, which serves all
+ * later ones.  nomas_moe_routing() reports the router's choice; under the caller's it is NOMAS_ERR_STATE. */
+int nomas_moe_forward_few(nomas_moe_t *h, const void *x, const int32_t *idx, const float *w, int fp8, void *y,
+                          int64_t rows, void *stream);
+
+/* Adds an 8-bit copy of the experts' weights (and the shared branch's) to a BF16 or F16
+ * handle, for nomas_moe_forward_few: e4m3 with a scale for each 128 x 128 square of a
+ * weight as its (out, in) layout has it, as nomas_quantize_fp8 with `square` makes them.  The
+ * weights themselves stay, and the other forwards are as before.  Synchronises. */
+int nomas_moe_quantize(nomas_moe_t *h);
+
 /* MoeLayer::forward on host tensors (the candle CPU-tensor case): copies x in,
  * runs the forward, copies y out and synchronises.  Pageable buffers are
  * staged through the handle's pinned buffers (a threaded host copy overlapping
@@ -231,6 +250,15 @@ int nomas_ffn_from_host(int64_t dim, int64_t hidden, int dtype, int device, cons
  * aligned) on `stream`, and on host rows (copied in and out). */
 int nomas_ffn_forward(nomas_ffn_t *h, const void *x, void *y, int64_t rows, void *stream);
 int nomas_ffn_forward_host(nomas_ffn_t *h, const void *x, void *y, int64_t rows);
+
+/* No counterpart in the reference: the feed-forward on 8-bit weights and activations.
+ * nomas_ffn_quantize adds the 8-bit copy of a BF16 or F16 handle's weights (squares of 128 x 128, as
+ * nomas_quantize_fp8 makes them; synchronises).  nomas_ffn_forward_fp8: x in blocks of
+ * 128 of a row to 8 bits, gate and up products, h = silu(gate) * up in f32 to 8 bits in the same
+ * way, down product, biases in f32, y rounded once; x, y and `stream` as in nomas_ffn_forward
+ * (y may be x). */
+int nomas_ffn_quantize(nomas_ffn_t *h);
+int nomas_ffn_forward_fp8(nomas_ffn_t *h, const void *x, void *y, int64_t rows, void *stream);
 
 /* FeedForward::n_params (mlp.rs:50-58). */
 int64_t nomas_ffn_n_params(const nomas_ffn_t *h);

@@ -103,3 +103,28 @@ def test_mirror_of_matmul(no_lib):
     refused("out", mm, a, sa, b, sb, out=fake(6, 41, dtype=torch.bfloat16))
     refused("out", mm, a, sa, b, sb, out=fake(6, 40))
     refused("contiguous", mm, a, sa, b, sb, out=fake(40, 6, dtype=torch.bfloat16).T)
+
+
+# ---- the layers -------------------------------------------------------------------
+
+def test_layers_need_a_handle():
+    lib = _lib.lib()
+    for call in (lambda: lib.nomas_moe_forward_few(None, P, None, None, 0, P, 4, None), lambda: lib.nomas_moe_quantize(None),
+                 lambda: lib.nomas_ffn_quantize(None), lambda: lib.nomas_ffn_forward_fp8(None, P, P, 4, None)):
+        assert call() == 2
+        assert "handle" in _lib.last_error()
+
+
+def test_mirror_of_the_layers(no_lib):
+    layer = object.__new__(nm.MoeLayer)
+    layer._h, layer.dim, layer.top_k, layer.dtype, layer.device = None, 16, 2, nm.DataType.F32, 0
+    x, i, w = torch.zeros(4, 16), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    refused("last dim", layer.forward_few, torch.zeros(4, 8))
+    refused("dtype", layer.forward_few, x.bfloat16())
+    refused("GPU", layer.forward_few, x)
+    refused("GPU", layer.forward_few, x, i, w)
+    ffn = object.__new__(nm.FeedForward)
+    ffn._h, ffn.dim, ffn.dtype, ffn.device = None, 16, nm.DataType.F32, 0
+    refused("last dim", ffn.forward_fp8, torch.zeros(4, 8))
+    refused("dtype", ffn.forward_fp8, x.bfloat16())
+    refused("GPU", ffn.forward_fp8, x)
