@@ -94,9 +94,9 @@ __device__ __forceinline__ u32x4_t load16u(const void* p) { return *reinterpret_
 struct Lists {
     uint64_t* mask;  // [Ecols] rows that chose the expert
     int* live;       // [Ecols] the chosen experts, ascending
-    int* off;        // [Ecols] by place in `live`: the expert's first place in `row`
+    int* off;        // [Ecols] the expert's first place in `row`
     int* info;       // [16] scratch; [0]: chosen experts
-    uint8_t* row;    // [rows * slots] the experts' rows, one after another
+    uint8_t* row;    // [places] the experts' rows, one after another
     float* gate;     // ... and their weights (second kernel)
     static __host__ __device__ size_t bytes(int ecols, int places, bool gates) {
         return (size_t)ecols * 16 + 64 + (size_t)(places + 15) / 16 * 16 + (gates ? (size_t)places * 4 : 0);
@@ -111,21 +111,23 @@ struct Lists {
     }
 };
 
-// Experts named twice by a row have the sum of their weights, at the first mention.
+// Experts named twice by a row have the sum of their weights.
 template <bool kGates>
 __device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
     const int tid = threadIdx.x, n = a.rows * a.k, lane = tid & 63, wave = tid >> 6;
+    const int first_e = tid < n ? a.idx[tid] : -1;  // (on its way while the masks are cleared)
     for (int e = tid; e < a.Ecols; e += kFewThreads)
         l.mask[e] = e < a.E ? 0 : ~0ull >> (64 - a.rows);  // (the shared branch: all rows)
     __syncthreads();
     for (int i = tid; i < n; i += kFewThreads) {
-        const int e = a.idx[i];
+        const int e = i == tid ? first_e : a.idx[i];
         if (e >= 0 && e < a.E) atomicOr(reinterpret_cast<unsigned long long*>(&l.mask[e]), 1ull << (i / a.k));
     }
     __syncthreads();
     // places: the chosen experts before, and their rows (512 threads hold all experts)
     static_assert(kMaxExperts + 1 <= kFewThreads, "an expert a thread");
-    const int c = tid < a.Ecols ? __popcll(l.mask[tid]) : 0;
+    const uint64_t mine = tid < a.Ecols ? l.mask[tid] : 0;
+    const int c = __popcll(mine);
     const uint64_t some = __ballot(c > 0);
     int sum = c;
 #pragma unroll
@@ -145,25 +147,25 @@ __device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
             first += v & 0xffff;
         }
     }
-    __syncthreads();
     if (c > 0) {
-        const int at = before + __popcll(some & ((1ull << lane) - 1));
-        l.live[at] = tid;
-        l.off[at] = first + sum - c;
+        l.live[before + __popcll(some & ((1ull << lane) - 1))] = tid;
         int p = first + sum - c;
-        for (uint64_t m = l.mask[tid]; m; m &= m - 1) {
-            const int r = __builtin_ctzll(m);
-            l.row[p] = (uint8_t)r;
-            if constexpr (kGates) {
-                float w = tid < a.E ? 0.0f : a.dense_coef;
-                if (tid < a.E)
-                    for (int t = 0; t < a.k; ++t) w += a.idx[r * a.k + t] == tid ? a.w[r * a.k + t] : 0.0f;
-                l.gate[p] = w;
-            }
-            ++p;
+        l.off[tid] = p;
+        for (uint64_t m = mine; m; m &= m - 1, ++p) {
+            l.row[p] = (uint8_t)__builtin_ctzll(m);
+            if constexpr (kGates) l.gate[p] = tid < a.E ? 0.0f : a.dense_coef;
         }
     }
+    __syncthreads();
     if (tid == 0) l.info[0] = all;
+    if constexpr (kGates) {
+        if (tid < a.rows)  // a row a thread: its slots in their order
+            for (int t = 0; t < a.k; ++t) {
+                const int e = a.idx[tid * a.k + t];
+                const float w = a.w[tid * a.k + t];
+                if (e >= 0 && e < a.E) l.gate[l.off[e] + __popcll(l.mask[e] & ((1ull << tid) - 1))] += w;
+            }
+    }
     __syncthreads();
 }
 
@@ -184,6 +186,7 @@ __device__ __forceinline__ uint32_t weight_lane(int l16, int lq) {
 template <typename T, bool W8, int NT, int S, int P>
 __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     typedef Step<T, W8> St;
+    constexpr int XP = W8 && NT == 4 ? 1 : 2;  // steps of rows in flight (they come from L2)
     constexpr int GP = kFewWaves / S;  // units a block has at a time
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_part[S > 1 ? kFewWaves : 1][2][NT][kWave];
@@ -206,9 +209,8 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     auto unit = [&](int u, Unit& t) {
         const int li = u / tiles, ht = u - li * tiles;
         t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
-        t.off = __builtin_amdgcn_readfirstlane(l.off[li]);
-        t.n = __popcll(l.mask[t.e]);
-        t.n = __builtin_amdgcn_readfirstlane(t.n);
+        t.off = __builtin_amdgcn_readfirstlane(l.off[t.e]);
+        t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
         t.n0 = ht / 2 * 64 + ht % 2 * 16;
         t.w = static_cast<const uint8_t*>(a.w1) + (int64_t)t.e * a.w1_expert + (int64_t)t.n0 * kKBlockBytes;
 #pragma unroll
@@ -219,16 +221,27 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
             t.su = t.sg + (int64_t)a.hb * a.kb1;
         }
     };
-    struct Data {
-        u32x4_t w[2][2], x[NT][St::XL];
+    struct Weights {
+        u32x4_t w[2][2];
         float s[2];
     };
-    auto fetch = [&](const Unit& t, int st, Data& d) {
+    struct Tokens {
+        u32x4_t x[NT][St::XL];
+    };
+    auto fetch_w = [&](const Unit& t, int st, Weights& d) {
         const uint8_t* p = t.w + 2 * st * kstep + wl;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int q = 0; q < 2; ++q) d.w[i][q] = load16u(p + q * kstep + i * 32 * kKBlockBytes);
+        if constexpr (W8) {
+            d.s[0] = t.sg[st];
+            d.s[1] = t.su[st];
+        } else {
+            d.s[0] = d.s[1] = a.w1_down;
+        }
+    };
+    auto fetch_x = [&](const Unit& t, int st, Tokens& d) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             if (j * 16 >= t.n) break;
@@ -238,12 +251,6 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
                 d.x[j][q] = u32x4_t{0, 0, 0, 0};
                 if (k < a.D) d.x[j][q] = load16u(t.x[j] + k * sizeof(T));
             }
-        }
-        if constexpr (W8) {
-            d.s[0] = t.sg[st];
-            d.s[1] = t.su[st];
-        } else {
-            d.s[0] = d.s[1] = a.w1_down;
         }
     };
     for (int u0 = blockIdx.x * GP; u0 < units; u0 += gridDim.x * GP) {
@@ -256,10 +263,14 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         unit(min(u0 + g, units - 1), t);
         if (mine) {
-            Data d[P];
+            Weights wd[P];
+            Tokens xd[XP];
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                if (s0 + p < s1) fetch(t, s0 + p, d[p]);
+                if (s0 + p < s1) fetch_w(t, s0 + p, wd[p]);
+#pragma unroll
+            for (int p = 0; p < XP; ++p)
+                if (s0 + p < s1) fetch_x(t, s0 + p, xd[p]);
             for (int st = s0; st < s1; st += P) {
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
@@ -268,9 +279,10 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
                     for (int j = 0; j < NT; ++j) {
                         if (j * 16 >= t.n) break;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) multiply<T, W8>(acc[i][j], d[p].w[i], d[p].x[j], d[p].s[i]);
+                        for (int i = 0; i < 2; ++i) multiply<T, W8>(acc[i][j], wd[p].w[i], xd[p % XP].x[j], wd[p].s[i]);
                     }
-                    if (st + p + P < s1) fetch(t, st + p + P, d[p]);
+                    if (st + p + P < s1) fetch_w(t, st + p + P, wd[p]);
+                    if (st + p + XP < s1) fetch_x(t, st + p + XP, xd[p % XP]);
                 }
             }
         }
@@ -318,6 +330,7 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
 template <typename T, bool W8, int NT, int P>
 __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     typedef Step<T, W8> St;
+    constexpr int XP = W8 && NT == 4 ? 1 : 2;  // steps of rows in flight
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_y[kFewWaves][16 * NT][4];  // [wave][row][4 columns each]
     __shared__ int s_last;
@@ -337,49 +350,54 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     const int live_h = (a.H + 15) / 16 * 16;  // columns of h that are written
 
     for (int r = lane; r < 16 * NT * 4; r += kWave) s_y[wave][r / 4][r % 4] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    struct Data {
-        u32x4_t w[2], x[NT][St::XL];
+    struct At {
+        int li, st, e, off, n;  // a chosen expert and a step of it
+    };
+    auto place = [&](At& t, int li, int st) {
+        t.li = li;
+        t.st = st;
+        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
+        t.off = __builtin_amdgcn_readfirstlane(l.off[t.e]);
+        t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
+    };
+    auto next = [&](At& t, int s) {  // to step s, the one after t's
+        if (++t.st == steps && s < s1) place(t, t.li + 1, 0);
+    };
+    struct Weights {
+        u32x4_t w[2];
         float s;
     };
-    struct At {
-        int e, off, n;
+    struct Tokens {
+        u32x4_t x[NT][St::XL];
     };
-    auto place = [&](int li) {
-        At t;
-        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
-        t.off = __builtin_amdgcn_readfirstlane(l.off[li]);
-        t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
-        return t;
-    };
-    auto fetch = [&](int s, Data& d) {
-        const int li = s / steps, st = s - li * steps;
-        const At t = place(li);
+    auto fetch_w = [&](const At& t, Weights& d) {
         const uint8_t* p = static_cast<const uint8_t*>(a.w2) + (int64_t)t.e * a.w2_expert + (int64_t)n0 * kKBlockBytes +
-                           2 * st * kstep + wl;
+                           2 * t.st * kstep + wl;
 #pragma unroll
         for (int q = 0; q < 2; ++q) d.w[q] = load16u(p + q * kstep);
+        if constexpr (W8) d.s = a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + t.st];
+        else d.s = a.w2_down;
+    };
+    auto fetch_x = [&](const At& t, Tokens& d) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             if (j * 16 >= t.n) break;
             const T* h = static_cast<const T*>(a.h) + (int64_t)(t.off + min(j * 16 + l16, t.n - 1)) * a.ldh;
 #pragma unroll
             for (int q = 0; q < St::XL; ++q) {
-                const int k = st * St::KS + St::xk(q, lq);
+                const int k = t.st * St::KS + St::xk(q, lq);
                 d.x[j][q] = u32x4_t{0, 0, 0, 0};
                 if (k < live_h) d.x[j][q] = load16u(h + k);
             }
         }
-        if constexpr (W8) d.s = a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + st];
-        else d.s = a.w2_down;
     };
     f32x4_t acc[NT];
     auto clear = [&] {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     };
-    // the sums of expert `li` so far, weighed, to the rows' (each row of it is one lane's)
-    auto flush = [&](int li, bool bias) {
-        const At t = place(li);
+    // the sums of an expert so far, weighed, to the rows' (each row of it is one lane's)
+    auto flush = [&](const At& t, bool bias) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int m = j * 16 + l16;
@@ -399,32 +417,52 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
         clear();
     };
     clear();
-    Data d[P];
+    if (s0 < s1) {
+        At at, aw, ax;  // of the products, of the weights' and the rows' loads
+        place(at, s0 / steps, s0 % steps);
+        aw = ax = at;
+        bool whole = at.st == 0;  // the expert's first step is this wave's
+        Weights wd[P];
+        Tokens xd[XP];
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-        if (s0 + p < s1) fetch(s0 + p, d[p]);
-    int li = s0 / steps, end = (li + 1) * steps, from = s0;
-    int n = s0 < s1 ? place(li).n : 0;
-    for (int s = s0; s < s1; s += P) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            if (s + p >= s1) break;
-            if (s + p == end) {
-                flush(li, from <= end - steps);
-                ++li;
-                from = end;
-                end += steps;
-                n = place(li).n;
+        for (int p = 0; p < P; ++p)
+            if (s0 + p < s1) {
+                fetch_w(aw, wd[p]);
+                next(aw, s0 + p + 1);
             }
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (j * 16 >= n) break;
-                multiply<T, W8>(acc[j], d[p].w, d[p].x[j], d[p].s);
+        for (int p = 0; p < XP; ++p)
+            if (s0 + p < s1) {
+                fetch_x(ax, xd[p]);
+                next(ax, s0 + p + 1);
             }
-            if (s + p + P < s1) fetch(s + p + P, d[p]);
+        for (int s = s0; s < s1; s += P) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                if (s + p >= s1) break;
+                if (at.st == steps) {
+                    flush(at, whole);
+                    place(at, at.li + 1, 0);
+                    whole = true;
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if (j * 16 >= at.n) break;
+                    multiply<T, W8>(acc[j], wd[p].w, xd[p % XP].x[j], wd[p].s);
+                }
+                ++at.st;
+                if (s + p + P < s1) {
+                    fetch_w(aw, wd[p]);
+                    next(aw, s + p + P + 1);
+                }
+                if (s + p + XP < s1) {
+                    fetch_x(ax, xd[p % XP]);
+                    next(ax, s + p + XP + 1);
+                }
+            }
         }
+        flush(at, whole);
     }
-    if (s0 < s1) flush(li, from <= end - steps);
     __syncthreads();
     // the waves' sums in wave order; thread (row, column quarter)
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -436,19 +474,35 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
         for (int w = 1; w < kFewWaves; ++w) v += s_y[w][row][c];
     }
     if (a.parts > 1) {
-        // the last block to arrive adds the shares, in their order
-        f32x4_t* ws = reinterpret_cast<f32x4_t*>(a.partial) + (int64_t)tile * a.parts * a.rows * 4;
-        if (row < a.rows) ws[((int64_t)part * a.rows + row) * 4 + c] = v;
-        __threadfence();
+        // The last block to arrive adds the shares, in their order.  Blocks of a tile run on
+        // different XCDs, whose L2 caches are not coherent: the shares are written and read past
+        // them (agent-scope cache policy), each block's increment is a release, and the
+        // one that completes the count acquires.  (A fence of every wave took 50 us of a call: it
+        // writes back and empties the L2.)
+        constexpr int kSc1 = 16;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(a.partial + (int64_t)tile * kFewParts * kFewRows * 16, 0,
+                                                          kFewParts * kFewRows * 64, 0x00020000);
+        if (row < a.rows)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), rs, (part * kFewRows + row) * 64 + c * 16, 0,
+                                                   kSc1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (tid == 0)
-            s_last = __hip_atomic_fetch_add(&a.arrived[tile], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+        if (tid == 0) {
+            s_last = __hip_atomic_fetch_add(&a.arrived[tile], 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+            if (s_last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        }
         __syncthreads();
         if (!s_last) return;
-        __threadfence();
         if (row < a.rows) {
-            v = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int p = 0; p < a.parts; ++p) v += ws[((int64_t)p * a.rows + row) * 4 + c];
+            f32x4_t t[kFewParts];
+#pragma unroll
+            for (int p = 0; p < kFewParts; ++p)  // (past the last part: any of them, not used)
+                t[p] = __builtin_bit_cast(
+                    f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (min(p, a.parts - 1) * kFewRows + row) * 64 + c * 16, 0, kSc1));
+            v = t[0];
+#pragma unroll
+            for (int p = 1; p < kFewParts; ++p)
+                if (p < a.parts) v += t[p];
         }
         if (tid == 0) __hip_atomic_store(&a.arrived[tile], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -477,24 +531,25 @@ hipError_t launch(F kernel, int64_t grid, size_t fixed, size_t lds, const FewArg
     return hipGetLastError();
 }
 
-constexpr int kTargetWaves = 256 * 8;  // that fill the chip
-
 template <typename T, bool W8, int NT>
 hipError_t launch_nt(FewArgs a, hipStream_t s) {
-    constexpr int P = W8 ? (NT == 1 ? 3 : NT == 2 ? 2 : 1) : NT == 1 ? 4 : 2;  // steps in flight
+    constexpr int P = 4;  // steps of weights in flight
+    typedef Step<T, W8> St;
     const int slots = a.k + a.Ecols - a.E, places = a.rows * slots;
     const int tiles = (a.H + 15) / 16, live = std::min(a.E, a.rows * a.k) + a.Ecols - a.E;
     const int64_t units = (int64_t)tiles * live;
     const size_t lds1 = Lists::bytes(a.Ecols, places, false), lds2 = Lists::bytes(a.Ecols, places, true);
-    const int S = units * 2 > kTargetWaves ? 2 : units * 4 > kTargetWaves ? 4 : 8;
-    const int grid = (int)std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 512);
+    const int S = units >= 256 * 6 ? 1 : units >= 256 * 3 ? 2 : units * 4 >= 256 * 6 ? 4 : 8;
+    const int64_t grid = std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 512);
     constexpr size_t fixed1 = kFewWaves * 2 * NT * kWave * 16, fixed2 = kFewWaves * NT * kWave * 16 + 16;
-    hipError_t e = S == 2   ? launch(few_up_kernel<T, W8, NT, 2, P>, grid, fixed1, lds1, a, s)
+    hipError_t e = S == 1   ? launch(few_up_kernel<T, W8, NT, 1, P>, grid, fixed1, lds1, a, s)
+                   : S == 2 ? launch(few_up_kernel<T, W8, NT, 2, P>, grid, fixed1, lds1, a, s)
                    : S == 4 ? launch(few_up_kernel<T, W8, NT, 4, P>, grid, fixed1, lds1, a, s)
                             : launch(few_up_kernel<T, W8, NT, 8, P>, grid, fixed1, lds1, a, s);
     if (e != hipSuccess) return e;
     const int ntiles = (a.D + 15) / 16;
-    a.parts = std::max(1, std::min(kFewParts, 256 / ntiles));
+    // (no part of a tile without work for all of its waves)
+    a.parts = std::max(1, std::min({kFewParts, 256 / ntiles, live * ((a.H + St::KS - 1) / St::KS) / (kFewWaves * 4)}));
     return launch(few_down_kernel<T, W8, NT, P>, ntiles * a.parts, fixed2, lds2, a, s);
 }
 
