@@ -90,6 +90,194 @@ __device__ __forceinline__ void multiply(f32x4_t& acc, const u32x4_t (&w)[2], co
 
 __device__ __forceinline__ u32x4_t load16u(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 
+// ---- the router's choice ---------------------------------------------------------
+// Softmax over the logits, top-k with ties to the lowest index, weights p / (sum of the chosen p + 1e-9)
+// in ascending order of experts: the layer's router (router.hip) for few rows.  16-bit products are exact
+// in f32, each MFMA's 32 of them summed there and those sums in f64; f32 inputs take f64 MFMAs.
+
+typedef double d4_t __attribute__((ext_vector_type(4)));
+
+// The logits of 16 rows and 16 experts, D shared by the block's waves; thread t < 256 returns that of
+// row t / 16 and expert t % 16.  s_part: 256 per wave.
+template <typename T>
+__device__ __forceinline__ double logit_tile(const FewArgs& a, int rg, int eg, double* s_part) {
+    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int CH = 16 / (int)sizeof(T), KS = 4 * CH;  // columns a lane, and of a step
+    const int steps = (a.D + KS - 1) / KS, s0 = steps * wave / kFewWaves, s1 = steps * (wave + 1) / kFewWaves;
+    const T* x = static_cast<const T*>(a.x) + (int64_t)min(rg * 16 + l16, a.rows - 1) * a.D + lq * CH;
+    const T* w = static_cast<const T*>(a.wr) + (int64_t)min(eg * 16 + l16, a.E - 1) * a.D + lq * CH;
+    d4_t acc = {0.0, 0.0, 0.0, 0.0};
+    constexpr int U = 8;
+    for (int st = s0; st < s1; st += U) {
+        u32x4_t xv[U], wv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (st + u) * KS;
+            xv[u] = wv[u] = u32x4_t{0, 0, 0, 0};
+            if (st + u < s1 && k + lq * CH < a.D) {
+                xv[u] = load16u(x + k);
+                wv[u] = load16u(w + k);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {  // (past the end: zeros)
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)__uint_as_float(xv[u][i]),
+                                                               (double)__uint_as_float(wv[u][i]), acc, 0, 0, 0);
+            } else {
+                typedef typename Mfma<T>::V V;
+                const f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+                const f32x4_t t = Mfma<T>::run(__builtin_bit_cast(V, xv[u]), __builtin_bit_cast(V, wv[u]), z);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[r] += (double)t[r];
+            }
+        }
+    }
+    // lane: expert l16 of rows 4 lq + r (f64 MFMAs: lq + 4 r)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_part[wave * 256 + (sizeof(T) == 4 ? lq + 4 * r : 4 * lq + r) * 16 + l16] = acc[r];
+    __syncthreads();
+    double v = 0.0;
+    if (tid < 256) {
+        v = s_part[tid];
+#pragma unroll
+        for (int i = 1; i < kFewWaves; ++i) v += s_part[i * 256 + tid];
+    }
+    return v;
+}
+
+// f64 as an integer of the same order; NaN above all, so that the choice is always k experts.
+__device__ __forceinline__ int64_t order_key(double v) {
+    if (v != v) return INT64_MAX;
+    const int64_t b = __double_as_longlong(v + 0.0);  // (-0 is 0)
+    return b ^ ((b >> 63) & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ double wave_max(double v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmax(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// One wave chooses for one row: its logits `l` (LDS, E of them), PL a lane.  An expert is chosen if
+// fewer than k others are before it: a count over all, without rounds.
+template <int PL, typename F>
+__device__ __forceinline__ void choose(const FewArgs& a, const double* l, int row, bool store, F chosen) {
+    const int lane = threadIdx.x & 63, E = a.E, k = a.top_k;
+    double v[PL];
+    int64_t key[PL];
+    int before[PL];
+    double m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+        const int e = lane + j * 64;
+        v[j] = e < E ? l[e] : -INFINITY;
+        key[j] = order_key(v[j]);
+        before[j] = e < E ? 0 : E;
+        m = fmax(m, v[j]);
+    }
+    for (int e = 0; e < E; ++e) {
+        const int64_t o = order_key(l[e]);
+#pragma unroll
+        for (int j = 0; j < PL; ++j) before[j] += o > key[j] || (o == key[j] && e < lane + j * 64);
+    }
+    m = wave_max(m);
+    float p[PL];
+    double sum = 0.0, sel = 0.0, kth = 0.0, next = 0.0;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+        p[j] = lane + j * 64 < E ? expf((float)(v[j] - m)) : 0.0f;
+        sum += (double)p[j];
+        sel += before[j] < k ? (double)p[j] : 0.0;
+        kth += before[j] == k - 1 ? v[j] : 0.0;  // (one lane's)
+        next += before[j] == k ? v[j] : 0.0;
+    }
+    sum = wave_sum(sum);
+    sel = wave_sum(sel);
+    const double inv = 1.0 / sum, norm = 1.0 / (sel * inv + 1e-9);
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+        const uint64_t c = __ballot(before[j] < k);
+        if (before[j] < k) {
+            const int e = lane + j * 64, t = at + __popcll(c & ((1ull << lane) - 1));
+            chosen(t, e);
+            if (store) {
+                a.out_idx[row * a.out_slots + t] = e;
+                a.out_w[row * a.out_slots + t] = (float)((double)p[j] * inv * norm);
+            }
+        }
+        at += __popcll(c);
+    }
+    if (store) {
+        kth = wave_sum(kth);
+        next = wave_sum(next);
+        if (lane == 0) {
+            a.out_gap[row] = k == E ? INFINITY : (float)(kth - next);
+            if (a.out_slots > k) {
+                a.out_idx[row * a.out_slots + k] = E;
+                a.out_w[row * a.out_slots + k] = a.dense_coef;
+            }
+        }
+    }
+}
+template <typename F>
+__device__ __forceinline__ void choose_any(const FewArgs& a, const double* l, int row, bool store, F chosen) {
+    if (a.E <= 64) choose<1>(a, l, row, store, chosen);
+    else choose<kMaxExperts / 64>(a, l, row, store, chosen);
+}
+
+// A kernel of its own: a block for 16 rows and 16 experts; the last one of 16 rows chooses.
+template <typename T>
+__global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
+    extern __shared__ __align__(16) uint8_t s_dyn[];  // 16 rows' logits
+    __shared__ double s_part[kFewWaves * 256];
+    __shared__ int s_count[kMaxExperts + 1], s_last;
+    double* s_logit = reinterpret_cast<double*>(s_dyn);
+    const int tid = threadIdx.x, wave = tid >> 6, eg = blockIdx.x, rg = blockIdx.y, groups = gridDim.x;
+    const double v = logit_tile<T>(a, rg, eg, s_part);
+    const int r = tid / 16, e = eg * 16 + tid % 16;
+    if (groups > 1) {
+        // as in few_down_kernel: past the L2 caches, release and acquire around the count
+        constexpr int kSc1 = 16;
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(a.logits, 0, kFewRows * kMaxExperts * 8, 0x00020000);
+        typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+        if (tid < 256 && e < a.E)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, v), rs, ((rg * 16 + r) * kMaxExperts + e) * 8, 0,
+                                                  kSc1);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        int32_t* count = a.arrived + a.tile_cap + rg;
+        if (tid == 0) {
+            s_last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+            if (s_last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        }
+        __syncthreads();
+        if (!s_last) return;
+        for (int i = tid; i < 16 * a.E; i += kFewThreads) {
+            const int row = i / a.E, ex = i - row * a.E;
+            s_logit[i] = __builtin_bit_cast(
+                double, __builtin_amdgcn_raw_buffer_load_b64(rs, ((rg * 16 + row) * kMaxExperts + ex) * 8, 0, kSc1));
+        }
+        if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else if (tid < 256 && e < a.E) {
+        s_logit[r * a.E + e] = v;
+    }
+    for (int i = tid; i < a.Ecols; i += kFewThreads) s_count[i] = i < a.E ? 0 : min(16, a.rows - rg * 16);
+    __syncthreads();
+    for (int i = wave; i < min(16, a.rows - rg * 16); i += kFewWaves)
+        choose_any(a, s_logit + i * a.E, rg * 16 + i, true, [&](int, int ex) { atomicAdd(&s_count[ex], 1); });
+    __syncthreads();
+    for (int i = tid; i < a.Ecols; i += kFewThreads) a.out_count[rg * a.Ecols + i] = s_count[i];
+}
+
 // What a block knows of the routing.
 struct Lists {
     uint64_t* mask;  // [Ecols] rows that chose the expert
@@ -553,8 +741,20 @@ hipError_t launch_nt(FewArgs a, hipStream_t s) {
     return launch(few_down_kernel<T, W8, NT, P>, ntiles * a.parts, fixed2, lds2, a, s);
 }
 
+template <typename T>
+hipError_t launch_route(const FewArgs& a, hipStream_t s) {
+    const size_t lds = (size_t)16 * a.E * sizeof(double);  // (at most 32 KB beside 17 KB)
+    launch_kernel(few_route_kernel<T>, dim3((unsigned)(a.E + 15) / 16, (unsigned)(a.rows + 15) / 16), dim3(kFewThreads),
+                  (uint32_t)lds, s, a);
+    return hipGetLastError();
+}
+
 template <typename T, bool W8>
 hipError_t launch_few_t(const FewArgs& a, hipStream_t s) {
+    if (a.wr) {
+        const hipError_t e = launch_route<T>(a, s);
+        if (e != hipSuccess) return e;
+    }
     if (a.rows <= 16) return launch_nt<T, W8, 1>(a, s);
     if (a.rows <= 32) return launch_nt<T, W8, 2>(a, s);
     return launch_nt<T, W8, 4>(a, s);

@@ -327,6 +327,7 @@ private:
     void* d_few_ = nullptr;
     Workspace few_ws_;
     float* few_partial_ = nullptr;
+    double* few_logits_ = nullptr;
     int32_t* few_arrived_ = nullptr;
     int ensure_few();
     bool last_few_given_ = false;  // the last forward was forward_few under the caller's routing

@@ -318,6 +318,7 @@ struct QuantSquareArgs {
 };
 // The MoE layer on few rows (few.hip).
 constexpr int kFewRows = 64;
+constexpr int kFewGroups = kFewRows / 16;
 constexpr int kFewParts = 4;  // blocks that share 16 columns of y, at most
 struct FewArgs {
     const void* x;       // rows x D, model dtype
@@ -337,9 +338,16 @@ struct FewArgs {
     void* h;             // hidden activations, ldh columns a place
     int64_t ldh;
     float* partial;      // tile_cap x kFewParts x rows x 16 sums
-    int32_t* arrived;    // tile_cap counters, zero between calls
+    int32_t* arrived;    // tile_cap + kFewGroups counters, zero between calls
     int tile_cap;
     int parts;           // (set by the launch)
+    // the router (wr non-null): its choice goes to idx and w too, which have out_slots a row
+    const void* wr;      // E x D
+    int top_k;
+    double* logits;      // kFewRows x kMaxExperts
+    int32_t *out_idx, *out_count;  // out_count: Ecols for each 16 rows
+    float *out_w, *out_gap;
+    int out_slots;
 };
 hipError_t launch_few(DType dt, const FewArgs& a, hipStream_t s);
 hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s);

@@ -942,12 +942,12 @@ int MoeLayer::ensure_few() {
     };
     auto lay = [&] {
         off = 0;
-        few_arrived_ = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * tiles));
+        few_arrived_ = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * (tiles + kFewGroups)));
+        few_logits_ = reinterpret_cast<double*>(take(sizeof(double) * kFewRows * kMaxExperts));
         w.idx = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * kFewRows * kslots_));
         w.w = reinterpret_cast<float*>(take(sizeof(float) * kFewRows * kslots_));
         w.gap = reinterpret_cast<float*>(take(sizeof(float) * kFewRows));
-        w.expert_count = w.chunk_counts = reinterpret_cast<int32_t*>(
-            take(sizeof(int32_t) * (kFewRows / kMinRouterBlockRows) * Ecols_));
+        w.expert_count = reinterpret_cast<int32_t*>(take(sizeof(int32_t) * kFewGroups * Ecols_));
         w.h = take(dtype_size(dt_) * kFewRows * kslots_ * round_up(H_, 16));
         few_partial_ = reinterpret_cast<float*>(take(sizeof(float) * tiles * kFewParts * kFewRows * 16));
     };
@@ -956,7 +956,7 @@ int MoeLayer::ensure_few() {
     HIP_TRY(hipMalloc(&p, off));
     base = static_cast<uint8_t*>(p);
     lay();
-    const hipError_t e = hipMemset(few_arrived_, 0, sizeof(int32_t) * tiles);
+    const hipError_t e = hipMemset(few_arrived_, 0, sizeof(int32_t) * (tiles + kFewGroups));
     if (e != hipSuccess || hipDeviceSynchronize() != hipSuccess) {
         (void)hipFree(p);
         return set_error(NOMAS_ERR_HIP, "clearing the counters failed: %s", hipGetErrorString(e));
@@ -985,26 +985,7 @@ int MoeLayer::forward_few(const void* x, const Given* g, bool fp8, void* y, int6
     if (rc != NOMAS_OK) return rc;
     if (done_recorded_ && s != last_stream_) HIP_TRY(hipStreamWaitEvent(s, done_, 0));
     const Workspace& w = few_ws_;
-    int count_rows = kRouterRows;
     last_rows_ = -1;  // (until all is launched)
-    if (!g) {
-        count_rows = router_block_rows(dt_, rows, (int)D_, (int)E_);
-        RouterArgs ra;
-        ra.x = x;
-        ra.wr = d_wr_;
-        ra.rows = rows;
-        ra.D = (int)D_;
-        ra.E = (int)E_;
-        ra.k = (int)k_;
-        ra.k_slots = (int)kslots_;
-        ra.dense_coef = (float)shared_dense_;
-        ra.topk_idx = w.idx;
-        ra.topk_w = w.w;
-        ra.gap = w.gap;
-        ra.chunk_counts = w.chunk_counts;
-        ra.block_rows = count_rows;
-        HIP_TRY(launch_router(dt_, ra, s));
-    }
     FewArgs a = {};
     a.x = x;
     a.y = y;
@@ -1041,9 +1022,19 @@ int MoeLayer::forward_few(const void* x, const Given* g, bool fp8, void* y, int6
     a.partial = few_partial_;
     a.arrived = few_arrived_;
     a.tile_cap = (int)((D_ + 15) / 16);
+    if (!g) {
+        a.wr = d_wr_;
+        a.top_k = (int)k_;
+        a.logits = few_logits_;
+        a.out_idx = w.idx;
+        a.out_w = w.w;
+        a.out_gap = w.gap;
+        a.out_count = w.expert_count;
+        a.out_slots = (int)kslots_;
+    }
     HIP_TRY(launch_few(dt_, a, s));
     last_in_scratch_ = false;
-    rc = finish_forward(rows, s, w, (int)((rows + count_rows - 1) / count_rows));
+    rc = finish_forward(rows, s, w, (int)((rows + 15) / 16));  // (expert counts of each 16 rows)
     last_few_given_ = g != nullptr;
     return rc;
 }

@@ -25,6 +25,7 @@ def case(rows, D, E, k, H, dtype, seed, s=0.0, fp8=False):
     layer = layer_from_tensors(t, dtype, D, H, E, k, s)
     rt, xm = rounded(t, x, dtype)
     p, dense = nm.workloads.oracle_params(rt, E)
+    layer.wr = p["wr"]
     names = ("wg", "bg", "wu", "bu", "wd", "bd")
     ffn = [[np.asarray(p[n][e], np.float64) for n in names] for e in range(E)]
     ffn += [[np.asarray(dense[n], np.float64) for n in names]] if s > 0 else []
@@ -82,9 +83,23 @@ def test_the_routers_choice(rows, D, E, k, H, s, dtype, fp8):
     idx, w, counts, gap = layer.routing(rows)
     near(y, *plain(xm, ffn, idx, w, dtype, s))
     assert bool((big[rows * D:] == 7.0).all())
-    layer.forward(x)  # the same routing, to the bit
+    # The layer's own router: of 16-bit products both sum 32 at a time in f32 (at most 32 steps of 2^-23 of their
+    # magnitudes; f32 inputs are summed in f64) and those sums in f64, in another order.  So two logits
+    # are that far apart twice; a weight is a ratio of exponentials of differences of logits, each exponential
+    # with an f32 argument and its own error.
+    layer.forward(x)
     i2, w2, c2, g2 = layer.routing(rows)
-    assert np.array_equal(idx, i2) and np.array_equal(w, w2) and np.array_equal(counts, c2) and np.array_equal(gap, g2)
+    dl = 2 * 32 * U * (np.abs(xm.astype(np.float64)) @ np.abs(layer.wr.astype(np.float64)).T).max(1)
+    dl = dl if dtype != "f32" else 2.0 ** -40 + 0 * dl
+    sure = (gap > dl) | np.isinf(gap)
+    assert sure.any() and np.array_equal(idx[sure], i2[sure]) and counts.sum() == rows * k
+    spread = 64.0  # (no logit here is further from the largest)
+    rel = np.expm1(2 * dl) + 4 * (spread + 4) * U
+    assert np.all(np.abs(w - w2)[sure] <= (rel[:, None] * np.abs(w2))[sure])
+    both = sure & np.isfinite(gap)
+    assert np.all(np.abs(gap - g2)[both] <= (2 * dl + U * np.abs(g2))[both]) and np.array_equal(np.isinf(gap), np.isinf(g2))
+    if sure.all():
+        assert np.array_equal(counts, c2)
 
 
 @pytest.mark.parametrize("dtype,fp8", [("f32", False), ("bf16", False), ("f16", True)])
