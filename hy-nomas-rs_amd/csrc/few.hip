@@ -155,15 +155,24 @@ __device__ __forceinline__ int64_t order_key(double v) {
     const int64_t b = __double_as_longlong(v + 0.0);  // (-0 is 0)
     return b ^ ((b >> 63) & 0x7fffffffffffffffll);
 }
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmax(v, __shfl_xor(v, o));
-    return v;
+template <int kCtrl>
+__device__ __forceinline__ float dpp_addf(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// Over a wave, in all lanes.
+__device__ __forceinline__ float wave_max(float v) {
+    const uint32_t b = __float_as_uint(v), m = max16(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u));  // (in their order)
+    auto lane = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)m, i); };
+    const uint32_t t = max(max(lane(0), lane(16)), max(lane(32), lane(48)));
+    return __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = dpp_addf<0xb1>(v);
+    v = dpp_addf<0x4e>(v);
+    v = dpp_addf<0x141>(v);
+    v = dpp_addf<0x140>(v);
+    auto lane = [&](int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
+    return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
 // One wave chooses for one row: its logits `l` (LDS, E of them), PL a lane.  An expert is chosen if
@@ -174,35 +183,35 @@ __device__ __forceinline__ void choose(const FewArgs& a, const double* l, int ro
     double v[PL];
     int64_t key[PL];
     int before[PL];
-    double m = -INFINITY;
+    float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
         const int e = lane + j * 64;
         v[j] = e < E ? l[e] : -INFINITY;
         key[j] = order_key(v[j]);
         before[j] = e < E ? 0 : E;
-        m = fmax(m, v[j]);
+        m = fmaxf(m, (float)v[j]);
     }
+#pragma unroll 8
     for (int e = 0; e < E; ++e) {
         const int64_t o = order_key(l[e]);
 #pragma unroll
         for (int j = 0; j < PL; ++j) before[j] += o > key[j] || (o == key[j] && e < lane + j * 64);
     }
-    m = wave_max(m);
-    float p[PL];
-    double sum = 0.0, sel = 0.0, kth = 0.0, next = 0.0;
+    m = wave_max(m);  // (any number near the largest does)
+    float p[PL], sum = 0.0f, sel = 0.0f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-        p[j] = lane + j * 64 < E ? expf((float)(v[j] - m)) : 0.0f;
-        sum += (double)p[j];
-        sel += before[j] < k ? (double)p[j] : 0.0;
-        kth += before[j] == k - 1 ? v[j] : 0.0;  // (one lane's)
-        next += before[j] == k ? v[j] : 0.0;
+        p[j] = lane + j * 64 < E ? expf((float)(v[j] - (double)m)) : 0.0f;
+        sum += p[j];
+        sel += before[j] < k ? p[j] : 0.0f;
     }
     sum = wave_sum(sum);
     sel = wave_sum(sel);
-    const double inv = 1.0 / sum, norm = 1.0 / (sel * inv + 1e-9);
+    // p / sum / (sel / sum + 1e-9)
+    const float norm = 1.0f / (sel + 1e-9f * sum);
     int at = 0;
+    double kth = 0.0, next = 0.0;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
         const uint64_t c = __ballot(before[j] < k);
@@ -211,20 +220,21 @@ __device__ __forceinline__ void choose(const FewArgs& a, const double* l, int ro
             chosen(t, e);
             if (store) {
                 a.out_idx[row * a.out_slots + t] = e;
-                a.out_w[row * a.out_slots + t] = (float)((double)p[j] * inv * norm);
+                a.out_w[row * a.out_slots + t] = p[j] * norm;
             }
         }
         at += __popcll(c);
+        if (store) {  // the logits of the last one chosen and the first one not
+            const uint64_t last = __ballot(before[j] == k - 1), first = __ballot(before[j] == k && lane + j * 64 < E);
+            if (last) kth = __shfl(v[j], __builtin_ctzll(last));
+            if (first) next = __shfl(v[j], __builtin_ctzll(first));
+        }
     }
-    if (store) {
-        kth = wave_sum(kth);
-        next = wave_sum(next);
-        if (lane == 0) {
-            a.out_gap[row] = k == E ? INFINITY : (float)(kth - next);
-            if (a.out_slots > k) {
-                a.out_idx[row * a.out_slots + k] = E;
-                a.out_w[row * a.out_slots + k] = a.dense_coef;
-            }
+    if (store && lane == 0) {
+        a.out_gap[row] = k == E ? INFINITY : (float)(kth - next);
+        if (a.out_slots > k) {
+            a.out_idx[row * a.out_slots + k] = E;
+            a.out_w[row * a.out_slots + k] = a.dense_coef;
         }
     }
 }
@@ -245,7 +255,7 @@ __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
     const double v = logit_tile<T>(a, rg, eg, s_part);
     const int r = tid / 16, e = eg * 16 + tid % 16;
     if (groups > 1) {
-        // as in few_down_kernel: past the L2 caches, release and acquire around the count
+        // as in few_down_kernel: past the L2 caches, written before the block is counted
         constexpr int kSc1 = 16;
         const auto rs = __builtin_amdgcn_make_buffer_rsrc(a.logits, 0, kFewRows * kMaxExperts * 8, 0x00020000);
         typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -255,10 +265,8 @@ __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         int32_t* count = a.arrived + a.tile_cap + rg;
-        if (tid == 0) {
-            s_last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
-            if (s_last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        }
+        if (tid == 0)
+            s_last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
         __syncthreads();
         if (!s_last) return;
         for (int i = tid; i < 16 * a.E; i += kFewThreads) {
@@ -299,17 +307,30 @@ struct Lists {
     }
 };
 
-// Experts named twice by a row have the sum of their weights.
+// The slots of a call in LDS (experts, weights); calls of more of them are read again where needed.
+constexpr int kStaged = 2048;
+
+// Experts named twice by a row have the sum of their weights, in the slots' order.
 template <bool kGates>
 __device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
+    __shared__ int16_t s_e[kGates ? kStaged : 1];
+    __shared__ float s_w[kGates ? kStaged : 1];
     const int tid = threadIdx.x, n = a.rows * a.k, lane = tid & 63, wave = tid >> 6;
-    const int first_e = tid < n ? a.idx[tid] : -1;  // (on its way while the masks are cleared)
+    const bool staged = n <= kStaged;
+    // (on their way while the masks are cleared)
+    const int first_e = tid < n ? a.idx[tid] : -1;
+    const float first_w = kGates && tid < n ? a.w[tid] : 0.0f;
     for (int e = tid; e < a.Ecols; e += kFewThreads)
         l.mask[e] = e < a.E ? 0 : ~0ull >> (64 - a.rows);  // (the shared branch: all rows)
     __syncthreads();
     for (int i = tid; i < n; i += kFewThreads) {
-        const int e = i == tid ? first_e : a.idx[i];
-        if (e >= 0 && e < a.E) atomicOr(reinterpret_cast<unsigned long long*>(&l.mask[e]), 1ull << (i / a.k));
+        const int in = i == tid ? first_e : a.idx[i], e = in >= 0 && in < a.E ? in : -1;
+        if (e >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&l.mask[e]), 1ull << (i / a.k));
+        if constexpr (kGates)
+            if (staged) {
+                s_e[i] = (int16_t)e;
+                s_w[i] = i == tid ? first_w : a.w[i];
+            }
     }
     __syncthreads();
     // places: the chosen experts before, and their rows (512 threads hold all experts)
@@ -341,18 +362,28 @@ __device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
         l.off[tid] = p;
         for (uint64_t m = mine; m; m &= m - 1, ++p) {
             l.row[p] = (uint8_t)__builtin_ctzll(m);
-            if constexpr (kGates) l.gate[p] = tid < a.E ? 0.0f : a.dense_coef;
+            if constexpr (kGates) l.gate[p] = a.dense_coef;  // (of the shared branch; the others' below)
         }
     }
     __syncthreads();
     if (tid == 0) l.info[0] = all;
     if constexpr (kGates) {
-        if (tid < a.rows)  // a row a thread: its slots in their order
-            for (int t = 0; t < a.k; ++t) {
-                const int e = a.idx[tid * a.k + t];
-                const float w = a.w[tid * a.k + t];
-                if (e >= 0 && e < a.E) l.gate[l.off[e] + __popcll(l.mask[e] & ((1ull << tid) - 1))] += w;
-            }
+        auto expert = [&](int i) {
+            if (staged) return (int)s_e[i];
+            const int e = a.idx[i];
+            return e >= 0 && e < a.E ? e : -1;
+        };
+        for (int i = tid; i < n; i += kFewThreads) {
+            const int r = i / a.k, e = expert(i);
+            if (e < 0) continue;
+            bool first_mention = true;
+            for (int t = r * a.k; t < i; ++t) first_mention &= expert(t) != e;
+            if (!first_mention) continue;
+            float w = staged ? s_w[i] : a.w[i];
+            for (int t = i + 1; t < r * a.k + a.k; ++t)
+                if (expert(t) == e) w += staged ? s_w[t] : a.w[t];
+            l.gate[l.off[e] + __popcll(l.mask[e] & ((1ull << r) - 1))] = w;
+        }
     }
     __syncthreads();
 }
@@ -369,12 +400,17 @@ __device__ __forceinline__ uint32_t weight_lane(int l16, int lq) {
     return W8 ? (uint32_t)(lq * 256 + l16 * 16) : (uint32_t)(l16 * 64 + lq * 16);
 }
 
+// Steps of rows in flight, as many as registers hold (of four: two made a step of the second kernel 2,200 cycles
+// long, an L2 read and a half).
+template <bool W8, int NT, bool kDown>
+constexpr int rows_ahead() { return W8 ? (NT == 1 ? 4 : NT == 2 ? 2 : 1) : NT < 4 || kDown ? 4 : 2; }
+
 // S waves share a unit (16 hidden units of one expert: 16 gate and 16 up rows), each its own
 // share of the steps.
 template <typename T, bool W8, int NT, int S, int P>
 __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     typedef Step<T, W8> St;
-    constexpr int XP = W8 && NT == 4 ? 1 : 2;  // steps of rows in flight (they come from L2)
+    constexpr int XP = rows_ahead<W8, NT, false>();
     constexpr int GP = kFewWaves / S;  // units a block has at a time
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_part[S > 1 ? kFewWaves : 1][2][NT][kWave];
@@ -388,27 +424,9 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     const uint32_t wl = weight_lane<T, W8>(l16, lq);
     const int64_t kstep = (int64_t)a.N1 * kKBlockBytes;
 
-    struct Unit {
-        int e, off, n, n0;         // expert, its first place and rows, the gate rows' place
-        const uint8_t* w;          // ... and address
-        const uint8_t* x[NT];      // the lane's token rows
-        const float *sg, *su;      // 8-bit weights: scales of its gate and up rows
-    };
-    auto unit = [&](int u, Unit& t) {
-        const int li = u / tiles, ht = u - li * tiles;
-        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
-        t.off = __builtin_amdgcn_readfirstlane(l.off[t.e]);
-        t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
-        t.n0 = ht / 2 * 64 + ht % 2 * 16;
-        t.w = static_cast<const uint8_t*>(a.w1) + (int64_t)t.e * a.w1_expert + (int64_t)t.n0 * kKBlockBytes;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-            t.x[j] = static_cast<const uint8_t*>(a.x) + (int64_t)l.row[t.off + min(j * 16 + l16, t.n - 1)] * a.D * sizeof(T);
-        if constexpr (W8) {
-            t.sg = a.s1 + ((int64_t)t.e * 2 * a.hb + ht / 8) * a.kb1;
-            t.su = t.sg + (int64_t)a.hb * a.kb1;
-        }
-    };
+    // rows through a range check: columns past D are at an offset that reads as zeros
+    const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.x), 0, (int)((uint32_t)a.rows * a.D * sizeof(T)),
+                                                      0x00020000);
     struct Weights {
         u32x4_t w[2][2];
         float s[2];
@@ -416,81 +434,88 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     struct Tokens {
         u32x4_t x[NT][St::XL];
     };
-    auto fetch_w = [&](const Unit& t, int st, Weights& d) {
-        const uint8_t* p = t.w + 2 * st * kstep + wl;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) d.w[i][q] = load16u(p + q * kstep + i * 32 * kKBlockBytes);
-        if constexpr (W8) {
-            d.s[0] = t.sg[st];
-            d.s[1] = t.su[st];
-        } else {
-            d.s[0] = d.s[1] = a.w1_down;
-        }
-    };
-    auto fetch_x = [&](const Unit& t, int st, Tokens& d) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            if (j * 16 >= t.n) break;
-#pragma unroll
-            for (int q = 0; q < St::XL; ++q) {
-                const int k = st * St::KS + St::xk(q, lq);
-                d.x[j][q] = u32x4_t{0, 0, 0, 0};
-                if (k < a.D) d.x[j][q] = load16u(t.x[j] + k * sizeof(T));
-            }
-        }
-    };
     for (int u0 = blockIdx.x * GP; u0 < units; u0 += gridDim.x * GP) {
-        const bool mine = u0 + g < units;
-        Unit t;
+        const bool has = u0 + g < units;
+        const int u = min(u0 + g, units - 1), li = u / tiles, ht = u - li * tiles;
+        const int e = __builtin_amdgcn_readfirstlane(l.live[li]), off = __builtin_amdgcn_readfirstlane(l.off[e]);
+        const int n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[e]));
+        const int n0 = ht / 2 * 64 + ht % 2 * 16;  // the gate rows' place; the up rows' is 32 further
+        const float* b = a.b1 + (int64_t)e * a.N1 + n0 + 4 * lq;
+        const float4 bg = *reinterpret_cast<const float4*>(b), bu = *reinterpret_cast<const float4*>(b + 32);
+        const uint8_t* w = static_cast<const uint8_t*>(a.w1) + (int64_t)e * a.w1_expert + (int64_t)n0 * kKBlockBytes;
+        const float* sg = W8 ? a.s1 + ((int64_t)e * 2 * a.hb + ht / 8) * a.kb1 : nullptr;
+        const float* su = W8 ? sg + (int64_t)a.hb * a.kb1 : nullptr;
+        uint32_t xo[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) xo[j] = (uint32_t)l.row[off + min(j * 16 + l16, n - 1)] * (uint32_t)(a.D * sizeof(T));
+        auto fetch_w = [&](int st, Weights& d) {
+            const uint8_t* p = w + 2 * st * kstep;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) d.w[i][q] = load16u(p + q * kstep + i * 32 * kKBlockBytes + wl);
+            d.s[0] = W8 ? sg[st] : a.w1_down;
+            d.s[1] = W8 ? su[st] : a.w1_down;
+        };
+        auto fetch_x = [&](int st, Tokens& d) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if (j * 16 >= n) break;
+#pragma unroll
+                for (int q = 0; q < St::XL; ++q) {
+                    const int k = st * St::KS + St::xk(q, lq);
+                    d.x[j][q] = __builtin_bit_cast(
+                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                     rx, k < a.D ? xo[j] + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
+                }
+            }
+        };
         f32x4_t acc[2][NT];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        unit(min(u0 + g, units - 1), t);
-        if (mine) {
+        if (has) {
             Weights wd[P];
             Tokens xd[XP];
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                if (s0 + p < s1) fetch_w(t, s0 + p, wd[p]);
+                if (s0 + p < s1) fetch_w(s0 + p, wd[p]);
 #pragma unroll
             for (int p = 0; p < XP; ++p)
-                if (s0 + p < s1) fetch_x(t, s0 + p, xd[p]);
+                if (s0 + p < s1) fetch_x(s0 + p, xd[p]);
             for (int st = s0; st < s1; st += P) {
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
                     if (st + p >= s1) break;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        if (j * 16 >= t.n) break;
+                        if (j * 16 >= n) break;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) multiply<T, W8>(acc[i][j], wd[p].w[i], xd[p % XP].x[j], wd[p].s[i]);
+                        for (int c = 0; c < 2; ++c) multiply<T, W8>(acc[c][j], wd[p].w[c], xd[p % XP].x[j], wd[p].s[c]);
                     }
-                    if (st + p + P < s1) fetch_w(t, st + p + P, wd[p]);
-                    if (st + p + XP < s1) fetch_x(t, st + p + XP, xd[p % XP]);
+                    if (st + p + P < s1) fetch_w(st + p + P, wd[p]);
+                    if (st + p + XP < s1) fetch_x(st + p + XP, xd[p % XP]);
                 }
             }
         }
         // lane (l16, lq): token row j * 16 + l16, hidden units 4 lq + (0..3) of the tile
-        const int ht = t.n0 / 64 * 2 + t.n0 % 64 / 16, hc = ht * 16 + 4 * lq;
+        const int hc = ht * 16 + 4 * lq;
         auto finish = [&](int j, const f32x4_t& gv, const f32x4_t& uv) {
             const int m = j * 16 + l16;
-            if (m >= t.n) return;
-            const float* b = a.b1 + (int64_t)t.e * a.N1 + t.n0 + 4 * lq;
+            if (m >= n) return;
+            const float fg[4] = {bg.x, bg.y, bg.z, bg.w}, fu[4] = {bu.x, bu.y, bu.z, bu.w};
             T o[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                o[r] = Elt<T>::from_f32(hc + r < a.H ? swiglu<T>(gv[r] + b[r], uv[r] + b[32 + r]) : 0.0f);
+                o[r] = Elt<T>::from_f32(hc + r < a.H ? swiglu<T>(gv[r] + fg[r], uv[r] + fu[r]) : 0.0f);
             typedef typename std::conditional<sizeof(T) == 2, uint2, uint4>::type Raw4;
             Raw4 raw;
             __builtin_memcpy(&raw, o, sizeof(raw));
-            *reinterpret_cast<Raw4*>(static_cast<T*>(a.h) + (int64_t)(t.off + m) * a.ldh + hc) = raw;
+            *reinterpret_cast<Raw4*>(static_cast<T*>(a.h) + (int64_t)(off + m) * a.ldh + hc) = raw;
         };
         if constexpr (S == 1) {
-            if (mine)
+            if (has)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) finish(j, acc[0][j], acc[1][j]);
         } else {
@@ -499,13 +524,13 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) s_part[wave][i][j][lane] = acc[i][j];
             lds_barrier();
-            if (mine)
+            if (has)
                 for (int j = part; j < NT; j += S) {
                     f32x4_t gv = s_part[g * S][0][j][lane], uv = s_part[g * S][1][j][lane];
 #pragma unroll
-                    for (int w = 1; w < S; ++w) {
-                        gv += s_part[g * S + w][0][j][lane];
-                        uv += s_part[g * S + w][1][j][lane];
+                    for (int i = 1; i < S; ++i) {
+                        gv += s_part[g * S + i][0][j][lane];
+                        uv += s_part[g * S + i][1][j][lane];
                     }
                     finish(j, gv, uv);
                 }
@@ -518,7 +543,7 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
 template <typename T, bool W8, int NT, int P>
 __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     typedef Step<T, W8> St;
-    constexpr int XP = W8 && NT == 4 ? 1 : 2;  // steps of rows in flight
+    constexpr int XP = rows_ahead<W8, NT, true>();
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_y[kFewWaves][16 * NT][4];  // [wave][row][4 columns each]
     __shared__ int s_last;
@@ -530,7 +555,7 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = blockIdx.x / a.parts, part = blockIdx.x % a.parts, n0 = tile * 16;
     const int steps = (a.H + St::KS - 1) / St::KS;  // of an expert
-    const int total = __builtin_amdgcn_readfirstlane(l.info[0]) * steps, shares = a.parts * kFewWaves;
+    const int chosen = __builtin_amdgcn_readfirstlane(l.info[0]), total = chosen * steps, shares = a.parts * kFewWaves;
     const int share = part * kFewWaves + wave;
     const int s0 = (int)((int64_t)total * share / shares), s1 = (int)((int64_t)total * (share + 1) / shares);
     const uint32_t wl = weight_lane<T, W8>(l16, lq);
@@ -541,15 +566,16 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     struct At {
         int li, st, e, off, n;  // a chosen expert and a step of it
     };
-    auto place = [&](At& t, int li, int st) {
-        t.li = li;
-        t.st = st;
-        t.e = __builtin_amdgcn_readfirstlane(l.live[li]);
+    auto place = [&](At& t) {
+        t.e = __builtin_amdgcn_readfirstlane(l.live[t.li]);
         t.off = __builtin_amdgcn_readfirstlane(l.off[t.e]);
         t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
     };
-    auto next = [&](At& t, int s) {  // to step s, the one after t's
-        if (++t.st == steps && s < s1) place(t, t.li + 1, 0);
+    // to the step after (past an expert's last one the next expert's; no branch between loads)
+    auto next = [&](At& t) {
+        const bool wrap = t.st + 1 == steps;
+        t.st = wrap ? 0 : t.st + 1;
+        t.li = min(t.li + (wrap ? 1 : 0), chosen - 1);
     };
     struct Weights {
         u32x4_t w[2];
@@ -558,32 +584,40 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     struct Tokens {
         u32x4_t x[NT][St::XL];
     };
-    auto fetch_w = [&](const At& t, Weights& d) {
+    const auto rh = __builtin_amdgcn_make_buffer_rsrc(a.h, 0, (int)((uint32_t)(a.rows * slots) * (uint32_t)(a.ldh * sizeof(T))),
+                                                      0x00020000);
+    auto fetch_w = [&](At& t, Weights& d) {
+        place(t);
         const uint8_t* p = static_cast<const uint8_t*>(a.w2) + (int64_t)t.e * a.w2_expert + (int64_t)n0 * kKBlockBytes +
-                           2 * t.st * kstep + wl;
+                           2 * t.st * kstep;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) d.w[q] = load16u(p + q * kstep);
-        if constexpr (W8) d.s = a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + t.st];
-        else d.s = a.w2_down;
+        for (int q = 0; q < 2; ++q) d.w[q] = load16u(p + q * kstep + wl);
+        d.s = W8 ? a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + t.st] : a.w2_down;
+        next(t);
     };
-    auto fetch_x = [&](const At& t, Tokens& d) {
+    auto fetch_x = [&](At& t, Tokens& d) {
+        place(t);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             if (j * 16 >= t.n) break;
-            const T* h = static_cast<const T*>(a.h) + (int64_t)(t.off + min(j * 16 + l16, t.n - 1)) * a.ldh;
+            const uint32_t h = (uint32_t)(t.off + min(j * 16 + l16, t.n - 1)) * (uint32_t)(a.ldh * sizeof(T));
 #pragma unroll
             for (int q = 0; q < St::XL; ++q) {
                 const int k = t.st * St::KS + St::xk(q, lq);
-                d.x[j][q] = u32x4_t{0, 0, 0, 0};
-                if (k < live_h) d.x[j][q] = load16u(h + k);
+                d.x[j][q] = __builtin_bit_cast(
+                    u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                 rh, k < live_h ? h + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
             }
         }
+        next(t);
     };
     f32x4_t acc[NT];
     auto clear = [&] {
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     };
+    float4 b2;  // the lane's biases of the expert at hand
+    auto biases = [&](const At& t) { b2 = *reinterpret_cast<const float4*>(a.b2 + (int64_t)t.e * a.N2 + n0 + 4 * lq); };
     // the sums of an expert so far, weighed, to the rows' (each row of it is one lane's)
     auto flush = [&](const At& t, bool bias) {
 #pragma unroll
@@ -592,11 +626,7 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
             if (m < t.n) {
                 const float w = l.gate[t.off + m];
                 f32x4_t v = acc[j];
-                if (bias) {
-                    const float* b = a.b2 + (int64_t)t.e * a.N2 + n0 + 4 * lq;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] += b[r];
-                }
+                if (bias) v += f32x4_t{b2.x, b2.y, b2.z, b2.w};
                 f32x4_t& to = s_y[wave][l.row[t.off + m]][lq];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) to[r] = __builtin_fmaf(v[r], w, to[r]);
@@ -606,31 +636,28 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     };
     clear();
     if (s0 < s1) {
-        At at, aw, ax;  // of the products, of the weights' and the rows' loads
-        place(at, s0 / steps, s0 % steps);
-        aw = ax = at;
+        At at = {s0 / steps, s0 % steps, 0, 0, 0}, aw = at, ax = at;  // of the products, of the weights' and the rows' loads
+        place(at);
         bool whole = at.st == 0;  // the expert's first step is this wave's
+        biases(at);
         Weights wd[P];
         Tokens xd[XP];
 #pragma unroll
         for (int p = 0; p < P; ++p)
-            if (s0 + p < s1) {
-                fetch_w(aw, wd[p]);
-                next(aw, s0 + p + 1);
-            }
+            if (s0 + p < s1) fetch_w(aw, wd[p]);
 #pragma unroll
         for (int p = 0; p < XP; ++p)
-            if (s0 + p < s1) {
-                fetch_x(ax, xd[p]);
-                next(ax, s0 + p + 1);
-            }
+            if (s0 + p < s1) fetch_x(ax, xd[p]);
         for (int s = s0; s < s1; s += P) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 if (s + p >= s1) break;
                 if (at.st == steps) {
                     flush(at, whole);
-                    place(at, at.li + 1, 0);
+                    ++at.li;
+                    at.st = 0;
+                    place(at);
+                    biases(at);
                     whole = true;
                 }
 #pragma unroll
@@ -639,14 +666,8 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
                     multiply<T, W8>(acc[j], wd[p].w, xd[p % XP].x[j], wd[p].s);
                 }
                 ++at.st;
-                if (s + p + P < s1) {
-                    fetch_w(aw, wd[p]);
-                    next(aw, s + p + P + 1);
-                }
-                if (s + p + XP < s1) {
-                    fetch_x(ax, xd[p % XP]);
-                    next(ax, s + p + XP + 1);
-                }
+                if (s + p + P < s1) fetch_w(aw, wd[p]);
+                if (s + p + XP < s1) fetch_x(ax, xd[p % XP]);
             }
         }
         flush(at, whole);
@@ -664,9 +685,9 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     if (a.parts > 1) {
         // The last block to arrive adds the shares, in their order.  Blocks of a tile run on
         // different XCDs, whose L2 caches are not coherent: the shares are written and read past
-        // them (agent-scope cache policy), each block's increment is a release, and the
-        // one that completes the count acquires.  (A fence of every wave took 50 us of a call: it
-        // writes back and empties the L2.)
+        // them (agent-scope cache policy), and written, as the wait says, before the block is
+        // counted.  So nothing has to be written back or thrown away: a release and an acquire
+        // around the count took 3 us, fences of every wave 50.
         constexpr int kSc1 = 16;
         const auto rs = __builtin_amdgcn_make_buffer_rsrc(a.partial + (int64_t)tile * kFewParts * kFewRows * 16, 0,
                                                           kFewParts * kFewRows * 64, 0x00020000);
@@ -675,10 +696,8 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
                                                    kSc1);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (tid == 0) {
-            s_last = __hip_atomic_fetch_add(&a.arrived[tile], 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
-            if (s_last) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-        }
+        if (tid == 0)
+            s_last = __hip_atomic_fetch_add(&a.arrived[tile], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
         __syncthreads();
         if (!s_last) return;
         if (row < a.rows) {
@@ -727,8 +746,20 @@ hipError_t launch_nt(FewArgs a, hipStream_t s) {
     const int tiles = (a.H + 15) / 16, live = std::min(a.E, a.rows * a.k) + a.Ecols - a.E;
     const int64_t units = (int64_t)tiles * live;
     const size_t lds1 = Lists::bytes(a.Ecols, places, false), lds2 = Lists::bytes(a.Ecols, places, true);
-    const int S = units >= 256 * 6 ? 1 : units >= 256 * 3 ? 2 : units * 4 >= 256 * 6 ? 4 : 8;
-    const int64_t grid = std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 512);
+    // The share of a unit's steps that a wave takes (1 / S) by the steps that the longest wave then walks, one block of
+    // eight waves a CU, a round's first loads as long as six steps; of equal ones the fewest waves a unit, which have the
+    // fewest sums to exchange.
+    const int steps = (a.D + St::KS - 1) / St::KS;
+    int S = 1;
+    int64_t least = INT64_MAX;
+    for (const int c : {1, 2, 4, 8}) {
+        const int64_t rounds = (units * c + 256 * kFewWaves - 1) / (256 * kFewWaves), walk = rounds * (6 + (steps + c - 1) / c);
+        if (walk < least) {
+            least = walk;
+            S = c;
+        }
+    }
+    const int64_t grid = std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 256);
     constexpr size_t fixed1 = kFewWaves * 2 * NT * kWave * 16, fixed2 = kFewWaves * NT * kWave * 16 + 16;
     hipError_t e = S == 1   ? launch(few_up_kernel<T, W8, NT, 1, P>, grid, fixed1, lds1, a, s)
                    : S == 2 ? launch(few_up_kernel<T, W8, NT, 2, P>, grid, fixed1, lds1, a, s)
@@ -764,7 +795,8 @@ hipError_t launch_few_t(const FewArgs& a, hipStream_t s) {
 
 hipError_t launch_few(DType dt, const FewArgs& a, hipStream_t s) {
     if (a.rows < 1 || a.rows > kFewRows || a.D < 8 || a.D % 8 != 0 || a.E < 1 || a.E > kMaxExperts || a.k < 1 ||
-        a.k > a.Ecols || (a.D + 15) / 16 > a.tile_cap)
+        a.k > a.Ecols || (int64_t)a.rows * a.D > (1 << 28) || (int64_t)a.rows * (a.k + 1) * a.ldh > (1 << 28) ||
+        (a.D + 15) / 16 > a.tile_cap)
         return hipErrorInvalidValue;
     const bool w8 = a.s1 != nullptr;
     switch (dt) {

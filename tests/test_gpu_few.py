@@ -97,7 +97,7 @@ def test_the_routers_choice(rows, D, E, k, H, s, dtype, fp8):
     rel = np.expm1(2 * dl) + 4 * (spread + 4) * U
     assert np.all(np.abs(w - w2)[sure] <= (rel[:, None] * np.abs(w2))[sure])
     both = sure & np.isfinite(gap)
-    assert np.all(np.abs(gap - g2)[both] <= (2 * dl + U * np.abs(g2))[both]) and np.array_equal(np.isinf(gap), np.isinf(g2))
+    assert np.all(np.abs(gap[both] - g2[both]) <= 2 * dl[both] + U * np.abs(g2[both])) and np.array_equal(np.isinf(gap), np.isinf(g2))
     if sure.all():
         assert np.array_equal(counts, c2)
 
