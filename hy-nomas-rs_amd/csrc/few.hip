@@ -90,6 +90,10 @@ __device__ __forceinline__ void multiply(f32x4_t& acc, const u32x4_t (&w)[2], co
 
 __device__ __forceinline__ u32x4_t load16u(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 
+// Who has chosen, or will (FewArgs::choice): a kernel before or the caller, or the first kernel, from
+// logits or from the rows themselves.
+enum { kChoiceMade = 0, kChoiceOfLogits = 1, kChoiceOfRows = 2 };
+
 // ---- the router's choice ---------------------------------------------------------
 // Softmax over the logits, top-k with ties to the lowest index, weights p / (sum of the chosen p + 1e-9)
 // in ascending order of experts: the layer's router (router.hip) for few rows.  16-bit products are exact
@@ -160,12 +164,6 @@ __device__ __forceinline__ float dpp_addf(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
 }
 // Over a wave, in all lanes.
-__device__ __forceinline__ float wave_max(float v) {
-    const uint32_t b = __float_as_uint(v), m = max16(b ^ ((uint32_t)((int)b >> 31) | 0x80000000u));  // (in their order)
-    auto lane = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)m, i); };
-    const uint32_t t = max(max(lane(0), lane(16)), max(lane(32), lane(48)));
-    return __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
-}
 __device__ __forceinline__ float wave_sum(float v) {
     v = dpp_addf<0xb1>(v);
     v = dpp_addf<0x4e>(v);
@@ -175,62 +173,132 @@ __device__ __forceinline__ float wave_sum(float v) {
     return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-// One wave chooses for one row: its logits `l` (LDS, E of them), PL a lane.  An expert is chosen if
-// fewer than k others are before it: a count over all, without rounds.
+__device__ __forceinline__ uint32_t wave_maxu(uint32_t v) {
+    const uint32_t m = max16(v);
+    auto lane = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)m, i); };
+    return max(max(lane(0), lane(16)), max(lane(32), lane(48)));
+}
+// f32 bits as an unsigned integer of the same order, NaN above all.
+__device__ __forceinline__ uint32_t order_key32(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v != v ? 0xffffffffu : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+}
+
+// Which of the lane's experts (bit j: lane + 64 j) are among the k of the largest logits, ties to the lowest
+// index.  By the logits as f32, whose order is that of f64 but for equal ones, and by f64 where more than
+// one choice is possible so.  Up to 64 experts: each lane counts those above its own; more: the k-th
+// value by bisection over its bits.  s_key: 64 words of the wave's.  (64-bit compares of all
+// with all took 4.5 us for one row of 64 experts.)
+template <int PL>
+__device__ __forceinline__ uint32_t choose_largest(const double* l, const double (&v)[PL], int E, int k, uint32_t* s_key) {
+    const int lane = threadIdx.x & 63;
+    uint32_t key[PL], mine = 0;
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) key[j] = lane + j * 64 < E ? order_key32((float)v[j]) : 0u;  // (0: below all)
+    if constexpr (PL == 1) {
+        s_key[lane] = key[0];  // (one wave: its LDS accesses are in order)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        int above = 0;
+        for (int e = 0; e < E; e += 16) {
+            u32x4_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const u32x4_t*>(s_key + e + i * 4);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) above += o[i / 4][i % 4] > key[0] ? 1 : 0;
+        }
+        mine = lane < E && above < k ? 1u : 0u;
+        count = __popcll(__ballot(mine));
+    } else {
+        uint32_t kth = 0;  // the largest value that at least k are not below
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < PL; ++j) n += __popcll(__ballot(key[j] >= (kth | bit)));
+            if (n >= k) kth |= bit;
+        }
+#pragma unroll
+        for (int j = 0; j < PL; ++j) {
+            const bool in = key[j] >= kth && lane + j * 64 < E;
+            mine |= in ? 1u << j : 0u;
+            count += __popcll(__ballot(in));
+        }
+    }
+    if (count == k) return mine;
+    mine = 0;
+    int64_t own[PL];
+    int before[PL];
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+        own[j] = order_key(v[j]);
+        before[j] = 0;
+    }
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+        const int64_t o = order_key(l[e]);
+#pragma unroll
+        for (int j = 0; j < PL; ++j) before[j] += o > own[j] || (o == own[j] && e < lane + j * 64);
+    }
+#pragma unroll
+    for (int j = 0; j < PL; ++j) mine |= lane + j * 64 < E && before[j] < k ? 1u << j : 0u;
+    return mine;
+}
+
+// One wave chooses for one row: its logits `l` (LDS, E of them), PL a lane.
 template <int PL, typename F>
-__device__ __forceinline__ void choose(const FewArgs& a, const double* l, int row, bool store, F chosen) {
+__device__ __forceinline__ void choose(const FewArgs& a, const double* l, int row, bool store, uint32_t* s_key, F chosen) {
     const int lane = threadIdx.x & 63, E = a.E, k = a.top_k;
     double v[PL];
-    int64_t key[PL];
-    int before[PL];
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
         const int e = lane + j * 64;
         v[j] = e < E ? l[e] : -INFINITY;
-        key[j] = order_key(v[j]);
-        before[j] = e < E ? 0 : E;
         m = fmaxf(m, (float)v[j]);
     }
-#pragma unroll 8
-    for (int e = 0; e < E; ++e) {
-        const int64_t o = order_key(l[e]);
+    const uint32_t mine = choose_largest<PL>(l, v, E, k, s_key);
+    int at = 0, t[PL];
 #pragma unroll
-        for (int j = 0; j < PL; ++j) before[j] += o > key[j] || (o == key[j] && e < lane + j * 64);
+    for (int j = 0; j < PL; ++j) {
+        const uint64_t c = __ballot(mine >> j & 1);
+        t[j] = at + __popcll(c & ((1ull << lane) - 1));  // (places in ascending order of experts)
+        at += __popcll(c);
+        if (mine >> j & 1) chosen(lane + j * 64);
     }
-    m = wave_max(m);  // (any number near the largest does)
+    if (!store) return;
+    {  // (any number near the largest does)
+        const uint32_t b = wave_maxu(order_key32(m));
+        m = __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+    }
     float p[PL], sum = 0.0f, sel = 0.0f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
         p[j] = lane + j * 64 < E ? expf((float)(v[j] - (double)m)) : 0.0f;
         sum += p[j];
-        sel += before[j] < k ? p[j] : 0.0f;
+        sel += mine >> j & 1 ? p[j] : 0.0f;
     }
     sum = wave_sum(sum);
     sel = wave_sum(sel);
     // p / sum / (sel / sum + 1e-9)
     const float norm = 1.0f / (sel + 1e-9f * sum);
-    int at = 0;
-    double kth = 0.0, next = 0.0;
+    // the last one chosen and the first one not, for the gap between them
+    double kth = INFINITY, next = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-        const uint64_t c = __ballot(before[j] < k);
-        if (before[j] < k) {
-            const int e = lane + j * 64, t = at + __popcll(c & ((1ull << lane) - 1));
-            chosen(t, e);
-            if (store) {
-                a.out_idx[row * a.out_slots + t] = e;
-                a.out_w[row * a.out_slots + t] = p[j] * norm;
-            }
-        }
-        at += __popcll(c);
-        if (store) {  // the logits of the last one chosen and the first one not
-            const uint64_t last = __ballot(before[j] == k - 1), first = __ballot(before[j] == k && lane + j * 64 < E);
-            if (last) kth = __shfl(v[j], __builtin_ctzll(last));
-            if (first) next = __shfl(v[j], __builtin_ctzll(first));
+        if (mine >> j & 1) {
+            a.out_idx[row * a.out_slots + t[j]] = lane + j * 64;
+            a.out_w[row * a.out_slots + t[j]] = p[j] * norm;
+            kth = fmin(kth, v[j]);
+        } else {
+            next = fmax(next, v[j]);  // (past E: -infinity)
         }
     }
-    if (store && lane == 0) {
+#pragma unroll 1
+    for (int o = 32; o >= 1; o >>= 1) {
+        kth = fmin(kth, __shfl_xor(kth, o));
+        next = fmax(next, __shfl_xor(next, o));
+    }
+    if (lane == 0) {
         a.out_gap[row] = k == E ? INFINITY : (float)(kth - next);
         if (a.out_slots > k) {
             a.out_idx[row * a.out_slots + k] = E;
@@ -239,9 +307,9 @@ __device__ __forceinline__ void choose(const FewArgs& a, const double* l, int ro
     }
 }
 template <typename F>
-__device__ __forceinline__ void choose_any(const FewArgs& a, const double* l, int row, bool store, F chosen) {
-    if (a.E <= 64) choose<1>(a, l, row, store, chosen);
-    else choose<kMaxExperts / 64>(a, l, row, store, chosen);
+__device__ __forceinline__ void choose_any(const FewArgs& a, const double* l, int row, bool store, uint32_t* s_key, F chosen) {
+    if (a.E <= 64) choose<1>(a, l, row, store, s_key, chosen);
+    else choose<kMaxExperts / 64>(a, l, row, store, s_key, chosen);
 }
 
 // A kernel of its own: a block for 16 rows and 16 experts; the last one of 16 rows chooses.
@@ -250,10 +318,15 @@ __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
     extern __shared__ __align__(16) uint8_t s_dyn[];  // 16 rows' logits
     __shared__ double s_part[kFewWaves * 256];
     __shared__ int s_count[kMaxExperts + 1], s_last;
+    __shared__ __align__(16) uint32_t s_key[kFewWaves * 64];
     double* s_logit = reinterpret_cast<double*>(s_dyn);
     const int tid = threadIdx.x, wave = tid >> 6, eg = blockIdx.x, rg = blockIdx.y, groups = gridDim.x;
     const double v = logit_tile<T>(a, rg, eg, s_part);
     const int r = tid / 16, e = eg * 16 + tid % 16;
+    if (a.choice == kChoiceOfLogits) {  // the first kernel chooses
+        if (tid < 256 && e < a.E) a.logits[(rg * 16 + r) * kMaxExperts + e] = v;
+        return;
+    }
     if (groups > 1) {
         // as in few_down_kernel: past the L2 caches, written before the block is counted
         constexpr int kSc1 = 16;
@@ -281,7 +354,7 @@ __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
     for (int i = tid; i < a.Ecols; i += kFewThreads) s_count[i] = i < a.E ? 0 : min(16, a.rows - rg * 16);
     __syncthreads();
     for (int i = wave; i < min(16, a.rows - rg * 16); i += kFewWaves)
-        choose_any(a, s_logit + i * a.E, rg * 16 + i, true, [&](int, int ex) { atomicAdd(&s_count[ex], 1); });
+        choose_any(a, s_logit + i * a.E, rg * 16 + i, true, s_key + wave * 64, [&](int ex) { atomicAdd(&s_count[ex], 1); });
     __syncthreads();
     for (int i = tid; i < a.Ecols; i += kFewThreads) a.out_count[rg * a.Ecols + i] = s_count[i];
 }
@@ -297,6 +370,7 @@ struct Lists {
     static __host__ __device__ size_t bytes(int ecols, int places, bool gates) {
         return (size_t)ecols * 16 + 64 + (size_t)(places + 15) / 16 * 16 + (gates ? (size_t)places * 4 : 0);
     }
+    // (a multiple of 8 bytes without gates)
     __device__ Lists(uint8_t* p, int ecols, int places) {
         mask = reinterpret_cast<uint64_t*>(p);
         live = reinterpret_cast<int*>(p + (size_t)ecols * 8);
@@ -311,11 +385,13 @@ struct Lists {
 constexpr int kStaged = 2048;
 
 // Experts named twice by a row have the sum of their weights, in the slots' order.
+// `logits`: where the routing is still to be chosen (by the first kernel; its block 0 keeps it for the second).
 template <bool kGates>
-__device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
+__device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l, const double* logits = nullptr) {
     __shared__ int16_t s_e[kGates ? kStaged : 1];
     __shared__ float s_w[kGates ? kStaged : 1];
-    const int tid = threadIdx.x, n = a.rows * a.k, lane = tid & 63, wave = tid >> 6;
+    __shared__ __align__(16) uint32_t s_key[kGates ? 4 : kFewWaves * 64];
+    const int tid = threadIdx.x, n = logits ? 0 : a.rows * a.k, lane = tid & 63, wave = tid >> 6;
     const bool staged = n <= kStaged;
     // (on their way while the masks are cleared)
     const int first_e = tid < n ? a.idx[tid] : -1;
@@ -331,6 +407,13 @@ __device__ __forceinline__ void make_lists(const FewArgs& a, const Lists& l) {
                 s_e[i] = (int16_t)e;
                 s_w[i] = i == tid ? first_w : a.w[i];
             }
+    }
+    if constexpr (!kGates) {
+        if (logits)
+            for (int r = wave; r < a.rows; r += kFewWaves)
+                choose_any(a, logits + r * a.E, r, blockIdx.x == 0, s_key + wave * 64, [&](int e) {
+                    atomicOr(reinterpret_cast<unsigned long long*>(&l.mask[e]), 1ull << r);
+                });
     }
     __syncthreads();
     // places: the chosen experts before, and their rows (512 threads hold all experts)
@@ -414,8 +497,23 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     constexpr int GP = kFewWaves / S;  // units a block has at a time
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_part[S > 1 ? kFewWaves : 1][2][NT][kWave];
-    const Lists l(s_dyn, a.Ecols, a.rows * (a.k + a.Ecols - a.E));
-    make_lists<false>(a, l);
+    const int places = a.rows * (a.k + a.Ecols - a.E);
+    const Lists l(s_dyn, a.Ecols, places);
+    if (NT == 1 && a.choice != kChoiceMade) {
+        double* s_logit = reinterpret_cast<double*>(s_dyn + Lists::bytes(a.Ecols, places, false));
+        if (a.choice == kChoiceOfLogits) {
+            for (int i = threadIdx.x; i < a.rows * a.E; i += kFewThreads)
+                s_logit[i] = a.logits[i / a.E * kMaxExperts + i % a.E];
+        } else {
+            const double v = logit_tile<T>(a, 0, 0, s_logit + a.rows * a.E);
+            const int r = threadIdx.x / 16, e = threadIdx.x % 16;
+            if (r < a.rows && e < a.E) s_logit[r * a.E + e] = v;
+        }
+        make_lists<false>(a, l, s_logit);  // (a barrier first)
+        if (blockIdx.x == 0 && (int)threadIdx.x < a.Ecols) a.out_count[threadIdx.x] = __popcll(l.mask[threadIdx.x]);
+    } else {
+        make_lists<false>(a, l);
+    }
 
     const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = wave / S, part = wave % S;
@@ -745,7 +843,9 @@ hipError_t launch_nt(FewArgs a, hipStream_t s) {
     const int slots = a.k + a.Ecols - a.E, places = a.rows * slots;
     const int tiles = (a.H + 15) / 16, live = std::min(a.E, a.rows * a.k) + a.Ecols - a.E;
     const int64_t units = (int64_t)tiles * live;
-    const size_t lds1 = Lists::bytes(a.Ecols, places, false), lds2 = Lists::bytes(a.Ecols, places, true);
+    const size_t lds1 = Lists::bytes(a.Ecols, places, false) + (a.choice != kChoiceMade ? (size_t)a.rows * a.E * 8 : 0) +
+                        (a.choice == kChoiceOfRows ? (size_t)kFewWaves * 256 * 8 : 0),
+                 lds2 = Lists::bytes(a.Ecols, places, true);
     // The share of a unit's steps that a wave takes (1 / S) by the steps that the longest wave then walks, one block of
     // eight waves a CU, a round's first loads as long as six steps; of equal ones the fewest waves a unit, which have the
     // fewest sums to exchange.
@@ -760,7 +860,7 @@ hipError_t launch_nt(FewArgs a, hipStream_t s) {
         }
     }
     const int64_t grid = std::min<int64_t>((units * S + kFewWaves - 1) / kFewWaves, 256);
-    constexpr size_t fixed1 = kFewWaves * 2 * NT * kWave * 16, fixed2 = kFewWaves * NT * kWave * 16 + 16;
+    constexpr size_t fixed1 = kFewWaves * (2 * NT * kWave * 16 + 256) + 64, fixed2 = kFewWaves * NT * kWave * 16 + kStaged * 6 + 64;
     hipError_t e = S == 1   ? launch(few_up_kernel<T, W8, NT, 1, P>, grid, fixed1, lds1, a, s)
                    : S == 2 ? launch(few_up_kernel<T, W8, NT, 2, P>, grid, fixed1, lds1, a, s)
                    : S == 4 ? launch(few_up_kernel<T, W8, NT, 4, P>, grid, fixed1, lds1, a, s)
@@ -781,8 +881,16 @@ hipError_t launch_route(const FewArgs& a, hipStream_t s) {
 }
 
 template <typename T, bool W8>
-hipError_t launch_few_t(const FewArgs& a, hipStream_t s) {
-    if (a.wr) {
+hipError_t launch_few_t(FewArgs a, hipStream_t s) {
+    // Who chooses.  Up to 16 rows: every block of the first kernel, from logits that it makes itself
+    // where the router's weights and the rows are a few KB, else from those of a kernel that has a
+    // block for 16 experts.  More rows: that kernel's last blocks.  (Two rows of 64, 4 experts: 21
+    // us a call with a kernel for the router, 15 without; one row of 2,048, 64 experts: the router's
+    // kernel 10 us with the choice, 4 without.)
+    a.choice = kChoiceMade;
+    if (a.wr && a.rows <= 16)
+        a.choice = a.E <= 16 && (int64_t)(a.rows + a.E) * a.D * (int)sizeof(T) <= 64 * 1024 ? kChoiceOfRows : kChoiceOfLogits;
+    if (a.wr && a.choice != kChoiceOfRows) {
         const hipError_t e = launch_route<T>(a, s);
         if (e != hipSuccess) return e;
     }

@@ -348,6 +348,7 @@ struct FewArgs {
     int32_t *out_idx, *out_count;  // out_count: Ecols for each 16 rows
     float *out_w, *out_gap;
     int out_slots;
+    int choice;          // (set by the launch)
 };
 hipError_t launch_few(DType dt, const FewArgs& a, hipStream_t s);
 hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s);

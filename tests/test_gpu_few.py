@@ -121,6 +121,34 @@ def test_the_callers_routing(rows, D, E, k, H, s, dtype, fp8):
         layer.routing(rows)
 
 
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("E,k", [(4, 1), (16, 3), (64, 8), (64, 64), (200, 6), (256, 1)])
+def test_ties_and_near_ties(rows, E, k):
+    """Equal logits: the lowest index; logits that differ by 2^-40 only, or by f32's last bit: the larger one."""
+    D, H = 64, 16
+    t, _ = small_case(rows, D, E, k, H, 11)
+    r = np.random.default_rng(E + k)
+    fine = r.permutation(E)
+    fine[: E // 2] = fine[0]  # half of them equal
+    wr = np.zeros((E, D), np.float32)
+    wr[:, 0], wr[:, 1], wr[:, 2] = 1.0, fine * 2.0 ** -20, r.integers(0, 2, E) * 2.0 ** -23
+    t["blocks.0.moe.router.weight"] = wr
+    layer = layer_from_tensors(t, "f32", D, H, E, k, 0.0)
+    x = np.zeros((rows, D), np.float32)
+    x[:, 0] = 1.0
+    x[:, 1] = 2.0 ** -20
+    x[1::2, 2] = 1.0
+    layer.forward_few(torch.from_numpy(x).cuda())
+    logits = x.astype(np.float64) @ wr.astype(np.float64).T
+    idx, w, counts, gap = layer.routing(rows)
+    for i in range(rows):
+        order = sorted(range(E), key=lambda e: (-logits[i, e], e))
+        assert list(idx[i]) == sorted(order[:k])
+        p = np.exp(logits[i] - logits[i].max())[idx[i]]
+        assert np.allclose(w[i], p / (p.sum() + 1e-9 * p.sum()), rtol=1e-6, atol=0)
+        assert gap[i] == (np.inf if k == E else np.float32(logits[i, order[k - 1]] - logits[i, order[k]]))
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 def test_rows_do_not_touch_each_other(fp8):
     layer, x, _, _ = case(20, 264, 6, 2, 200, "bf16", 7, fp8=fp8)
