@@ -44,31 +44,28 @@ template <typename T, int U>
 __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a) {
     const int l = threadIdx.x % kLanes;
     const uint32_t kb = (uint32_t)((a.ld_q + kFp8Block - 1) / kFp8Block), total = (uint32_t)a.rows * kb;
-    const uint32_t step = gridDim.x * kGroups;
     const T* x = static_cast<const T*>(a.x);
-    for (uint32_t at = blockIdx.x * kGroups + threadIdx.x / kLanes; at < total; at += U * step) {
-        In8<T> in[U];
-        uint32_t row[U], b[U];
+    // (a group's blocks are next to each other for a wave's four groups, U steps apart)
+    const uint32_t first = blockIdx.x * (uint32_t)(U * kGroups) + threadIdx.x / kLanes;
+    In8<T> in[U];
+    uint32_t row[U];
+    int col[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            // (past the end the last block again, whose lanes store the same bytes)
-            const uint32_t u = total - at > i * step ? at + i * step : total - 1;
-            row[i] = u / kb;
-            b[i] = u - row[i] * kb;
-            const int col = (int)b[i] * kFp8Block + l * 8;
-            in[i] = In8<T>{};
-            if (col < a.cols) in[i] = fetch(x + (int64_t)row[i] * a.cols + col);
-        }
+    for (int i = 0; i < U; ++i) {
+        const uint32_t u = min(first + i * kGroups, total - 1);
+        row[i] = u / kb;
+        col[i] = (int)(u - row[i] * kb) * kFp8Block + l * 8;
+        in[i] = In8<T>{};
+        if (col[i] < a.cols) in[i] = fetch(x + (int64_t)row[i] * a.cols + col[i]);
+    }
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-            float v[8];
-            widen<T>(in[i], v);
-            const float s = fp8_scale(max16(largest(v)));
-            const int col = (int)b[i] * kFp8Block + l * 8;
-            if (col < a.ld_q)
-                *reinterpret_cast<uint2*>(a.q + (int64_t)row[i] * a.ld_q + col) = pack8(v, Fp8Quot(s));
-            if (l == 0) a.scale[(int64_t)row[i] * kb + b[i]] = s;
-        }
+    for (int i = 0; i < U; ++i) {
+        if (first + i * kGroups >= total) break;
+        float v[8];
+        widen<T>(in[i], v);
+        const float s = fp8_scale(max16(largest(v)));
+        if (col[i] < a.ld_q) *reinterpret_cast<uint2*>(a.q + (int64_t)row[i] * a.ld_q + col[i]) = pack8(v, Fp8Quot(s));
+        if (l == 0) a.scale[(int64_t)row[i] * kb + col[i] / kFp8Block] = s;
     }
 }
 
@@ -131,7 +128,7 @@ hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s) {
         a.rows * kb >= ((int64_t)1 << 31))
         return hipErrorInvalidValue;
     constexpr int U = 4;
-    const int64_t blocks = std::min<int64_t>((a.rows * kb + kGroups - 1) / kGroups, 4096);
+    const int64_t blocks = (a.rows * kb + U * kGroups - 1) / (U * kGroups);
     const dim3 grid((unsigned)blocks), block(kQuantThreads);
     switch (dt) {
         case DType::F32: launch_kernel(quant_rows_kernel<float, U>, grid, block, 0, s, a); break;
