@@ -96,7 +96,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
     constexpr int NW = WN * WM, BN = 16 * NI * WN, BM = 16 * NJ * WM;
     constexpr int kStage = (BN + BM) * kFp8Block;
     __shared__ __align__(1024) uint8_t s_ring[2][kStage];
-    __shared__ float s_sa[2][BM];
+    __shared__ float s_sa[2][BM], s_sb[2][kWave];
     constexpr int QN = BN / 8 / NW, QM = BM / 8 / NW;  // loads of 8 rows a wave
 
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
@@ -130,6 +130,12 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
     // the scales of the rows: one per thread of the first BM / 64 waves (past the end the last row's)
     const uint32_t vs = (uint32_t)min(tid % BM, rows_m - 1) * (uint32_t)kb * 4;
     const float* as = a.as + m0 * kb;
+    // ... and of the tile's weights: blocks of 128 rows, with kGlu the gate rows' and the up rows'.  (A
+    // load of them to registers waited for all the direct loads issued before it.)
+    static_assert(kFp8Block % (16 * NI) == 0 && BN / kFp8Block <= 2, "one weight scale a wave");
+    const uint32_t vsb = MODE == kGlu ? (uint32_t)(tn + (lane & 1) * tiles_n) * (uint32_t)kb * 4
+                                      : (uint32_t)min(n0 / kFp8Block + (lane & 1), (a.N - 1) / kFp8Block) * (uint32_t)kb * 4;
+    const uint32_t sbs = lds_addr(&s_sb[0][0]);
     const uint32_t ring = lds_addr(&s_ring[0][0]), sas = lds_addr(&s_sa[0][0]);
 
     auto issue = [&](int kt) {
@@ -142,6 +148,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
         for (int q = 0; q < QM; ++q)
             lds_dma16_buf_s(ra, out ? 0xfffffff0u : vm[q], k0, at + (BN / 8 + wave * QM + q) * 1024);
         if (wave < BM / kWave) lds_dma4(as + kt, vs, sas + (kt & 1) * BM * 4 + wave * 256);
+        if (wave == NW - 1) lds_dma4(a.bs + kt, vsb, sbs + (kt & 1) * kWave * 4);
     };
 
     f32x4_t acc[NI][NJ];
@@ -150,12 +157,6 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // (a wave's weight rows lie in one block of 128)
-    static_assert(kFp8Block % (16 * NI) == 0, "one weight scale a wave");
-    // (of the gate rows with kGlu, whose up rows' scales are `up` further on)
-    const float* __restrict__ bs =
-        a.bs + (int64_t)(MODE == kGlu ? tn : min((n0 + wn * 16 * NI) / kFp8Block, (a.N - 1) / kFp8Block)) * kb;
-    const int64_t up = MODE == kGlu ? (int64_t)tiles_n * kb : 0;
     const int sw = l16 & 7;
     const int c0 = (2 * lq) ^ sw, c1 = (2 * lq + 1) ^ sw;
 
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             return join(*reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c0 * 16),
                         *reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c1 * 16));
         };
-        const float sb = bs[kt], sb2 = bs[up + kt];
+        const float sb = s_sb[kt & 1][MODE == kGlu ? 0 : wn * 16 * NI / kFp8Block], sb2 = s_sb[kt & 1][1];
         FragOf<T> x[NJ];
         float s[NJ], s2[NJ];
 #pragma unroll
