@@ -121,12 +121,9 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
                                                       (int)((uint32_t)rows_n * (uint32_t)K), 0x00020000);
     const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.a) + m0 * K, 0,
                                                       (int)((uint32_t)rows_m * (uint32_t)K), 0x00020000);
+    // (the first of the wave's loads of 8 rows; the others' offsets are made where they go out: registers are short)
     const int chunk = (lane & 7) ^ (lane >> 3);
-    uint32_t vn[QN], vm[QM];
-#pragma unroll
-    for (int q = 0; q < QN; ++q) vn[q] = (uint32_t)((wave * QN + q) * 8 + (lane >> 3)) * (uint32_t)K + chunk * 16;
-#pragma unroll
-    for (int q = 0; q < QM; ++q) vm[q] = (uint32_t)((wave * QM + q) * 8 + (lane >> 3)) * (uint32_t)K + chunk * 16;
+    const uint32_t v0 = (uint32_t)(lane >> 3) * (uint32_t)K + chunk * 16;
     // the scales of the rows: one per thread of the first BM / 64 waves (past the end the last row's)
     const uint32_t vs = (uint32_t)min(tid % BM, rows_m - 1) * (uint32_t)kb * 4;
     const float* as = a.as + m0 * kb;
@@ -136,20 +133,32 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
     const uint32_t vsb = MODE == kGlu ? (uint32_t)(tn + (lane & 1) * tiles_n) * (uint32_t)kb * 4
                                       : (uint32_t)min(n0 / kFp8Block + (lane & 1), (a.N - 1) / kFp8Block) * (uint32_t)kb * 4;
     const uint32_t sbs = lds_addr(&s_sb[0][0]);
+    // the first waves load the rows' scales, the others the weights'
+    static_assert(NW > BM / kWave, "a wave for the weights' scales");
+    const bool rows_scales = wave < BM / kWave;
+    const float* scales = rows_scales ? as : a.bs;
+    const uint32_t scales_stage = rows_scales ? BM * 4 : kWave * 4;
     const uint32_t ring = lds_addr(&s_ring[0][0]), sas = lds_addr(&s_sa[0][0]);
 
-    auto issue = [&](int kt) {
+    // load q of a wave for block kt: of the QN + QM tile loads, then the scales
+    auto issue = [&](int kt, int q) {
         const uint32_t at = ring + (kt & 1) * kStage, k0 = (uint32_t)kt * kFp8Block;
-        const bool out = (int)k0 + chunk * 16 >= K;  // (only in the last block)
-#pragma unroll
-        for (int q = 0; q < QN; ++q)
-            lds_dma16_buf_s(rb, out ? 0xfffffff0u : vn[q], k0, at + (wave * QN + q) * 1024);
-#pragma unroll
-        for (int q = 0; q < QM; ++q)
-            lds_dma16_buf_s(ra, out ? 0xfffffff0u : vm[q], k0, at + (BN / 8 + wave * QM + q) * 1024);
-        if (wave < BM / kWave) lds_dma4(as + kt, vs, sas + (kt & 1) * BM * 4 + wave * 256);
-        if (wave == NW - 1) lds_dma4(a.bs + kt, vsb, sbs + (kt & 1) * kWave * 4);
+        const bool out = (int)k0 + chunk * 16 >= K;  // (only in the last block, or past it)
+        uint32_t v = v0;
+        asm volatile("" : "+v"(v));  // (else all loads' offsets are kept, and registers spilled)
+        if (q < QN) {
+            lds_dma16_buf_s(rb, out ? 0xfffffff0u : v + (uint32_t)(wave * QN + q) * 8 * (uint32_t)K, k0,
+                            at + (wave * QN + q) * 1024);
+        } else if (q < QN + QM) {
+            const int m = q - QN;
+            lds_dma16_buf_s(ra, out ? 0xfffffff0u : v + (uint32_t)(wave * QM + m) * 8 * (uint32_t)K, k0,
+                            at + (BN / 8 + wave * QM + m) * 1024);
+        } else {
+            // (no branch here: the compiler moved all scaling behind it)
+            lds_dma4(scales + min(kt, kb - 1), rows_scales ? vs : vsb, (rows_scales ? sas + wave * 256 : sbs) + (kt & 1) * scales_stage);
+        }
     };
+    constexpr int kLoads = QN + QM + 1;
 
     f32x4_t acc[NI][NJ];
 #pragma unroll
@@ -160,13 +169,13 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
     const int sw = l16 & 7;
     const int c0 = (2 * lq) ^ sw, c1 = (2 * lq + 1) ^ sw;
 
-    issue(0);
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) issue(0, q);
     for (int kt = 0; kt < kb; ++kt) {
         wait_vmcnt<0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();  // stage kt has landed, and all have read the other one
         asm volatile("" ::: "memory");
-        if (kt + 1 < kb) issue(kt + 1);
         const uint8_t* wt = s_ring[kt & 1] + (wn * NI * 16 + l16) * kFp8Block;
         const uint8_t* xt = s_ring[kt & 1] + (BN + wm * NJ * 16 + l16) * kFp8Block;
         auto frag = [&](const uint8_t* p, int i) {
@@ -174,28 +183,46 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
                         *reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c1 * 16));
         };
         const float sb = s_sb[kt & 1][MODE == kGlu ? 0 : wn * 16 * NI / kFp8Block], sb2 = s_sb[kt & 1][1];
-        FragOf<T> x[NJ];
+        FragOf<T> x[NJ], w[2];
         float s[NJ], s2[NJ];
+        w[0].set(frag(wt, 0));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) x[j].set(frag(xt, j));
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            x[j].set(frag(xt, j));
             const float sa = s_sa[kt & 1][wm * NJ * 16 + j * 16 + l16];
             s[j] = sa * sb;
             s2[j] = MODE == kGlu ? sa * sb2 : 0.0f;
         }
+        // Two products a turn; beside them the scaling of the two before, the next weights' read and a share of the
+        // loads of block kt + 1: a direct load goes out every 35 cycles a CU at most, and all of them at a
+        // step's start held its first products back.
+        constexpr int kTurns = NI * NJ / 2, kPer = (kLoads + kTurns - 1) / kTurns;
+        f32x4_t t[2][2];
+        auto scale = [&](int u) {
+            const int i = u / (NJ / 2);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            FragOf<T> w;
-            w.set(frag(wt, i));
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const f32x4_t t = dot(w, x[j]);
+            for (int h = 0; h < 2; ++h) {
+                const int j = u % (NJ / 2) * 2 + h;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[i][j][r] = __builtin_fmaf(t[r], MODE == kGlu && i % 4 >= 2 ? s2[j] : s[j], acc[i][j][r]);
+                    acc[i][j][r] = __builtin_fmaf(t[u % 2][h][r], MODE == kGlu && i % 4 >= 2 ? s2[j] : s[j], acc[i][j][r]);
             }
+        };
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int i = u / (NJ / 2), j = u % (NJ / 2) * 2;
+            if (j == 0 && i + 1 < NI) w[(i + 1) % 2].set(frag(wt, i + 1));
+            t[u % 2][0] = dot(w[i % 2], x[j]);
+            t[u % 2][1] = dot(w[i % 2], x[j + 1]);
+#pragma unroll
+            for (int q = u * kPer; q < (u + 1) * kPer && q < kLoads; ++q) issue(kt + 1, q);  // (past the end: zeros)
+            if (u > 0) scale(u - 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        scale(kTurns - 1);
     }
+    wait_vmcnt<0>();  // (the loads past the end have written their zeros)
 
     if constexpr (MODE == kGlu) {
         // a lane's gate values of weight blocks i and up values of i + 2 are of the same hidden
@@ -413,7 +440,8 @@ hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
     if (a.M <= 32) return rows<T, kStore, 2, 2, 8, 2>(a, s);
     if (a.M <= 512) return rows<T, kStore, 4, 4, 4, 2>(a, s);
     if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<T, kStore, 4, 4, 2, 2>(a, s);
-    return tile<T, kStore, 8, 4, 2, 4>(a, s);
+    // (f32 results: widened fragments take twice the registers)
+    return tile<T, kStore, 8, sizeof(T) == 4 ? 2 : 4, 2, 4>(a, s);
 }
 
 }  // namespace
