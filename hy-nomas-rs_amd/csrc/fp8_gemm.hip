@@ -278,18 +278,53 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
         return;
     }
     T* y = static_cast<T*>(a.y);
+    float bias[NI][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = n0 + (wn * NI + i) * 16 + 4 * lq + r;
+            bias[i][r] = a.bias && n < a.N ? a.bias[n] : 0.0f;
+        }
+    constexpr int V = 16 / (int)sizeof(T), kWide = 16 * NI;  // outputs of a 16-byte store, and of a row of the wave
+    if (n0 + BN <= a.N && a.N % V == 0) {
+        // Sixteen rows at a time through LDS of the wave's own: a lane has four neighbouring outputs of a
+        // row, and stores of those (32 bytes of each row at a time) took a third of a product of 2,048 columns.
+        constexpr int kRow = kWide * (int)sizeof(T) + 16;  // (16 bytes more: rows start at other banks)
+        static_assert(NW * 16 * kRow <= 2 * kStage, "in the ring");
+        __syncthreads();  // (all have read the last stage)
+        uint8_t* lds = &s_ring[0][0] + wave * 16 * kRow;
+        constexpr int kLanesRow = kWide / V, kRowsStore = kWave / kLanesRow;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                T o[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] = Elt<T>::from_f32(acc[i][j][r] + bias[i][r]);
+                __builtin_memcpy(lds + l16 * kRow + (i * 16 + 4 * lq) * sizeof(T), o, sizeof(o));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (one wave: nothing else to wait for)
+#pragma unroll
+            for (int q = 0; q < 16 / kRowsStore; ++q) {
+                const int row = q * kRowsStore + lane / kLanesRow, c = lane % kLanesRow;
+                const u32x4_t v = *reinterpret_cast<const u32x4_t*>(lds + row * kRow + c * 16);
+                const int m = (wm * NJ + j) * 16 + row;
+                if (m < rows_m) *reinterpret_cast<u32x4_t*>(y + (m0 + m) * a.N + n0 + wn * kWide + c * V) = v;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        return;
+    }
     const bool whole = a.N % 4 == 0;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const int n = n0 + (wn * NI + i) * 16 + 4 * lq;
-        f32x4_t bias = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (a.bias)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bias[r] = n + r < a.N ? a.bias[n + r] : 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int m = (wm * NJ + j) * 16 + l16;
-            if (m < rows_m) put4(y + (m0 + m) * a.N, n, a.N, acc[i][j] + bias, whole);
+            const f32x4_t v = acc[i][j] + f32x4_t{bias[i][0], bias[i][1], bias[i][2], bias[i][3]};
+            if (m < rows_m) put4(y + (m0 + m) * a.N, n, a.N, v, whole);
         }
     }
 }
