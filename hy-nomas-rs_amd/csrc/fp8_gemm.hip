@@ -469,11 +469,20 @@ hipError_t rows(const Fp8GemmArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Few rows: as many blocks as fill the chip (256), then as many weight rows a block as leave so many.
+template <typename T, int NT, int P>
+hipError_t rows_by_n(const Fp8GemmArgs& a, hipStream_t s) {
+    const int64_t tm = (a.M + 16 * NT - 1) / (16 * NT);
+    if ((a.N + 63) / 64 * tm >= 256) return rows<T, kStore, 4, NT, NT == 4 ? 4 : 8, P>(a, s);
+    if ((a.N + 31) / 32 * tm >= 256) return rows<T, kStore, 2, NT, 8, P>(a, s);
+    return rows<T, kStore, 1, NT, 8, P>(a, s);
+}
+
 template <typename T>
 hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
-    if (a.M <= 16) return rows<T, kStore, 2, 1, 8, 2>(a, s);
-    if (a.M <= 32) return rows<T, kStore, 2, 2, 8, 2>(a, s);
-    if (a.M <= 512) return rows<T, kStore, 4, 4, 4, 2>(a, s);
+    if (a.M <= 16) return rows_by_n<T, 1, 2>(a, s);
+    if (a.M <= 32) return rows_by_n<T, 2, 2>(a, s);
+    if (a.M <= 512) return rows_by_n<T, 4, 2>(a, s);
     if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<T, kStore, 4, 4, 2, 2>(a, s);
     // (f32 results: widened fragments take twice the registers)
     return tile<T, kStore, 8, sizeof(T) == 4 ? 2 : 4, 2, 4>(a, s);
