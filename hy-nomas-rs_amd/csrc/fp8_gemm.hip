@@ -16,6 +16,7 @@
 #include "mfma.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace nomas {
@@ -469,22 +470,39 @@ hipError_t rows(const Fp8GemmArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Few rows: as many blocks as fill the chip (256), then as many weight rows a block as leave so many.
-template <typename T, int NT, int P>
-hipError_t rows_by_n(const Fp8GemmArgs& a, hipStream_t s) {
-    const int64_t tm = (a.M + 16 * NT - 1) / (16 * NT);
-    if ((a.N + 63) / 64 * tm >= 256) return rows<T, kStore, 4, NT, NT == 4 ? 4 : 8, P>(a, s);
-    if ((a.N + 31) / 32 * tm >= 256) return rows<T, kStore, 2, NT, 8, P>(a, s);
-    return rows<T, kStore, 1, NT, 8, P>(a, s);
+// Weight rows (16 NI) of a block of the kernel for few rows: as many as leave a block for each CU.
+template <int NT>
+int rows_ni(int64_t M, int N) {
+    const int64_t tm = (M + 16 * NT - 1) / (16 * NT);
+    return (N + 63) / 64 * tm >= 256 ? 4 : (N + 31) / 32 * tm >= 256 ? 2 : 1;
+}
+constexpr int rows_waves(int ni, int nt) { return ni == 4 && nt == 4 ? 4 : 8; }
+template <typename T, int NT>
+hipError_t few_rows(const Fp8GemmArgs& a, hipStream_t s) {
+    switch (rows_ni<NT>(a.M, a.N)) {
+        case 4: return rows<T, kStore, 4, NT, rows_waves(4, NT), 2>(a, s);
+        case 2: return rows<T, kStore, 2, NT, 8, 2>(a, s);
+    }
+    return rows<T, kStore, 1, NT, 8, 2>(a, s);
 }
 
+// Up to 32 rows the kernel for few rows; more: the least estimate, in us. Measured, in bf16 (few rows in tiles of
+// 64; tiles of 128 x 128; of 256 x 256): 128 x 8,192 x 2,048 15.3, 18.0, 31.7; 512 x 8,192 x 2,048 50, 19.8, 33;
+// 256 x 2,048 x 2,048 11.2, 17.6, 31; 64 x 2,048 x 8,192 28, 55, 105; 2,048 x 8,192 x 2,048 -, 50, 41; 4,744 x 4,096 x 2,048
+// -, 58, 68; 4,744 x 2,048 x 8,192 -, 131, 117.
 template <typename T>
 hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
-    if (a.M <= 16) return rows_by_n<T, 1, 2>(a, s);
-    if (a.M <= 32) return rows_by_n<T, 2, 2>(a, s);
-    if (a.M <= 512) return rows_by_n<T, 4, 2>(a, s);
-    if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<T, kStore, 4, 4, 2, 2>(a, s);
-    // (f32 results: widened fragments take twice the registers)
+    if (a.M <= 16) return few_rows<T, 1>(a, s);
+    if (a.M <= 32) return few_rows<T, 2>(a, s);
+    const double kt = (a.K + kFp8Block - 1) / kFp8Block;
+    auto rounds = [&](int bm, int bn) { return (double)(((a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) + 255) / 256); };
+    const int ni = rows_ni<4>(a.M, a.N);
+    const double few = 5 + rounds(64, 16 * ni) * (2 + 2.2 * std::ceil(kt / rows_waves(ni, 4)));
+    const double r128 = rounds(128, 128), t128 = 4 + kt * (r128 <= 1 ? 0.78 : 0.7 * r128);
+    const double t256 = 4 + rounds(256, 256) * (3 + 1.65 * kt);
+    if (few <= t128 && few <= t256 && a.M <= 65535 * 64) return few_rows<T, 4>(a, s);
+    if (t128 <= t256) return tile<T, kStore, 4, 4, 2, 2>(a, s);
+    // (f32 results: widened fragments take twice the registers, 128 rows a tile)
     return tile<T, kStore, 8, sizeof(T) == 4 ? 2 : 4, 2, 4>(a, s);
 }
 
