@@ -979,6 +979,14 @@ int MoeLayer::forward_few(const void* x, const Given* g, bool fp8, void* y, int6
     int rc = check_forward(x, y, rows);
     if (rc != NOMAS_OK) return rc;
     if (rows == 0) { last_rows_ = 0; last_in_scratch_ = false; return NOMAS_OK; }
+    if (g) {  // (x is read before y is written, the routing beside it)
+        const uintptr_t y0 = reinterpret_cast<uintptr_t>(y), y1 = y0 + (uintptr_t)(rows * D_) * dtype_size(dt_);
+        for (const void* p : {static_cast<const void*>(g->idx), static_cast<const void*>(g->w)}) {
+            const uintptr_t p0 = reinterpret_cast<uintptr_t>(p);
+            if (p0 < y1 && y0 < p0 + (uintptr_t)(rows * k_) * 4)
+                return set_error(NOMAS_ERR_INVALID_ARGUMENT, "y shares memory with idx or w");
+        }
+    }
     DeviceGuard guard(device_);
     if (!guard.ok) return set_error(NOMAS_ERR_HIP, "hipSetDevice(%d) failed", device_);
     rc = ensure_few();

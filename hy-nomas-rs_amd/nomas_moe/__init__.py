@@ -499,33 +499,40 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     scales.  K a multiple of 16; bias: (N,).  Sums in f32, rounded once; for 16-bit results the
     matrix instructions keep 13 bits below the largest of each 8 products (1.4e-5 of a result on
     random values), f32 results have exact products."""
-    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != b.shape[1]:
+    lead, (N, K) = a.shape[:-1], b.shape if b.dim() == 2 else (0, 0)
+    if a.dim() < 1 or b.dim() != 2 or a.shape[-1] != K:
         raise NomasError(2, f"expected (..., K) and (N, K) values, got {tuple(a.shape)} and "
                             f"{tuple(b.shape)}")
     if a.dtype is not FP8 or b.dtype is not FP8:
         raise NomasError(2, f"a and b must be {FP8}, got {a.dtype} and {b.dtype}")
-    if not a.is_cuda or b.device != a.device:
-        raise NomasError(2, f"matmul_fp8 takes tensors on one GPU, got {a.device} and {b.device}")
-    if dtype not in _CODES:
+    device = a.device
+    if not a.is_cuda or b.device != device:
+        raise NomasError(2, f"matmul_fp8 takes tensors on one GPU, got {device} and {b.device}")
+    code = _CODES.get(dtype)
+    if code is None:
         raise NomasError(2, f"the result must be f32, bf16 or f16, got {dtype}")
-    N, K = b.shape
     if K < 16 or K % 16:
         raise NomasError(2, f"K must be a positive multiple of 16, got {K}")
-    for t, n, want in ((a_scale, "a_scale", a.shape[:-1] + (_blocks(K),)),
-                       (b_scale, "b_scale", (_blocks(N), _blocks(K)))):
-        if t.shape != want or t.dtype is not torch.float32 or t.device != a.device:
-            raise NomasError(2, f"{n}: expected {tuple(want)} f32 on {a.device}, got "
-                                f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    kb = (K + 127) // 128
+    if a_scale.shape != lead + (kb,) or a_scale.dtype is not torch.float32 or a_scale.device != device:
+        raise _bad_scale("a_scale", a_scale, lead + (kb,), device)
+    if b_scale.shape != ((N + 127) // 128, kb) or b_scale.dtype is not torch.float32 or \
+            b_scale.device != device:
+        raise _bad_scale("b_scale", b_scale, ((N + 127) // 128, kb), device)
     ac, bc, sa, sb = a.contiguous(), b.contiguous(), a_scale.contiguous(), b_scale.contiguous()
     bias = _param(bias, ac, (N,), "bias")
-    shape = a.shape[:-1] + (N,)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=ac.device)
+        out = torch.empty(lead + (N,), dtype=dtype, device=device)
     else:
-        _check_out(out, torch.empty((), dtype=dtype, device=ac.device).expand(shape))
-    _call(_lib.lib().nomas_matmul_fp8, ac, _CODES[dtype], ac.data_ptr(), sa.data_ptr(),
-          bc.data_ptr(), sb.data_ptr(), _ptr(bias), out.data_ptr(), ac.numel() // K, N, K)
+        _check_out(out, torch.empty((), dtype=dtype, device=device).expand(lead + (N,)))
+    _call(_lib.lib().nomas_matmul_fp8, ac, code, ac.data_ptr(), sa.data_ptr(), bc.data_ptr(),
+          sb.data_ptr(), _ptr(bias), out.data_ptr(), ac.numel() // K, N, K)
     return out
+
+
+def _bad_scale(name: str, t: torch.Tensor, want, device) -> NomasError:
+    return NomasError(2, f"{name}: expected {tuple(want)} f32 on {device}, got {tuple(t.shape)} "
+                         f"{t.dtype} on {t.device}")
 
 
 class Weights:

@@ -245,6 +245,10 @@ def test_states_refused():
         layer.forward_few(x[:, :32])
     with pytest.raises(nm.NomasError, match="GPU"):
         layer.forward_few(x.cpu())
+    both = torch.zeros(4 * 64 * 2 + 64, dtype=torch.uint8, device="cuda")
+    y, i = both[:512].view(torch.bfloat16).view(4, 64), both[480:512].view(torch.int32).view(4, 2)
+    with pytest.raises(nm.NomasError, match="shares"):
+        layer.forward_few(x, i, w, out=y)
     f32, *_ = case(4, 64, 4, 2, 96, "f32", 1)
     with pytest.raises(nm.InvalidConfig, match="f32"):
         f32.quantize()

@@ -77,7 +77,8 @@ def test_quantize_shapes_strides_and_nothing():
 # from one row to the sizes that take each of the kernels
 SIZES = [(1, 1, 16), (1, 40, 128), (3, 130, 272), (16, 64, 1024), (17, 129, 400), (32, 96, 640), (33, 257, 144),
          (64, 512, 2048), (200, 321, 1008), (512, 64, 128), (600, 515, 272), (1111, 2667, 1008), (4100, 3077, 144),
-         (3333, 4096, 400)]
+         (3333, 4096, 400), (3333, 4099, 400), (1, 8200, 272), (5, 16400, 144), (20, 8200, 144), (20, 16400, 144),
+         (128, 8192, 1024), (256, 2048, 1024)]
 
 
 @pytest.mark.parametrize("bias", [False, True])
