@@ -669,11 +669,12 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
         t.off = __builtin_amdgcn_readfirstlane(l.off[t.e]);
         t.n = __builtin_amdgcn_readfirstlane(__popcll(l.mask[t.e]));
     };
-    // to the step after (past an expert's last one the next expert's; no branch between loads)
+    // to the step after: past an expert's last one the next expert's
     auto next = [&](At& t) {
-        const bool wrap = t.st + 1 == steps;
-        t.st = wrap ? 0 : t.st + 1;
-        t.li = min(t.li + (wrap ? 1 : 0), chosen - 1);
+        if (++t.st < steps) return;
+        t.st = 0;
+        t.li = min(t.li + 1, chosen - 1);
+        place(t);
     };
     struct Weights {
         u32x4_t w[2];
@@ -685,7 +686,6 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     const auto rh = __builtin_amdgcn_make_buffer_rsrc(a.h, 0, (int)((uint32_t)(a.rows * slots) * (uint32_t)(a.ldh * sizeof(T))),
                                                       0x00020000);
     auto fetch_w = [&](At& t, Weights& d) {
-        place(t);
         const uint8_t* p = static_cast<const uint8_t*>(a.w2) + (int64_t)t.e * a.w2_expert + (int64_t)n0 * kKBlockBytes +
                            2 * t.st * kstep;
 #pragma unroll
@@ -694,7 +694,6 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
         next(t);
     };
     auto fetch_x = [&](At& t, Tokens& d) {
-        place(t);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             if (j * 16 >= t.n) break;
@@ -734,8 +733,9 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     };
     clear();
     if (s0 < s1) {
-        At at = {s0 / steps, s0 % steps, 0, 0, 0}, aw = at, ax = at;  // of the products, of the weights' and the rows' loads
+        At at = {s0 / steps, s0 % steps, 0, 0, 0};
         place(at);
+        At aw = at, ax = at;  // of the products, of the weights' and the rows' loads
         bool whole = at.st == 0;  // the expert's first step is this wave's
         biases(at);
         Weights wd[P];
