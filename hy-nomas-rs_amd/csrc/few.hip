@@ -48,44 +48,65 @@ template <> struct Widen8<_Float16> {
     }
 };
 
+// The rows' fragments of a step, 16 J rows.
+template <typename T, bool W8, int J> struct Rows {
+    u32x4_t x[J][Step<T, W8>::XL];
+};
+
 // acc += the step's products.  `s`: the scale of 8-bit weights, else what f32 weights are taken down by.
-template <typename T, bool W8>
-__device__ __forceinline__ void multiply(f32x4_t& acc, const u32x4_t (&w)[2], const u32x4_t (&x)[Step<T, W8>::XL],
-                                         float s) {
+template <typename T, bool W8, int J>
+__device__ __forceinline__ void multiply(f32x4_t* acc, const u32x4_t (&w)[2], const u32x4_t (*x)[Step<T, W8>::XL], float s) {
     if constexpr (W8) {
         typedef typename Mfma<T>::V V;
-        f32x4_t t = {0.0f, 0.0f, 0.0f, 0.0f};
+        V a[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            V a;
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const auto v = Widen8<T>::run(w[q / 2][q % 2 * 2 + i], h);
-                    a[i * 4 + h * 2] = v[0];
-                    a[i * 4 + h * 2 + 1] = v[1];
+                    a[q][i * 4 + h * 2] = v[0];
+                    a[q][i * 4 + h * 2 + 1] = v[1];
                 }
-            t = Mfma<T>::run(a, __builtin_bit_cast(V, x[q]), t);
-        }
-        // The result is there 8 wait states after the last MFMA.  The compiler moved its use behind a
-        // branch that skips the next rows' products and counted the waits along the longer
-        // way only: every fourth column was wrong.  So the wait stands here.
-        asm volatile("s_nop 8" : "+v"(t));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(t[r], s, acc[r]);
+        for (int j = 0; j < J; ++j) {
+            f32x4_t t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) t = Mfma<T>::run(a[q], __builtin_bit_cast(V, x[j][q]), t);
+            // The result is there 8 wait states after the last MFMA.  The compiler moved its use behind a
+            // branch that skipped the next rows' products and counted the waits along the longer
+            // way only: every fourth column was wrong.  So the wait stands here.
+            asm volatile("s_nop 8" : "+v"(t));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(t[r], s, acc[j][r]);
+        }
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                acc = mfma_f32(__uint_as_float(w[q][k]) * s, __uint_as_float(x[q][k]), acc);
+            for (int k = 0; k < 4; ++k) {
+                const float v = __uint_as_float(w[q][k]) * s;
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[j] = mfma_f32(v, __uint_as_float(x[j][q][k]), acc[j]);
+            }
     } else {
         typedef typename Mfma<T>::V V;
 #pragma unroll
         for (int q = 0; q < 2; ++q)
-            acc = Mfma<T>::run(__builtin_bit_cast(V, w[q]), __builtin_bit_cast(V, x[q]), acc);
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                acc[j] = Mfma<T>::run(__builtin_bit_cast(V, w[q]), __builtin_bit_cast(V, x[j][q]), acc[j]);
     }
+}
+
+// f(J) with 16 J >= n rows, J of 1, 2, 4 up to NT: code with the loads ahead that so few rows leave registers for.
+template <int NT, typename F>
+__device__ __forceinline__ void for_rows(int n, F f) {
+    using std::integral_constant;
+    if (NT == 1 || n <= 16) f(integral_constant<int, 1>{});
+    else if (NT == 2 || n <= 32) f(integral_constant<int, NT < 2 ? NT : 2>{});
+    else f(integral_constant<int, NT>{});
 }
 
 __device__ __forceinline__ u32x4_t load16u(const void* p) { return *reinterpret_cast<const u32x4_t*>(p); }
@@ -483,17 +504,16 @@ __device__ __forceinline__ uint32_t weight_lane(int l16, int lq) {
     return W8 ? (uint32_t)(lq * 256 + l16 * 16) : (uint32_t)(l16 * 64 + lq * 16);
 }
 
-// Steps of rows in flight, as many as registers hold (of four: two made a step of the second kernel 2,200 cycles
-// long, an L2 read and a half).
-template <bool W8, int NT, bool kDown>
-constexpr int rows_ahead() { return W8 ? (NT == 1 ? 4 : NT == 2 ? 2 : 1) : NT < 4 || kDown ? 4 : 2; }
+// Steps of 16 J rows in flight, as many as registers hold (of four: two made a step of the second kernel 2,200
+// cycles long, an L2 read and a half).
+template <bool W8, int J, bool kDown>
+constexpr int rows_ahead() { return W8 ? (J == 1 ? 4 : J == 2 ? 2 : 1) : J < 4 || kDown ? 4 : 2; }
 
 // S waves share a unit (16 hidden units of one expert: 16 gate and 16 up rows), each its own
 // share of the steps.
 template <typename T, bool W8, int NT, int S, int P>
 __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     typedef Step<T, W8> St;
-    constexpr int XP = rows_ahead<W8, NT, false>();
     constexpr int GP = kFewWaves / S;  // units a block has at a time
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_part[S > 1 ? kFewWaves : 1][2][NT][kWave];
@@ -529,9 +549,6 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
         u32x4_t w[2][2];
         float s[2];
     };
-    struct Tokens {
-        u32x4_t x[NT][St::XL];
-    };
     for (int u0 = blockIdx.x * GP; u0 < units; u0 += gridDim.x * GP) {
         const bool has = u0 + g < units;
         const int u = min(u0 + g, units - 1), li = u / tiles, ht = u - li * tiles;
@@ -555,33 +572,68 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
             d.s[0] = W8 ? sg[st] : a.w1_down;
             d.s[1] = W8 ? su[st] : a.w1_down;
         };
-        auto fetch_x = [&](int st, Tokens& d) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (j * 16 >= n) break;
-#pragma unroll
-                for (int q = 0; q < St::XL; ++q) {
-                    const int k = st * St::KS + St::xk(q, lq);
-                    d.x[j][q] = __builtin_bit_cast(
-                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                                     rx, k < a.D ? xo[j] + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
-                }
-            }
-        };
         f32x4_t acc[2][NT];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (has) {
+        auto fetch_x = [&](int j, int st, u32x4_t (&d)[St::XL]) {
+#pragma unroll
+            for (int q = 0; q < St::XL; ++q) {
+                const int k = st * St::KS + St::xk(q, lq);
+                d[q] = __builtin_bit_cast(
+                    u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                 rx, k < a.D ? xo[j] + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
+            }
+        };
+        // 8-bit weights in code of so many row groups, as a step's values are widened once for all of them (64
+        // rows, 2,048 x 768, 8 of 64 experts: 100 -> 91 us a call).  Others in one: with code for each
+        // number the first kernel of 64 rows, 1,024 x 2,048, 2 of 16 experts took 37 us for 30, and loops without
+        // branches, which never wait for more than the loads they need, 41.
+        if constexpr (W8) {
+            if (has)
+                for_rows<NT>(n, [&](auto jj) {
+                    constexpr int J = decltype(jj)::value, XP = rows_ahead<W8, J, false>();
+                    Weights wd[P];
+                    Rows<T, W8, J> xd[XP];
+#pragma unroll
+                    for (int p = 0; p < P; ++p)
+                        if (s0 + p < s1) fetch_w(s0 + p, wd[p]);
+#pragma unroll
+                    for (int p = 0; p < XP; ++p)
+                        if (s0 + p < s1)
+#pragma unroll
+                            for (int j = 0; j < J; ++j) fetch_x(j, s0 + p, xd[p].x[j]);
+                    for (int st = s0; st < s1; st += P) {
+#pragma unroll
+                        for (int p = 0; p < P; ++p) {
+                            if (st + p >= s1) break;
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) multiply<T, W8, J>(acc[c], wd[p].w[c], xd[p % XP].x, wd[p].s[c]);
+                            if (st + p + P < s1) fetch_w(st + p + P, wd[p]);
+                            if (st + p + XP < s1)
+#pragma unroll
+                                for (int j = 0; j < J; ++j) fetch_x(j, st + p + XP, xd[p % XP].x[j]);
+                        }
+                    }
+                });
+        } else if (has) {
+            constexpr int XP = rows_ahead<W8, NT, false>();
             Weights wd[P];
-            Tokens xd[XP];
+            Rows<T, W8, NT> xd[XP];
+            auto fetch_rows = [&](int st, Rows<T, W8, NT>& d) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if (j * 16 >= n) break;
+                    fetch_x(j, st, d.x[j]);
+                }
+            };
 #pragma unroll
             for (int p = 0; p < P; ++p)
                 if (s0 + p < s1) fetch_w(s0 + p, wd[p]);
 #pragma unroll
             for (int p = 0; p < XP; ++p)
-                if (s0 + p < s1) fetch_x(s0 + p, xd[p]);
+                if (s0 + p < s1) fetch_rows(s0 + p, xd[p]);
             for (int st = s0; st < s1; st += P) {
 #pragma unroll
                 for (int p = 0; p < P; ++p) {
@@ -590,10 +642,10 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
                     for (int j = 0; j < NT; ++j) {
                         if (j * 16 >= n) break;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) multiply<T, W8>(acc[c][j], wd[p].w[c], xd[p % XP].x[j], wd[p].s[c]);
+                        for (int c = 0; c < 2; ++c) multiply<T, W8, 1>(acc[c] + j, wd[p].w[c], xd[p % XP].x + j, wd[p].s[c]);
                     }
                     if (st + p + P < s1) fetch_w(st + p + P, wd[p]);
-                    if (st + p + XP < s1) fetch_x(st + p + XP, xd[p % XP]);
+                    if (st + p + XP < s1) fetch_rows(st + p + XP, xd[p % XP]);
                 }
             }
         }
@@ -641,7 +693,6 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
 template <typename T, bool W8, int NT, int P>
 __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     typedef Step<T, W8> St;
-    constexpr int XP = rows_ahead<W8, NT, true>();
     extern __shared__ __align__(16) uint8_t s_dyn[];
     __shared__ f32x4_t s_y[kFewWaves][16 * NT][4];  // [wave][row][4 columns each]
     __shared__ int s_last;
@@ -680,9 +731,6 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
         u32x4_t w[2];
         float s;
     };
-    struct Tokens {
-        u32x4_t x[NT][St::XL];
-    };
     const auto rh = __builtin_amdgcn_make_buffer_rsrc(a.h, 0, (int)((uint32_t)(a.rows * slots) * (uint32_t)(a.ldh * sizeof(T))),
                                                       0x00020000);
     auto fetch_w = [&](At& t, Weights& d) {
@@ -691,21 +739,6 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) d.w[q] = load16u(p + q * kstep + wl);
         d.s = W8 ? a.s2[((int64_t)t.e * a.nb2 + n0 / kFp8Block) * a.kb2 + t.st] : a.w2_down;
-        next(t);
-    };
-    auto fetch_x = [&](At& t, Tokens& d) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            if (j * 16 >= t.n) break;
-            const uint32_t h = (uint32_t)(t.off + min(j * 16 + l16, t.n - 1)) * (uint32_t)(a.ldh * sizeof(T));
-#pragma unroll
-            for (int q = 0; q < St::XL; ++q) {
-                const int k = t.st * St::KS + St::xk(q, lq);
-                d.x[j][q] = __builtin_bit_cast(
-                    u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                                 rh, k < live_h ? h + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
-            }
-        }
         next(t);
     };
     f32x4_t acc[NT];
@@ -734,40 +767,63 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     clear();
     if (s0 < s1) {
         At at = {s0 / steps, s0 % steps, 0, 0, 0};
+        int most = 0;  // rows of an expert of this wave's
+        for (int li = at.li; li <= (s1 - 1) / steps; ++li)
+            most = max(most, __builtin_amdgcn_readfirstlane(__popcll(l.mask[l.live[li]])));
         place(at);
-        At aw = at, ax = at;  // of the products, of the weights' and the rows' loads
         bool whole = at.st == 0;  // the expert's first step is this wave's
         biases(at);
-        Weights wd[P];
-        Tokens xd[XP];
+        for_rows<NT>(most, [&](auto jj) {
+            constexpr int J = decltype(jj)::value, XP = rows_ahead<W8, J, true>();
+            auto fetch_x = [&](At& t, Rows<T, W8, J>& d) {
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-            if (s0 + p < s1) fetch_w(aw, wd[p]);
+                for (int j = 0; j < J; ++j) {
+                    if (J > 1 && j * 16 >= t.n) break;
+                    const uint32_t h = (uint32_t)(t.off + min(j * 16 + l16, t.n - 1)) * (uint32_t)(a.ldh * sizeof(T));
 #pragma unroll
-        for (int p = 0; p < XP; ++p)
-            if (s0 + p < s1) fetch_x(ax, xd[p]);
-        for (int s = s0; s < s1; s += P) {
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                if (s + p >= s1) break;
-                if (at.st == steps) {
-                    flush(at, whole);
-                    ++at.li;
-                    at.st = 0;
-                    place(at);
-                    biases(at);
-                    whole = true;
+                    for (int q = 0; q < St::XL; ++q) {
+                        const int k = t.st * St::KS + St::xk(q, lq);
+                        d.x[j][q] = __builtin_bit_cast(
+                            u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                         rh, k < live_h ? h + (uint32_t)(k * sizeof(T)) : 0xfffffff0u, 0, 0));
+                    }
                 }
+                next(t);
+            };
+            At aw = at, ax = at;  // of the weights' and the rows' loads
+            Weights wd[P];
+            Rows<T, W8, J> xd[XP];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if (j * 16 >= at.n) break;
-                    multiply<T, W8>(acc[j], wd[p].w, xd[p % XP].x[j], wd[p].s);
+            for (int p = 0; p < XP; ++p)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int q = 0; q < St::XL; ++q) xd[p].x[j][q] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (s0 + p < s1) fetch_w(aw, wd[p]);
+#pragma unroll
+            for (int p = 0; p < XP; ++p)
+                if (s0 + p < s1) fetch_x(ax, xd[p]);
+            for (int s = s0; s < s1; s += P) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    if (s + p >= s1) break;
+                    if (at.st == steps) {
+                        flush(at, whole);
+                        ++at.li;
+                        at.st = 0;
+                        place(at);
+                        biases(at);
+                        whole = true;
+                    }
+                    multiply<T, W8, J>(acc, wd[p].w, xd[p % XP].x, wd[p].s);  // (rows past the expert's: not used)
+                    ++at.st;
+                    if (s + p + P < s1) fetch_w(aw, wd[p]);
+                    if (s + p + XP < s1) fetch_x(ax, xd[p % XP]);
                 }
-                ++at.st;
-                if (s + p + P < s1) fetch_w(aw, wd[p]);
-                if (s + p + XP < s1) fetch_x(ax, xd[p % XP]);
             }
-        }
+        });
         flush(at, whole);
     }
     __syncthreads();
