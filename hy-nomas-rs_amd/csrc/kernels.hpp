@@ -378,7 +378,7 @@ hipError_t launch_fp8_gemm(DType dt, const Fp8GemmArgs& a, hipStream_t s);
 // 128 == 0; scales 2 x N / 256 x K / 128): 8-bit (M x N / 2) with y_scale where fp8_glu_fused, else f32.
 constexpr int kFp8GluRows = 128;  // (more rows: always fused)
 bool fp8_glu_fused(int64_t M, int N);
-hipError_t launch_fp8_glu(const Fp8GemmArgs& a, hipStream_t s);
+hipError_t launch_fp8_glu(DType dt, const Fp8GemmArgs& a, hipStream_t s);
 int64_t block_seam_workspace(int64_t rows, int64_t D, int64_t seq);
 hipError_t launch_block_seam(DType dt, const BlockSeamArgs& a, hipStream_t s);
 hipError_t launch_block_seam_backward(DType dt, const BlockSeamBackwardArgs& a, hipStream_t s);

@@ -1102,7 +1102,7 @@ int MoeLayer::forward_fp8(const void* x, void* y, int64_t rows, hipStream_t s) {
     const bool fused = fp8_glu_fused(rows, a.N);
     a.y = fused ? static_cast<void*>(h8.q) : const_cast<void*>(h8.x);
     a.y_scale = h8.scale;
-    HIP_TRY(launch_fp8_glu(a, s));
+    HIP_TRY(launch_fp8_glu(dt_, a, s));
     if (!fused) {
         h8.rows = rows;
         h8.cols = h8.ld_q = (int)Hp_;

@@ -74,6 +74,10 @@ extern "C" {
     pub fn nomas_moe_forward_routed(h: *mut nomas_moe_t, x: *const c_void, idx: *const i32,
                                     w: *const f32, y: *mut c_void, rows: i64,
                                     stream: *mut c_void) -> c_int;
+    pub fn nomas_moe_forward_few(h: *mut nomas_moe_t, x: *const c_void, idx: *const i32,
+                                 w: *const f32, fp8: c_int, y: *mut c_void, rows: i64,
+                                 stream: *mut c_void) -> c_int;
+    pub fn nomas_moe_quantize(h: *mut nomas_moe_t) -> c_int;
     pub fn nomas_moe_forward_block(h: *mut nomas_moe_t, x: *const c_void, out: *mut c_void,
                                    rows: i64, seq: i64, norm_w: *const f32, eps: f64,
                                    shift: *const f32, scale: *const f32, gate: *const f32,
@@ -101,6 +105,9 @@ extern "C" {
                                out: *mut *mut nomas_ffn_t) -> c_int;
     pub fn nomas_ffn_forward(h: *mut nomas_ffn_t, x: *const c_void, y: *mut c_void, rows: i64,
                              stream: *mut c_void) -> c_int;
+    pub fn nomas_ffn_quantize(h: *mut nomas_ffn_t) -> c_int;
+    pub fn nomas_ffn_forward_fp8(h: *mut nomas_ffn_t, x: *const c_void, y: *mut c_void, rows: i64,
+                                 stream: *mut c_void) -> c_int;
     pub fn nomas_ffn_forward_host(h: *mut nomas_ffn_t, x: *const c_void, y: *mut c_void,
                                   rows: i64) -> c_int;
     pub fn nomas_ffn_n_params(h: *const nomas_ffn_t) -> i64;
@@ -113,6 +120,13 @@ extern "C" {
                                dim: i64, seq: i64, norm_w: *const f32, eps: f64,
                                shift: *const f32, scale: *const f32,
                                stream: *mut c_void) -> c_int;
+    pub fn nomas_quantize_fp8(dtype: c_int, x: *const c_void, rows: i64, cols: i64,
+                              square: c_int, q: *mut c_void, scale: *mut f32,
+                              stream: *mut c_void) -> c_int;
+    pub fn nomas_matmul_fp8(dtype: c_int, a: *const c_void, a_scale: *const f32,
+                            b: *const c_void, b_scale: *const f32, bias: *const f32,
+                            y: *mut c_void, rows: i64, n: i64, k: i64,
+                            stream: *mut c_void) -> c_int;
     pub fn nomas_gated_residual(dtype: c_int, x: *const c_void, y: *const c_void,
                                 gate: *const f32, out: *mut c_void, rows: i64, dim: i64,
                                 seq: i64, stream: *mut c_void) -> c_int;
