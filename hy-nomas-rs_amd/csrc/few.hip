@@ -368,7 +368,6 @@ __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
             s_logit[i] = __builtin_bit_cast(
                 double, __builtin_amdgcn_raw_buffer_load_b64(rs, ((rg * 16 + row) * kMaxExperts + ex) * 8, 0, kSc1));
         }
-        if (tid == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else if (tid < 256 && e < a.E) {
         s_logit[r * a.E + e] = v;
     }
@@ -535,6 +534,12 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
         make_lists<false>(a, l);
     }
 
+    // The second kernel's counts.  Each kernel clears the other's: what a call finds does not depend on how the
+    // one before it ended.
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.tile_cap; i += kFewThreads)
+            __hip_atomic_store(&a.arrived[i], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+
     const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = wave / S, part = wave % S;
     const int tiles = (a.H + 15) / 16, units = __builtin_amdgcn_readfirstlane(l.info[0]) * tiles;
@@ -699,6 +704,8 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     const int slots = a.k + a.Ecols - a.E;
     const Lists l(s_dyn, a.Ecols, a.rows * slots);
     make_lists<true>(a, l);
+    if (blockIdx.x == 0 && threadIdx.x < kFewGroups)  // the router's kernel's counts
+        __hip_atomic_store(&a.arrived[a.tile_cap + threadIdx.x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -865,7 +872,6 @@ __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
             for (int p = 1; p < kFewParts; ++p)
                 if (p < a.parts) v += t[p];
         }
-        if (tid == 0) __hip_atomic_store(&a.arrived[tile], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     const int col = n0 + 4 * c;
     if (row < a.rows && col < a.D) {  // (D % 8 == 0: four columns are real or padding)

@@ -333,6 +333,7 @@ private:
     bool last_few_given_ = false;  // the last forward was forward_few under the caller's routing
     // forward_fp8's: x and the hidden activations in 8 bits, and the latter in f32 where few
     void* d_f8_ = nullptr;
+    std::vector<void*> f8_old_;  // outgrown ones: a captured graph may use them
     int64_t f8_rows_ = 0;
 
     // the handle's workspace (sized for ws_.cap_rows rows)

@@ -338,7 +338,7 @@ struct FewArgs {
     void* h;             // hidden activations, ldh columns a place
     int64_t ldh;
     float* partial;      // tile_cap x kFewParts x rows x 16 sums
-    int32_t* arrived;    // tile_cap + kFewGroups counters, zero between calls
+    int32_t* arrived;    // tile_cap + kFewGroups counters, the last ones zero at first
     int tile_cap;
     int parts;           // (set by the launch)
     // the router (wr non-null): its choice goes to idx and w too, which have out_slots a row

@@ -203,6 +203,7 @@ MoeLayer::~MoeLayer() {
     for (void* p : {d_wr_, d_w1_, (void*)d_b1_, d_w2_, (void*)d_b2_, d_hio_, d_route_, (void*)d_q1_, (void*)d_q2_,
                     (void*)d_s1_, (void*)d_s2_, d_few_, d_f8_})
         if (p) (void)hipFree(p);
+    for (void* p : f8_old_) (void)hipFree(p);
     for (hipEvent_t e : events_) (void)hipEventDestroy(e);
     for (int i = 0; i < kHostMaxPieces; ++i) {
         if (hev_in_[i]) (void)hipEventDestroy(hev_in_[i]);
@@ -1076,10 +1077,11 @@ int MoeLayer::forward_fp8(const void* x, void* y, int64_t rows, hipStream_t s) {
     if (rows > f8_rows_) {
         const int64_t cap = round_up(std::max(rows, f8_rows_ + f8_rows_ / 2), kRouterRows);
         const size_t bytes = lay(cap, nullptr, &x8, &h8);
-        if (d_f8_) HIP_TRY(hipFree(d_f8_));
-        d_f8_ = nullptr;
-        f8_rows_ = 0;
-        HIP_TRY(hipMalloc(&d_f8_, bytes));
+        void* p = nullptr;
+        f8_old_.reserve(f8_old_.size() + 1);
+        HIP_TRY(hipMalloc(&p, bytes));
+        if (d_f8_) f8_old_.push_back(d_f8_);
+        d_f8_ = p;
         f8_rows_ = cap;
     }
     lay(f8_rows_, static_cast<uint8_t*>(d_f8_), &x8, &h8);

@@ -256,7 +256,8 @@ int nomas_ffn_forward_host(nomas_ffn_t *h, const void *x, void *y, int64_t rows)
  * nomas_quantize_fp8 makes them; synchronises).  nomas_ffn_forward_fp8: x in blocks of
  * 128 of a row to 8 bits, gate and up products, h = silu(gate) * up in f32 to 8 bits in the same
  * way, down product, biases in f32, y rounded once; x, y and `stream` as in nomas_ffn_forward
- * (y may be x). */
+ * (y may be x).  A call of more rows than any before allocates a workspace; those outgrown stay until
+ * the handle's end, for graphs that were captured with them. */
 int nomas_ffn_quantize(nomas_ffn_t *h);
 int nomas_ffn_forward_fp8(nomas_ffn_t *h, const void *x, void *y, int64_t rows, void *stream);
 

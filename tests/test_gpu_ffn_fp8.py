@@ -157,6 +157,27 @@ def test_states_refused():
         f32.quantize()
 
 
+def test_a_graph_outlives_its_workspace():
+    """A call of more rows takes a new workspace; a graph captured before keeps the old one."""
+    x, w, b = case(700, 256, 384, 2)
+    layer = layer_of(w, b, torch.bfloat16)
+    xd = x.bfloat16().cuda()
+    small = xd[:40].clone()
+    want = layer.forward_fp8(small)
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        y = layer.forward_fp8(small)
+    for rows in (300, 700):
+        whole = layer.forward_fp8(xd[:rows])
+        torch.cuda.synchronize()
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        assert torch.equal(layer.forward_fp8(xd[:rows]), whole)
+
+
 @pytest.mark.parametrize("rows,D,H", [(515, 96, 2093), (41, 136, 640), (932, 912, 1805)])
 def test_f16_keeps_its_accuracy(rows, D, H):
     """On values of every kind the error is the outputs' rounding, at most 2^-11 of each, and that of
