@@ -333,7 +333,9 @@ __device__ __forceinline__ void choose_any(const FewArgs& a, const double* l, in
     else choose<kMaxExperts / 64>(a, l, row, store, s_key, chosen);
 }
 
-// A kernel of its own: a block for 16 rows and 16 experts; the last one of 16 rows chooses.
+// A kernel of its own: a block for 16 rows and 16 experts; with more than 16 rows in all the last block of each 16
+// chooses for them.  Latencies bound it: the router's weights once from HBM, a sum over the waves, the logits' way
+// past the caches.  4.6 us for one row of 2,048 and 64 experts, 6.8 for 48 rows of 1,024 and 16.
 template <typename T>
 __global__ __launch_bounds__(kFewThreads) void few_route_kernel(FewArgs a) {
     extern __shared__ __align__(16) uint8_t s_dyn[];  // 16 rows' logits
@@ -509,7 +511,9 @@ template <bool W8, int J, bool kDown>
 constexpr int rows_ahead() { return W8 ? (J == 1 ? 4 : J == 2 ? 2 : 1) : J < 4 || kDown ? 4 : 2; }
 
 // S waves share a unit (16 hidden units of one expert: 16 gate and 16 up rows), each its own
-// share of the steps.
+// share of the steps: as many small units as there are feed all CUs from the first load on, with no tile of rows to
+// wait for.  Bound by the weights' bytes: 134 MB for 48 rows, 1,024 x 2,048, 16 experts in f16 take 29.8 us (4.5 TB/s); the
+// 50 MB of one row's 8 experts, 2,048 x 768, 13.8 us (3.6 TB/s).
 template <typename T, bool W8, int NT, int S, int P>
 __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     typedef Step<T, W8> St;
@@ -593,7 +597,7 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
         };
         // 8-bit weights in code of so many row groups, as a step's values are widened once for all of them (64
         // rows, 2,048 x 768, 8 of 64 experts: 100 -> 91 us a call).  Others in one: with code for each
-        // number the first kernel of 64 rows, 1,024 x 2,048, 2 of 16 experts took 37 us for 30, and loops without
+        // number the first kernel of 48 rows, 1,024 x 2,048, 2 of 16 experts took 37 us for 30, and loops without
         // branches, which never wait for more than the loads they need, 41.
         if constexpr (W8) {
             if (has)
@@ -694,7 +698,9 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     }
 }
 
-// A block has 16 columns of y, or with parts > 1 a share of their sums' steps.
+// A block has 16 columns of y, or with parts > 1 a share of their sums' steps: all experts of a row end in one
+// block (or kFewParts), so nothing is written between.  67 MB for 48 rows, 1,024 x 2,048, 16 experts in f16: 18.4 us (3.6
+// TB/s; 64 tiles of 16 columns in 4 parts, a block a CU); 25 MB of one row's 8 experts, 2,048 x 768: 9.5 us.
 template <typename T, bool W8, int NT, int P>
 __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     typedef Step<T, W8> St;
@@ -947,8 +953,8 @@ hipError_t launch_few_t(FewArgs a, hipStream_t s) {
     // Who chooses.  Up to 16 rows: every block of the first kernel, from logits that it makes itself
     // where the router's weights and the rows are a few KB, else from those of a kernel that has a
     // block for 16 experts.  More rows: that kernel's last blocks.  (Two rows of 64, 4 experts: 21
-    // us a call with a kernel for the router, 15 without; one row of 2,048, 64 experts: the router's
-    // kernel 10 us with the choice, 4 without.)
+    // us a call with a kernel for the router, 18 without; one row of 2,048, 64 experts: the router's
+    // kernel 10 us with the choice, 4.6 without.)
     a.choice = kChoiceMade;
     if (a.wr && a.rows <= 16)
         a.choice = a.E <= 16 && (int64_t)(a.rows + a.E) * a.D * (int)sizeof(T) <= 64 * 1024 ? kChoiceOfRows : kChoiceOfLogits;
