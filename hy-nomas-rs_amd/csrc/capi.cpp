@@ -895,7 +895,7 @@ int nomas_quantize_fp8(int dtype, const void* x, int64_t rows, int64_t cols, int
         if (cols < 16 || cols % 16 != 0 || cols > 0x7fffff00)
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "cols must be a positive multiple of 16 (got %lld)",
                              (long long)cols);
-        if (rows < 0 || rows > 0x7fffffffLL || rows * fp8_blocks(cols) > 0x7fffffffLL ||
+        if (rows < 0 || rows > 0x7fffffffLL || rows * fp8_blocks(cols) >= (1LL << 30) ||
             (square && fp8_blocks(rows) > 65535))
             return set_error(NOMAS_ERR_INVALID_ARGUMENT, "rows=%lld out of range", (long long)rows);
         if (rows == 0) return NOMAS_OK;

@@ -460,7 +460,7 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
 template <typename T, int MODE, int NI, int NJ, int WN, int WM>
 hipError_t tile(const Fp8GemmArgs& a, hipStream_t s) {
     const int64_t tm = (a.M + 16 * NJ * WM - 1) / (16 * NJ * WM), tn = (a.N + 16 * NI * WN - 1) / (16 * NI * WN);
-    if (tm * tn > 0x7fffff00) return hipErrorInvalidValue;
+    if (tm * tn >= ((int64_t)1 << 32) / (WN * WM * kWave) - kNumXcd) return hipErrorInvalidValue;
     launch_kernel(fp8_tile_kernel<T, MODE, NI, NJ, WN, WM>, dim3((unsigned)round_up(tm * tn, kNumXcd)),
                   dim3(WN * WM * kWave), 0, s, a, (int)tm, (int)tn);
     return hipGetLastError();

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_squares_kernel(QuantSquar
 hipError_t launch_quant_rows(DType dt, const QuantArgs& a, hipStream_t s) {
     const int64_t kb = (a.ld_q + kFp8Block - 1) / kFp8Block;
     if (a.rows < 1 || a.cols < 8 || a.cols % 8 != 0 || a.ld_q < a.cols || a.ld_q % 8 != 0 ||
-        a.rows * kb >= ((int64_t)1 << 31))
+        a.rows * kb >= ((int64_t)1 << 30))  // (four threads a block of 128: 2^32 in a grid)
         return hipErrorInvalidValue;
     constexpr int U = 4;
     const int64_t blocks = (a.rows * kb + U * kGroups - 1) / (U * kGroups);

@@ -374,7 +374,7 @@ int nomas_block_seam_backward(int dtype, const void *dout, const void *dh, const
 /* x (rows, cols) in `dtype` -> q (rows, cols) and scale: (rows, ceil(cols / 128)) for blocks
  * along the rows (activations), or (ceil(rows / 128), ceil(cols / 128)) with `square` for
  * blocks of 128 x 128 (weights).  cols % 16 == 0; x and q 16-byte, scale 4-byte aligned; outputs
- * share no memory with x or each other.  rows * ceil(cols / 128) < 2^31. */
+ * share no memory with x or each other.  rows * ceil(cols / 128) < 2^30. */
 int nomas_quantize_fp8(int dtype, const void* x, int64_t rows, int64_t cols, int square, void* q, float* scale,
                        void* stream);
 

@@ -128,3 +128,9 @@ def test_mirror_of_the_layers(no_lib):
     refused("last dim", ffn.forward_fp8, torch.zeros(4, 8))
     refused("dtype", ffn.forward_fp8, x.bfloat16())
     refused("GPU", ffn.forward_fp8, x)
+
+
+def test_quantize_refuses_more_blocks_than_a_grid_holds():
+    kw = dict(rows=1 << 30, cols=16, q=P + (1 << 40), scale=P + (1 << 41))
+    assert _lib.lib().nomas_quantize_fp8(*{**QUANT, **kw}.values(), None) == 2
+    assert "rows" in _lib.last_error()
