@@ -11,6 +11,10 @@
 // columns for all rows and experts, or shares it with a few others.  Weights are read in the layouts that
 // the layer keeps (K-blocked, kernels.hpp), a 16 x 16-byte fragment of an MFMA per instruction, straight
 // into registers, or as 8-bit values in fragment order, widened there.
+//
+// h is rounded to the layer's type, in which the second kernel's MFMAs take it and in which the layer's
+// forward of many rows keeps it (an output's error is then 1.4 times that of its own rounding);
+// y's sums stay f32 over all experts and are rounded once.
 #include "fp8.hpp"
 #include "mfma.hpp"
 

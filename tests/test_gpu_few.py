@@ -252,3 +252,31 @@ def test_states_refused():
     f32, *_ = case(4, 64, 4, 2, 96, "f32", 1)
     with pytest.raises(nm.InvalidConfig, match="f32"):
         f32.quantize()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_graphs_that_share_a_workspace_and_layers_side_by_side(fp8):
+    """Two graphs of one layer, of few and of many rows, replayed in turn, while another layer runs on another stream."""
+    layer, x, _, _ = case(64, 512, 8, 2, 768, "bf16", 9, fp8=fp8)
+    beside, xb, _, _ = case(20, 256, 16, 3, 200, "bf16", 10, fp8=fp8)
+    want = {n: layer.forward_few(x[:n], fp8=fp8) for n in (3, 64)}
+    wb = beside.forward_few(xb, fp8=fp8)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs = {}
+    for n in want:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            y = layer.forward_few(x[:n], fp8=fp8)
+        graphs[n] = g, y
+    outs = []
+    for _ in range(4):
+        for n in (64, 3, 3):
+            g, y = graphs[n]
+            with torch.cuda.stream(s):
+                y.zero_()
+                g.replay()
+                outs.append((y.clone(), want[n]))
+            outs.append((beside.forward_few(xb, fp8=fp8), wb))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in outs)
