@@ -87,6 +87,56 @@ __device__ __forceinline__ void put4(T* row, int n, int N, const f32x4_t& v, boo
 //          128 of them (tile kernel: a tile has whole blocks) or as they are (few rows)
 enum { kStore = 0, kGlu = 1 };
 
+// ---- the scales' product ---------------------------------------------------------
+// sa sb leaves f32's range where the results do not: two of 2^-70 beside sums of 2^20, two of 2^70 beside sums
+// of 2^-14, or beside a sum of 0.  So the sums are taken times 2^32.  Products of scales down to 2^-158 are
+// then normal numbers, and the bits that smaller ones lose are below 2^-156 of a result: under 1/64 of f32's
+// last bit.  Products from 2^55 on (a row's sum can add 2^40 of one) and infinities are seen by a compare a
+// step; a wave that saw one makes its sums again, with the scales' powers of two apart.  (NaN needs no second try.)
+constexpr float kScaleUp = 0x1p32f, kScaleDown = 0x1p-32f, kScaleMost = 0x1p87f;
+__device__ __forceinline__ bool too_large(float s) { return __builtin_fabsf(s) >= kScaleMost; }
+
+// The wave's sums over blocks kt0, kt0 + step, ... for any scales, to put(i, j, sums): a block's sum times the scales'
+// mantissas, then their powers of two in one step.  w, x: the wave's first rows; rows past last_n, last_m (the
+// matrices' last ones, as seen from there) are the last one again.  bs: the scales of its weights' block, with kGlu of
+// the gate rows, the up rows' `up` further.  One fragment at a time from global memory, to keep out of the other
+// path's registers: 1,111 x 2,667 x 1,008 in bf16 59 us for 18, 14,232 x 8,192 x 2,048 4,180 for 280.
+template <typename T, int MODE, int NI, int NJ, typename F>
+__device__ __forceinline__ void sum_any_scales(const Fp8GemmArgs& a, const uint8_t* w, const uint8_t* x, const float* as,
+                                               const float* bs, int64_t up, int last_n, int last_m, int kt0, int step, F put) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+    const int kb = (a.K + kFp8Block - 1) / kFp8Block;
+    auto frag = [&](const uint8_t* p, int k) {
+        const i32x4_t z = {0, 0, 0, 0};
+        FragOf<T> f;
+        f.set(join(k < a.K ? *reinterpret_cast<const i32x4_t*>(p + k) : z,
+                   k + 16 < a.K ? *reinterpret_cast<const i32x4_t*>(p + k + 16) : z));
+        return f;
+    };
+#pragma unroll 1
+    for (int i = 0; i < NI; ++i) {
+        const uint8_t* wi = w + (int64_t)min(i * 16 + l16, last_n) * a.K;
+        const float* sbs = bs + (MODE == kGlu && i % 4 >= 2 ? up : 0);
+#pragma unroll 1
+        for (int j = 0; j < NJ; ++j) {
+            const int m = min(j * 16 + l16, last_m);
+            const uint8_t* xj = x + (int64_t)m * a.K;
+            f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+            for (int kt = kt0; kt < kb; kt += step) {
+                const int k = kt * kFp8Block + lq * 32;
+                const f32x4_t t = dot(frag(wi, k), frag(xj, k));
+                const float sa = as[(int64_t)m * kb + kt], sb = sbs[kt];
+                const float f = __builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sb);
+                const int e = __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sb);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum[r] += __builtin_ldexpf(t[r] * f, e);
+            }
+            put(i, j, sum);
+        }
+    }
+}
+
 // ---- tiles through LDS ---------------------------------------------------------
 // A block's WN x WM waves share a tile of 16 NI WN weight rows and 16 NJ WM rows;
 // K-blocks of 128 bytes a row go through a ring of two LDS stages, filled by direct loads of
@@ -169,6 +219,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+    bool beyond = false;
     const int sw = l16 & 7;
     const int c0 = (2 * lq) ^ sw, c1 = (2 * lq + 1) ^ sw;
 
@@ -185,7 +236,9 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             return join(*reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c0 * 16),
                         *reinterpret_cast<const i32x4_t*>(p + i * 16 * kFp8Block + c1 * 16));
         };
-        const float sb = s_sb[kt & 1][MODE == kGlu ? 0 : wn * 16 * NI / kFp8Block], sb2 = s_sb[kt & 1][1];
+        const float sb = s_sb[kt & 1][MODE == kGlu ? 0 : wn * 16 * NI / kFp8Block] * kScaleUp;
+        const float sb2 = MODE == kGlu ? s_sb[kt & 1][1] * kScaleUp : 0.0f;
+        beyond |= too_large(sb) | too_large(sb2);  // (times a scale of 0: NaN)
         FragOf<T> x[NJ], w[2];
         float s[NJ], s2[NJ];
         w[0].set(frag(wt, 0));
@@ -196,6 +249,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             const float sa = s_sa[kt & 1][wm * NJ * 16 + j * 16 + l16];
             s[j] = sa * sb;
             s2[j] = MODE == kGlu ? sa * sb2 : 0.0f;
+            beyond |= too_large(s[j]) | too_large(s2[j]);
         }
         // Two products a turn; beside them the scaling of the two before, the next weights' read and a share of the
         // loads of block kt + 1: a direct load goes out every 35 cycles a CU at most, and all of them at a
@@ -226,6 +280,21 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
         scale(kTurns - 1);
     }
     wait_vmcnt<0>();  // (the loads past the end have written their zeros)
+    float down = kScaleDown;
+    if (__any(beyond)) {
+        const int wr = n0 + wn * NI * 16;  // the wave's first weight row, and row
+        const int64_t xr = m0 + wm * NJ * 16;
+        const int block = MODE == kGlu ? tn : min(wr, a.N - 1) / kFp8Block;
+        f32x4_t sums[NI][NJ];
+        sum_any_scales<T, MODE, NI, NJ>(a, a.b + (int64_t)wr * K, a.a + xr * K, a.as + xr * kb, a.bs + (int64_t)block * kb,
+                                        (int64_t)tiles_n * kb, a.N - 1 - wr, (int)min<int64_t>(a.M - 1 - xr, BM), 0, 1,
+                                        [&](int i, int j, const f32x4_t& v) { sums[i][j] = v; });
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = sums[i][j];
+        down = 1.0f;
+    }
 
     if constexpr (MODE == kGlu) {
         // a lane's gate values of weight blocks i and up values of i + 2 are of the same hidden
@@ -245,8 +314,8 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             const float4 bu = *reinterpret_cast<const float4*>(a.bias + at + 32);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                acc[i][j] += f32x4_t{bg.x, bg.y, bg.z, bg.w};
-                acc[i + 2][j] += f32x4_t{bu.x, bu.y, bu.z, bu.w};
+                acc[i][j] = acc[i][j] * down + f32x4_t{bg.x, bg.y, bg.z, bg.w};
+                acc[i + 2][j] = acc[i + 2][j] * down + f32x4_t{bu.x, bu.y, bu.z, bu.w};
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float h = hc[p] + r < a.hidden ? swiglu<__bf16>(acc[i][j][r], acc[i + 2][j][r]) : 0.0f;
@@ -304,7 +373,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             for (int i = 0; i < NI; ++i) {
                 T o[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = Elt<T>::from_f32(acc[i][j][r] + bias[i][r]);
+                for (int r = 0; r < 4; ++r) o[r] = Elt<T>::from_f32(__builtin_fmaf(acc[i][j][r], down, bias[i][r]));
                 __builtin_memcpy(lds + l16 * kRow + (i * 16 + 4 * lq) * sizeof(T), o, sizeof(o));
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (one wave: nothing else to wait for)
@@ -326,7 +395,9 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int m = (wm * NJ + j) * 16 + l16;
-            const f32x4_t v = acc[i][j] + f32x4_t{bias[i][0], bias[i][1], bias[i][2], bias[i][3]};
+            f32x4_t v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(acc[i][j][r], down, bias[i][r]);
             if (m < rows_m) put4(y + (m0 + m) * a.N, n, a.N, v, whole);
         }
     }
@@ -389,6 +460,7 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
     for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    bool beyond = false;
     Step st[P];
 #pragma unroll
     for (int p = 0; p < P; ++p)
@@ -403,7 +475,8 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
             for (int i = 0; i < NI; ++i) w[i].set(join(s.w[i][0], s.w[i][1]));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const float f = s.sa[j] * s.sb, f2 = s.sa[j] * s.sb2;
+                const float up = s.sb * kScaleUp, up2 = s.sb2 * kScaleUp, f = s.sa[j] * up, f2 = s.sa[j] * up2;
+                beyond |= too_large(up) | too_large(f) | too_large(up2) | too_large(f2);
                 FragOf<T> x;
                 x.set(join(s.x[j][0], s.x[j][1]));
 #pragma unroll
@@ -420,7 +493,10 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) s_part[wave][i][j][lane] = acc[i][j];
+        for (int j = 0; j < NT; ++j) s_part[wave][i][j][lane] = acc[i][j] * kScaleDown;
+    if (__any(beyond))
+        sum_any_scales<T, MODE, NI, NT>(a, bt, at, as, bs, (int64_t)hb * kb, a.N - 1 - n0, rows_m - 1, wave, NW,
+                                        [&](int i, int j, const f32x4_t& v) { s_part[wave][i][j][lane] = v; });
     __syncthreads();
     if constexpr (MODE == kGlu) {
         static_assert(MODE != kGlu || NI == 4, "32 gate rows and their 32 up rows");
