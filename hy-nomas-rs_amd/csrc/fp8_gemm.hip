@@ -238,7 +238,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
         };
         const float sb = s_sb[kt & 1][MODE == kGlu ? 0 : wn * 16 * NI / kFp8Block] * kScaleUp;
         const float sb2 = MODE == kGlu ? s_sb[kt & 1][1] * kScaleUp : 0.0f;
-        beyond |= too_large(sb) | too_large(sb2);  // (times a scale of 0: NaN)
+        beyond = beyond || too_large(sb) || too_large(sb2);  // (times a scale of 0: NaN)
         FragOf<T> x[NJ], w[2];
         float s[NJ], s2[NJ];
         w[0].set(frag(wt, 0));
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
             const float sa = s_sa[kt & 1][wm * NJ * 16 + j * 16 + l16];
             s[j] = sa * sb;
             s2[j] = MODE == kGlu ? sa * sb2 : 0.0f;
-            beyond |= too_large(s[j]) | too_large(s2[j]);
+            beyond = beyond || too_large(s[j]) || too_large(s2[j]);
         }
         // Two products a turn; beside them the scaling of the two before, the next weights' read and a share of the
         // loads of block kt + 1: a direct load goes out every 35 cycles a CU at most, and all of them at a
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const float up = s.sb * kScaleUp, up2 = s.sb2 * kScaleUp, f = s.sa[j] * up, f2 = s.sa[j] * up2;
-                beyond |= too_large(up) | too_large(f) | too_large(up2) | too_large(f2);
+                beyond = beyond || too_large(up) || too_large(f) || too_large(up2) || too_large(f2);
                 FragOf<T> x;
                 x.set(join(s.x[j][0], s.x[j][1]));
 #pragma unroll
