@@ -291,14 +291,22 @@ __device__ __forceinline__ void choose(const FewArgs& a, const double* l, int ro
         if (mine >> j & 1) chosen(lane + j * 64);
     }
     if (!store) return;
-    {  // (any number near the largest does)
-        const uint32_t b = wave_maxu(order_key32(m));
-        m = __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+    // Any number within 1 of the largest does: as f32 up to 2^24, from there on (and past f32) the f64 one,
+    // which takes six more shuffles of two words.
+    const uint32_t b = wave_maxu(order_key32(m));
+    m = __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+    double top = (double)m;
+    if (!(__builtin_fabsf(m) < 0x1p24f)) {
+        top = v[0];
+#pragma unroll
+        for (int j = 1; j < PL; ++j) top = fmax(top, v[j]);
+#pragma unroll 1
+        for (int o = 32; o >= 1; o >>= 1) top = fmax(top, __shfl_xor(top, o));
     }
     float p[PL], sum = 0.0f, sel = 0.0f;
 #pragma unroll
     for (int j = 0; j < PL; ++j) {
-        p[j] = lane + j * 64 < E ? expf((float)(v[j] - (double)m)) : 0.0f;
+        p[j] = lane + j * 64 < E ? expf((float)(v[j] - top)) : 0.0f;
         sum += p[j];
         sel += mine >> j & 1 ? p[j] : 0.0f;
     }
