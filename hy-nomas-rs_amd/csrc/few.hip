@@ -36,17 +36,29 @@ template <typename T, bool W8> struct Step {
     }
 };
 
+// 8-bit weights as 16-bit values, and what those are short of the weights' scale `s`: v * rest = w * s.  A block's
+// sum of bf16 rows by weights of up to 448 leaves f32 from 2^112 on, where its product with a scale below 1 does
+// not: such weights are taken times 2^-16 (and stay normal bf16 numbers), so that no sum can.  A scale from 1 on makes
+// the sum larger still.  f16 rows end at 2^16.
 template <typename T> struct Widen8;
 template <> struct Widen8<__bf16> {
     typedef __bf16 V2 __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ V2 run(uint32_t w, bool hi) {
-        return hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, true)
-                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false);
+    float down, rest;
+    __device__ __forceinline__ explicit Widen8(float s) {
+        const bool less = __builtin_fabsf(s) < 1.0f;
+        down = less ? 0x1p-16f : 1.0f;
+        rest = less ? s * 0x1p16f : s;
+    }
+    __device__ __forceinline__ V2 run(uint32_t w, bool hi) const {
+        return hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, down, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, down, false);
     }
 };
 template <> struct Widen8<_Float16> {
     typedef _Float16 V2 __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ V2 run(uint32_t w, bool hi) {
+    float rest;
+    __device__ __forceinline__ explicit Widen8(float s) : rest(s) {}
+    __device__ __forceinline__ V2 run(uint32_t w, bool hi) const {
         return hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, true)
                   : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, false);
     }
@@ -62,6 +74,7 @@ template <typename T, bool W8, int J>
 __device__ __forceinline__ void multiply(f32x4_t* acc, const u32x4_t (&w)[2], const u32x4_t (*x)[Step<T, W8>::XL], float s) {
     if constexpr (W8) {
         typedef typename Mfma<T>::V V;
+        const Widen8<T> to16(s);
         V a[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -69,7 +82,7 @@ __device__ __forceinline__ void multiply(f32x4_t* acc, const u32x4_t (&w)[2], co
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const auto v = Widen8<T>::run(w[q / 2][q % 2 * 2 + i], h);
+                    const auto v = to16.run(w[q / 2][q % 2 * 2 + i], h);
                     a[q][i * 4 + h * 2] = v[0];
                     a[q][i * 4 + h * 2 + 1] = v[1];
                 }
@@ -83,7 +96,7 @@ __device__ __forceinline__ void multiply(f32x4_t* acc, const u32x4_t (&w)[2], co
             // way only: every fourth column was wrong.  So the wait stands here.
             asm volatile("s_nop 8" : "+v"(t));
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(t[r], s, acc[j][r]);
+            for (int r = 0; r < 4; ++r) acc[j][r] = __builtin_fmaf(t[r], to16.rest, acc[j][r]);
         }
     } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
