@@ -1283,7 +1283,7 @@ int MoeLayer::forward_host_pieces(const void* x, void* y, int64_t rows, int np, 
 int MoeLayer::routing(int32_t* idx, float* w, int32_t* counts, float* gap) {
     if (dense_only_) return set_error(NOMAS_ERR_STATE, "a dense feed-forward has no routing");
     if (last_rows_ < 0) return set_error(NOMAS_ERR_STATE, "no forward has run on this handle");
-    if (last_few_given_)
+    if (last_few_given_ && last_rows_ > 0)  // (a forward of no rows has an empty routing)
         return set_error(NOMAS_ERR_STATE, "the last forward of few rows ran under the caller's routing");
     if (last_in_scratch_ && last_rows_ > 0 && scratch_generation(device_) != last_scratch_gen_)
         return set_error(NOMAS_ERR_STATE,
