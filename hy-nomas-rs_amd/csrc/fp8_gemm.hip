@@ -565,10 +565,14 @@ hipError_t few_rows(const Fp8GemmArgs& a, hipStream_t s) {
     return rows<T, kStore, 1, NT, 8, 2>(a, s);
 }
 
-// Up to 32 rows the kernel for few rows; more: the least estimate, in us. Measured, in bf16 (few rows in tiles of
-// 64; tiles of 128 x 128; of 256 x 256): 128 x 8,192 x 2,048 15.3, 18.0, 31.7; 512 x 8,192 x 2,048 50, 19.8, 33;
-// 256 x 2,048 x 2,048 11.2, 17.6, 31; 64 x 2,048 x 8,192 28, 55, 105; 2,048 x 8,192 x 2,048 -, 50, 41; 4,744 x 4,096 x 2,048
-// -, 58, 68; 4,744 x 2,048 x 8,192 -, 131, 117.
+// Up to 32 rows the kernel for few rows; more: the least estimate, in us, from rounds of 256 CUs and steps of 128
+// columns. Measured in bf16 (few rows in tiles of 64; tiles of 128 x 128; of 256 x 256): 128 x 8,192 x 2,048 14.6, 18.1,
+// 31.9; 512 x 8,192 x 2,048 51, 20.4, 33; 256 x 2,048 x 2,048 10.7, 17.6, 31; 40 x 2,048 x 8,192 22, 56, 106; 2,048 x 8,192
+// x 2,048 190, 50, 40; 4,744 x 4,096 x 2,048 -, 58, 68; 4,744 x 2,048 x 8,192 -, 138, 113; 14,232 x 8,192 x 2,048 -, 326, 247.
+// f32 results take twice the MFMA time and registers for widened fragments. Measured (few rows; tiles of 128 x 128; of
+// 256 weight rows x 128, which were 24% slower to 2% faster and are not built): 128 x 8,192 x 2,048 16.8, 23.7, 32.7;
+// 256 x 2,048 x 8,192 34, 78, 116; 1,024 x 1,536 x 4,096 48, 43, 63; 2,048 x 512 x 1,008 9.0, 14.5, 19.7; 4,744 x 2,048 x 8,192
+// -, 188, 233; 14,232 x 8,192 x 2,048 -, 497, 488.
 template <typename T>
 hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
     if (a.M <= 16) return few_rows<T, 1>(a, s);
@@ -576,13 +580,19 @@ hipError_t gemm(const Fp8GemmArgs& a, hipStream_t s) {
     const double kt = (a.K + kFp8Block - 1) / kFp8Block;
     auto rounds = [&](int bm, int bn) { return (double)(((a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) + 255) / 256); };
     const int ni = rows_ni<4>(a.M, a.N);
-    const double few = 5 + rounds(64, 16 * ni) * (2 + 2.2 * std::ceil(kt / rows_waves(ni, 4)));
-    const double r128 = rounds(128, 128), t128 = 4 + kt * (r128 <= 1 ? 0.78 : 0.7 * r128);
-    const double t256 = 4 + rounds(256, 256) * (3 + 1.65 * kt);
-    if (few <= t128 && few <= t256 && a.M <= 65535 * 64) return few_rows<T, 4>(a, s);
-    if (t128 <= t256) return tile<T, kStore, 4, 4, 2, 2>(a, s);
-    // (f32 results: widened fragments take twice the registers, 128 rows a tile)
-    return tile<T, kStore, 8, sizeof(T) == 4 ? 2 : 4, 2, 4>(a, s);
+    const double walk = std::ceil(kt / rows_waves(ni, 4)), r64 = rounds(64, 16 * ni), r128 = rounds(128, 128);
+    if constexpr (sizeof(T) == 4) {
+        const double few = 2 + r64 * (ni == 4 ? 3 + 2.6 * walk : ni == 2 ? 1.3 + 3.85 * walk : 3.4 * walk);
+        const double t128 = 4 + kt * (r128 <= 1 ? 1.17 : 1.05 * r128);
+        if (few <= t128 && a.M <= 65535 * 64) return few_rows<T, 4>(a, s);
+        return tile<T, kStore, 4, 4, 2, 2>(a, s);
+    } else {
+        const double few = 5 + r64 * (2 + 2.2 * walk);
+        const double t128 = 4 + kt * (r128 <= 1 ? 0.78 : 0.7 * r128), t256 = 4 + rounds(256, 256) * (3 + 1.65 * kt);
+        if (few <= t128 && few <= t256 && a.M <= 65535 * 64) return few_rows<T, 4>(a, s);
+        if (t128 <= t256) return tile<T, kStore, 4, 4, 2, 2>(a, s);
+        return tile<T, kStore, 8, 4, 2, 4>(a, s);
+    }
 }
 
 }  // namespace
@@ -617,7 +627,10 @@ hipError_t launch_fp8_glu(DType dt, const Fp8GemmArgs& a, hipStream_t s) {
         return rows<float, kGlu, 4, 4, 4, 2>(a, s);
     }
     if (dt != DType::BF16) return tile<float, kGlu, 8, 2, 2, 4>(a, s);
-    if (a.M * a.N < (int64_t)256 * 256 * 192) return tile<__bf16, kGlu, 8, 2, 2, 4>(a, s);
+    // Tiles of 128 rows while they are one round of the CUs, else of 256 (us a feed-forward, 128 and 256 rows a tile: 512 rows
+    // of 2,048 x 8,192, 256 tiles, 75 and 85; 4,744 of 512 x 512, 152 tiles, 28 and 34; 1,500 of 1,536 x 4,096, 384 tiles, 79
+    // and 71; 9,000 of 2,048 x 512, 284 tiles, 87 and 77; 4,744 of 2,048 x 8,192 358 and 308).
+    if ((a.M + 127) / 128 * (a.N / 256) <= 256) return tile<__bf16, kGlu, 8, 2, 2, 4>(a, s);
     return tile<__bf16, kGlu, 8, 4, 2, 4>(a, s);
 }
 
