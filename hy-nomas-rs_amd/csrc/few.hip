@@ -537,8 +537,10 @@ constexpr int rows_ahead() { return W8 ? (J == 1 ? 4 : J == 2 ? 2 : 1) : J < 4 |
 
 // S waves share a unit (16 hidden units of one expert: 16 gate and 16 up rows), each its own
 // share of the steps: as many small units as there are feed all CUs from the first load on, with no tile of rows to
-// wait for.  Bound by the weights' bytes: 134 MB for 48 rows, 1,024 x 2,048, 16 experts in f16 take 29.8 us (4.5 TB/s); the
-// 50 MB of one row's 8 experts, 2,048 x 768, 13.8 us (3.6 TB/s).
+// wait for.  Bound by the weights' bytes: 134 MB for 48 rows, 1,024 x 2,048, 16 experts in f16 take 29.2 us (4.6 TB/s) where each
+// call has another layer, 24.9 where the same one again finds a part of them in the last-level cache; the 50 MB of one
+// row's 8 experts, 2,048 x 768, 15.2 us (3.3 TB/s) and 13.6; 134 MB of 16 rows, 8 experts in f32 40 us and 34.  With 8-bit
+// weights and more than 32 rows 4 to 10 vector and 78 scalar registers are spilled: 64 rows, 64 experts of 2,048 x 768 46 us.
 template <typename T, bool W8, int NT, int S, int P>
 __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
     typedef Step<T, W8> St;
@@ -724,8 +726,9 @@ __global__ __launch_bounds__(kFewThreads) void few_up_kernel(FewArgs a) {
 }
 
 // A block has 16 columns of y, or with parts > 1 a share of their sums' steps: all experts of a row end in one
-// block (or kFewParts), so nothing is written between.  67 MB for 48 rows, 1,024 x 2,048, 16 experts in f16: 18.4 us (3.6
-// TB/s; 64 tiles of 16 columns in 4 parts, a block a CU); 25 MB of one row's 8 experts, 2,048 x 768: 9.5 us.
+// block (or kFewParts), so nothing is written between.  67 MB for 48 rows, 1,024 x 2,048, 16 experts in f16: 18.0 us (3.7
+// TB/s; 64 tiles of 16 columns in 4 parts, a block a CU); 25 MB of one row's 8 experts, 2,048 x 768: 10.4 us (both from HBM: each
+// call another layer).
 template <typename T, bool W8, int NT, int P>
 __global__ __launch_bounds__(kFewThreads) void few_down_kernel(FewArgs a) {
     typedef Step<T, W8> St;

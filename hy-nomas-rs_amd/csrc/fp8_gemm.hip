@@ -142,8 +142,10 @@ __device__ __forceinline__ void sum_any_scales(const Fp8GemmArgs& a, const uint8
 // K-blocks of 128 bytes a row go through a ring of two LDS stages, filled by direct loads of
 // whole 128-byte rows.  16-byte chunk c of row r is kept at chunk c ^ (r % 8), so that the
 // fragment reads (one chunk of 8 rows at a time) touch every bank once.  Bound by the matrix pipes and the scaling's
-// vector instructions beside them: 14,232 x 8,192 x 2,048 in bf16 248 us (1,930 TFLOP/s), 8,192 x 8,192 x 8,192 541 us
-// (2,034); the rest of a tile's time is its first loads and its outputs.
+// vector instructions beside them: 14,232 x 8,192 x 2,048 in bf16 245-280 us by the card's clock (1,710-1,950 TFLOP/s; the pipes
+// are busy 41% of the cycles); the rest of a tile's time is its first loads and its outputs.  f32 results 487 us.  Where there is less
+// than a round of tiles, a step waits for its loads (0.8 us; f32 1.2): 1,111 x 2,667 x 1,008 in f16, 189 tiles of 128 x 128, takes
+// 16.5 us, and 13.4 with 2,672 columns, whose outputs leave in whole lines.
 template <typename T, int MODE, int NI, int NJ, int WN, int WM>
 __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a, int tiles_m, int tiles_n) {
     constexpr int NW = WN * WM, BN = 16 * NI * WN, BM = 16 * NJ * WM;
@@ -406,7 +408,8 @@ __global__ __launch_bounds__(WN * WM * kWave) void fp8_tile_kernel(Fp8GemmArgs a
 // ---- few rows --------------------------------------------------------------------
 // 16 NT rows x 16 NI weight rows a block; its NW waves take the K-blocks in turn, operands
 // straight from global memory, and add their sums in LDS in wave order: LDS holds nothing that two waves
-// read, and every CU has loads under way at once.  Bound by latency: 16.8 MB of one row's 8,192 x 2,048 take 7.5 us.
+// read, and every CU has loads under way at once.  Bound by latency: 16.8 MB of one row's 8,192 x 2,048 take 5 us, 40
+// rows of 1,536 x 4,096 in f32 12.4 (96 blocks, each of them all of K).  The gate and up kernel of 17 to 32 rows spills 9 registers.
 template <typename T, int MODE, int NI, int NT, int NW, int P>
 __global__ __launch_bounds__(NW * kWave) void fp8_rows_kernel(Fp8GemmArgs a) {
     constexpr int BN = 16 * NI, BM = 16 * NT;

@@ -382,7 +382,8 @@ int nomas_quantize_fp8(int dtype, const void* x, int64_t rows, int64_t cols, int
  * with scales (ceil(n / 128), ceil(k / 128)), any f32 values; bias n f32 or NULL.  A block's
  * sums are scaled and added in f32, and rounded once.  For 16-bit results the 8-bit matrix
  * instructions make them, which keep 13 bits below the largest of each 8 products (1.4e-5 of a
- * result on random values); f32 results have exact products and f32 sums.  The order of the
+ * result on random values); f32 results have exact products and f32 sums.  Scales whose product
+ * leaves f32's range are taken apart, at 2 to 15 times the time from products of 2^55 on.  The order of the
  * sums depends on the sizes.  1 <= k <= 2^22 with k % 16 == 0; a, b and y 16-byte, the
  * others 4-byte aligned; y shares no memory with the inputs. */
 int nomas_matmul_fp8(int dtype, const void* a, const float* a_scale, const void* b, const float* b_scale,
